@@ -18,7 +18,7 @@ static const char* const kKernelNames[KID_NUM] = {
     "indptr_from_sorted", "relabel_setup", "relabel_pcount", "relabel_pscan", "relabel_scatter",
     "relabel_dedupe", "relabel_mark", "relabel_prefix", "relabel_rank", "relabel_emit",
     "slice_rows", "edge_sum", "edge_op", "list_sample", "walk", "sort", "sample_probs_short",
-    "sample_probs_long", "misc"};
+    "sample_probs_long", "misc", "embed", "embed_sort", "embed_grad", "dropout", "loss", "loss_grad", "loss_join"};
 
 struct TimedLaunch {
   int id, tag;

@@ -271,7 +271,8 @@ enum KernelId {
   KID_SAMPLE = 0, KID_SAMPLE_PROBS, KID_COUNT, KID_SLICE_FILL, KID_GATHER, KID_EXPAND,
   KID_INDPTR_SORTED, KID_RL_SETUP, KID_RL_PCOUNT, KID_RL_PSCAN, KID_RL_SCATTER, KID_RL_DEDUPE,
   KID_RL_COUNT, KID_RL_TILES, KID_RL_SCAN, KID_RL_EDGES, KID_SLICE_ROWS, KID_EDGE_SUM,
-  KID_EDGE_OP, KID_LIST_SAMPLE, KID_WALK, KID_SORT, KID_SAMPLE_PROBS_SHORT, KID_SAMPLE_PROBS_LONG, KID_MISC, KID_NUM
+  KID_EDGE_OP, KID_LIST_SAMPLE, KID_WALK, KID_SORT, KID_SAMPLE_PROBS_SHORT, KID_SAMPLE_PROBS_LONG, KID_MISC,
+  KID_EMBED, KID_EMBED_SORT, KID_EMBED_GRAD, KID_DROPOUT, KID_LOSS, KID_LOSS_GRAD, KID_LOSS_JOIN, KID_NUM
 };
 struct LaunchScope {
   LaunchScope(int id, cudaStream_t st);

@@ -858,8 +858,27 @@ torch::Tensor& AsyncErrorWord(const torch::Device& dev) {
   static auto* words = new std::map<int, torch::Tensor>();
   std::lock_guard<std::mutex> lock(mu);
   auto it = words->find(dev.index());
-  if (it == words->end())
-    it = words->emplace(dev.index(), torch::zeros({1}, torch::dtype(torch::kInt32).device(dev))).first;
+  if (it == words->end()) {
+    // Not from the caching allocator: the first call may be recorded into a CUDA graph, whose pool
+    // (and zero fill) would then own the word.  The fill is waited for on a stream of its own, so
+    // that every stream finds it done.
+    c10::cuda::CUDAGuard guard(dev);
+    void* word = nullptr;
+    cudaStream_t st = nullptr;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e == cudaSuccess) {
+      e = cudaMalloc(&word, 256);
+      if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+      if (e == cudaSuccess) e = cudaMemsetAsync(word, 0, 256, st);
+      if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+      if (st) cudaStreamDestroy(st);
+      cudaThreadExchangeStreamCaptureMode(&mode);
+    }
+    if (e != cudaSuccess && word) cudaFree(word);
+    TORCH_CHECK(e == cudaSuccess, "gsb200: no device memory for the error word (", cudaGetErrorString(e), ")");
+    it = words->emplace(dev.index(), torch::from_blob(word, {1}, torch::dtype(torch::kInt32).device(dev))).first;
+  }
   return it->second;
 }
 
@@ -868,7 +887,7 @@ void CheckAsyncErrors() {
   auto& w = AsyncErrorWord(dev);
   const int bits = w.item<int>();
   if (bits) w.zero_();
-  CheckDeviceError(bits, "an earlier sync-free operator (row gather, single-list sampling, walks)");
+  CheckDeviceError(bits, "an earlier sync-free operator (row gather, single-list sampling, walks, embedding, loss)");
 }
 
 // out[i, ...] = data[index[i], ...].  `data` lives on the GPU or in page-locked

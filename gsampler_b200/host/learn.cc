@@ -1,0 +1,139 @@
+#include "learn.h"
+
+#include <c10/cuda/CUDAGuard.h>
+
+#include <atomic>
+#include <cmath>
+#include <mutex>
+
+#include "graph.h"
+#include "gsb200.h"
+
+namespace gsb_host {
+
+static int ValueType(const torch::Tensor& t, const char* op, const char* name) {
+  TORCH_CHECK(t.defined(), op, ": ", name, " is undefined");
+  TORCH_CHECK(t.is_cuda(), op, ": ", name, " must be a CUDA tensor (this library has no CPU path)");
+  switch (t.scalar_type()) {
+    case torch::kFloat32: return GSB_F32;
+    case torch::kFloat16: return GSB_F16;
+    case torch::kBFloat16: return GSB_BF16;
+    default: TORCH_CHECK(false, op, ": ", name, " must be float32, float16 or bfloat16, got ", t.scalar_type());
+  }
+}
+
+static void CheckIndex(const torch::Tensor& t, const char* op, const char* name) {
+  TORCH_CHECK(t.defined() && t.is_cuda(), op, ": ", name, " must be a CUDA tensor (this library has no CPU path)");
+  TORCH_CHECK(t.scalar_type() == torch::kInt64, op, ": ", name, " must be int64");
+}
+
+static int* ErrorWord(const torch::Device& dev) { return AsyncErrorWord(dev).data_ptr<int>(); }
+
+// ------------------------------------------------------------------ embedding
+torch::Tensor Embedding(torch::Tensor weight, torch::Tensor index, double scale, int64_t padding) {
+  const int dt = ValueType(weight, "Embedding", "weight");
+  CheckIndex(index, "Embedding", "index");
+  TORCH_CHECK(weight.device() == index.device(), "Embedding: weight and index live on different devices");
+  TORCH_CHECK(weight.dim() == 2, "Embedding: weight must be two-dimensional");
+  TORCH_CHECK(std::isfinite(scale), "Embedding: scale must be finite");
+  c10::cuda::CUDAGuard guard(index.device());
+  // rows may be strided (a column slice of a wider table is read in place)
+  if (weight.size(1) > 1 && weight.stride(1) != 1) weight = weight.contiguous();
+  if (weight.size(0) > 1 && weight.stride(0) < weight.size(1)) weight = weight.contiguous();
+  index = index.contiguous();
+  auto sizes = index.sizes().vec();
+  sizes.push_back(weight.size(1));
+  auto out = torch::empty(sizes, weight.options());
+  const int64_t ld = weight.size(0) > 1 ? weight.stride(0) : weight.size(1);
+  CheckStatus(gsb_embedding(weight.data_ptr(), dt, ld, weight.size(0), weight.size(1), index.data_ptr<int64_t>(),
+                            index.numel(), (float)scale, padding, out.data_ptr(), ErrorWord(index.device()),
+                            CurrentStream()),
+              "embedding");
+  return out;
+}
+
+static void CheckEmbeddingGrad(const torch::Tensor& grad, const torch::Tensor& index, int64_t num_rows) {
+  CheckIndex(index, "EmbeddingGrad", "index");
+  TORCH_CHECK(grad.device() == index.device(), "EmbeddingGrad: grad and index live on different devices");
+  TORCH_CHECK(grad.dim() == index.dim() + 1 && grad.sizes().slice(0, index.dim()) == index.sizes(),
+              "EmbeddingGrad: grad must have the shape of index and one more dimension");
+  TORCH_CHECK(num_rows >= 0 && num_rows < 0xFFFFFFFFll, "EmbeddingGrad: the table must have fewer than 2^32 - 1 rows");
+  TORCH_CHECK(index.numel() < (1ll << 31), "EmbeddingGrad: at most 2^31 - 1 ids a call");
+}
+
+torch::Tensor EmbeddingGrad(torch::Tensor grad, torch::Tensor index, int64_t num_rows, double scale, int64_t padding) {
+  const int dt = ValueType(grad, "EmbeddingGrad", "grad");
+  CheckEmbeddingGrad(grad, index, num_rows);
+  c10::cuda::CUDAGuard guard(index.device());
+  grad = grad.contiguous();
+  index = index.contiguous();
+  const int64_t n = index.numel(), D = grad.size(-1);
+  auto out = torch::empty({num_rows, D}, grad.options());
+  auto ws = NewWorkspace(gsb_embedding_grad_workspace_bytes(n, num_rows, D), index.device());
+  CheckStatus(gsb_embedding_grad(grad.data_ptr(), dt, D, index.data_ptr<int64_t>(), n, num_rows, (float)scale, padding,
+                                 out.data_ptr(), ws.data_ptr(), (size_t)ws.numel(), ErrorWord(index.device()),
+                                 CurrentStream()),
+              "embedding_grad");
+  return out;
+}
+
+std::tuple<torch::Tensor, torch::Tensor> EmbeddingSparseGrad(torch::Tensor grad, torch::Tensor index, int64_t num_rows,
+                                                             double scale, int64_t padding) {
+  const int dt = ValueType(grad, "EmbeddingSparseGrad", "grad");
+  CheckEmbeddingGrad(grad, index, num_rows);
+  c10::cuda::CUDAGuard guard(index.device());
+  grad = grad.contiguous();
+  index = index.contiguous();
+  const int64_t n = index.numel(), D = grad.size(-1);
+  if (n == 0) return {torch::empty({0}, index.options()), torch::empty({0, D}, grad.options())};
+  auto ws = NewWorkspace(gsb_embedding_grad_workspace_bytes(n, num_rows, D), index.device());
+  auto ids = torch::empty({n}, index.options());
+  auto num = torch::empty({1}, index.options());
+  CheckStatus(gsb_embedding_sort(index.data_ptr<int64_t>(), n, num_rows, D, padding, ids.data_ptr<int64_t>(),
+                                 num.data_ptr<int64_t>(), ws.data_ptr(), (size_t)ws.numel(), ErrorWord(index.device()),
+                                 CurrentStream()),
+              "embedding_sort");
+  const int64_t U = num.item<int64_t>();
+  auto rows = torch::empty({U, D}, grad.options());
+  CheckStatus(gsb_embedding_grad_rows(grad.data_ptr(), dt, D, n, num_rows, U, (float)scale, rows.data_ptr(),
+                                      ws.data_ptr(), (size_t)ws.numel(), CurrentStream()),
+              "embedding_grad_rows");
+  return {ids.narrow(0, 0, U).clone(), rows};
+}
+
+// ------------------------------------------------------------------ dropout
+torch::Tensor Dropout(torch::Tensor data, double p, int64_t seed, int64_t stream, c10::optional<torch::Tensor> step) {
+  const int dt = ValueType(data, "Dropout", "data");
+  TORCH_CHECK(p >= 0.0 && p <= 1.0, "Dropout: p must lie in [0, 1], got ", p);
+  c10::cuda::CUDAGuard guard(data.device());
+  const int64_t* step_ptr = nullptr;
+  if (step.has_value()) {
+    CheckIndex(*step, "Dropout", "step");
+    TORCH_CHECK(step->numel() == 1 && step->device() == data.device(),
+                "Dropout: step must have one element on data's device");
+    step_ptr = step->data_ptr<int64_t>();
+  }
+  data = data.contiguous();
+  auto out = torch::empty(data.sizes(), data.options());
+  CheckStatus(gsb_dropout(data.data_ptr(), dt, data.numel(), p, (uint64_t)seed, (uint32_t)stream, step_ptr,
+                          out.data_ptr(), CurrentStream()),
+              "dropout");
+  return out;
+}
+
+static std::mutex g_dropout_mutex;
+static uint64_t g_dropout_seed = 7777;
+static uint32_t g_dropout_calls = 0;
+
+void SetDropoutSeed(int64_t seed) {
+  std::lock_guard<std::mutex> lock(g_dropout_mutex);
+  g_dropout_seed = (uint64_t)seed;
+  g_dropout_calls = 0;
+}
+
+std::tuple<int64_t, int64_t> NextDropoutStream() {
+  std::lock_guard<std::mutex> lock(g_dropout_mutex);
+  return {(int64_t)g_dropout_seed, (int64_t)g_dropout_calls++};
+}
+
+}  // namespace gsb_host

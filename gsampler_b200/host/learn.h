@@ -1,0 +1,22 @@
+// Operators on learned node values behind torch.ops.gs_ops.*: embedding lookup, dropout and the
+// softmax cross entropy over a vocabulary, each with its gradient.  They have no counterpart in
+// the reference, whose examples hand these steps to torch.
+#pragma once
+#include <torch/script.h>
+
+#include <tuple>
+
+namespace gsb_host {
+
+torch::Tensor Embedding(torch::Tensor weight, torch::Tensor index, double scale, int64_t padding);
+torch::Tensor EmbeddingGrad(torch::Tensor grad, torch::Tensor index, int64_t num_rows, double scale, int64_t padding);
+// (ids, rows): the touched rows, ids ascending; one read-back (their number)
+std::tuple<torch::Tensor, torch::Tensor> EmbeddingSparseGrad(torch::Tensor grad, torch::Tensor index, int64_t num_rows,
+                                                             double scale, int64_t padding);
+// `step` (optional one-element int64 tensor on the GPU) is added to `stream` when the kernel runs
+torch::Tensor Dropout(torch::Tensor data, double p, int64_t seed, int64_t stream, c10::optional<torch::Tensor> step);
+// default random state of dropout: a seed and a per-process call counter, as for list sampling
+void SetDropoutSeed(int64_t seed);
+std::tuple<int64_t, int64_t> NextDropoutStream();
+
+}  // namespace gsb_host

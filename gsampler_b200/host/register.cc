@@ -4,6 +4,7 @@
 #include <torch/script.h>
 
 #include "graph.h"
+#include "learn.h"
 #include "ops.h"
 
 using gsb_host::Graph;
@@ -90,4 +91,11 @@ TORCH_LIBRARY(gs_ops, m) {
   m.def("_CAPI_SetListSamplingSeed", &gsb_host::SetListSamplingSeed);
   m.def("_CAPI_GatherRows", &gsb_host::GatherRows);
   m.def("_CAPI_CheckAsyncErrors", &gsb_host::CheckAsyncErrors);
+  // operators on learned node values (no counterpart in the reference)
+  m.def("_CAPI_Embedding", &gsb_host::Embedding);
+  m.def("_CAPI_EmbeddingGrad", &gsb_host::EmbeddingGrad);
+  m.def("_CAPI_EmbeddingSparseGrad", &gsb_host::EmbeddingSparseGrad);
+  m.def("_CAPI_Dropout", &gsb_host::Dropout);
+  m.def("_CAPI_SetDropoutSeed", &gsb_host::SetDropoutSeed);
+  m.def("_CAPI_NextDropoutStream", &gsb_host::NextDropoutStream);
 }

@@ -49,6 +49,9 @@ enum {
 /* indices_dtype */
 enum { GSB_I32 = 0, GSB_I64 = 1 };
 
+/* element types of the operators on learned values (embedding, dropout, loss) */
+enum { GSB_F32 = 0, GSB_F16 = 1, GSB_BF16 = 2 };
+
 /* bits of the device error word (`d_err`, an int in device memory that the
  * caller zeroes once and may poll after synchronising) */
 enum {
@@ -214,6 +217,53 @@ GSB_API int gsb_gather_i64(const int64_t* src, const int64_t* idx, int64_t n, in
 GSB_API int gsb_gather_rows(const void* src, int64_t row_bytes, int64_t src_rows,
                             const int64_t* idx, int64_t n, void* out, int* d_err,
                             void* cuda_stream);
+
+/* ------------------------------------------------------------------ learned node values
+ * What a model does with the ids that sampling and walks produce when the node
+ * values are learned (no counterpart in the reference, whose examples hand that
+ * to torch).  Values are fp32, fp16 or bf16 (`dtype`, GSB_F32 ...); sums are
+ * held in 32 bits and rounded once.  No call allocates or synchronises.
+ *
+ * gsb_embedding: out[i,:] = scale * weight[idx[i],:], rows of D elements; a row
+ * of `weight` starts ld elements after the one before.  idx[i] == padding gives
+ * a row of zeros; any other id outside [0, rows) does too and sets
+ * GSB_ERRBIT_BAD_INPUT. */
+#define GSB_EMBED_MAX_D (1 << 20)
+GSB_API int gsb_embedding(const void* weight, int dtype, int64_t ld, int64_t rows, int64_t D,
+                          const int64_t* idx, int64_t n, float scale, int64_t padding, void* out,
+                          int* d_err, void* cuda_stream);
+
+/* The gradient of gsb_embedding with respect to weight, dense: out[rows, D],
+ * out[v,:] = scale * sum of grad[i,:] over idx[i] == v in ascending order of i
+ * (grad contiguous [n, D]), zeros for rows that no id names.  The order of the
+ * sums depends on the ids alone: the same inputs give the same bits.
+ * n < 2^31, rows < 2^32 - 1. */
+GSB_API size_t gsb_embedding_grad_workspace_bytes(int64_t n, int64_t rows, int64_t D);
+GSB_API int gsb_embedding_grad(const void* grad, int dtype, int64_t D, const int64_t* idx, int64_t n,
+                               int64_t rows, float scale, int64_t padding, void* out, void* workspace,
+                               size_t workspace_bytes, int* d_err, void* cuda_stream);
+
+/* The same gradient for the touched rows only, in two calls on one workspace:
+ * gsb_embedding_sort writes the distinct ids in ascending order to ids[n] and
+ * their number to *d_num (device); gsb_embedding_grad_rows, given that number,
+ * writes their gradients to out[num, D].  n > 0. */
+GSB_API int gsb_embedding_sort(const int64_t* idx, int64_t n, int64_t rows, int64_t D, int64_t padding,
+                               int64_t* ids, int64_t* d_num, void* workspace, size_t workspace_bytes,
+                               int* d_err, void* cuda_stream);
+GSB_API int gsb_embedding_grad_rows(const void* grad, int dtype, int64_t D, int64_t n, int64_t rows,
+                                    int64_t num, float scale, void* out, void* workspace,
+                                    size_t workspace_bytes, void* cuda_stream);
+
+/* Dropout from the counter-based streams: with T = floor(65536 p + 0.5),
+ * y[e] = x[e] * 65536 / (65536 - T) where the 16-bit number of element e is at
+ * least T, else 0 (also where x[e] is not finite).  The number is halfword e % 8
+ * (low halves first) of the Philox4x32-10 block with counter
+ * {e / 8 low, e / 8 high, 0, stream} and key = seed; stream_dev (optional device
+ * int64) is added to `stream` when the kernel runs, so that a recorded CUDA
+ * graph can draw a new mask at every replay.  The backward pass is the same
+ * call on the gradient.  x and y contiguous, n elements; y may be x. */
+GSB_API int gsb_dropout(const void* x, int dtype, int64_t n, double p, uint64_t seed, uint32_t stream,
+                        const int64_t* stream_dev, void* y, void* cuda_stream);
 
 /* ------------------------------------------------------------------ format conversion
  * CSC -> COO column expansion: out[e] = column owning edge e.  Replaces
