@@ -136,4 +136,96 @@ std::tuple<int64_t, int64_t> NextDropoutStream() {
   return {(int64_t)g_dropout_seed, (int64_t)g_dropout_calls++};
 }
 
+// ------------------------------------------------------------------ vocabulary cross entropy
+// rows of a matrix may be strided; anything else is copied
+static torch::Tensor Rows(torch::Tensor t) {
+  if (t.size(1) > 1 && t.stride(1) != 1) return t.contiguous();
+  if (t.size(0) > 1 && t.stride(0) < t.size(1)) return t.contiguous();
+  return t;
+}
+static int64_t RowStep(const torch::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+static int CheckLoss(const torch::Tensor& x, const torch::Tensor& weight, const torch::Tensor& target, double scale) {
+  const char* op = "LinearCrossEntropy";
+  const int dt = ValueType(x, op, "x");
+  ValueType(weight, op, "weight");
+  CheckIndex(target, op, "target");
+  TORCH_CHECK(x.scalar_type() == weight.scalar_type(), op, ": x and weight have different types");
+  TORCH_CHECK(x.device() == weight.device() && x.device() == target.device(), op,
+              ": x, weight and target live on different devices");
+  TORCH_CHECK(x.dim() == 2 && weight.dim() == 2 && x.size(1) == weight.size(1), op,
+              ": x must be [N, D] and weight [V, D], got ", x.sizes(), " and ", weight.sizes());
+  TORCH_CHECK(target.dim() == 1 && target.size(0) == x.size(0), op, ": target must be [N]");
+  TORCH_CHECK(weight.size(0) >= 1 && weight.size(1) >= 1, op, ": weight must have a row and a column");
+  TORCH_CHECK(weight.size(1) <= GSB_LOSS_MAX_D, op, ": at most ", GSB_LOSS_MAX_D, " columns");
+  TORCH_CHECK(x.size(0) < (1ll << 31) && weight.size(0) < (1ll << 31), op, ": at most 2^31 - 1 rows");
+  TORCH_CHECK(std::isfinite(scale), op, ": scale must be finite");
+  return dt;
+}
+
+std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropy(torch::Tensor x, torch::Tensor weight, torch::Tensor target,
+                                                            double scale, int64_t ignore) {
+  const int dt = CheckLoss(x, weight, target, scale);
+  c10::cuda::CUDAGuard guard(x.device());
+  x = Rows(x);
+  weight = Rows(weight);
+  target = target.contiguous();
+  const int64_t N = x.size(0), V = weight.size(0), D = x.size(1);
+  auto f32 = x.options().dtype(torch::kFloat32);
+  auto loss = torch::empty({N}, f32), lse2 = torch::empty({N}, f32);
+  auto ws = NewWorkspace(gsb_linear_ce_workspace_bytes(N, V, D), x.device());
+  CheckStatus(gsb_linear_ce(x.data_ptr(), dt, RowStep(x), N, weight.data_ptr(), RowStep(weight), V, D,
+                            target.data_ptr<int64_t>(), ignore, (float)scale, loss.data_ptr<float>(),
+                            lse2.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), ErrorWord(x.device()),
+                            CurrentStream()),
+              "linear_ce");
+  return {loss, lse2};
+}
+
+std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyTotal(torch::Tensor loss, torch::Tensor target,
+                                                                 int64_t vocabulary, int64_t ignore, bool mean) {
+  CheckIndex(target, "LinearCrossEntropyTotal", "target");
+  TORCH_CHECK(loss.is_cuda() && loss.scalar_type() == torch::kFloat32 && loss.is_contiguous() &&
+                  loss.sizes() == target.sizes() && loss.device() == target.device(),
+              "LinearCrossEntropyTotal: loss must be the contiguous float32 losses of target's rows");
+  c10::cuda::CUDAGuard guard(loss.device());
+  target = target.contiguous();
+  auto total = torch::empty({}, loss.options()), count = torch::empty({}, loss.options());
+  CheckStatus(gsb_linear_ce_total(loss.data_ptr<float>(), target.data_ptr<int64_t>(), ignore, vocabulary, loss.numel(),
+                                  mean, total.data_ptr<float>(), count.data_ptr<float>(), CurrentStream()),
+              "linear_ce_total");
+  return {total, count};
+}
+
+std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyGrad(torch::Tensor x, torch::Tensor weight,
+                                                                torch::Tensor target, torch::Tensor lse2,
+                                                                torch::Tensor upstream,
+                                                                c10::optional<torch::Tensor> count, double scale,
+                                                                int64_t ignore, bool want_dx, bool want_dw) {
+  const int dt = CheckLoss(x, weight, target, scale);
+  const int64_t N = x.size(0), V = weight.size(0), D = x.size(1);
+  auto good = [&](const torch::Tensor& t, int64_t n) {
+    return t.is_cuda() && t.device() == x.device() && t.scalar_type() == torch::kFloat32 && t.numel() == n;
+  };
+  const bool per_row = upstream.dim() == 1;
+  TORCH_CHECK(good(lse2, N) && lse2.is_contiguous(), "LinearCrossEntropyGrad: lse2 must be float32 [N]");
+  TORCH_CHECK(good(upstream, per_row ? N : 1), "LinearCrossEntropyGrad: upstream must be float32, one value or [N]");
+  TORCH_CHECK(!count.has_value() || good(*count, 1), "LinearCrossEntropyGrad: count must be one float32 value");
+  c10::cuda::CUDAGuard guard(x.device());
+  x = Rows(x);
+  weight = Rows(weight);
+  target = target.contiguous();
+  upstream = upstream.contiguous();
+  auto dx = want_dx ? torch::empty({N, D}, x.options()) : torch::empty({0}, x.options());
+  auto dw = want_dw ? torch::empty({V, D}, x.options()) : torch::empty({0}, x.options());
+  auto ws = NewWorkspace(gsb_linear_ce_grad_workspace_bytes(N, V, D, want_dx, want_dw), x.device());
+  CheckStatus(gsb_linear_ce_grad(x.data_ptr(), dt, RowStep(x), N, weight.data_ptr(), RowStep(weight), V, D,
+                                 target.data_ptr<int64_t>(), ignore, (float)scale, lse2.data_ptr<float>(),
+                                 upstream.data_ptr<float>(), per_row, count.has_value() ? count->data_ptr<float>() : nullptr,
+                                 want_dx ? dx.data_ptr() : nullptr, want_dw ? dw.data_ptr() : nullptr, ws.data_ptr(),
+                                 (size_t)ws.numel(), CurrentStream()),
+              "linear_ce_grad");
+  return {dx, dw};
+}
+
 }  // namespace gsb_host

@@ -98,4 +98,7 @@ TORCH_LIBRARY(gs_ops, m) {
   m.def("_CAPI_Dropout", &gsb_host::Dropout);
   m.def("_CAPI_SetDropoutSeed", &gsb_host::SetDropoutSeed);
   m.def("_CAPI_NextDropoutStream", &gsb_host::NextDropoutStream);
+  m.def("_CAPI_LinearCrossEntropy", &gsb_host::LinearCrossEntropy);
+  m.def("_CAPI_LinearCrossEntropyTotal", &gsb_host::LinearCrossEntropyTotal);
+  m.def("_CAPI_LinearCrossEntropyGrad", &gsb_host::LinearCrossEntropyGrad);
 }
