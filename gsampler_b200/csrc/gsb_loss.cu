@@ -4,8 +4,8 @@
 //   dx_i = g_i s (sum_j p_ij w_j - w_{t_i})     dW_j = s sum_i g_i (p_ij - [t_i = j]) x_i
 //   p_ij = exp(l_ij - lse_i)
 //
-// This file has the form that takes every type and width: products by 32-bit multiply-adds on
-// 128 x 64 tiles.  The forward pass runs over the vocabulary once with the running maximum and
+// This file has the form that takes every type and width (gsb_loss_tc.cu has the one for 16-bit
+// types of up to 256 columns): products by 32-bit multiply-adds on 128 x 64 tiles.  The forward pass runs over the vocabulary once with the running maximum and
 // sum of every row.  The backward pass takes the vocabulary in pieces: the logits of a piece are
 // computed again, turned into g (p - target) in a workspace of at most PIECE_ELEMS values, and
 // multiplied with W (for dx) and with x (for dW).  Bound by the 32-bit multiply-add rate.
@@ -409,26 +409,36 @@ static bool loss_sizes_ok(i64 N, i64 V, i64 D, i64 ldx, i64 ldw) {
          (V < 2 || ldw >= D);
 }
 
-extern "C" size_t gsb_linear_ce_workspace_bytes(int64_t N, int64_t V, int64_t D) {
+extern "C" int gsb_linear_ce_has_pull(int dtype, int64_t N, int64_t V, int64_t D) { return tc_loss_takes(dtype, N, V, D); }
+
+extern "C" size_t gsb_linear_ce_workspace_bytes(int dtype, const void* weight, int64_t ldw, int64_t N, int64_t V, int64_t D,
+                                                int want_pull) {
   if (!loss_sizes_ok(N, V, D, D, D)) return 0;
+  if (tc_loss_takes(dtype, N, V, D)) return tc_loss_workspace(N, V, D, want_pull != 0, tc_loss_packs(weight, ldw));
   return simt_loss_workspace(N, V, D);
 }
 
 extern "C" int gsb_linear_ce(const void* x, int dtype, int64_t ldx, int64_t N, const void* weight, int64_t ldw, int64_t V,
                              int64_t D, const int64_t* target, int64_t ignore, float scale, float* loss, float* lse2,
-                             void* workspace, size_t workspace_bytes, int* d_err, void* cuda_stream) {
+                             float* pull, void* workspace, size_t workspace_bytes, int* d_err, void* cuda_stream) {
   if (!loss_sizes_ok(N, V, D, ldx, ldw) || !(scale - scale == 0.f)) return GSB_ERR_INVALID;
   if (dtype != GSB_F32 && dtype != GSB_F16 && dtype != GSB_BF16) return GSB_ERR_INVALID;
+  if (pull && !gsb_linear_ce_has_pull(dtype, N, V, D)) return GSB_ERR_UNSUPPORTED;
   if (N == 0) return GSB_OK;
   if (!x || !weight || !target || !loss || !lse2) return GSB_ERR_INVALID;
-  if (!workspace || workspace_bytes < gsb_linear_ce_workspace_bytes(N, V, D)) return GSB_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < gsb_linear_ce_workspace_bytes(dtype, weight, ldw, N, V, D, pull != nullptr))
+    return GSB_ERR_WORKSPACE;
   LossArgs a = {};
   a.x = x; a.ldx = ldx; a.N = N; a.w = weight; a.ldw = ldw; a.V = V; a.D = D;
   a.target = (const i64*)target; a.ignore = ignore; a.scale = scale; a.loss = loss; a.lse2 = lse2;
   a.ws = workspace; a.err = d_err; a.st = (cudaStream_t)cuda_stream;
-  if (dtype == GSB_F32) simt_forward<float>(a);
+  int rc = GSB_OK;
+  if (tc_loss_takes(dtype, N, V, D))
+    rc = dtype == GSB_F16 ? tc_loss_forward<__half>(a, pull) : tc_loss_forward<__nv_bfloat16>(a, pull);
+  else if (dtype == GSB_F32) simt_forward<float>(a);
   else if (dtype == GSB_F16) simt_forward<__half>(a);
   else simt_forward<__nv_bfloat16>(a);
+  if (rc != GSB_OK) return rc;
   GSB_CUDA_OK(cudaGetLastError());
   return GSB_OK;
 }
@@ -443,15 +453,25 @@ extern "C" int gsb_linear_ce_total(const float* loss, const int64_t* target, int
   return GSB_OK;
 }
 
-extern "C" size_t gsb_linear_ce_grad_workspace_bytes(int64_t N, int64_t V, int64_t D, int want_dx, int want_dw) {
+extern "C" size_t gsb_linear_ce_grad_workspace_bytes(int dtype, const void* weight, int64_t ldw, int64_t N, int64_t V, int64_t D,
+                                                     int have_pull, int want_dx, int want_dw) {
   if (!loss_sizes_ok(N, V, D, D, D)) return 0;
-  return up256(4 * (size_t)N) + 256 + simt_loss_grad_workspace(N, V, D, want_dx != 0, want_dw != 0);
+  const size_t head = up256(4 * (size_t)N) + 256;
+  const bool tc = tc_loss_takes(dtype, N, V, D);
+  const bool simt_dx = want_dx && !(tc && have_pull), simt_dw = want_dw && !tc;
+  size_t need = simt_dx || simt_dw ? simt_loss_grad_workspace(N, V, D, simt_dx, simt_dw) : 0;
+  if (tc && want_dw) {
+    const size_t b = tc_loss_grad_workspace(N, V, D, tc_loss_packs(weight, ldw));
+    if (b > need) need = b;
+  }
+  return head + need;
 }
 
 extern "C" int gsb_linear_ce_grad(const void* x, int dtype, int64_t ldx, int64_t N, const void* weight, int64_t ldw,
                                   int64_t V, int64_t D, const int64_t* target, int64_t ignore, float scale,
-                                  const float* lse2, const float* upstream, int per_row, const float* count, void* dx,
-                                  void* dw, void* workspace, size_t workspace_bytes, void* cuda_stream) {
+                                  const float* lse2, const float* pull, const float* upstream, int per_row,
+                                  const float* count, void* dx, void* dw, void* workspace, size_t workspace_bytes,
+                                  int* d_err, void* cuda_stream) {
   if (!loss_sizes_ok(N, V, D, ldx, ldw) || !(scale - scale == 0.f)) return GSB_ERR_INVALID;
   if (dtype != GSB_F32 && dtype != GSB_F16 && dtype != GSB_BF16) return GSB_ERR_INVALID;
   cudaStream_t st = (cudaStream_t)cuda_stream;
@@ -461,7 +481,8 @@ extern "C" int gsb_linear_ce_grad(const void* x, int dtype, int64_t ldx, int64_t
   }
   if (!dx && !dw) return GSB_OK;
   if (!x || !weight || !target || !lse2 || !upstream) return GSB_ERR_INVALID;
-  if (!workspace || workspace_bytes < gsb_linear_ce_grad_workspace_bytes(N, V, D, dx != nullptr, dw != nullptr))
+  if (!workspace || workspace_bytes < gsb_linear_ce_grad_workspace_bytes(dtype, weight, ldw, N, V, D, pull != nullptr,
+                                                                         dx != nullptr, dw != nullptr))
     return GSB_ERR_WORKSPACE;
   char* ws = (char*)workspace;
   float* g = (float*)ws;
@@ -476,10 +497,25 @@ extern "C" int gsb_linear_ce_grad(const void* x, int dtype, int64_t ldx, int64_t
   LossArgs a = {};
   a.x = x; a.ldx = ldx; a.N = N; a.w = weight; a.ldw = ldw; a.V = V; a.D = D;
   a.target = (const i64*)target; a.ignore = ignore; a.scale = scale; a.lse2 = const_cast<float*>(lse2);
-  a.g = g; a.top = top; a.dx = dx; a.dw = dw; a.ws = ws + up256(4 * (size_t)N) + 256; a.st = st;
-  if (dtype == GSB_F32) simt_backward<float>(a);
-  else if (dtype == GSB_F16) simt_backward<__half>(a);
-  else simt_backward<__nv_bfloat16>(a);
+  a.g = g; a.top = top; a.dx = dx; a.dw = dw; a.ws = ws + up256(4 * (size_t)N) + 256; a.err = d_err; a.st = st;
+  if (tc_loss_takes(dtype, N, V, D)) {
+    const bool half = dtype == GSB_F16;
+    if (a.dx && pull) {
+      if (half) tc_loss_dx<__half>(a, pull);
+      else tc_loss_dx<__nv_bfloat16>(a, pull);
+      a.dx = nullptr;
+    }
+    if (a.dw) {
+      const int rc = half ? tc_loss_grad_w<__half>(a) : tc_loss_grad_w<__nv_bfloat16>(a);
+      if (rc != GSB_OK) return rc;
+      a.dw = nullptr;
+    }
+  }
+  if (a.dx || a.dw) {
+    if (dtype == GSB_F32) simt_backward<float>(a);
+    else if (dtype == GSB_F16) simt_backward<__half>(a);
+    else simt_backward<__nv_bfloat16>(a);
+  }
   GSB_CUDA_OK(cudaGetLastError());
   return GSB_OK;
 }

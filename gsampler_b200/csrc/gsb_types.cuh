@@ -18,6 +18,9 @@ __device__ __forceinline__ __half from_float<__half>(float x) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+template <typename T> struct IsBf16 { static constexpr bool value = false; };
+template <> struct IsBf16<__nv_bfloat16> { static constexpr bool value = true; };
+
 template <int BYTES> struct Raw;
 template <> struct Raw<2> { typedef unsigned short type; };
 template <> struct Raw<4> { typedef unsigned int type; };

@@ -163,8 +163,9 @@ static int CheckLoss(const torch::Tensor& x, const torch::Tensor& weight, const 
   return dt;
 }
 
-std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropy(torch::Tensor x, torch::Tensor weight, torch::Tensor target,
-                                                            double scale, int64_t ignore) {
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> LinearCrossEntropy(torch::Tensor x, torch::Tensor weight,
+                                                                           torch::Tensor target, double scale,
+                                                                           int64_t ignore, bool want_dx) {
   const int dt = CheckLoss(x, weight, target, scale);
   c10::cuda::CUDAGuard guard(x.device());
   x = Rows(x);
@@ -173,13 +174,15 @@ std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropy(torch::Tensor x, tor
   const int64_t N = x.size(0), V = weight.size(0), D = x.size(1);
   auto f32 = x.options().dtype(torch::kFloat32);
   auto loss = torch::empty({N}, f32), lse2 = torch::empty({N}, f32);
-  auto ws = NewWorkspace(gsb_linear_ce_workspace_bytes(N, V, D), x.device());
+  const bool want_pull = want_dx && gsb_linear_ce_has_pull(dt, N, V, D);
+  auto pull = torch::empty(want_pull ? std::vector<int64_t>{N, D} : std::vector<int64_t>{0}, f32);
+  auto ws = NewWorkspace(gsb_linear_ce_workspace_bytes(dt, weight.data_ptr(), RowStep(weight), N, V, D, want_pull), x.device());
   CheckStatus(gsb_linear_ce(x.data_ptr(), dt, RowStep(x), N, weight.data_ptr(), RowStep(weight), V, D,
                             target.data_ptr<int64_t>(), ignore, (float)scale, loss.data_ptr<float>(),
-                            lse2.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), ErrorWord(x.device()),
-                            CurrentStream()),
+                            lse2.data_ptr<float>(), want_pull ? pull.data_ptr<float>() : nullptr, ws.data_ptr(),
+                            (size_t)ws.numel(), ErrorWord(x.device()), CurrentStream()),
               "linear_ce");
-  return {loss, lse2};
+  return {loss, lse2, pull};
 }
 
 std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyTotal(torch::Tensor loss, torch::Tensor target,
@@ -199,7 +202,7 @@ std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyTotal(torch::Tensor l
 
 std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyGrad(torch::Tensor x, torch::Tensor weight,
                                                                 torch::Tensor target, torch::Tensor lse2,
-                                                                torch::Tensor upstream,
+                                                                torch::Tensor pull, torch::Tensor upstream,
                                                                 c10::optional<torch::Tensor> count, double scale,
                                                                 int64_t ignore, bool want_dx, bool want_dw) {
   const int dt = CheckLoss(x, weight, target, scale);
@@ -209,6 +212,8 @@ std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyGrad(torch::Tensor x,
   };
   const bool per_row = upstream.dim() == 1;
   TORCH_CHECK(good(lse2, N) && lse2.is_contiguous(), "LinearCrossEntropyGrad: lse2 must be float32 [N]");
+  const bool have_pull = pull.numel() > 0;
+  TORCH_CHECK(!have_pull || (good(pull, N * D) && pull.is_contiguous()), "LinearCrossEntropyGrad: pull must be float32 [N, D]");
   TORCH_CHECK(good(upstream, per_row ? N : 1), "LinearCrossEntropyGrad: upstream must be float32, one value or [N]");
   TORCH_CHECK(!count.has_value() || good(*count, 1), "LinearCrossEntropyGrad: count must be one float32 value");
   c10::cuda::CUDAGuard guard(x.device());
@@ -218,12 +223,14 @@ std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyGrad(torch::Tensor x,
   upstream = upstream.contiguous();
   auto dx = want_dx ? torch::empty({N, D}, x.options()) : torch::empty({0}, x.options());
   auto dw = want_dw ? torch::empty({V, D}, x.options()) : torch::empty({0}, x.options());
-  auto ws = NewWorkspace(gsb_linear_ce_grad_workspace_bytes(N, V, D, want_dx, want_dw), x.device());
+  auto ws = NewWorkspace(gsb_linear_ce_grad_workspace_bytes(dt, weight.data_ptr(), RowStep(weight), N, V, D, have_pull, want_dx,
+                                                            want_dw),
+                         x.device());
   CheckStatus(gsb_linear_ce_grad(x.data_ptr(), dt, RowStep(x), N, weight.data_ptr(), RowStep(weight), V, D,
                                  target.data_ptr<int64_t>(), ignore, (float)scale, lse2.data_ptr<float>(),
-                                 upstream.data_ptr<float>(), per_row, count.has_value() ? count->data_ptr<float>() : nullptr,
+                                 have_pull ? pull.data_ptr<float>() : nullptr, upstream.data_ptr<float>(), per_row, count.has_value() ? count->data_ptr<float>() : nullptr,
                                  want_dx ? dx.data_ptr() : nullptr, want_dw ? dw.data_ptr() : nullptr, ws.data_ptr(),
-                                 (size_t)ws.numel(), CurrentStream()),
+                                 (size_t)ws.numel(), ErrorWord(x.device()), CurrentStream()),
               "linear_ce_grad");
   return {dx, dw};
 }

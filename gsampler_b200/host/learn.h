@@ -19,16 +19,18 @@ torch::Tensor Dropout(torch::Tensor data, double p, int64_t seed, int64_t stream
 void SetDropoutSeed(int64_t seed);
 std::tuple<int64_t, int64_t> NextDropoutStream();
 
-// softmax cross entropy over a vocabulary: (loss of every row, log-sum-exp of every row in base 2)
-std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropy(torch::Tensor x, torch::Tensor weight, torch::Tensor target,
-                                                            double scale, int64_t ignore);
+// softmax cross entropy over a vocabulary: (loss of every row, log-sum-exp of every row in base 2, and
+// -- empty unless asked for and available -- what the gradient of x is made from)
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> LinearCrossEntropy(torch::Tensor x, torch::Tensor weight,
+                                                                           torch::Tensor target, double scale,
+                                                                           int64_t ignore, bool want_dx);
 // (sum or mean of the rows' losses, number of rows that count)
 std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyTotal(torch::Tensor loss, torch::Tensor target,
                                                                  int64_t vocabulary, int64_t ignore, bool mean);
 // (dx, dw); one that is not asked for comes back empty
 std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyGrad(torch::Tensor x, torch::Tensor weight,
                                                                 torch::Tensor target, torch::Tensor lse2,
-                                                                torch::Tensor upstream,
+                                                                torch::Tensor pull, torch::Tensor upstream,
                                                                 c10::optional<torch::Tensor> count, double scale,
                                                                 int64_t ignore, bool want_dx, bool want_dw);
 

@@ -8,21 +8,22 @@ __all__ = ["linear_cross_entropy"]
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, scale, ignore_index, reduction):
-        loss, lse2 = torch.ops.gs_ops._CAPI_LinearCrossEntropy(x, weight, target, scale, ignore_index)
+        loss, lse2, pull = torch.ops.gs_ops._CAPI_LinearCrossEntropy(x, weight, target, scale, ignore_index,
+                                                                     ctx.needs_input_grad[0])
         count = None
         if reduction != "none":
             loss, count = torch.ops.gs_ops._CAPI_LinearCrossEntropyTotal(loss, target, weight.shape[0], ignore_index,
                                                                          reduction == "mean")
-        ctx.save_for_backward(x, weight, target, lse2, count if reduction == "mean" else None)
+        ctx.save_for_backward(x, weight, target, lse2, pull, count if reduction == "mean" else None)
         ctx.scale, ctx.ignore_index = scale, ignore_index
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x, weight, target, lse2, count = ctx.saved_tensors
+        x, weight, target, lse2, pull, count = ctx.saved_tensors
         want_dx, want_dw = ctx.needs_input_grad[:2]
-        dx, dw = torch.ops.gs_ops._CAPI_LinearCrossEntropyGrad(x, weight, target, lse2, grad, count, ctx.scale,
+        dx, dw = torch.ops.gs_ops._CAPI_LinearCrossEntropyGrad(x, weight, target, lse2, pull, grad, count, ctx.scale,
                                                                ctx.ignore_index, want_dx, want_dw)
         return dx if want_dx else None, dw if want_dw else None, None, None, None, None
 

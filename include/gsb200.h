@@ -271,24 +271,32 @@ GSB_API int gsb_dropout(const void* x, int dtype, int64_t n, double p, uint64_t 
  * count (its loss and gradients are 0, whatever x holds there); another target
  * sets GSB_ERRBIT_BAD_INPUT and does not count either.
  *   loss[i] = lse_i - scale x_i . w_target       lse2[i] = lse_i / ln 2
+ * pull (optional, fp32 [N, D]; only where gsb_linear_ce_has_pull says 1) receives
+ * sum_j p_ij w_j - w_target of every row, from which gsb_linear_ce_grad makes dx
+ * without going over the vocabulary again.
  * gsb_linear_ce_total: *total = sum (mean: divided by the number of rows that
  * count, 0 when there are none) of the rows' losses, *count = max(that number, 1).
  * gsb_linear_ce_grad: dx[N, D] and / or dw[V, D] (either may be NULL) from the
  * upstream gradient: upstream[N] when per_row, else one value, divided by *count
  * when count is given.  Sums are made in an order that depends on the sizes
- * alone.  N, V < 2^31. */
+ * alone.  N, V < 2^31.  A workspace is sized for the device that is current. */
 #define GSB_LOSS_MAX_D 65536
-GSB_API size_t gsb_linear_ce_workspace_bytes(int64_t N, int64_t V, int64_t D);
+GSB_API int gsb_linear_ce_has_pull(int dtype, int64_t N, int64_t V, int64_t D);
+GSB_API size_t gsb_linear_ce_workspace_bytes(int dtype, const void* weight, int64_t ldw, int64_t N, int64_t V,
+                                             int64_t D, int want_pull);
 GSB_API int gsb_linear_ce(const void* x, int dtype, int64_t ldx, int64_t N, const void* weight, int64_t ldw,
                           int64_t V, int64_t D, const int64_t* target, int64_t ignore, float scale, float* loss,
-                          float* lse2, void* workspace, size_t workspace_bytes, int* d_err, void* cuda_stream);
+                          float* lse2, float* pull, void* workspace, size_t workspace_bytes, int* d_err,
+                          void* cuda_stream);
 GSB_API int gsb_linear_ce_total(const float* loss, const int64_t* target, int64_t ignore, int64_t V, int64_t N,
                                 int mean, float* total, float* count, void* cuda_stream);
-GSB_API size_t gsb_linear_ce_grad_workspace_bytes(int64_t N, int64_t V, int64_t D, int want_dx, int want_dw);
+GSB_API size_t gsb_linear_ce_grad_workspace_bytes(int dtype, const void* weight, int64_t ldw, int64_t N, int64_t V,
+                                                  int64_t D, int have_pull, int want_dx, int want_dw);
 GSB_API int gsb_linear_ce_grad(const void* x, int dtype, int64_t ldx, int64_t N, const void* weight, int64_t ldw,
                                int64_t V, int64_t D, const int64_t* target, int64_t ignore, float scale,
-                               const float* lse2, const float* upstream, int per_row, const float* count, void* dx,
-                               void* dw, void* workspace, size_t workspace_bytes, void* cuda_stream);
+                               const float* lse2, const float* pull, const float* upstream, int per_row,
+                               const float* count, void* dx, void* dw, void* workspace, size_t workspace_bytes,
+                               int* d_err, void* cuda_stream);
 
 /* ------------------------------------------------------------------ format conversion
  * CSC -> COO column expansion: out[e] = column owning edge e.  Replaces

@@ -23,16 +23,17 @@ def test_c_entry_points_check_their_arguments():
     for p in (-0.1, 1.1, float("nan")):
         assert L.gsb_dropout(nul, 0, abi.i64(0), C.c_double(p), C.c_uint64(1), C.c_uint32(1), nul, nul, nul) == invalid
     lce = lambda x, dt, N, V, D: L.gsb_linear_ce(x, dt, abi.i64(D), abi.i64(N), x, abi.i64(D), abi.i64(V), abi.i64(D), nul,
-                                                 abi.i64(-1), f, nul, nul, nul, C.c_size_t(0), nul, nul)
+                                                 abi.i64(-1), f, nul, nul, nul, nul, C.c_size_t(0), nul, nul)
     assert lce(nul, 0, 0, 5, 4) == ok
     assert lce(nul, 0, 3, 5, 4) == invalid and lce(nul, 9, 0, 5, 4) == invalid
     assert lce(nul, 0, 0, 0, 4) == invalid and lce(nul, 0, 0, 5, 0) == invalid
-    assert L.gsb_linear_ce_workspace_bytes(abi.i64(1 << 31), abi.i64(5), abi.i64(4)) == 0
+    assert L.gsb_linear_ce_workspace_bytes(0, nul, abi.i64(4), abi.i64(1 << 31), abi.i64(5), abi.i64(4), 0) == 0
     for n in (0, 1):
-        L.gsb_linear_ce_workspace_bytes(abi.i64(n), abi.i64(5), abi.i64(4))
-        L.gsb_linear_ce_grad_workspace_bytes(abi.i64(n), abi.i64(5), abi.i64(4), 1, 1)
+        for dt in (0, 1, 2):
+            L.gsb_linear_ce_workspace_bytes(dt, nul, abi.i64(4), abi.i64(n), abi.i64(5), abi.i64(4), 1)
+            L.gsb_linear_ce_grad_workspace_bytes(dt, nul, abi.i64(4), abi.i64(n), abi.i64(5), abi.i64(4), 1, 1, 1)
         L.gsb_embedding_grad_workspace_bytes(abi.i64(n), abi.i64(0), abi.i64(0))
-    assert L.gsb_linear_ce_workspace_bytes(abi.i64(100), abi.i64(5), abi.i64(4)) > 0
+    assert L.gsb_linear_ce_workspace_bytes(0, nul, abi.i64(4), abi.i64(100), abi.i64(5), abi.i64(4), 0) > 0
 
 
 def test_there_is_no_cpu_path():
