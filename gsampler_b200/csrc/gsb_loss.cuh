@@ -5,6 +5,34 @@
 namespace gsb {
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int FWD_SHIFT = 7;    // the forward pass holds p at 2^7 times its value relative to the row's reference
+constexpr int GRAD_SHIFT = 14;  // the backward pass holds g (p - target) at 2^14 / max |g| times its value
+constexpr float MOVE_REFERENCE = 8.f;  // a row's reference moves when its maximum passes it by 2^8
+
+// Factor from x . w to a base-2 logit, |scale| log2 e (the sign goes into x).  Not zero, so that a
+// masked logit of -inf stays one; times any finite product 1e-38 is as good as zero.
+inline float logit_factor(float scale) { return fmaxf(fabsf(scale) * LOG2E, 1e-38f); }
+
+inline size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+inline int blocks_for(i64 threads) {
+  const i64 b = (threads + 255) / 256, most = (i64)sm_count() * 16;
+  return (int)(b < 1 ? 1 : b < most ? b : most);
+}
+
+// Tiles B a CTA runs over.  `groups` CTAs cover the rows A; the tiles are split until the CTAs fill
+// the SMs' `slots` evenly: the time is (rounds of CTAs) x (tiles of one + about 3 for its start and end).
+inline int split_count(i64 groups, i64 tiles, i64 slots) {
+  int best = 1;
+  double best_t = 1e300;
+  for (i64 s = 1; s <= tiles && s <= 2 * slots && (s == 1 || groups * s <= 3 * slots); ++s) {
+    const i64 per = (tiles + s - 1) / s;
+    if ((tiles + per - 1) / per != s) continue;  // the same as fewer splits
+    const double t = (double)((groups * s + slots - 1) / slots) * (double)(per + 3);
+    if (t < best_t * 0.999) { best_t = t; best = (int)s; }
+  }
+  return best;
+}
+
 
 struct LossArgs {
   const void* x;
@@ -35,6 +63,17 @@ bool tc_loss_takes(int dtype, i64 N, i64 V, i64 D);
 bool tc_loss_packs(const void* w, i64 ldw);  // whether the rows of W have to be copied for it
 size_t tc_loss_workspace(i64 N, i64 V, i64 D, bool pull, bool pack_w);
 size_t tc_loss_grad_workspace(i64 N, i64 V, i64 D, bool pack_w);
+// The general form (gsb_loss_gemm.cu).
+size_t gemm_loss_workspace(int dtype, i64 N, i64 V, i64 D, bool pack_w);
+size_t gemm_loss_grad_workspace(int dtype, i64 N, i64 V, i64 D, bool dx, bool dw, bool pack_w);
+template <typename T>
+int gemm_loss_forward(const LossArgs& a);
+template <typename T>
+int gemm_loss_backward(const LossArgs& a);
+// losses (and pulls) of all rows from the parts of their statistics (gsb_loss_tc.cu)
+template <typename T>
+void launch_loss_join(const LossArgs& a, const float2* part_ms, int parts, const float* part_o, float* pull);
+
 template <typename T>
 int tc_loss_forward(const LossArgs& a, float* pull);
 template <typename T>

@@ -1,10 +1,13 @@
 // The vocabulary cross entropy of 16-bit types on the tensor cores (tcgen05, TMA, TMEM).
 //
-// Both passes are one shape of computation: a tile of 128 rows A stays in shared memory, tiles B of
-// the other matrix stream past it, and for each
+// Both passes are one shape of computation: a tile of 128 rows A stays in TMEM, tiles B of the other
+// matrix stream past it, and for each
 //     S = A B^T   ->   P = f(S)   ->   O += P B
 // where one copy of the B tile in shared memory serves both products (read along its rows for S,
-// across them for O).  S, P (16-bit, in the place of S) and O live in TMEM.
+// across them for O).  S, P (16-bit, in the place of S) and O live in TMEM too.  A there, and not in
+// shared memory, halves what a product reads from shared memory: S alone ran at 984 TFLOP/s with
+// both operands in shared memory (128 x 128 tiles, 8192 x 300000 x 128), the second product, whose
+// first operand was in TMEM already, at 2000.
 //   forward   A = rows of x, B = the vocabulary.  P = exp2(l - m) against a running reference m;
 //             O / sum P is the expected row of W, which is all that dx needs; log2 sum P + m is
 //             the log-sum-exp.  Without a gradient for x there is no second product.
@@ -15,175 +18,50 @@
 // The reference m moves only when a row's maximum passes it by 2^8, because moving it rescales O;
 // P stays below 2^15, which fp16 holds.  Sums and O are 32 bits; P is rounded to the type, half a
 // step each, which is the rounding that the tensor cores' operands ask for.
-#include <cuda.h>
-
 #include "gsb_common.cuh"
 #include "gsb_loss.cuh"
+#include "gsb_tc.cuh"
 #include "gsb_types.cuh"
 
 namespace gsb {
 
 enum { TC_STATS = 0, TC_PULL = 1, TC_GRAD_W = 2 };
 
-constexpr int FWD_SHIFT = 7;    // P is held at 2^7 times its value relative to the reference
-constexpr int GRAD_SHIFT = 14;  // g (p - target) is held at 2^14 / max |g| times its value
-constexpr float MOVE_REFERENCE = 8.f;
-
-// ---------------------------------------------------------------- instructions
-__device__ __forceinline__ u32 smem_addr(const void* p) { return (u32)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void bar_init(u32 bar, u32 count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_expect(u32 bar, u32 bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(u32 bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool bar_try(u32 bar, u32 parity) {
-  u32 ok;
-  asm volatile(
-      "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.b32 %0, 1, 0, p;\n}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Every wait ends: after two seconds, or once another warp of the CTA gave up, it reports and the
-// kernel runs out without touching anything more.
-__device__ __noinline__ bool bar_wait_slow(u32 bar, u32 parity, volatile int* gave_up, int* err) {
-  u64 t0;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
-  for (;;) {
-    for (int k = 0; k < 64; ++k)
-      if (bar_try(bar, parity)) return true;
-    u64 now;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
-    if (*gave_up) return false;
-    if (now - t0 > 2000000000ull) {
-      *gave_up = 1;
-      raise(err, ERRBIT_LOOKBACK_TIMEOUT);
-      return false;
-    }
-  }
-}
-__device__ __forceinline__ bool bar_wait(u32 bar, u32 parity, volatile int* gave_up, int* err) {
-  if (bar_try(bar, parity)) return true;
-  return bar_wait_slow(bar, parity, gave_up, err);
-}
-
-__device__ __forceinline__ void tma_tile(u32 dst, const CUtensorMap* map, int x, int y, u32 bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-               "l"(map), "r"(x), "r"(y), "r"(bar)
-               : "memory");
-}
-__device__ __forceinline__ void bulk_copy(u32 dst, const void* src, u32 bytes, u32 bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-               "r"(bytes), "r"(bar)
-               : "memory");
-}
-__device__ __forceinline__ void tc_commit(u32 bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_mma(u32 d, u64 a, u64 b, u32 idesc, bool add) {
-  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
-               "l"(b), "r"(idesc), "r"((u32)add)
-               : "memory");
-}
-__device__ __forceinline__ void tc_mma_ta(u32 d, u32 a, u64 b, u32 idesc, bool add) {
-  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a),
-               "l"(b), "r"(idesc), "r"((u32)add)
-               : "memory");
-}
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-#define GSB_R4(a, i) "=f"(a[i]), "=f"(a[i + 1]), "=f"(a[i + 2]), "=f"(a[i + 3])
-#define GSB_R16(a, i) GSB_R4(a, i), GSB_R4(a, i + 4), GSB_R4(a, i + 8), GSB_R4(a, i + 12)
-__device__ __forceinline__ void tc_ld32(float* v, u32 addr) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
-      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : GSB_R16(v, 0), GSB_R16(v, 16)
-      : "r"(addr));
-}
-#define GSB_U4(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3])
-#define GSB_U16(a, i) GSB_U4(a, i), GSB_U4(a, i + 4), GSB_U4(a, i + 8), GSB_U4(a, i + 12)
-__device__ __forceinline__ void tc_st16(u32 addr, const u32* v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
-      GSB_U16(v, 0)
-      : "memory");
-}
-__device__ __forceinline__ void tc_st32(u32 addr, const u32* v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
-      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
-      GSB_U16(v, 0), GSB_U16(v, 16)
-      : "memory");
-}
-
-// Shared-memory matrix descriptor, 128-byte swizzle.  Along rows (K-major): 8-row groups 1024 bytes
-// apart.  Across rows (MN-major): 64-element pieces `lead` bytes apart, 8-row groups 1024 bytes apart.
-__device__ __forceinline__ u64 tc_desc(u32 addr, u32 lead) {
-  return (u64)((addr & 0x3FFFF) >> 4) | ((u64)(lead >> 4) << 16) | ((u64)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-// Instruction descriptor of kind::f16 with a 32-bit accumulator and M = 128.
-__device__ __forceinline__ u32 tc_idesc(bool bf16, u32 n, bool b_across) {
-  const u32 t = bf16 ? 1 : 0;
-  return (1u << 4) | (t << 7) | (t << 10) | ((b_across ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ u32 pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ u32 pack2<__half>(float lo, float hi) {
-  u32 r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-template <>
-__device__ __forceinline__ u32 pack2<__nv_bfloat16>(float lo, float hi) {
-  u32 r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
 // ---------------------------------------------------------------- shapes of the kernel
 // DP    columns a row may have (64, 128, 256)
-// NA    tiles A a CTA works on at once, WG  warpgroups that turn S into P
+// NA    tiles A a CTA works on at once
 // NB    S buffers, BT  rows of a tile B, ST  stages of the B pipeline, CTAS  CTAs an SM
-// An item is (tile B j, tile A a), numbered w = j NA + a; it uses buffer w % NB and warpgroup w % WG.
-template <int MODE_, int DP_, int NA_, int WG_, int NB_, int BT_, int ST_, int CTAS_>
+// An item is (tile B j, tile A a), numbered w = j NA + a; it uses buffer w % NB.  Two warpgroups turn
+// an item's S into P, half of its columns each: a warp alone issues an instruction every three
+// cycles or so, which made the tensor cores wait (41 % busy with one warpgroup an item, 8192 x 60000 x 128).
+constexpr int HALVES = 2;
+
+template <int MODE_, int DP_, int NA_, int NB_, int BT_, int ST_, int CTAS_>
 struct TcShape {
-  static constexpr int MODE = MODE_, DP = DP_, NA = NA_, WG = WG_, NB = NB_, BT = BT_, ST = ST_, CTAS = CTAS_;
+  static constexpr int MODE = MODE_, DP = DP_, NA = NA_, NB = NB_, BT = BT_, ST = ST_, CTAS = CTAS_;
   static constexpr bool SECOND = MODE != TC_STATS;  // the product with P
+  static constexpr int WG = NA * HALVES, HC = BT / HALVES;
   static constexpr int SUBS = DP / 64;
-  static constexpr int A_BYTES = SUBS * 128 * 128, B_BYTES = SUBS * BT * 128;
+  static constexpr int B_BYTES = SUBS * BT * 128;
   static constexpr int META = MODE == TC_GRAD_W ? BT * 14 : 0;
-  static constexpr int O_COL = NB * BT;
+  static constexpr int A_COL = NB * BT, O_COL = A_COL + NA * (DP / 2);
   static constexpr int USED = O_COL + (SECOND ? NA * DP : 0);
   static constexpr int COLS = USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
   static constexpr int THREADS = WG * 128 + 64;
-  static constexpr int OFF_B = NA * A_BYTES, OFF_META = OFF_B + ST * B_BYTES;
-  static constexpr int OFF_BAR = (OFF_META + ST * META + 15) / 16 * 16;
-  static constexpr int BARS = 2 * ST + 2 * NB + 3;
+  static constexpr int OFF_B = 0, OFF_META = ST * B_BYTES;
+  static constexpr int OFF_TOP = OFF_META + ST * META;                                     // row maxima of the halves
+  static constexpr int OFF_BAR = OFF_TOP + (MODE == TC_PULL ? 2 * WG * 128 * 4 : 0);
+  static constexpr bool TURNS = SECOND && NA == 2;
+  static constexpr int BARS = 2 * ST + 2 * NB + 3 + 8 + (MODE == TC_PULL ? 4 * NA : 0);
   static constexpr int BYTES = OFF_BAR + 8 * BARS + 16 + 1024;  // and room to align the base
   static_assert(USED <= 512 && COLS * CTAS <= 512, "TMEM");
   static_assert(BYTES * CTAS <= 227 * 1024, "shared memory");
-  static_assert(WG % NA == 0 || NA % WG == 0, "a tile A keeps its warpgroup");
-  static_assert(MODE != TC_PULL || WG == NA, "a row's running state has one owner");
+  static_assert(HC % 32 == 0 && META % 16 == 0 && OFF_TOP % 16 == 0 && OFF_BAR % 8 == 0, "");
 };
 
 struct TcParams {
+  const void* a;            // rows of lda elements, 16-byte aligned
+  i64 lda;
   int rows_a, rows_b, D;
   int tiles_per_split;      // tiles B a CTA runs over
   float c;                  // |scale| log2 e
@@ -198,7 +76,7 @@ struct TcParams {
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(C::THREADS, C::CTAS)
-loss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const TcParams p) {
+loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
   extern __shared__ unsigned char smem_raw[];
   const u32 base = (smem_addr(smem_raw) + 1023) & ~1023u;
   unsigned char* smem = smem_raw + (base - smem_addr(smem_raw));
@@ -208,6 +86,9 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   auto s_full = [&](int b) { return bar0 + 8 * (2 * C::ST + b); };
   auto p_full = [&](int b) { return bar0 + 8 * (2 * C::ST + C::NB + b); };
   const u32 a_full = bar0 + 8 * (2 * C::ST + 2 * C::NB), o_full = a_full + 8, pv_done = a_full + 16;
+  // whose turn the exponentials of a scheduler's four warps are: tile a is through with its tile j
+  auto turn = [&](int a, int quarter) { return a_full + 24 + 8 * (4 * a + quarter); };
+  auto pair = [&](int a, int quarter) { return a_full + 24 + 64 + 8 * (4 * a + quarter); };  // the two warps that share 32 rows
   u32* tmem_slot = reinterpret_cast<u32*>(smem + C::OFF_BAR + 8 * C::BARS);
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -221,10 +102,16 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 
   if (warp == C::WG * 4 && lane == 0) {
     for (int s = 0; s < C::ST; ++s) { bar_init(full(s), 1); bar_init(empty(s), 1); }
-    for (int b = 0; b < C::NB; ++b) { bar_init(s_full(b), 1); bar_init(p_full(b), 4); }
-    bar_init(a_full, 1);
+    for (int b = 0; b < C::NB; ++b) { bar_init(s_full(b), 1); bar_init(p_full(b), 4 * HALVES); }
+    bar_init(a_full, 4 * C::WG);
     bar_init(o_full, 1);
     bar_init(pv_done, 1);
+    if (C::TURNS)
+      for (int a = 0; a < 2; ++a)
+        for (int q = 0; q < 4; ++q) bar_init(turn(a, q), HALVES);
+    if (C::MODE == TC_PULL)
+      for (int a = 0; a < C::NA; ++a)
+        for (int q = 0; q < 4; ++q) bar_init(pair(a, q), 2);
     *gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -237,45 +124,50 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   tc_before();
   __syncthreads();
   tc_after();
-  const u32 tmem = *tmem_slot;
+  const u32 tmem = __reduce_max_sync(0xffffffffu, *tmem_slot);  // the same in every lane, and known to be
 
   if (warp == C::WG * 4) {
     // ------------------------------------------------ loads
     if (lane == 0 && my_tiles > 0) {
-      bar_expect(a_full, (u32)(C::NA * subs * 16384));
-      for (int a = 0; a < C::NA; ++a)
-        for (int s = 0; s < subs; ++s) tma_tile(base + a * C::A_BYTES + s * 16384, &map_a, s * 64, row0 + a * 128, a_full);
       int issued = 0;
       for (int j = 0; j < my_tiles; ++j) {
         const int st = j % C::ST;
         if (j >= C::ST && !bar_wait(empty(st), ((j / C::ST) - 1) & 1, gave_up, p.err)) break;
         bar_expect(full(st), (u32)(subs * C::BT * 128 + C::META));
         for (int s = 0; s < subs; ++s)
-          tma_tile(base + C::OFF_B + st * C::B_BYTES + s * (C::BT * 128), &map_b, s * 64, (t0 + j) * C::BT, full(st));
+          tma_tile(base + C::OFF_B + st * C::B_BYTES + s * (C::BT * 128), &map_b, s * 64, (t0 + j) * C::BT, 0, full(st));
         if (C::META) bulk_copy(base + C::OFF_META + st * C::META, p.meta + (i64)(t0 + j) * C::META, C::META, full(st));
         ++issued;
       }
       // no copy may be in flight when the CTA ends (only after a wait that gave up can one be)
-      bar_wait(a_full, 0, gave_up, p.err);
       for (int j = issued > C::ST ? issued - C::ST : 0; j < issued; ++j)
         for (int k = 0; k < (1 << 16) && !bar_try(full(j % C::ST), (j / C::ST) & 1); ++k) __nanosleep(32);
     }
   } else if (warp == C::WG * 4 + 1) {
     // ------------------------------------------------ products
-    if (lane == 0 && my_tiles > 0) {
+    // The whole warp walks the items and one lane issues: unrolled, with descriptors that differ by
+    // constants.  A product of 128 x 128 x 16 takes 64 cycles; issued from a divergent lane with its
+    // descriptors made one by one it took 130.
+    if (my_tiles > 0) {
       const bool bf = IsBf16<T>::value;
-      const u32 id_s = tc_idesc(bf, C::BT, false), id_o = tc_idesc(bf, (u32)ksteps * 16, true);
+      const u32 id_s = tc_idesc(bf, C::BT, false, false), id_o = tc_idesc(bf, (u32)ksteps * 16, false, true);
+      const bool leader = elect_one();
       bool ok = bar_wait(a_full, 0, gave_up, p.err);
+      tc_after();
       auto product_s = [&](int w) {
         const int j = w / C::NA, a = w % C::NA, st = j % C::ST;
-        if (a == 0 || C::NA == 1) ok = ok && bar_wait(full(st), (j / C::ST) & 1, gave_up, p.err);
+        if (a == 0) ok = ok && bar_wait(full(st), (j / C::ST) & 1, gave_up, p.err);
         if (!ok) return;
         tc_after();
-        const u32 A = base + a * C::A_BYTES, B = base + C::OFF_B + st * C::B_BYTES, d = tmem + (w % C::NB) * C::BT;
-        for (int k = 0; k < ksteps; ++k)
-          tc_mma(d, tc_desc(A + (k >> 2) * 16384 + (k & 3) * 32, 16), tc_desc(B + (k >> 2) * (C::BT * 128) + (k & 3) * 32, 16), id_s, k > 0);
-        tc_commit(s_full(w % C::NB));
-        if (!C::SECOND && a == C::NA - 1) tc_commit(empty(st));
+        const u32 A = tmem + C::A_COL + a * (C::DP / 2), d = tmem + (w % C::NB) * C::BT;
+        const u64 B = tc_desc(base + C::OFF_B + st * C::B_BYTES, 16);
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < C::DP / 16; ++k)
+            if (k < ksteps) tc_mma_ta(d, A + k * 8, B + ((k >> 2) * (C::BT * 128) + (k & 3) * 32) / 16, id_s, k > 0);
+          tc_commit(s_full(w % C::NB));
+          if (!C::SECOND && a == C::NA - 1) tc_commit(empty(st));
+        }
       };
       for (int w = 0; w < C::NB && w < items; ++w) product_s(w);
       for (int w = 0; w < items && ok; ++w) {
@@ -284,27 +176,62 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         if (!ok) break;
         if (C::SECOND) {
           tc_after();
-          const u32 B = base + C::OFF_B + st * C::B_BYTES, P = tmem + b * C::BT, d = tmem + C::O_COL + a * C::DP;
-          for (int k = 0; k < C::BT / 16; ++k) tc_mma_ta(d, P + k * 8, tc_desc(B + k * 2048, C::BT * 128), id_o, j > 0 || k > 0);
-          if (a == C::NA - 1) tc_commit(empty(st));
-          if (C::MODE == TC_PULL && C::NA == 1 && C::NB > 1) tc_commit(pv_done);
+          const u32 P = tmem + b * C::BT, d = tmem + C::O_COL + a * C::DP;
+          const u64 B = tc_desc(base + C::OFF_B + st * C::B_BYTES, C::BT * 128);
+          if (leader) {
+#pragma unroll
+            for (int k = 0; k < C::BT / 16; ++k)
+              tc_mma_ta(d, P + (k / (C::HC / 16)) * C::HC + (k % (C::HC / 16)) * 8, B + k * (2048 / 16), id_o, j > 0 || k > 0);
+            if (a == C::NA - 1) tc_commit(empty(st));
+            if (C::MODE == TC_PULL && C::NA == 1 && C::NB > 1) tc_commit(pv_done);
+          }
         }
         if (w + C::NB < items) product_s(w + C::NB);
       }
-      tc_commit(o_full);
+      if (leader) tc_commit(o_full);
       // the products that were issued end by themselves; a bounded look keeps the order when a wait gave up
       for (int k = 0; k < (1 << 16) && !bar_try(o_full, 0); ++k) __nanosleep(32);
     }
   } else {
     // ------------------------------------------------ S -> P
-    const int wg = warp >> 2, quarter = warp & 3;
+    const int wg = warp >> 2, quarter = warp & 3, a = wg / HALVES, half = wg % HALVES;
     const u32 lanes = (u32)(quarter * 32) << 16;
-    const int a_mine = C::NA == 1 ? 0 : wg;
-    const int row = row0 + a_mine * 128 + quarter * 32 + lane;
-    const bool warp_live = row0 + a_mine * 128 + quarter * 32 < p.rows_a;
+    const int row = row0 + a * 128 + quarter * 32 + lane;
+    const bool warp_live = row0 + a * 128 + quarter * 32 < p.rows_a;
+    // the rows of A into TMEM: a thread its row, pairs of elements a column; zeros behind the last
+    // column (nothing there may meet the zeros of B as a NaN) and row
+    for (int k = half * 32; k < ksteps * 16; k += 32 * HALVES) {
+      const T* from = (const T*)p.a + (i64)row * p.lda + k;
+      Pack<T, 32> piece;
+#pragma unroll
+      for (int q = 0; q < 32; q += 8) {
+        if (row < p.rows_a && k + q + 8 <= p.D) {
+          reinterpret_cast<Pack<T, 8>*>(piece.v + q)->load(from + q);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) piece.v[q + e] = row < p.rows_a && k + q + e < p.D ? from[q + e] : from_float<T>(0.f);
+        }
+      }
+      tc_st16(tmem + C::A_COL + a * (C::DP / 2) + k / 2 + lanes, reinterpret_cast<const u32*>(piece.v));
+    }
+    tc_wait_st();
+    tc_before();
+    __syncwarp();
+    if (lane == 0) bar_arrive(a_full);
     float m = -INFINITY, sum = 0.f;
+    const u64 c2 = join2(p.c, p.c);
     bool ok = true;
-    for (int w = wg; w < items; w += C::WG) {
+    // The two tiles' warps on a scheduler take the exponentials in turns.  Left alone they run into
+    // step: both wait for the special-function unit while the tensor cores idle, then both wait for
+    // the tensor cores.
+    auto my_turn = [&](int j) {
+      if (C::TURNS && (a == 1 || j > 0)) ok = ok && bar_wait(turn(a ^ 1, quarter), (a == 1 ? j : j - 1) & 1, gave_up, p.err);
+    };
+    auto next_turn = [&]() {
+      __syncwarp();
+      if (C::TURNS && lane == 0) bar_arrive(turn(a, quarter));
+    };
+    for (int w = a; w < items; w += C::NA) {
       const int j = w / C::NA, st = j % C::ST, b = w % C::NB;
       ok = bar_wait(s_full(b), (w / C::NB) & 1, gave_up, p.err);
       if (C::META) ok = ok && bar_wait(full(st), (j / C::ST) & 1, gave_up, p.err);
@@ -312,106 +239,132 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       if (!ok) break;
       tc_after();
       if (warp_live) {
-        const u32 S = tmem + b * C::BT + lanes;
-        float v[C::BT];
+        const u32 S = tmem + b * C::BT + half * C::HC + lanes;
+        float v[C::HC];
 #pragma unroll
-        for (int k = 0; k < C::BT; k += 32) tc_ld32(v + k, S + k);
+        for (int k = 0; k < C::HC; k += 32) tc_ld32(v + k, S + k);
         tc_wait_ld();
         if constexpr (C::MODE == TC_GRAD_W) {
-          const unsigned char* meta = smem + C::OFF_META + st * C::META;
-          const float4* bias = reinterpret_cast<const float4*>(meta);
+          const unsigned char* meta = smem + C::OFF_META + st * C::META + half * C::HC * 4;
+          const ulonglong2* bias = reinterpret_cast<const ulonglong2*>(meta);  // negative
 #pragma unroll
-          for (int k = 0; k < C::BT / 4; ++k) {
-            const float4 q = bias[k];
-            v[4 * k] = ex2(fmaf(v[4 * k], p.c, -q.x));
-            v[4 * k + 1] = ex2(fmaf(v[4 * k + 1], p.c, -q.y));
-            v[4 * k + 2] = ex2(fmaf(v[4 * k + 2], p.c, -q.z));
-            v[4 * k + 3] = ex2(fmaf(v[4 * k + 3], p.c, -q.w));
+          for (int k = 0; k < C::HC / 4; ++k) {
+            const ulonglong2 q = bias[k];
+            part2(fma2(join2(v[4 * k], v[4 * k + 1]), c2, q.x), v[4 * k], v[4 * k + 1]);
+            part2(fma2(join2(v[4 * k + 2], v[4 * k + 3]), c2, q.y), v[4 * k + 2], v[4 * k + 3]);
           }
+          my_turn(j);
+#pragma unroll
+          for (int k = 0; k < C::HC; ++k) v[k] = ex2(v[k]);
+          next_turn();
           const int* tgt = reinterpret_cast<const int*>(meta + 4 * C::BT);
           const float* gs = reinterpret_cast<const float*>(meta + 8 * C::BT);
           bool near = false;
 #pragma unroll
-          for (int k = 0; k < C::BT / 32; ++k) near |= (u32)(tgt[k * 32 + lane] - (row - lane)) < 32u;
+          for (int k = 0; k < C::HC / 32; ++k) near |= (u32)(tgt[k * 32 + lane] - (row - lane)) < 32u;
           if (__any_sync(0xffffffffu, near)) {  // some row's target is one of this warp's vocabulary rows
 #pragma unroll
-            for (int k = 0; k < C::BT; ++k)
+            for (int k = 0; k < C::HC; ++k)
               if (tgt[k] == row) v[k] -= gs[k];
           }
         } else {
-          const int col0 = (t0 + j) * C::BT;
-          if (col0 + C::BT > p.rows_b) {
+          const int col0 = (t0 + j) * C::BT + half * C::HC;
+          if (col0 + C::HC > p.rows_b) {
 #pragma unroll
-            for (int k = 0; k < C::BT; ++k)
+            for (int k = 0; k < C::HC; ++k)
               if (col0 + k >= p.rows_b) v[k] = -INFINITY;
           }
           float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-          for (int k = 4; k < C::BT; k += 4) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) top[q] = fmaxf(top[q], v[k + q]);
+          for (int k = 4; k < C::HC; k += 4) {
+            const int q = (k >> 2) & 1 ? 2 : 0;
+            top[q] = max3(top[q], v[k], v[k + 1]);
+            top[q + 1] = max3(top[q + 1], v[k + 2], v[k + 3]);
           }
-          const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.c;
-          const bool move = t > m + MOVE_REFERENCE || (m == -INFINITY && t > m);
+          float t = fmaxf(max3(top[0], top[1], top[2]), top[3]) * p.c;
+          if (C::MODE == TC_PULL) {
+            // one reference a row: the halves' maxima meet in shared memory (two sets, by turns, so that
+            // one barrier an item of the two warps is enough)
+            float* tops = reinterpret_cast<float*>(smem + C::OFF_TOP) + (j & 1) * (C::WG * 128) + quarter * 32 + lane;
+            tops[wg * 128] = t;
+            __syncwarp();
+            if (lane == 0) bar_arrive(pair(a, quarter));
+            ok = __all_sync(0xffffffffu, bar_wait(pair(a, quarter), j & 1, gave_up, p.err));
+            if (!ok) break;
+            t = fmaxf(t, tops[(wg ^ 1) * 128]);
+          }
+          const bool move = t > m + MOVE_REFERENCE;
           if (__any_sync(0xffffffffu, move)) {
             const float f = move ? (m == -INFINITY ? 0.f : ex2(m - t)) : 1.f;
-            sum *= f;
+            sum = m == -INFINITY ? sum : sum * f;
             if (move) m = t;
-            if (C::MODE == TC_PULL && w >= C::WG) {
+            if (C::MODE == TC_PULL && j > 0) {
               // O was made against the old reference
               if (C::NA == 1 && C::NB > 1) {
                 ok = bar_wait(pv_done, (w - 1) & 1, gave_up, p.err);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
                 tc_after();
               }
-              for (int k = 0; k < ksteps * 16; k += 32) {
-                float o[32];
-                const u32 at = tmem + C::O_COL + a_mine * C::DP + k + lanes;
-                tc_ld32(o, at);
+              for (int k = half * 16; k < ksteps * 16; k += 32) {
+                float o[16];
+                const u32 at = tmem + C::O_COL + a * C::DP + k + lanes;
+                tc_ld16(o, at);
                 tc_wait_ld();
 #pragma unroll
-                for (int q = 0; q < 32; ++q) o[q] *= f;
-                tc_st32(at, reinterpret_cast<const u32*>(o));
+                for (int q = 0; q < 16; ++q) o[q] *= f;
+                tc_st16(at, reinterpret_cast<const u32*>(o));
               }
             }
           }
           const float off = (float)FWD_SHIFT - (m == -INFINITY ? 0.f : m);
-          float add[4] = {0.f, 0.f, 0.f, 0.f};
+          const u64 off2 = join2(off, off);
+          u64 add[2] = {0, 0};
+          my_turn(j);
 #pragma unroll
-          for (int k = 0; k < C::BT; ++k) {
-            v[k] = ex2(fmaf(v[k], p.c, off));
-            add[k & 3] += v[k];
+          for (int k = 0; k < C::HC; k += 2) {
+            part2(fma2(join2(v[k], v[k + 1]), c2, off2), v[k], v[k + 1]);
+            v[k] = ex2(v[k]);
+            v[k + 1] = ex2(v[k + 1]);
+            add[(k >> 1) & 1] = add2(add[(k >> 1) & 1], join2(v[k], v[k + 1]));
           }
-          sum += (add[0] + add[1]) + (add[2] + add[3]);
+          next_turn();
+          float lo, hi;
+          part2(add2(add[0], add[1]), lo, hi);
+          sum += lo + hi;
         }
         if constexpr (C::SECOND) {
+          // each half's P takes the first columns of the half's own S: a warp overwrites what it has read itself
+          u32 h[C::HC / 2];
 #pragma unroll
-          for (int k = 0; k < C::BT; k += 32) {
-            u32 h[16];
+          for (int q = 0; q < C::HC / 2; ++q) h[q] = pack2<T>(v[2 * q], v[2 * q + 1]);
+          if constexpr (C::MODE == TC_GRAD_W) {
+            // rows with a negative upstream gradient: the sign of their whole column
+            const u32* sign = reinterpret_cast<const u32*>(smem + C::OFF_META + st * C::META + 12 * C::BT) + half * (C::HC / 2);
+            const u32 own = sign[lane % (C::HC / 2)];
+            if (__any_sync(0xffffffffu, own != 0)) {
 #pragma unroll
-            for (int q = 0; q < 16; ++q) h[q] = pack2<T>(v[k + 2 * q], v[k + 2 * q + 1]);
-            if constexpr (C::MODE == TC_GRAD_W) {
-              // rows with a negative upstream gradient: the sign of their whole column
-              const u32* sign = reinterpret_cast<const u32*>(smem + C::OFF_META + st * C::META + 12 * C::BT) + k / 2;
-              const u32 own = sign[lane & 15];
-              if (__any_sync(0xffffffffu, own != 0)) {
-#pragma unroll
-                for (int q = 0; q < 16; ++q) h[q] ^= sign[q];
-              }
+              for (int q = 0; q < C::HC / 2; ++q) h[q] ^= sign[q];
             }
-            tc_st16(S + k / 2, h);
           }
+#pragma unroll
+          for (int q = 0; q < C::HC / 2; q += 16) tc_st16(S + q, h + q);
           tc_wait_st();
         }
+      } else {
+        next_turn();
       }
       tc_before();
       __syncwarp();
       if (lane == 0) bar_arrive(p_full(b));
     }
-    if (C::MODE != TC_GRAD_W && row < p.rows_a && ok) {
-      const int part = blockIdx.y * (C::WG / C::NA) + (C::NA == 1 ? wg : 0);
-      p.part_ms[(i64)part * p.rows_a + row] = make_float2(m, sum);
+    if (C::MODE == TC_STATS && row < p.rows_a && ok)
+      p.part_ms[(i64)(blockIdx.y * HALVES + half) * p.rows_a + row] = make_float2(m, sum);
+    if (C::MODE == TC_PULL) {
+      float* sums = reinterpret_cast<float*>(smem + C::OFF_TOP) + (my_tiles & 1) * (C::WG * 128) + quarter * 32 + lane;
+      sums[wg * 128] = sum;
+      __syncwarp();
+      if (lane == 0) bar_arrive(pair(a, quarter));
+      ok = ok && (!warp_live || bar_wait(pair(a, quarter), my_tiles & 1, gave_up, p.err));
+      if (half == 0 && row < p.rows_a && ok) p.part_ms[(i64)blockIdx.y * p.rows_a + row] = make_float2(m, sum + sums[(wg ^ 1) * 128]);
     }
     if (C::SECOND && my_tiles > 0) {
       ok = ok && bar_wait(o_full, 0, gave_up, p.err);
@@ -419,11 +372,9 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       if (ok && warp_live) {
         tc_after();
         const float f = C::MODE == TC_GRAD_W ? p.out_scale * __uint_as_float(*p.top) : 1.f;
-        // with two warpgroups and one tile each takes half the columns
-        const int step = C::WG > C::NA ? 64 : 32;
-        for (int k = C::WG > C::NA ? wg * 32 : 0; k < p.D; k += step) {
+        for (int k = half * 32; k < p.D; k += 32 * HALVES) {
           float o[32];
-          tc_ld32(o, tmem + C::O_COL + a_mine * C::DP + k + lanes);
+          tc_ld32(o, tmem + C::O_COL + a * C::DP + k + lanes);
           tc_wait_ld();
           if (row < p.rows_a) {
             const bool slab = C::MODE == TC_PULL || gridDim.y > 1;
@@ -490,7 +441,7 @@ __global__ void loss_pack_kernel(const T* __restrict__ src, i64 ld, i64 rows, in
   }
 }
 
-// What the dW pass needs of every row of x, by tiles of BT rows: bias (p g = exp2(l - bias)), target,
+// What the dW pass needs of every row of x, by tiles of BT rows: -bias (p g = exp2(l - bias)), target,
 // |g| as P holds it, and the sign as a mask of the packed element.  Rows that do not count, and the
 // rows behind the last, have an infinite bias: P = 0.
 __global__ void loss_meta_kernel(const float* __restrict__ lse2, const i64* __restrict__ target, const float* __restrict__ g,
@@ -509,7 +460,7 @@ __global__ void loss_meta_kernel(const float* __restrict__ lse2, const i64* __re
     t = (int)target[r];
     sign = g[r] < 0.f ? 0x8000u : 0u;
   }
-  reinterpret_cast<float*>(tile)[k] = bias;
+  reinterpret_cast<float*>(tile)[k] = -bias;
   reinterpret_cast<int*>(tile + 4 * BT)[k] = t;
   reinterpret_cast<float*>(tile + 8 * BT)[k] = gs;
   reinterpret_cast<unsigned short*>(tile + 12 * BT)[k] = (unsigned short)sign;
@@ -585,54 +536,6 @@ __global__ void loss_join_dw_kernel(const float* __restrict__ slab, i64 size, in
 }
 
 // ---------------------------------------------------------------- host side
-static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
-static int blocks_for(i64 threads) {
-  const i64 b = (threads + 255) / 256, most = (i64)sm_count() * 16;
-  return (int)(b < 1 ? 1 : b < most ? b : most);
-}
-
-typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static EncodeFn encode_fn() {
-  static EncodeFn fn = []() -> EncodeFn {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      return nullptr;
-    return (EncodeFn)f;
-  }();
-  return fn;
-}
-
-static bool make_map(CUtensorMap* map, const void* p, bool bf16, i64 rows, i64 D, i64 ld, int box_rows) {
-  EncodeFn fn = encode_fn();
-  if (!fn) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, step[2] = {1, 1};
-  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(p), dims, strides,
-            box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-static bool tma_ready(const void* p, i64 ld) { return ((uintptr_t)p & 15) == 0 && ld * 2 % 16 == 0; }
-static i64 packed_ld(i64 D) { return (D + 7) / 8 * 8; }
-
-// Tiles B a CTA runs over.  `groups` CTAs cover the rows A; the tiles are split until the CTAs fill
-// the SMs' `slots` evenly: the time is (rounds of CTAs) x (tiles of one + about 3 for its start and end).
-static int split_count(i64 groups, i64 tiles, i64 slots) {
-  int best = 1;
-  double best_t = 1e300;
-  for (i64 s = 1; s <= tiles && s <= 2 * slots && (s == 1 || groups * s <= 3 * slots); ++s) {
-    const i64 per = (tiles + s - 1) / s;
-    if ((tiles + per - 1) / per != s) continue;  // the same as fewer splits
-    const double t = (double)((groups * s + slots - 1) / slots) * (double)(per + 3);
-    if (t < best_t * 0.999) { best_t = t; best = (int)s; }
-  }
-  return best;
-}
-
 struct TcPlan {
   int NA, BT, ctas, splits, per, parts;
   i64 groups;
@@ -652,26 +555,26 @@ static TcPlan plan_of(i64 rows_a, i64 rows_b) {
   const int s = split_count(p.groups, tiles, (i64)sm_count() * C::CTAS);
   p.per = (int)((tiles + s - 1) / s);
   p.splits = (int)((tiles + p.per - 1) / p.per);
-  p.parts = p.splits * (C::MODE == TC_GRAD_W ? 1 : C::WG / C::NA);
+  p.parts = p.splits * (C::MODE == TC_STATS ? HALVES : 1);
   return p;
 }
 
-//                     MODE      DP  NA WG NB  BT ST CTAS
-typedef TcShape<TC_STATS, 64, 2, 2, 4, 128, 6, 1> Stats64;
-typedef TcShape<TC_STATS, 128, 2, 2, 4, 128, 4, 1> Stats128;
-typedef TcShape<TC_STATS, 256, 1, 2, 4, 128, 2, 1> Stats256;
-typedef TcShape<TC_STATS, 64, 1, 1, 2, 128, 4, 2> StatsFew64;
-typedef TcShape<TC_STATS, 128, 1, 1, 2, 128, 2, 2> StatsFew128;
-typedef TcShape<TC_PULL, 64, 2, 2, 2, 128, 6, 1> Pull64;
-typedef TcShape<TC_PULL, 128, 2, 2, 2, 128, 4, 1> Pull128;
-typedef TcShape<TC_PULL, 256, 1, 1, 2, 64, 4, 1> Pull256;
-typedef TcShape<TC_PULL, 64, 1, 1, 1, 128, 4, 2> PullFew64;
-typedef TcShape<TC_PULL, 128, 1, 1, 1, 128, 2, 2> PullFew128;
-typedef TcShape<TC_GRAD_W, 64, 2, 2, 2, 128, 6, 1> Grad64;
-typedef TcShape<TC_GRAD_W, 128, 2, 2, 2, 128, 4, 1> Grad128;
-typedef TcShape<TC_GRAD_W, 256, 1, 2, 2, 64, 4, 1> Grad256;
-typedef TcShape<TC_GRAD_W, 64, 1, 1, 1, 128, 4, 2> GradFew64;
-typedef TcShape<TC_GRAD_W, 128, 1, 1, 1, 128, 2, 2> GradFew128;
+//               MODE      DP  NA NB  BT ST CTAS
+typedef TcShape<TC_STATS, 64, 2, 3, 128, 6, 1> Stats64;
+typedef TcShape<TC_STATS, 128, 2, 3, 128, 5, 1> Stats128;
+typedef TcShape<TC_STATS, 256, 2, 2, 128, 3, 1> Stats256;
+typedef TcShape<TC_STATS, 64, 1, 3, 64, 8, 2> StatsFew64;
+typedef TcShape<TC_STATS, 128, 1, 3, 64, 6, 2> StatsFew128;
+typedef TcShape<TC_PULL, 64, 2, 2, 128, 6, 1> Pull64;
+typedef TcShape<TC_PULL, 128, 2, 2, 64, 8, 1> Pull128;
+typedef TcShape<TC_PULL, 256, 1, 2, 64, 5, 1> Pull256;
+typedef TcShape<TC_PULL, 64, 1, 2, 64, 8, 2> PullFew64;
+typedef TcShape<TC_PULL, 128, 1, 1, 64, 6, 2> PullFew128;
+typedef TcShape<TC_GRAD_W, 64, 2, 2, 128, 6, 1> Grad64;
+typedef TcShape<TC_GRAD_W, 128, 2, 2, 64, 8, 1> Grad128;
+typedef TcShape<TC_GRAD_W, 256, 1, 2, 64, 5, 1> Grad256;
+typedef TcShape<TC_GRAD_W, 64, 1, 2, 64, 8, 2> GradFew64;
+typedef TcShape<TC_GRAD_W, 128, 1, 1, 64, 6, 2> GradFew128;
 
 // f(shape) for the shape that the sizes ask for
 template <typename F>
@@ -698,8 +601,9 @@ static TcPlan tc_plan(int mode, i64 N, i64 V, i64 D) {
 }
 
 bool tc_loss_takes(int dtype, i64 N, i64 V, i64 D) {
-  // tile counts and coordinates stay in 31 bits, and the grid in its limits
-  return dtype != GSB_F32 && D <= 256 && N < (1ll << 30) && V < (1ll << 30);
+  (void)N;
+  (void)V;
+  return dtype != GSB_F32 && D <= 256;
 }
 
 struct TcFwdLayout { size_t ms, o, x, w, bytes; };
@@ -749,16 +653,20 @@ static const T* pack_rows(const void* src, i64 ld, i64 rows, i64 D, bool negate,
 }
 
 template <typename T, typename C>
-static int launch_tc(const CUtensorMap& a, const CUtensorMap& b, const TcPlan& plan, const TcParams& p, int kid, cudaStream_t st) {
+static int launch_tc(const CUtensorMap& b, const TcPlan& plan, const TcParams& p, int kid, cudaStream_t st) {
   // the attribute belongs to the device's copy of the kernel; setting it is cheap and not a stream operation
   GSB_CUDA_OK(cudaFuncSetAttribute(loss_tc_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
   LaunchScope ls(kid, st);
-  loss_tc_kernel<T, C><<<dim3((unsigned)plan.groups, (unsigned)plan.splits), C::THREADS, C::BYTES, st>>>(a, b, p);
+  loss_tc_kernel<T, C><<<dim3((unsigned)plan.groups, (unsigned)plan.splits), C::THREADS, C::BYTES, st>>>(b, p);
   return GSB_OK;
 }
 
-// not zero, so that a masked logit of -inf stays one; times any finite product it is as good as zero
-static float logit_factor(float scale) { return fmaxf(fabsf(scale) * LOG2E, 1e-38f); }
+template <typename T>
+void launch_loss_join(const LossArgs& a, const float2* part_ms, int parts, const float* part_o, float* pull) {
+  LaunchScope ls(KID_LOSS_JOIN, a.st);
+  loss_join_kernel<T><<<ceil_div_i(a.N, 8), 256, 0, a.st>>>(part_ms, parts, part_o, (const T*)a.x, a.ldx, a.N, (const T*)a.w, a.ldw, a.V,
+                                                            (int)a.D, a.scale, a.target, a.ignore, a.loss, a.lse2, pull, a.err);
+}
 
 template <typename T>
 int tc_loss_forward(const LossArgs& a, float* pull) {
@@ -773,9 +681,11 @@ int tc_loss_forward(const LossArgs& a, float* pull) {
   i64 ldx = a.ldx, ldw = a.ldw;
   if (negate || !tma_ready(x, ldx)) { x = pack_rows<T>(x, ldx, a.N, a.D, negate, nullptr, ws + L.x, a.st); ldx = packed_ld(a.D); }
   if (!tma_ready(w, ldw)) { w = pack_rows<T>(w, ldw, a.V, a.D, false, nullptr, ws + L.w, a.st); ldw = packed_ld(a.D); }
-  CUtensorMap ma, mb;
-  if (!make_map(&ma, x, IsBf16<T>::value, a.N, a.D, ldx, 128) || !make_map(&mb, w, IsBf16<T>::value, a.V, a.D, ldw, plan.BT)) return GSB_ERR_CUDA;
+  CUtensorMap mb;
+  if (!tc_map(&mb, w, IsBf16<T>::value, a.V, a.D, ldw, 1, 64, plan.BT)) return GSB_ERR_CUDA;
   TcParams p = {};
+  p.a = x;
+  p.lda = ldx;
   p.rows_a = (int)a.N;
   p.rows_b = (int)a.V;
   p.D = (int)a.D;
@@ -784,11 +694,9 @@ int tc_loss_forward(const LossArgs& a, float* pull) {
   p.part_ms = (float2*)(ws + L.ms);
   p.part_o = (float*)(ws + L.o);
   p.err = a.err;
-  const int rc = with_shape(mode, a.N, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(ma, mb, plan, p, KID_LOSS, a.st); });
+  const int rc = with_shape(mode, a.N, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS, a.st); });
   if (rc != GSB_OK) return rc;
-  LaunchScope ls(KID_LOSS_JOIN, a.st);
-  loss_join_kernel<T><<<ceil_div_i(a.N, 8), 256, 0, a.st>>>(p.part_ms, plan.parts, p.part_o, (const T*)a.x, a.ldx, a.N, (const T*)a.w, a.ldw,
-                                                            a.V, (int)a.D, a.scale, a.target, a.ignore, a.loss, a.lse2, pull, a.err);
+  launch_loss_join<T>(a, p.part_ms, plan.parts, p.part_o, pull);
   return GSB_OK;
 }
 
@@ -806,10 +714,12 @@ int tc_loss_grad_w(const LossArgs& a) {
     LaunchScope ls(KID_LOSS_JOIN, a.st);
     loss_meta_kernel<<<ceil_div_i(npad, 256), 256, 0, a.st>>>(a.lse2, a.target, a.g, a.top, a.N, npad, plan.BT, (unsigned char*)(ws + L.meta));
   }
-  CUtensorMap ma, mb;
-  if (!make_map(&ma, w, IsBf16<T>::value, a.V, a.D, ldw, 128) || !make_map(&mb, x, IsBf16<T>::value, a.N, a.D, packed_ld(a.D), plan.BT))
+  CUtensorMap mb;
+  if (!tc_map(&mb, x, IsBf16<T>::value, a.N, a.D, packed_ld(a.D), 1, 64, plan.BT))
     return GSB_ERR_CUDA;
   TcParams p = {};
+  p.a = w;
+  p.lda = ldw;
   p.rows_a = (int)a.V;
   p.rows_b = (int)a.N;
   p.D = (int)a.D;
@@ -821,7 +731,7 @@ int tc_loss_grad_w(const LossArgs& a) {
   p.top = a.top;
   p.out_scale = fabsf(a.scale) / (float)(1 << GRAD_SHIFT);
   p.err = a.err;
-  const int rc = with_shape(TC_GRAD_W, a.N, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(ma, mb, plan, p, KID_LOSS_GRAD, a.st); });
+  const int rc = with_shape(TC_GRAD_W, a.N, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS_GRAD, a.st); });
   if (rc != GSB_OK) return rc;
   if (plan.splits > 1) {
     LaunchScope ls(KID_LOSS_JOIN, a.st);
@@ -836,6 +746,9 @@ void tc_loss_dx(const LossArgs& a, const float* pull) {
   loss_dx_kernel<T><<<blocks_for(a.N * a.D), 256, 0, a.st>>>(pull, a.g, a.scale, a.N, (int)a.D, (T*)a.dx);
 }
 
+template void launch_loss_join<float>(const LossArgs&, const float2*, int, const float*, float*);
+template void launch_loss_join<__half>(const LossArgs&, const float2*, int, const float*, float*);
+template void launch_loss_join<__nv_bfloat16>(const LossArgs&, const float2*, int, const float*, float*);
 template int tc_loss_forward<__half>(const LossArgs&, float*);
 template int tc_loss_forward<__nv_bfloat16>(const LossArgs&, float*);
 template int tc_loss_grad_w<__half>(const LossArgs&);

@@ -158,7 +158,7 @@ static int CheckLoss(const torch::Tensor& x, const torch::Tensor& weight, const 
   TORCH_CHECK(target.dim() == 1 && target.size(0) == x.size(0), op, ": target must be [N]");
   TORCH_CHECK(weight.size(0) >= 1 && weight.size(1) >= 1, op, ": weight must have a row and a column");
   TORCH_CHECK(weight.size(1) <= GSB_LOSS_MAX_D, op, ": at most ", GSB_LOSS_MAX_D, " columns");
-  TORCH_CHECK(x.size(0) < (1ll << 31) && weight.size(0) < (1ll << 31), op, ": at most 2^31 - 1 rows");
+  TORCH_CHECK(x.size(0) <= (1ll << 30) && weight.size(0) <= (1ll << 30), op, ": at most 2^30 rows");
   TORCH_CHECK(std::isfinite(scale), op, ": scale must be finite");
   return dt;
 }

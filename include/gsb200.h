@@ -279,7 +279,7 @@ GSB_API int gsb_dropout(const void* x, int dtype, int64_t n, double p, uint64_t 
  * gsb_linear_ce_grad: dx[N, D] and / or dw[V, D] (either may be NULL) from the
  * upstream gradient: upstream[N] when per_row, else one value, divided by *count
  * when count is given.  Sums are made in an order that depends on the sizes
- * alone.  N, V < 2^31.  A workspace is sized for the device that is current. */
+ * alone.  N, V <= 2^30.  A workspace is sized for the device that is current. */
 #define GSB_LOSS_MAX_D 65536
 GSB_API int gsb_linear_ce_has_pull(int dtype, int64_t N, int64_t V, int64_t D);
 GSB_API size_t gsb_linear_ce_workspace_bytes(int dtype, const void* weight, int64_t ldw, int64_t N, int64_t V,

@@ -214,7 +214,12 @@ def test_one_of_the_gradients(gsb, dt):
     (dx,) = torch.autograd.grad(gsb.ops.linear_cross_entropy(xl, w, t), [xl])
     wl = w.clone().requires_grad_()
     (dw,) = torch.autograd.grad(gsb.ops.linear_cross_entropy(x, wl, t), [wl])
-    assert torch.equal(dx, both[1]) and torch.equal(dw, both[2])
+    assert torch.equal(dx, both[1])
+    # without a gradient for x the forward pass adds the log-sum-exp in another order, and dW is made
+    # from it: each of the two lies within the tolerance of the formula, not at the same bits
+    f = Formula(x, w, t, 1.0, dt)
+    g = torch.full((200,), 1.0 / int(f.live.sum()), device="cuda")
+    within(dw, f.grads(g, dt)[2], f.grads(g, dt)[3], "dW alone")
     tied = w[:200].clone().requires_grad_()     # one leaf on both sides: the gradients add up
     (d,) = torch.autograd.grad(gsb.ops.linear_cross_entropy(tied, tied, t % 200), [tied])
     a, b = tied.detach().clone().requires_grad_(), tied.detach().clone().requires_grad_()
