@@ -52,12 +52,6 @@ struct LossArgs {
   cudaStream_t st;
 };
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // The tensor-core form (gsb_loss_tc.cu): 16-bit types, up to 256 columns.
 bool tc_loss_takes(int dtype, i64 N, i64 V, i64 D);
 bool tc_loss_packs(const void* w, i64 ldw);  // whether the rows of W have to be copied for it

@@ -29,12 +29,17 @@ struct GmShape {
   static constexpr bool A_ACROSS = MODE == GM_DW, B_ACROSS = MODE == GM_DX || MODE == GM_DW;
   static constexpr int A_PLANE = 128 * 128, B_PLANE = BN * 128;
   static constexpr int STAGE = PL * (A_PLANE + B_PLANE);
-  static constexpr int COLS = 2 * BN < 128 ? 128 : 2 * BN;
+  // The products of two high planes have an accumulator of their own: every addition into a 32-bit
+  // accumulator truncates, and the five small products would truncate the large sum five times more.
+  static constexpr int ACCS = PL == 3 ? 2 : 1;
+  static constexpr int COLS = 2 * ACCS * BN;
   static constexpr int THREADS = 8 * 32 + 64;
-  static constexpr int OFF_BAR = ST * STAGE;
+  static constexpr int OFF_OUT = ST * STAGE;  // GM_PIECE: 32 rows x 64 columns a warp on their way out
+  static constexpr int OFF_BAR = OFF_OUT + (MODE == GM_PIECE ? 8 * 4096 : 0);
   static constexpr int BARS = 2 * ST + 4;
   static constexpr int BYTES = OFF_BAR + 8 * BARS + 16 + 1024;
-  static_assert(BYTES <= 227 * 1024 && COLS <= 512, "");
+  static_assert(BYTES <= 227 * 1024 && COLS >= 128 && COLS <= 512, "");
+  static_assert(MODE != GM_PIECE || BN % 128 == 0, "");
 };
 
 struct GmParams {
@@ -49,8 +54,6 @@ struct GmParams {
   const i64* target;
   const u32* top;
   int v0;                   // GM_PIECE: id of the piece's first column
-  void* piece;              // GM_PIECE: [PL][M][ld_piece]
-  i64 ld_piece, plane;
   float* slab;              // GM_DX / GM_DW: [units along z][M][N]
   int add;
   int* err;
@@ -58,7 +61,8 @@ struct GmParams {
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(C::THREADS, 1)
-loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GmParams p) {
+loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                 const __grid_constant__ CUtensorMap map_out, const GmParams p) {
   extern __shared__ unsigned char smem_raw[];
   const u32 base = (smem_addr(smem_raw) + 1023) & ~1023u;
   unsigned char* smem = smem_raw + (base - smem_addr(smem_raw));
@@ -107,7 +111,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
   tc_before();
   __syncthreads();
   tc_after();
-  const u32 tmem = *tmem_slot;
+  const u32 tmem = __reduce_max_sync(0xffffffffu, *tmem_slot);  // the same in every lane, and known to be
 
   if (warp == 8) {
     // ------------------------------------------------ loads
@@ -143,44 +147,46 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         for (int k = 0; k < (1 << 16) && !bar_try(full(j % C::ST), (j / C::ST) & 1); ++k) __nanosleep(32);
     }
   } else if (warp == 9) {
-    // ------------------------------------------------ products
-    if (lane == 0) {
-      const u32 id = tc_idesc(C::PL == 3 || IsBf16<T>::value, C::BN, C::A_ACROSS, C::B_ACROSS);
-      int it = 0, i = 0;
-      bool ok = true;
-      int m, n, z;
-      for (; ok && tile_at(i, m, n, z); ++i) {
-        int k0, blocks;
-        depth(z, k0, blocks);
-        const int b = i & 1;
-        if (i >= 2) ok = bar_wait(acc_empty(b), ((i >> 1) - 1) & 1, gave_up, p.err);
+    // ------------------------------------------------ products (the warp together, one lane issues)
+    const u32 id = tc_idesc(C::PL == 3 || IsBf16<T>::value, C::BN, C::A_ACROSS, C::B_ACROSS);
+    const bool leader = elect_one();
+    int it = 0, i = 0;
+    bool ok = true;
+    int m, n, z;
+    for (; ok && tile_at(i, m, n, z); ++i) {
+      int k0, blocks;
+      depth(z, k0, blocks);
+      const int b = i & 1;
+      if (i >= 2) ok = bar_wait(acc_empty(b), ((i >> 1) - 1) & 1, gave_up, p.err);
+      tc_after();
+      const u32 d = tmem + b * (C::ACCS * C::BN);
+      for (int kb = 0; ok && kb < blocks; ++kb, ++it) {
+        const int st = it % C::ST;
+        ok = bar_wait(full(st), (it / C::ST) & 1, gave_up, p.err);
+        if (!ok) break;
         tc_after();
-        const u32 d = tmem + b * C::BN;
-        for (int kb = 0; ok && kb < blocks; ++kb, ++it) {
-          const int st = it % C::ST;
-          ok = bar_wait(full(st), (it / C::ST) & 1, gave_up, p.err);
-          if (!ok) break;
-          tc_after();
-          const u32 A = base + st * C::STAGE, B = A + C::PL * C::A_PLANE;
-          // small products first within a slice
-          constexpr int PAIRS = C::PL == 3 ? 6 : 1;
-          constexpr int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
+        const u64 A = tc_desc(base + st * C::STAGE, C::A_ACROSS ? 8192 : 16);
+        const u64 B = tc_desc(base + st * C::STAGE + C::PL * C::A_PLANE, C::B_ACROSS ? 8192 : 16);
+        constexpr int PAIRS = C::PL == 3 ? 6 : 1;
+        constexpr int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
+        if (leader) {
 #pragma unroll
           for (int q = 0; q < PAIRS; ++q) {
-            const u32 a0 = A + (C::PL == 3 ? pa[q] : 0) * C::A_PLANE, b0 = B + (C::PL == 3 ? pb[q] : 0) * C::B_PLANE;
+            const bool high = q == PAIRS - 1;
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              tc_mma(d, tc_desc(a0 + k * (C::A_ACROSS ? 2048 : 32), C::A_ACROSS ? 8192 : 16),
-                     tc_desc(b0 + k * (C::B_ACROSS ? 2048 : 32), C::B_ACROSS ? 8192 : 16), id, kb > 0 || q > 0 || k > 0);
+              tc_mma(d + (high ? (C::ACCS - 1) * C::BN : 0), A + ((C::PL == 3 ? pa[q] : 0) * C::A_PLANE + k * (C::A_ACROSS ? 2048 : 32)) / 16,
+                     B + ((C::PL == 3 ? pb[q] : 0) * C::B_PLANE + k * (C::B_ACROSS ? 2048 : 32)) / 16, id,
+                     kb > 0 || k > 0 || (q > 0 && !high));
           }
           tc_commit(empty(st));
         }
-        if (ok) tc_commit(acc_full(b));
       }
-      // what was issued ends by itself; a bounded look keeps the order when a wait gave up
-      for (int j = i > 2 ? i - 2 : 0; j < i; ++j)
-        for (int k = 0; k < (1 << 16) && !bar_try(acc_full(j & 1), (j >> 1) & 1); ++k) __nanosleep(32);
+      if (ok && leader) tc_commit(acc_full(b));
     }
+    // what was issued ends by itself; a bounded look keeps the order when a wait gave up
+    for (int j = i > 2 ? i - 2 : 0; j < i; ++j)
+      for (int k = 0; k < (1 << 16) && !bar_try(acc_full(j & 1), (j >> 1) & 1); ++k) __nanosleep(32);
   } else {
     // ------------------------------------------------ epilogue: a thread has a row and half the columns
     const int half = warp >> 2, quarter = warp & 3;
@@ -204,13 +210,68 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         gs = p.g[row] / __uint_as_float(*p.top) * (float)(1 << GRAD_SHIFT);
         hot = (int)(p.target[row] - p.v0);
       }
+      auto columns = [&](float* v, int q) {  // 32 of the tile's columns, the accumulators added
+        const u32 from = tmem + b * (C::ACCS * C::BN) + q + lanes;
+        tc_ld32(v, from);
+        if constexpr (C::ACCS == 2) {
+          float u[32];
+          tc_ld32(u, from + C::BN);
+          tc_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += u[j];
+        } else {
+          tc_wait_ld();
+        }
+      };
+      if constexpr (C::MODE == GM_PIECE) {
+        // 64 columns at a time through shared memory, so that they leave as whole lines: row by row a
+        // warp's stores touch 32 lines an instruction (52 us for 4000 x 4096 columns of three planes)
 #pragma unroll 1
-      for (int q = half * (C::BN / 2); q < (half + 1) * (C::BN / 2); q += 32) {
+        for (int q = half * (C::BN / 2); q < (half + 1) * (C::BN / 2); q += 64) {
+          const int col = n * C::BN + q;
+          if (col >= p.N || m * 128 + quarter * 32 >= p.M) break;
+          float v[64];
+          columns(v, q);
+          columns(v + 32, q + 32);
+#pragma unroll
+          for (int j = 0; j < 64; ++j) {
+            v[j] = ex2(fmaf(v[j], p.c, -lse));
+            if (col + j == hot) v[j] -= 1.f;
+            v[j] = gs == 0.f ? 0.f : v[j] * gs;  // rows that do not count
+          }
+          const u32 out = base + C::OFF_OUT + warp * 4096;
+#pragma unroll
+          for (int pl = 0; pl < C::PL; ++pl) {
+            if (lane == 0) tma_store_read();  // the tile before has left
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 64; j += 8) {
+              u32 h[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                h[e] = pack2<T>(v[j + 2 * e], v[j + 2 * e + 1]);
+                if (pl + 1 < C::PL) {  // what this plane does not hold
+                  const T* t = reinterpret_cast<const T*>(h + e);
+                  v[j + 2 * e] -= to_float(t[0]);
+                  v[j + 2 * e + 1] -= to_float(t[1]);
+                }
+              }
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out + lane * 128 + ((j / 8) ^ (lane & 7)) * 16), "r"(h[0]), "r"(h[1]),
+                           "r"(h[2]), "r"(h[3])
+                           : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tma_store(&map_out, col, m * 128 + quarter * 32, pl, out);
+          }
+        }
+      }
+#pragma unroll 1
+      for (int q = half * (C::BN / 2); C::MODE != GM_PIECE && q < (half + 1) * (C::BN / 2); q += 32) {
         const int col = n * C::BN + q;
         if (col >= p.N) break;
         float v[32];
-        tc_ld32(v, tmem + b * C::BN + q + lanes);
-        tc_wait_ld();
+        columns(v, q);
         if (blocks == 0) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = 0.f;
@@ -232,34 +293,6 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 #pragma unroll
           for (int j = 0; j < 32; ++j) s[j & 3] += ex2(fmaf(v[j], p.c, off));
           run_s += (s[0] + s[1]) + (s[2] + s[3]);
-        } else if (C::MODE == GM_PIECE) {
-          if (row < p.M) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              v[j] = ex2(fmaf(v[j], p.c, -lse));
-              if (col + j == hot) v[j] -= 1.f;
-              v[j] = gs == 0.f ? 0.f : v[j] * gs;  // rows that do not count
-            }
-            const bool whole = col + 32 <= p.N;
-#pragma unroll
-            for (int pl = 0; pl < C::PL; ++pl) {
-              T* to = (T*)p.piece + pl * p.plane + (i64)row * p.ld_piece + col;
-              T h[32];
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                h[j] = from_float<T>(v[j]);
-                if (pl + 1 < C::PL) v[j] -= to_float(h[j]);  // what this plane does not hold
-              }
-              if (whole) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) reinterpret_cast<uint4*>(to)[j] = reinterpret_cast<const uint4*>(h)[j];
-              } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (col + j < p.N) to[j] = h[j];
-              }
-            }
-          }
         } else if (row < p.M) {
           float* to = p.slab + ((i64)z * p.M + row) * p.N + col;
           if (col + 32 <= p.N && (p.N & 3) == 0) {
@@ -284,6 +317,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       __syncwarp();
       if (lane == 0) bar_arrive(acc_empty(b));
     }
+    if (C::MODE == GM_PIECE && lane == 0) tma_store_done();
     if (C::MODE == GM_STATS && ok) {
       const int row = blockIdx.x * 128 + quarter * 32 + lane;
       if (row < p.M) p.part_ms[(i64)(blockIdx.y * 2 + half) * p.M + row] = make_float2(run_m, run_s);
@@ -355,7 +389,8 @@ static i64 piece_columns(i64 N, i64 V) {
   if (c < 128) c = 128;
   return c < V ? c : V;
 }
-static int bn_of(int planes, i64 cols) { return planes == 3 ? (cols <= 64 ? 64 : 128) : 256; }
+static int bn_of(int planes, i64 cols) { return planes == 3 ? (cols <= 64 ? 64 : 128) : 256; }  // dx, dW
+static int bn_wide(int planes) { return planes == 3 ? 128 : 256; }                               // logits
 
 struct GmLayout {
   size_t ms, x, w, piece, dx_slab, dw_slab, bytes;
@@ -369,7 +404,7 @@ static GmLayout gemm_layout(int planes, i64 N, i64 V, i64 D, bool forward, bool 
   L.ldp = packed_ld(D);
   L.x = take(2 * (size_t)planes * N * L.ldp);
   if (forward) {
-    const i64 tiles = (V + bn_of(planes, V) - 1) / bn_of(planes, V);
+    const i64 tiles = (V + bn_wide(planes) - 1) / bn_wide(planes);
     const int s = split_count(N > 0 ? (N + 127) / 128 : 1, tiles, sm_count());
     L.per = (int)((tiles + s - 1) / s);
     L.splits = (int)((tiles + L.per - 1) / L.per);
@@ -407,20 +442,21 @@ static void make_planes(const void* src, i64 ld, i64 rows, i64 D, bool negate, c
 }
 
 template <typename T, typename C>
-static int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GmParams& p, dim3 grid, int kid, cudaStream_t st) {
+static int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const GmParams& p, dim3 grid, int kid, cudaStream_t st) {
   GSB_CUDA_OK(cudaFuncSetAttribute(loss_gemm_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
   LaunchScope ls(kid, st);
-  loss_gemm_kernel<T, C><<<grid, C::THREADS, C::BYTES, st>>>(a, b, p);
+  loss_gemm_kernel<T, C><<<grid, C::THREADS, C::BYTES, st>>>(a, b, out, p);
   return GSB_OK;
 }
-// the shape for `cols` columns of the result
+// the shape for `cols` columns of the result (dx and dW of few columns: 64 of them, with a stage more)
 template <typename T, int MODE, int PL>
-static int launch_mode(i64 cols, const CUtensorMap& a, const CUtensorMap& b, const GmParams& p, dim3 grid, int kid, cudaStream_t st) {
+static int launch_mode(i64 cols, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const GmParams& p, dim3 grid, int kid, cudaStream_t st) {
   if constexpr (PL == 3) {
-    if (bn_of(3, cols) == 64) return launch_gemm<T, GmShape<MODE, 3, 64, 3>>(a, b, p, grid, kid, st);
-    return launch_gemm<T, GmShape<MODE, 3, 128, 2>>(a, b, p, grid, kid, st);
+    if constexpr (MODE == GM_DX || MODE == GM_DW)
+      if (bn_of(3, cols) == 64) return launch_gemm<T, GmShape<MODE, 3, 64, 3>>(a, b, out, p, grid, kid, st);
+    return launch_gemm<T, GmShape<MODE, 3, 128, 2>>(a, b, out, p, grid, kid, st);
   } else {
-    return launch_gemm<T, GmShape<MODE, 1, 256, 4>>(a, b, p, grid, kid, st);
+    return launch_gemm<T, GmShape<MODE, 1, 256, 4>>(a, b, out, p, grid, kid, st);
   }
 }
 
@@ -434,7 +470,7 @@ int gemm_loss_forward(const LossArgs& a) {
   i64 ldx = a.ldx, ldw = a.ldw;
   if (PL == 3 || a.scale < 0.f || !tma_ready(x, ldx)) { make_planes<S>(x, ldx, a.N, a.D, a.scale < 0.f, nullptr, ws + L.x, a.st); x = ws + L.x; ldx = L.ldp; }
   if (PL == 3 || !tma_ready(w, ldw)) { make_planes<S>(w, ldw, a.V, a.D, false, nullptr, ws + L.w, a.st); w = ws + L.w; ldw = L.ldp; }
-  const int bn = bn_of(PL, a.V);
+  const int bn = bn_wide(PL);
   CUtensorMap ma, mb;
   if (!tc_map(&ma, x, IsBf16<T>::value, a.N, a.D, ldx, PL, 64, 128) || !tc_map(&mb, w, IsBf16<T>::value, a.V, a.D, ldw, PL, 64, bn)) return GSB_ERR_CUDA;
   GmParams p = {};
@@ -448,7 +484,7 @@ int gemm_loss_forward(const LossArgs& a) {
   p.c = logit_factor(a.scale);
   p.part_ms = (float2*)(ws + L.ms);
   p.err = a.err;
-  const int rc = launch_mode<T, GM_STATS, PL>(a.V, ma, mb, p, dim3(p.m_tiles, L.splits), KID_LOSS, a.st);
+  const int rc = launch_mode<T, GM_STATS, PL>(a.V, ma, mb, mb, p, dim3(p.m_tiles, L.splits), KID_LOSS, a.st);
   if (rc != GSB_OK) return rc;
   launch_loss_join<S>(a, p.part_ms, 2 * L.splits, nullptr, nullptr);
   return GSB_OK;
@@ -480,10 +516,12 @@ int gemm_loss_backward(const LossArgs& a) {
   for (i64 v0 = 0; v0 < a.V; v0 += L.cols) {
     const i64 c = v0 + L.cols < a.V ? L.cols : a.V - v0;
     const T* wv = w + v0 * ldw;
-    CUtensorMap ma, mb;
+    CUtensorMap ma, mb, mo;
     {
-      const int bn = bn_of(PL, c);
-      if (!tc_map(&ma, x, bf, a.N, a.D, L.ldp, PL, 64, 128) || !tc_map(&mb, wv, bf, c, a.D, ldw, PL, 64, bn, a.V)) return GSB_ERR_CUDA;
+      const int bn = bn_wide(PL);
+      if (!tc_map(&ma, x, bf, a.N, a.D, L.ldp, PL, 64, 128) || !tc_map(&mb, wv, bf, c, a.D, ldw, PL, 64, bn, a.V) ||
+          !tc_map(&mo, piece, bf, a.N, c, ldq, PL, 64, 32))
+        return GSB_ERR_CUDA;
       GmParams p = {};
       p.M = (int)a.N;
       p.N = (int)c;
@@ -497,12 +535,9 @@ int gemm_loss_backward(const LossArgs& a) {
       p.target = a.target;
       p.top = a.top;
       p.v0 = (int)v0;
-      p.piece = piece;
-      p.ld_piece = ldq;
-      p.plane = a.N * ldq;
       p.err = a.err;
       const dim3 grid = units_grid(p, 1);
-      const int rc = launch_mode<T, GM_PIECE, PL>(c, ma, mb, p, grid, KID_LOSS_GRAD, a.st);
+      const int rc = launch_mode<T, GM_PIECE, PL>(c, ma, mb, mo, p, grid, KID_LOSS_GRAD, a.st);
       if (rc != GSB_OK) return rc;
     }
     if (a.dx) {
@@ -518,7 +553,7 @@ int gemm_loss_backward(const LossArgs& a) {
       p.add = v0 > 0;
       p.err = a.err;
       const dim3 grid = units_grid(p, L.dx_slabs);
-      const int rc = launch_mode<T, GM_DX, PL>(a.D, ma, mb, p, grid, KID_LOSS_GRAD, a.st);
+      const int rc = launch_mode<T, GM_DX, PL>(a.D, ma, mb, mb, p, grid, KID_LOSS_GRAD, a.st);
       if (rc != GSB_OK) return rc;
     }
     if (a.dw) {
@@ -533,7 +568,7 @@ int gemm_loss_backward(const LossArgs& a) {
       p.slab = dws;
       p.err = a.err;
       const dim3 grid = units_grid(p, L.dw_slabs);
-      const int rc = launch_mode<T, GM_DW, PL>(a.D, ma, mb, p, grid, KID_LOSS_GRAD, a.st);
+      const int rc = launch_mode<T, GM_DW, PL>(a.D, ma, mb, mb, p, grid, KID_LOSS_GRAD, a.st);
       if (rc != GSB_OK) return rc;
       LaunchScope ls(KID_LOSS_JOIN, a.st);
       loss_slabs_kernel<S><<<blocks_for(c * a.D), 256, 0, a.st>>>(dws, c * a.D, L.dw_slabs, fabsf(a.scale) * unit, a.top, nullptr, a.D,

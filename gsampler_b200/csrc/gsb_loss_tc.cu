@@ -31,32 +31,33 @@ enum { TC_STATS = 0, TC_PULL = 1, TC_GRAD_W = 2 };
 // DP    columns a row may have (64, 128, 256)
 // NA    tiles A a CTA works on at once
 // NB    S buffers, BT  rows of a tile B, ST  stages of the B pipeline, CTAS  CTAs an SM
-// An item is (tile B j, tile A a), numbered w = j NA + a; it uses buffer w % NB.  Two warpgroups turn
-// an item's S into P, half of its columns each: a warp alone issues an instruction every three
-// cycles or so, which made the tensor cores wait (41 % busy with one warpgroup an item, 8192 x 60000 x 128).
-constexpr int HALVES = 2;
-
-template <int MODE_, int DP_, int NA_, int NB_, int BT_, int ST_, int CTAS_>
+// HV    warpgroups that turn an item's S into P, each an equal share of its columns
+// ATM   tiles A in TMEM, where there is room beside O and two S buffers; else in shared memory
+// An item is (tile B j, tile A a), numbered w = j NA + a; it uses buffer w % NB.
+template <int MODE_, int DP_, int NA_, int NB_, int BT_, int ST_, int CTAS_, int HV_, bool ATM_>
 struct TcShape {
   static constexpr int MODE = MODE_, DP = DP_, NA = NA_, NB = NB_, BT = BT_, ST = ST_, CTAS = CTAS_;
+  static constexpr int HV = HV_;
+  static constexpr int POLY = MODE == TC_STATS ? 8 : 0;
+  static constexpr bool ATM = ATM_;  // tiles A in TMEM, else in shared memory
   static constexpr bool SECOND = MODE != TC_STATS;  // the product with P
-  static constexpr int WG = NA * HALVES, HC = BT / HALVES;
+  static constexpr int WG = NA * HV, HC = BT / HV;
   static constexpr int SUBS = DP / 64;
   static constexpr int B_BYTES = SUBS * BT * 128;
   static constexpr int META = MODE == TC_GRAD_W ? BT * 14 : 0;
-  static constexpr int A_COL = NB * BT, O_COL = A_COL + NA * (DP / 2);
+  static constexpr int A_COL = NB * BT, O_COL = A_COL + (ATM ? NA * (DP / 2) : 0);
   static constexpr int USED = O_COL + (SECOND ? NA * DP : 0);
   static constexpr int COLS = USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
   static constexpr int THREADS = WG * 128 + 64;
-  static constexpr int OFF_B = 0, OFF_META = ST * B_BYTES;
-  static constexpr int OFF_TOP = OFF_META + ST * META;                                     // row maxima of the halves
-  static constexpr int OFF_BAR = OFF_TOP + (MODE == TC_PULL ? 2 * WG * 128 * 4 : 0);
-  static constexpr bool TURNS = SECOND && NA == 2;
-  static constexpr int BARS = 2 * ST + 2 * NB + 3 + 8 + (MODE == TC_PULL ? 4 * NA : 0);
+  static constexpr int A_BYTES = ATM ? 0 : SUBS * 128 * 128;
+  static constexpr int OFF_B = NA * A_BYTES, OFF_META = OFF_B + ST * B_BYTES;
+  static constexpr int OFF_BAR = OFF_META + ST * META;
+  static constexpr int BARS = 2 * ST + 2 * NB + 3;
   static constexpr int BYTES = OFF_BAR + 8 * BARS + 16 + 1024;  // and room to align the base
   static_assert(USED <= 512 && COLS * CTAS <= 512, "TMEM");
-  static_assert(BYTES * CTAS <= 227 * 1024, "shared memory");
-  static_assert(HC % 32 == 0 && META % 16 == 0 && OFF_TOP % 16 == 0 && OFF_BAR % 8 == 0, "");
+  static_assert(BYTES * CTAS <= 226 * 1024, "shared memory");
+  static_assert(MODE != TC_PULL || HV == 1, "a row's running state has one owner");
+  static_assert(HC % 32 == 0 && META % 16 == 0 && OFF_BAR % 8 == 0, "");
 };
 
 struct TcParams {
@@ -86,9 +87,6 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
   auto s_full = [&](int b) { return bar0 + 8 * (2 * C::ST + b); };
   auto p_full = [&](int b) { return bar0 + 8 * (2 * C::ST + C::NB + b); };
   const u32 a_full = bar0 + 8 * (2 * C::ST + 2 * C::NB), o_full = a_full + 8, pv_done = a_full + 16;
-  // whose turn the exponentials of a scheduler's four warps are: tile a is through with its tile j
-  auto turn = [&](int a, int quarter) { return a_full + 24 + 8 * (4 * a + quarter); };
-  auto pair = [&](int a, int quarter) { return a_full + 24 + 64 + 8 * (4 * a + quarter); };  // the two warps that share 32 rows
   u32* tmem_slot = reinterpret_cast<u32*>(smem + C::OFF_BAR + 8 * C::BARS);
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -102,16 +100,10 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
 
   if (warp == C::WG * 4 && lane == 0) {
     for (int s = 0; s < C::ST; ++s) { bar_init(full(s), 1); bar_init(empty(s), 1); }
-    for (int b = 0; b < C::NB; ++b) { bar_init(s_full(b), 1); bar_init(p_full(b), 4 * HALVES); }
+    for (int b = 0; b < C::NB; ++b) { bar_init(s_full(b), 1); bar_init(p_full(b), 4 * C::HV); }
     bar_init(a_full, 4 * C::WG);
     bar_init(o_full, 1);
     bar_init(pv_done, 1);
-    if (C::TURNS)
-      for (int a = 0; a < 2; ++a)
-        for (int q = 0; q < 4; ++q) bar_init(turn(a, q), HALVES);
-    if (C::MODE == TC_PULL)
-      for (int a = 0; a < C::NA; ++a)
-        for (int q = 0; q < 4; ++q) bar_init(pair(a, q), 2);
     *gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -160,11 +152,12 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
         if (!ok) return;
         tc_after();
         const u32 A = tmem + C::A_COL + a * (C::DP / 2), d = tmem + (w % C::NB) * C::BT;
-        const u64 B = tc_desc(base + C::OFF_B + st * C::B_BYTES, 16);
+        const u64 B = tc_desc(base + C::OFF_B + st * C::B_BYTES, 16), As = tc_desc(base + a * C::A_BYTES, 16);
         if (leader) {
 #pragma unroll
           for (int k = 0; k < C::DP / 16; ++k)
-            if (k < ksteps) tc_mma_ta(d, A + k * 8, B + ((k >> 2) * (C::BT * 128) + (k & 3) * 32) / 16, id_s, k > 0);
+            if (k < ksteps && C::ATM) tc_mma_ta(d, A + k * 8, B + ((k >> 2) * (C::BT * 128) + (k & 3) * 32) / 16, id_s, k > 0);
+            else if (k < ksteps) tc_mma(d, As + ((k >> 2) * 16384 + (k & 3) * 32) / 16, B + ((k >> 2) * (C::BT * 128) + (k & 3) * 32) / 16, id_s, k > 0);
           tc_commit(s_full(w % C::NB));
           if (!C::SECOND && a == C::NA - 1) tc_commit(empty(st));
         }
@@ -194,13 +187,13 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
     }
   } else {
     // ------------------------------------------------ S -> P
-    const int wg = warp >> 2, quarter = warp & 3, a = wg / HALVES, half = wg % HALVES;
+    const int wg = warp >> 2, quarter = warp & 3, a = wg / C::HV, half = wg % C::HV;
     const u32 lanes = (u32)(quarter * 32) << 16;
     const int row = row0 + a * 128 + quarter * 32 + lane;
     const bool warp_live = row0 + a * 128 + quarter * 32 < p.rows_a;
     // the rows of A into TMEM: a thread its row, pairs of elements a column; zeros behind the last
     // column (nothing there may meet the zeros of B as a NaN) and row
-    for (int k = half * 32; k < ksteps * 16; k += 32 * HALVES) {
+    for (int k = half * 32; k < ksteps * 16; k += 32 * C::HV) {
       const T* from = (const T*)p.a + (i64)row * p.lda + k;
       Pack<T, 32> piece;
 #pragma unroll
@@ -212,25 +205,33 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
           for (int e = 0; e < 8; ++e) piece.v[q + e] = row < p.rows_a && k + q + e < p.D ? from[q + e] : from_float<T>(0.f);
         }
       }
-      tc_st16(tmem + C::A_COL + a * (C::DP / 2) + k / 2 + lanes, reinterpret_cast<const u32*>(piece.v));
+      if constexpr (C::ATM) {
+        tc_st16(tmem + C::A_COL + a * (C::DP / 2) + k / 2 + lanes, reinterpret_cast<const u32*>(piece.v));
+      } else {  // as a swizzled tile: 16-byte piece c of row r lies at c ^ (r & 7)
+        const int r = quarter * 32 + lane;
+        unsigned char* to = smem + a * C::A_BYTES + (k >> 6) * 16384 + r * 128;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<uint4*>(to + ((((k & 63) >> 3) + q) ^ (r & 7)) * 16) = reinterpret_cast<const uint4*>(piece.v)[q];
+      }
     }
-    tc_wait_st();
+    if (C::ATM) tc_wait_st();
+    else asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     tc_before();
     __syncwarp();
     if (lane == 0) bar_arrive(a_full);
+    // one pair in POLY by the polynomial
+    auto exponentials = [](float& lo, float& hi, int k) {
+      if (C::POLY && (k / 2) % (C::POLY ? C::POLY : 1) == C::POLY - 1) {
+        ex2_poly(lo, hi);
+      } else {
+        lo = ex2(lo);
+        hi = ex2(hi);
+      }
+    };
     float m = -INFINITY, sum = 0.f;
     const u64 c2 = join2(p.c, p.c);
     bool ok = true;
-    // The two tiles' warps on a scheduler take the exponentials in turns.  Left alone they run into
-    // step: both wait for the special-function unit while the tensor cores idle, then both wait for
-    // the tensor cores.
-    auto my_turn = [&](int j) {
-      if (C::TURNS && (a == 1 || j > 0)) ok = ok && bar_wait(turn(a ^ 1, quarter), (a == 1 ? j : j - 1) & 1, gave_up, p.err);
-    };
-    auto next_turn = [&]() {
-      __syncwarp();
-      if (C::TURNS && lane == 0) bar_arrive(turn(a, quarter));
-    };
     for (int w = a; w < items; w += C::NA) {
       const int j = w / C::NA, st = j % C::ST, b = w % C::NB;
       ok = bar_wait(s_full(b), (w / C::NB) & 1, gave_up, p.err);
@@ -253,10 +254,8 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
             part2(fma2(join2(v[4 * k], v[4 * k + 1]), c2, q.x), v[4 * k], v[4 * k + 1]);
             part2(fma2(join2(v[4 * k + 2], v[4 * k + 3]), c2, q.y), v[4 * k + 2], v[4 * k + 3]);
           }
-          my_turn(j);
 #pragma unroll
-          for (int k = 0; k < C::HC; ++k) v[k] = ex2(v[k]);
-          next_turn();
+          for (int k = 0; k < C::HC; k += 2) exponentials(v[k], v[k + 1], k);
           const int* tgt = reinterpret_cast<const int*>(meta + 4 * C::BT);
           const float* gs = reinterpret_cast<const float*>(meta + 8 * C::BT);
           bool near = false;
@@ -281,18 +280,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
             top[q] = max3(top[q], v[k], v[k + 1]);
             top[q + 1] = max3(top[q + 1], v[k + 2], v[k + 3]);
           }
-          float t = fmaxf(max3(top[0], top[1], top[2]), top[3]) * p.c;
-          if (C::MODE == TC_PULL) {
-            // one reference a row: the halves' maxima meet in shared memory (two sets, by turns, so that
-            // one barrier an item of the two warps is enough)
-            float* tops = reinterpret_cast<float*>(smem + C::OFF_TOP) + (j & 1) * (C::WG * 128) + quarter * 32 + lane;
-            tops[wg * 128] = t;
-            __syncwarp();
-            if (lane == 0) bar_arrive(pair(a, quarter));
-            ok = __all_sync(0xffffffffu, bar_wait(pair(a, quarter), j & 1, gave_up, p.err));
-            if (!ok) break;
-            t = fmaxf(t, tops[(wg ^ 1) * 128]);
-          }
+          const float t = fmaxf(max3(top[0], top[1], top[2]), top[3]) * p.c;
           const bool move = t > m + MOVE_REFERENCE;
           if (__any_sync(0xffffffffu, move)) {
             const float f = move ? (m == -INFINITY ? 0.f : ex2(m - t)) : 1.f;
@@ -304,7 +292,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
                 ok = bar_wait(pv_done, (w - 1) & 1, gave_up, p.err);
                 tc_after();
               }
-              for (int k = half * 16; k < ksteps * 16; k += 32) {
+              for (int k = 0; k < ksteps * 16; k += 16) {
                 float o[16];
                 const u32 at = tmem + C::O_COL + a * C::DP + k + lanes;
                 tc_ld16(o, at);
@@ -318,15 +306,12 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
           const float off = (float)FWD_SHIFT - (m == -INFINITY ? 0.f : m);
           const u64 off2 = join2(off, off);
           u64 add[2] = {0, 0};
-          my_turn(j);
 #pragma unroll
           for (int k = 0; k < C::HC; k += 2) {
             part2(fma2(join2(v[k], v[k + 1]), c2, off2), v[k], v[k + 1]);
-            v[k] = ex2(v[k]);
-            v[k + 1] = ex2(v[k + 1]);
+            exponentials(v[k], v[k + 1], k);
             add[(k >> 1) & 1] = add2(add[(k >> 1) & 1], join2(v[k], v[k + 1]));
           }
-          next_turn();
           float lo, hi;
           part2(add2(add[0], add[1]), lo, hi);
           sum += lo + hi;
@@ -349,30 +334,21 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
           for (int q = 0; q < C::HC / 2; q += 16) tc_st16(S + q, h + q);
           tc_wait_st();
         }
-      } else {
-        next_turn();
       }
       tc_before();
       __syncwarp();
       if (lane == 0) bar_arrive(p_full(b));
     }
     if (C::MODE == TC_STATS && row < p.rows_a && ok)
-      p.part_ms[(i64)(blockIdx.y * HALVES + half) * p.rows_a + row] = make_float2(m, sum);
-    if (C::MODE == TC_PULL) {
-      float* sums = reinterpret_cast<float*>(smem + C::OFF_TOP) + (my_tiles & 1) * (C::WG * 128) + quarter * 32 + lane;
-      sums[wg * 128] = sum;
-      __syncwarp();
-      if (lane == 0) bar_arrive(pair(a, quarter));
-      ok = ok && (!warp_live || bar_wait(pair(a, quarter), my_tiles & 1, gave_up, p.err));
-      if (half == 0 && row < p.rows_a && ok) p.part_ms[(i64)blockIdx.y * p.rows_a + row] = make_float2(m, sum + sums[(wg ^ 1) * 128]);
-    }
+      p.part_ms[(i64)(blockIdx.y * C::HV + half) * p.rows_a + row] = make_float2(m, sum);
+    if (C::MODE == TC_PULL && row < p.rows_a && ok) p.part_ms[(i64)blockIdx.y * p.rows_a + row] = make_float2(m, sum);
     if (C::SECOND && my_tiles > 0) {
       ok = ok && bar_wait(o_full, 0, gave_up, p.err);
       ok = __all_sync(0xffffffffu, ok);
       if (ok && warp_live) {
         tc_after();
         const float f = C::MODE == TC_GRAD_W ? p.out_scale * __uint_as_float(*p.top) : 1.f;
-        for (int k = half * 32; k < p.D; k += 32 * HALVES) {
+        for (int k = half * 32; k < p.D; k += 32 * C::HV) {
           float o[32];
           tc_ld32(o, tmem + C::O_COL + a * C::DP + k + lanes);
           tc_wait_ld();
@@ -555,26 +531,26 @@ static TcPlan plan_of(i64 rows_a, i64 rows_b) {
   const int s = split_count(p.groups, tiles, (i64)sm_count() * C::CTAS);
   p.per = (int)((tiles + s - 1) / s);
   p.splits = (int)((tiles + p.per - 1) / p.per);
-  p.parts = p.splits * (C::MODE == TC_STATS ? HALVES : 1);
+  p.parts = p.splits * (C::MODE == TC_STATS ? C::HV : 1);
   return p;
 }
 
-//               MODE      DP  NA NB  BT ST CTAS
-typedef TcShape<TC_STATS, 64, 2, 3, 128, 6, 1> Stats64;
-typedef TcShape<TC_STATS, 128, 2, 3, 128, 5, 1> Stats128;
-typedef TcShape<TC_STATS, 256, 2, 2, 128, 3, 1> Stats256;
-typedef TcShape<TC_STATS, 64, 1, 3, 64, 8, 2> StatsFew64;
-typedef TcShape<TC_STATS, 128, 1, 3, 64, 6, 2> StatsFew128;
-typedef TcShape<TC_PULL, 64, 2, 2, 128, 6, 1> Pull64;
-typedef TcShape<TC_PULL, 128, 2, 2, 64, 8, 1> Pull128;
-typedef TcShape<TC_PULL, 256, 1, 2, 64, 5, 1> Pull256;
-typedef TcShape<TC_PULL, 64, 1, 2, 64, 8, 2> PullFew64;
-typedef TcShape<TC_PULL, 128, 1, 1, 64, 6, 2> PullFew128;
-typedef TcShape<TC_GRAD_W, 64, 2, 2, 128, 6, 1> Grad64;
-typedef TcShape<TC_GRAD_W, 128, 2, 2, 64, 8, 1> Grad128;
-typedef TcShape<TC_GRAD_W, 256, 1, 2, 64, 5, 1> Grad256;
-typedef TcShape<TC_GRAD_W, 64, 1, 2, 64, 8, 2> GradFew64;
-typedef TcShape<TC_GRAD_W, 128, 1, 1, 64, 6, 2> GradFew128;
+//               MODE      DP  NA NB  BT ST CTAS HV ATM
+typedef TcShape<TC_STATS, 64, 2, 3, 128, 6, 1, 2, true> Stats64;
+typedef TcShape<TC_STATS, 128, 2, 3, 128, 5, 1, 2, true> Stats128;
+typedef TcShape<TC_STATS, 256, 2, 2, 128, 3, 1, 2, true> Stats256;
+typedef TcShape<TC_STATS, 64, 1, 3, 64, 8, 2, 2, true> StatsFew64;
+typedef TcShape<TC_STATS, 128, 1, 3, 64, 6, 2, 2, true> StatsFew128;
+typedef TcShape<TC_PULL, 64, 2, 2, 128, 6, 1, 1, true> Pull64;
+typedef TcShape<TC_PULL, 128, 2, 2, 128, 4, 1, 1, false> Pull128;
+typedef TcShape<TC_PULL, 256, 1, 2, 64, 5, 1, 1, true> Pull256;
+typedef TcShape<TC_PULL, 64, 1, 2, 64, 8, 2, 1, true> PullFew64;
+typedef TcShape<TC_PULL, 128, 1, 1, 64, 6, 2, 1, true> PullFew128;
+typedef TcShape<TC_GRAD_W, 64, 2, 2, 128, 6, 1, 2, true> Grad64;
+typedef TcShape<TC_GRAD_W, 128, 1, 2, 128, 4, 1, 2, true> Grad128;
+typedef TcShape<TC_GRAD_W, 256, 1, 2, 64, 5, 1, 2, true> Grad256;
+typedef TcShape<TC_GRAD_W, 64, 1, 2, 64, 8, 2, 2, true> GradFew64;
+typedef TcShape<TC_GRAD_W, 128, 1, 1, 64, 6, 2, 2, true> GradFew128;
 
 // f(shape) for the shape that the sizes ask for
 template <typename F>

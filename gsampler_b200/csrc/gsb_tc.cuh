@@ -56,6 +56,15 @@ __device__ __forceinline__ void tma_tile(u32 dst, const CUtensorMap* map, int x,
                "l"(map), "r"(x), "r"(y), "r"(plane), "r"(bar)
                : "memory");
 }
+// a tile from shared memory to the tensor; what lies outside the tensor is not written
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, int x, int y, int plane, u32 src) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x), "r"(y), "r"(plane),
+               "r"(src)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void tma_store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_copy(u32 dst, const void* src, u32 bytes, u32 bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
                "r"(bytes), "r"(bar)
@@ -121,6 +130,11 @@ __device__ __forceinline__ u32 tc_idesc(bool bf16, u32 n, bool a_across, bool b_
          ((128u >> 4) << 24);
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -147,6 +161,31 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
+  u64 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ u64 both(float v) { return join2(v, v); }
+// 2^x of two values on the multiply-add pipe, for the share of them that would otherwise queue for
+// the special-function unit (16 results a cycle and SM).  x = n + f with n the nearest integer, which
+// the addition of 1.5 2^23 leaves in the low bits (127 more makes them an exponent field); 2^f by
+// the polynomial of degree 5 that is nearest to it in relative error on [-1/2, 1/2] (weighted least
+// squares on Chebyshev points, 7.5e-8; 2.1e-7 with the roundings of its evaluation).  x below -126
+// gives 2^-126; a NaN and an infinity give NaN.  x < 128.
+__device__ __forceinline__ void ex2_poly(float& lo, float& hi) {
+  const u64 x = join2(max_nan(lo, -126.f), max_nan(hi, -126.f));
+  const u64 t = add2(x, both(12582912.f + 127.f));
+  const u64 f = fma2(add2(t, both(-12582912.f - 127.f)), both(-1.f), x);
+  u64 r = fma2(f, both(0.0013276472f), both(0.009675541f));
+  r = fma2(r, f, both(0.05550713f));
+  r = fma2(r, f, both(0.2402212f));
+  r = fma2(r, f, both(0.69314694f));
+  r = fma2(r, f, both(1.0000001f));
+  float tl, th;
+  part2(t, tl, th);
+  part2(mul2(r, join2(__uint_as_float(__float_as_uint(tl) << 23), __uint_as_float(__float_as_uint(th) << 23))), lo, hi);
 }
 template <typename T>
 __device__ __forceinline__ u32 pack2(float lo, float hi);
