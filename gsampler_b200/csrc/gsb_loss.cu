@@ -12,32 +12,54 @@
 
 namespace gsb {
 
-// One CTA: sum of the rows' losses (in 64 bits) and the number of rows that count.
-__global__ void __launch_bounds__(1024)
+// Sum of the rows' losses (in 64 bits) and the number of rows that count: CTA b adds its share to
+// part[b], or finishes when it is the only one; then one CTA adds the parts in order.
+__device__ __forceinline__ void block_total(double s, double c, double* shared, double* out_s, double* out_c) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, d);
+    c += __shfl_xor_sync(0xffffffffu, c, d);
+  }
+  if ((threadIdx.x & 31) == 0) { shared[threadIdx.x >> 5] = s; shared[32 + (threadIdx.x >> 5)] = c; }
+  __syncthreads();
+  *out_s = *out_c = 0;
+  for (int k = 0; k < (int)blockDim.x / 32; ++k) { *out_s += shared[k]; *out_c += shared[32 + k]; }
+}
+__device__ __forceinline__ void write_total(double s, double c, int mean, float* total, float* count) {
+  if (c < 1) c = 1;  // no row counts: the loss is 0, and so are the gradients
+  *total = (float)(mean ? s / c : s);
+  *count = (float)c;
+}
+__global__ void __launch_bounds__(512)
 loss_total_kernel(const float* __restrict__ loss, const i64* __restrict__ target, i64 ignore, i64 V, i64 N, int mean,
-                  float* __restrict__ total, float* __restrict__ count) {
-  __shared__ double ws[32];
-  __shared__ i64 wc[32];
-  double s = 0;
-  i64 c = 0;
-  for (i64 i = threadIdx.x; i < N; i += 1024) {
+                  double2* __restrict__ part, float* __restrict__ total, float* __restrict__ count) {
+  __shared__ double shared[64];
+  double s = 0, c = 0;
+  for (i64 i = (i64)blockIdx.x * 512 + threadIdx.x; i < N; i += (i64)gridDim.x * 512) {
     s += loss[i];
     const i64 t = target[i];
-    c += t != ignore && t >= 0 && t < V;
+    c += t != ignore && t >= 0 && t < V ? 1.0 : 0.0;
   }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-  c = warp_sum(c);
-  if ((threadIdx.x & 31) == 0) { ws[threadIdx.x >> 5] = s; wc[threadIdx.x >> 5] = c; }
-  __syncthreads();
+  double all_s, all_c;
+  block_total(s, c, shared, &all_s, &all_c);
   if (threadIdx.x == 0) {
-    s = 0;
-    c = 0;
-    for (int k = 0; k < 32; ++k) { s += ws[k]; c += wc[k]; }
-    if (c < 1) c = 1;  // no row counts: the loss is 0, and so are the gradients
-    *total = (float)(mean ? s / (double)c : s);
-    *count = (float)c;
+    if (gridDim.x == 1) write_total(all_s, all_c, mean, total, count);
+    else part[blockIdx.x] = make_double2(all_s, all_c);
   }
+}
+__global__ void __launch_bounds__(512)
+loss_total_join_kernel(const double2* __restrict__ part, int parts, int mean, float* __restrict__ total, float* __restrict__ count) {
+  __shared__ double shared[64];
+  const double2 mine = (int)threadIdx.x < parts ? part[threadIdx.x] : make_double2(0, 0);
+  double all_s, all_c;
+  block_total(mine.x, mine.y, shared, &all_s, &all_c);
+  if (threadIdx.x == 0) write_total(all_s, all_c, mean, total, count);
+}
+// up to 8192 rows take one CTA less time than a second launch
+static int total_blocks(i64 N) {
+  if (N <= 8192) return 1;
+  const i64 b = (N + 4095) / 4096;
+  return (int)(b < 512 ? b : 512);
 }
 
 // g[i] = upstream gradient of row i's loss (divided by the count for the mean), 0 where the row
@@ -67,12 +89,12 @@ static bool loss_sizes_ok(i64 N, i64 V, i64 D, i64 ldx, i64 ldw) {
          (V < 2 || ldw >= D);
 }
 
-extern "C" int gsb_linear_ce_has_pull(int dtype, int64_t N, int64_t V, int64_t D) { return tc_loss_takes(dtype, N, V, D); }
+extern "C" int gsb_linear_ce_has_pull(int dtype, int64_t V, int64_t D) { return tc_loss_takes(dtype, D) && tc_loss_pulls(V); }
 
 extern "C" size_t gsb_linear_ce_workspace_bytes(int dtype, const void* weight, int64_t ldw, int64_t N, int64_t V, int64_t D,
                                                 int want_pull) {
   if (!loss_sizes_ok(N, V, D, D, D)) return 0;
-  if (tc_loss_takes(dtype, N, V, D)) return tc_loss_workspace(N, V, D, want_pull != 0, tc_loss_packs(weight, ldw));
+  if (tc_loss_takes(dtype, D)) return tc_loss_workspace(N, V, D, want_pull != 0, tc_loss_packs(weight, ldw));
   return gemm_loss_workspace(dtype, N, V, D, tc_loss_packs(weight, ldw));
 }
 
@@ -81,7 +103,7 @@ extern "C" int gsb_linear_ce(const void* x, int dtype, int64_t ldx, int64_t N, c
                              float* pull, void* workspace, size_t workspace_bytes, int* d_err, void* cuda_stream) {
   if (!loss_sizes_ok(N, V, D, ldx, ldw) || !(scale - scale == 0.f)) return GSB_ERR_INVALID;
   if (dtype != GSB_F32 && dtype != GSB_F16 && dtype != GSB_BF16) return GSB_ERR_INVALID;
-  if (pull && !gsb_linear_ce_has_pull(dtype, N, V, D)) return GSB_ERR_UNSUPPORTED;
+  if (pull && !gsb_linear_ce_has_pull(dtype, V, D)) return GSB_ERR_UNSUPPORTED;
   if (N == 0) return GSB_OK;
   if (!x || !weight || !target || !loss || !lse2) return GSB_ERR_INVALID;
   if (!workspace || workspace_bytes < gsb_linear_ce_workspace_bytes(dtype, weight, ldw, N, V, D, pull != nullptr))
@@ -91,7 +113,7 @@ extern "C" int gsb_linear_ce(const void* x, int dtype, int64_t ldx, int64_t N, c
   a.target = (const i64*)target; a.ignore = ignore; a.scale = scale; a.loss = loss; a.lse2 = lse2;
   a.ws = workspace; a.err = d_err; a.st = (cudaStream_t)cuda_stream;
   int rc = GSB_OK;
-  if (tc_loss_takes(dtype, N, V, D))
+  if (tc_loss_takes(dtype, D))
     rc = dtype == GSB_F16 ? tc_loss_forward<__half>(a, pull) : tc_loss_forward<__nv_bfloat16>(a, pull);
   else
     rc = dtype == GSB_F32 ? gemm_loss_forward<float>(a)
@@ -101,12 +123,23 @@ extern "C" int gsb_linear_ce(const void* x, int dtype, int64_t ldx, int64_t N, c
   return GSB_OK;
 }
 
+extern "C" size_t gsb_linear_ce_total_workspace_bytes(int64_t N) { return sizeof(double2) * (size_t)total_blocks(N); }
+
 extern "C" int gsb_linear_ce_total(const float* loss, const int64_t* target, int64_t ignore, int64_t V, int64_t N,
-                                   int mean, float* total, float* count, void* cuda_stream) {
+                                   int mean, float* total, float* count, void* workspace, size_t workspace_bytes,
+                                   void* cuda_stream) {
   if (N < 0 || !total || !count || (N > 0 && (!loss || !target))) return GSB_ERR_INVALID;
+  const int blocks = total_blocks(N);
+  if (blocks > 1 && (!workspace || workspace_bytes < gsb_linear_ce_total_workspace_bytes(N))) return GSB_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)cuda_stream;
-  LaunchScope ls(KID_LOSS_JOIN, st);
-  loss_total_kernel<<<1, 1024, 0, st>>>(loss, (const i64*)target, ignore, V, N, mean, total, count);
+  {
+    LaunchScope ls(KID_LOSS_JOIN, st);
+    loss_total_kernel<<<blocks, 512, 0, st>>>(loss, (const i64*)target, ignore, V, N, mean, (double2*)workspace, total, count);
+  }
+  if (blocks > 1) {
+    LaunchScope ls(KID_LOSS_JOIN, st);
+    loss_total_join_kernel<<<1, 512, 0, st>>>((const double2*)workspace, blocks, mean, total, count);
+  }
   GSB_CUDA_OK(cudaGetLastError());
   return GSB_OK;
 }
@@ -115,14 +148,9 @@ extern "C" size_t gsb_linear_ce_grad_workspace_bytes(int dtype, const void* weig
                                                      int have_pull, int want_dx, int want_dw) {
   if (!loss_sizes_ok(N, V, D, D, D)) return 0;
   const size_t head = up256(4 * (size_t)N) + 256;
-  const bool tc = tc_loss_takes(dtype, N, V, D);
-  const bool rest_dx = want_dx && !(tc && have_pull), rest_dw = want_dw && !tc, pack = tc_loss_packs(weight, ldw);
-  size_t need = rest_dx || rest_dw ? gemm_loss_grad_workspace(dtype, N, V, D, rest_dx, rest_dw, pack) : 0;
-  if (tc && want_dw) {
-    const size_t b = tc_loss_grad_workspace(N, V, D, pack);
-    if (b > need) need = b;
-  }
-  return head + need;
+  if (!tc_loss_takes(dtype, D))
+    return head + gemm_loss_grad_workspace(dtype, N, V, D, want_dx != 0, want_dw != 0, tc_loss_packs(weight, ldw));
+  return head + tc_loss_grad_workspace(N, V, D, want_dx && !have_pull, want_dw != 0);
 }
 
 extern "C" int gsb_linear_ce_grad(const void* x, int dtype, int64_t ldx, int64_t N, const void* weight, int64_t ldw,
@@ -156,24 +184,22 @@ extern "C" int gsb_linear_ce_grad(const void* x, int dtype, int64_t ldx, int64_t
   a.x = x; a.ldx = ldx; a.N = N; a.w = weight; a.ldw = ldw; a.V = V; a.D = D;
   a.target = (const i64*)target; a.ignore = ignore; a.scale = scale; a.lse2 = const_cast<float*>(lse2);
   a.g = g; a.top = top; a.dx = dx; a.dw = dw; a.ws = ws + up256(4 * (size_t)N) + 256; a.err = d_err; a.st = st;
-  if (tc_loss_takes(dtype, N, V, D)) {
+  int rc = GSB_OK;
+  if (!tc_loss_takes(dtype, D)) {
+    rc = dtype == GSB_F32 ? gemm_loss_backward<float>(a)
+         : dtype == GSB_F16 ? gemm_loss_backward<__half>(a) : gemm_loss_backward<__nv_bfloat16>(a);
+  } else {
     const bool half = dtype == GSB_F16;
     if (a.dx && pull) {
       if (half) tc_loss_dx<__half>(a, pull);
       else tc_loss_dx<__nv_bfloat16>(a, pull);
-      a.dx = nullptr;
+      a.dx = nullptr;  // what is left below
+    } else if (a.dx) {
+      rc = half ? tc_loss_grad_x<__half>(a) : tc_loss_grad_x<__nv_bfloat16>(a);
     }
-    if (a.dw) {
-      const int rc = half ? tc_loss_grad_w<__half>(a) : tc_loss_grad_w<__nv_bfloat16>(a);
-      if (rc != GSB_OK) return rc;
-      a.dw = nullptr;
-    }
+    if (rc == GSB_OK && a.dw) rc = half ? tc_loss_grad_w<__half>(a) : tc_loss_grad_w<__nv_bfloat16>(a);
   }
-  if (a.dx || a.dw) {
-    const int rc = dtype == GSB_F32 ? gemm_loss_backward<float>(a)
-                   : dtype == GSB_F16 ? gemm_loss_backward<__half>(a) : gemm_loss_backward<__nv_bfloat16>(a);
-    if (rc != GSB_OK) return rc;
-  }
+  if (rc != GSB_OK) return rc;
   GSB_CUDA_OK(cudaGetLastError());
   return GSB_OK;
 }

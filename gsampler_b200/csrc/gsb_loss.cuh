@@ -53,10 +53,11 @@ struct LossArgs {
 };
 
 // The tensor-core form (gsb_loss_tc.cu): 16-bit types, up to 256 columns.
-bool tc_loss_takes(int dtype, i64 N, i64 V, i64 D);
+bool tc_loss_takes(int dtype, i64 D);
+bool tc_loss_pulls(i64 V);  // whether the forward pass delivers what dx is made from, or dx makes the logits again
 bool tc_loss_packs(const void* w, i64 ldw);  // whether the rows of W have to be copied for it
 size_t tc_loss_workspace(i64 N, i64 V, i64 D, bool pull, bool pack_w);
-size_t tc_loss_grad_workspace(i64 N, i64 V, i64 D, bool pack_w);
+size_t tc_loss_grad_workspace(i64 N, i64 V, i64 D, bool dx, bool dw);
 // The general form (gsb_loss_gemm.cu).
 size_t gemm_loss_workspace(int dtype, i64 N, i64 V, i64 D, bool pack_w);
 size_t gemm_loss_grad_workspace(int dtype, i64 N, i64 V, i64 D, bool dx, bool dw, bool pack_w);
@@ -72,6 +73,8 @@ template <typename T>
 int tc_loss_forward(const LossArgs& a, float* pull);
 template <typename T>
 int tc_loss_grad_w(const LossArgs& a);
+template <typename T>
+int tc_loss_grad_x(const LossArgs& a);
 template <typename T>
 void tc_loss_dx(const LossArgs& a, const float* pull);
 

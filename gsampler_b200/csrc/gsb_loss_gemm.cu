@@ -21,7 +21,7 @@ namespace gsb {
 
 enum { GM_STATS = 0, GM_PIECE = 1, GM_DX = 2, GM_DW = 3 };
 
-constexpr i64 PIECE_ELEMS = 1ll << 24;
+constexpr i64 PIECE_ELEMS = 1ll << 25;
 
 template <int MODE_, int PL_, int BN_, int ST_>
 struct GmShape {
@@ -54,6 +54,8 @@ struct GmParams {
   const i64* target;
   const u32* top;
   int v0;                   // GM_PIECE: id of the piece's first column
+  void* piece;              // GM_PIECE: [PL][M][ld_piece]
+  i64 ld_piece, plane;
   float* slab;              // GM_DX / GM_DW: [units along z][M][N]
   int add;
   int* err;
@@ -61,8 +63,7 @@ struct GmParams {
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(C::THREADS, 1)
-loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                 const __grid_constant__ CUtensorMap map_out, const GmParams p) {
+loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GmParams p) {
   extern __shared__ unsigned char smem_raw[];
   const u32 base = (smem_addr(smem_raw) + 1023) & ~1023u;
   unsigned char* smem = smem_raw + (base - smem_addr(smem_raw));
@@ -240,10 +241,10 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             v[j] = gs == 0.f ? 0.f : v[j] * gs;  // rows that do not count
           }
           const u32 out = base + C::OFF_OUT + warp * 4096;
+          const int first = m * 128 + quarter * 32;
 #pragma unroll
           for (int pl = 0; pl < C::PL; ++pl) {
-            if (lane == 0) tma_store_read();  // the tile before has left
-            __syncwarp();
+            __syncwarp();  // the plane before has been read
 #pragma unroll
             for (int j = 0; j < 64; j += 8) {
               u32 h[4];
@@ -260,9 +261,19 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                            "r"(h[2]), "r"(h[3])
                            : "memory");
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) tma_store(&map_out, col, m * 128 + quarter * 32, pl, out);
+            // eight lanes a row
+            T* to = (T*)p.piece + pl * p.plane + (i64)(first + (lane >> 3)) * p.ld_piece + col + (lane & 7) * 8;
+#pragma unroll
+            for (int r = 0; r < 32; r += 4) {
+              uint4 h;
+              const int mine = r + (lane >> 3);
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(h.x), "=r"(h.y), "=r"(h.z), "=r"(h.w)
+                           : "r"(out + mine * 128 + ((lane & 7) ^ (mine & 7)) * 16));
+              // whole pieces of 8: a row has room for them (packed_ld), and nobody reads behind its last column
+              if (first + mine < p.M && col + (lane & 7) * 8 < p.N) *reinterpret_cast<uint4*>(to + (i64)r * p.ld_piece) = h;
+            }
           }
         }
       }
@@ -317,7 +328,6 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       __syncwarp();
       if (lane == 0) bar_arrive(acc_empty(b));
     }
-    if (C::MODE == GM_PIECE && lane == 0) tma_store_done();
     if (C::MODE == GM_STATS && ok) {
       const int row = blockIdx.x * 128 + quarter * 32 + lane;
       if (row < p.M) p.part_ms[(i64)(blockIdx.y * 2 + half) * p.M + row] = make_float2(run_m, run_s);
@@ -442,21 +452,21 @@ static void make_planes(const void* src, i64 ld, i64 rows, i64 D, bool negate, c
 }
 
 template <typename T, typename C>
-static int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const GmParams& p, dim3 grid, int kid, cudaStream_t st) {
+static int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GmParams& p, dim3 grid, int kid, cudaStream_t st) {
   GSB_CUDA_OK(cudaFuncSetAttribute(loss_gemm_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
   LaunchScope ls(kid, st);
-  loss_gemm_kernel<T, C><<<grid, C::THREADS, C::BYTES, st>>>(a, b, out, p);
+  loss_gemm_kernel<T, C><<<grid, C::THREADS, C::BYTES, st>>>(a, b, p);
   return GSB_OK;
 }
 // the shape for `cols` columns of the result (dx and dW of few columns: 64 of them, with a stage more)
 template <typename T, int MODE, int PL>
-static int launch_mode(i64 cols, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out, const GmParams& p, dim3 grid, int kid, cudaStream_t st) {
+static int launch_mode(i64 cols, const CUtensorMap& a, const CUtensorMap& b, const GmParams& p, dim3 grid, int kid, cudaStream_t st) {
   if constexpr (PL == 3) {
     if constexpr (MODE == GM_DX || MODE == GM_DW)
-      if (bn_of(3, cols) == 64) return launch_gemm<T, GmShape<MODE, 3, 64, 3>>(a, b, out, p, grid, kid, st);
-    return launch_gemm<T, GmShape<MODE, 3, 128, 2>>(a, b, out, p, grid, kid, st);
+      if (bn_of(3, cols) == 64) return launch_gemm<T, GmShape<MODE, 3, 64, 3>>(a, b, p, grid, kid, st);
+    return launch_gemm<T, GmShape<MODE, 3, 128, 2>>(a, b, p, grid, kid, st);
   } else {
-    return launch_gemm<T, GmShape<MODE, 1, 256, 4>>(a, b, out, p, grid, kid, st);
+    return launch_gemm<T, GmShape<MODE, 1, 256, 4>>(a, b, p, grid, kid, st);
   }
 }
 
@@ -484,7 +494,7 @@ int gemm_loss_forward(const LossArgs& a) {
   p.c = logit_factor(a.scale);
   p.part_ms = (float2*)(ws + L.ms);
   p.err = a.err;
-  const int rc = launch_mode<T, GM_STATS, PL>(a.V, ma, mb, mb, p, dim3(p.m_tiles, L.splits), KID_LOSS, a.st);
+  const int rc = launch_mode<T, GM_STATS, PL>(a.V, ma, mb, p, dim3(p.m_tiles, L.splits), KID_LOSS, a.st);
   if (rc != GSB_OK) return rc;
   launch_loss_join<S>(a, p.part_ms, 2 * L.splits, nullptr, nullptr);
   return GSB_OK;
@@ -516,12 +526,10 @@ int gemm_loss_backward(const LossArgs& a) {
   for (i64 v0 = 0; v0 < a.V; v0 += L.cols) {
     const i64 c = v0 + L.cols < a.V ? L.cols : a.V - v0;
     const T* wv = w + v0 * ldw;
-    CUtensorMap ma, mb, mo;
+    CUtensorMap ma, mb;
     {
       const int bn = bn_wide(PL);
-      if (!tc_map(&ma, x, bf, a.N, a.D, L.ldp, PL, 64, 128) || !tc_map(&mb, wv, bf, c, a.D, ldw, PL, 64, bn, a.V) ||
-          !tc_map(&mo, piece, bf, a.N, c, ldq, PL, 64, 32))
-        return GSB_ERR_CUDA;
+      if (!tc_map(&ma, x, bf, a.N, a.D, L.ldp, PL, 64, 128) || !tc_map(&mb, wv, bf, c, a.D, ldw, PL, 64, bn, a.V)) return GSB_ERR_CUDA;
       GmParams p = {};
       p.M = (int)a.N;
       p.N = (int)c;
@@ -535,9 +543,12 @@ int gemm_loss_backward(const LossArgs& a) {
       p.target = a.target;
       p.top = a.top;
       p.v0 = (int)v0;
+      p.piece = piece;
+      p.ld_piece = ldq;
+      p.plane = a.N * ldq;
       p.err = a.err;
       const dim3 grid = units_grid(p, 1);
-      const int rc = launch_mode<T, GM_PIECE, PL>(c, ma, mb, mo, p, grid, KID_LOSS_GRAD, a.st);
+      const int rc = launch_mode<T, GM_PIECE, PL>(c, ma, mb, p, grid, KID_LOSS_GRAD, a.st);
       if (rc != GSB_OK) return rc;
     }
     if (a.dx) {
@@ -553,7 +564,7 @@ int gemm_loss_backward(const LossArgs& a) {
       p.add = v0 > 0;
       p.err = a.err;
       const dim3 grid = units_grid(p, L.dx_slabs);
-      const int rc = launch_mode<T, GM_DX, PL>(a.D, ma, mb, mb, p, grid, KID_LOSS_GRAD, a.st);
+      const int rc = launch_mode<T, GM_DX, PL>(a.D, ma, mb, p, grid, KID_LOSS_GRAD, a.st);
       if (rc != GSB_OK) return rc;
     }
     if (a.dw) {
@@ -568,7 +579,7 @@ int gemm_loss_backward(const LossArgs& a) {
       p.slab = dws;
       p.err = a.err;
       const dim3 grid = units_grid(p, L.dw_slabs);
-      const int rc = launch_mode<T, GM_DW, PL>(a.D, ma, mb, mb, p, grid, KID_LOSS_GRAD, a.st);
+      const int rc = launch_mode<T, GM_DW, PL>(a.D, ma, mb, p, grid, KID_LOSS_GRAD, a.st);
       if (rc != GSB_OK) return rc;
       LaunchScope ls(KID_LOSS_JOIN, a.st);
       loss_slabs_kernel<S><<<blocks_for(c * a.D), 256, 0, a.st>>>(dws, c * a.D, L.dw_slabs, fabsf(a.scale) * unit, a.top, nullptr, a.D,

@@ -12,6 +12,8 @@
 //             O / sum P is the expected row of W, which is all that dx needs; log2 sum P + m is
 //             the log-sum-exp.  Without a gradient for x there is no second product.
 //   dW        A = rows of W, B = rows of x.  P = g (p - target) with the known log-sum-exp.
+//   dx        (small vocabularies) A = rows of x, B = the vocabulary, P = g p (the target's row is taken off in 32 bits): making the logits
+//             once more costs less than 16 bytes of pull traffic an element of x.
 // So training costs four products of N V D multiply-adds (the logits twice, dx, dW) and no array of
 // N x V values exists anywhere.
 //
@@ -25,7 +27,7 @@
 
 namespace gsb {
 
-enum { TC_STATS = 0, TC_PULL = 1, TC_GRAD_W = 2 };
+enum { TC_STATS = 0, TC_PULL = 1, TC_GRAD_W = 2, TC_GRAD_X = 3 };
 
 // ---------------------------------------------------------------- shapes of the kernel
 // DP    columns a row may have (64, 128, 256)
@@ -48,11 +50,11 @@ struct TcShape {
   static constexpr int A_COL = NB * BT, O_COL = A_COL + (ATM ? NA * (DP / 2) : 0);
   static constexpr int USED = O_COL + (SECOND ? NA * DP : 0);
   static constexpr int COLS = USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
-  static constexpr int THREADS = WG * 128 + 64;
+  static constexpr int THREADS = WG * 128 + 64 + (MODE == TC_GRAD_W ? 32 : 0);
   static constexpr int A_BYTES = ATM ? 0 : SUBS * 128 * 128;
   static constexpr int OFF_B = NA * A_BYTES, OFF_META = OFF_B + ST * B_BYTES;
   static constexpr int OFF_BAR = OFF_META + ST * META;
-  static constexpr int BARS = 2 * ST + 2 * NB + 3;
+  static constexpr int BARS = 3 * ST + 2 * NB + 3;
   static constexpr int BYTES = OFF_BAR + 8 * BARS + 16 + 1024;  // and room to align the base
   static_assert(USED <= 512 && COLS * CTAS <= 512, "TMEM");
   static_assert(BYTES * CTAS <= 226 * 1024, "shared memory");
@@ -61,19 +63,51 @@ struct TcShape {
 };
 
 struct TcParams {
-  const void* a;            // rows of lda elements, 16-byte aligned
+  const void* a;            // rows of lda elements
   i64 lda;
+  int a_bytes;              // 16, 8, 4 or 2: what the address and step of a row are multiples of
+  u32 a_sign;               // 0x80008000 where A is taken with the other sign, else 0
   int rows_a, rows_b, D;
   int tiles_per_split;      // tiles B a CTA runs over
   float c;                  // |scale| log2 e
   const unsigned char* meta;  // TC_GRAD_W: BT * 14 bytes a tile B
+  const void* w;            // TC_GRAD_X: the vocabulary, for the targets' rows
+  i64 ldw;
+  int w_bytes;
+  const float* lse2;        // TC_GRAD_X, by row
+  const float* g;           // TC_GRAD_X
+  const i64* target;        // TC_STATS, TC_GRAD_X
+  float* hot;               // TC_STATS: [rows_a] the target's product, where the target lies in the vocabulary
   float2* part_ms;          // TC_STATS / TC_PULL: [parts][rows_a] reference and sum
   float* part_o;            // TC_PULL: [splits][rows_a][D]; TC_GRAD_W with splits: the same
-  void* out;                // TC_GRAD_W without splits: [rows_a][D]
-  const u32* top;           // TC_GRAD_W: bits of max |g|
-  float out_scale;          // |scale| 2^-GRAD_SHIFT
+  void* out;                // TC_GRAD_W without splits, TC_GRAD_X: [rows_a][D]
+  const u32* top;           // gradients: bits of max |g|
+  float out_scale;          // scale 2^-GRAD_SHIFT
   int* err;
 };
+
+// 32 elements of a row of which `left` are there (zeros behind them); rows start at multiples of `bytes`
+template <typename T>
+__device__ __forceinline__ void row_piece(Pack<T, 32>& piece, const T* from, int left, int bytes) {
+#pragma unroll
+  for (int q = 0; q < 32; q += 8) {
+    Pack<T, 8>* to = reinterpret_cast<Pack<T, 8>*>(piece.v + q);
+    if (q + 8 <= left && bytes >= 4) {
+      if (bytes == 16) {
+        to->load(from + q);
+      } else if (bytes == 8) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) reinterpret_cast<uint2*>(to)[e] = __ldg(reinterpret_cast<const uint2*>(from + q) + e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) reinterpret_cast<u32*>(to)[e] = __ldg(reinterpret_cast<const u32*>(from + q) + e);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) piece.v[q + e] = q + e < left ? from[q + e] : from_float<T>(0.f);
+    }
+  }
+}
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(C::THREADS, C::CTAS)
@@ -87,6 +121,8 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
   auto s_full = [&](int b) { return bar0 + 8 * (2 * C::ST + b); };
   auto p_full = [&](int b) { return bar0 + 8 * (2 * C::ST + C::NB + b); };
   const u32 a_full = bar0 + 8 * (2 * C::ST + 2 * C::NB), o_full = a_full + 8, pv_done = a_full + 16;
+  // a tile of B may be read: with dW, after the rows that do not count were wiped
+  auto ready = [&](int s) { return C::MODE == TC_GRAD_W ? a_full + 24 + 8 * s : full(s); };
   u32* tmem_slot = reinterpret_cast<u32*>(smem + C::OFF_BAR + 8 * C::BARS);
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -99,7 +135,11 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
   const int subs = (p.D + 63) / 64, ksteps = (p.D + 15) / 16;
 
   if (warp == C::WG * 4 && lane == 0) {
-    for (int s = 0; s < C::ST; ++s) { bar_init(full(s), 1); bar_init(empty(s), 1); }
+    for (int s = 0; s < C::ST; ++s) {
+      bar_init(full(s), 1);
+      bar_init(empty(s), 1);
+      if (C::MODE == TC_GRAD_W) bar_init(ready(s), 1);
+    }
     for (int b = 0; b < C::NB; ++b) { bar_init(s_full(b), 1); bar_init(p_full(b), 4 * C::HV); }
     bar_init(a_full, 4 * C::WG);
     bar_init(o_full, 1);
@@ -148,7 +188,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
       tc_after();
       auto product_s = [&](int w) {
         const int j = w / C::NA, a = w % C::NA, st = j % C::ST;
-        if (a == 0) ok = ok && bar_wait(full(st), (j / C::ST) & 1, gave_up, p.err);
+        if (a == 0) ok = ok && bar_wait(ready(st), (j / C::ST) & 1, gave_up, p.err);
         if (!ok) return;
         tc_after();
         const u32 A = tmem + C::A_COL + a * (C::DP / 2), d = tmem + (w % C::NB) * C::BT;
@@ -185,6 +225,27 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
       // the products that were issued end by themselves; a bounded look keeps the order when a wait gave up
       for (int k = 0; k < (1 << 16) && !bar_try(o_full, 0); ++k) __nanosleep(32);
     }
+  } else if (C::MODE == TC_GRAD_W && warp == C::WG * 4 + 2) {
+    // ------------------------------------------------ rows that do not count become zeros, whatever they hold
+    for (int j = 0; j < my_tiles; ++j) {
+      const int st = j % C::ST;
+      const bool ok = __all_sync(0xffffffffu, bar_wait(full(st), (j / C::ST) & 1, gave_up, p.err));
+      if (!ok) break;
+      const float* bias = reinterpret_cast<const float*>(smem + C::OFF_META + st * C::META);
+      bool wiped = false;
+      for (int r0 = 0; r0 < C::BT; r0 += 32) {
+        u32 dead = __ballot_sync(0xffffffffu, bias[r0 + lane] == -INFINITY);
+        wiped |= dead != 0;
+        for (; dead; dead &= dead - 1) {
+          const int r = r0 + __ffs(dead) - 1;
+          for (int k = lane; k < subs * 8; k += 32)
+            *reinterpret_cast<uint4*>(smem + C::OFF_B + st * C::B_BYTES + (k >> 3) * (C::BT * 128) + r * 128 + (k & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      if (wiped) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(ready(st));
+    }
   } else {
     // ------------------------------------------------ S -> P
     const int wg = warp >> 2, quarter = warp & 3, a = wg / C::HV, half = wg % C::HV;
@@ -193,18 +254,12 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
     const bool warp_live = row0 + a * 128 + quarter * 32 < p.rows_a;
     // the rows of A into TMEM: a thread its row, pairs of elements a column; zeros behind the last
     // column (nothing there may meet the zeros of B as a NaN) and row
+    const bool row_live = row < p.rows_a && (C::MODE != TC_GRAD_X || p.g[row < p.rows_a ? row : 0] != 0.f);
     for (int k = half * 32; k < ksteps * 16; k += 32 * C::HV) {
-      const T* from = (const T*)p.a + (i64)row * p.lda + k;
       Pack<T, 32> piece;
+      row_piece(piece, (const T*)p.a + (i64)row * p.lda + k, row_live ? p.D - k : 0, p.a_bytes);
 #pragma unroll
-      for (int q = 0; q < 32; q += 8) {
-        if (row < p.rows_a && k + q + 8 <= p.D) {
-          reinterpret_cast<Pack<T, 8>*>(piece.v + q)->load(from + q);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) piece.v[q + e] = row < p.rows_a && k + q + e < p.D ? from[q + e] : from_float<T>(0.f);
-        }
-      }
+      for (int q = 0; q < 16; ++q) reinterpret_cast<u32*>(piece.v)[q] ^= p.a_sign;
       if constexpr (C::ATM) {
         tc_st16(tmem + C::A_COL + a * (C::DP / 2) + k / 2 + lanes, reinterpret_cast<const u32*>(piece.v));
       } else {  // as a swizzled tile: 16-byte piece c of row r lies at c ^ (r & 7)
@@ -231,11 +286,23 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
     };
     float m = -INFINITY, sum = 0.f;
     const u64 c2 = join2(p.c, p.c);
+    // the target, and for dx the row's scaled gradient (an infinite bias: P = 0)
+    int hot = -1;
+    float gs = 0.f, row_bias = -INFINITY;
+    if (C::MODE == TC_STATS && row < p.rows_a) {
+      const i64 t = p.target[row];
+      if (t >= 0 && t < p.rows_b) hot = (int)t;
+    }
+    if (C::MODE == TC_GRAD_X && row_live) {
+      hot = (int)p.target[row];  // in range: the row counts
+      gs = p.g[row] / __uint_as_float(*p.top) * (float)(1 << GRAD_SHIFT);
+      row_bias = -p.lse2[row];
+    }
     bool ok = true;
     for (int w = a; w < items; w += C::NA) {
       const int j = w / C::NA, st = j % C::ST, b = w % C::NB;
       ok = bar_wait(s_full(b), (w / C::NB) & 1, gave_up, p.err);
-      if (C::META) ok = ok && bar_wait(full(st), (j / C::ST) & 1, gave_up, p.err);
+      if (C::META) ok = ok && bar_wait(ready(st), (j / C::ST) & 1, gave_up, p.err);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_after();
@@ -266,8 +333,26 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
             for (int k = 0; k < C::HC; ++k)
               if (tgt[k] == row) v[k] -= gs[k];
           }
+        } else if constexpr (C::MODE == TC_GRAD_X) {
+          const u64 bias2 = both(row_bias), gs2 = both(gs);
+#pragma unroll
+          for (int k = 0; k < C::HC; k += 2) {
+            part2(fma2(join2(v[k], v[k + 1]), c2, bias2), v[k], v[k + 1]);
+            exponentials(v[k], v[k + 1], k);
+            part2(mul2(join2(v[k], v[k + 1]), gs2), v[k], v[k + 1]);
+          }
         } else {
           const int col0 = (t0 + j) * C::BT + half * C::HC;
+          if (C::MODE == TC_STATS) {
+            const int at = hot - col0;
+            if (__any_sync(0xffffffffu, (u32)at < (u32)C::HC)) {  // the target's product, on its way past
+              float mine = 0.f;
+#pragma unroll
+              for (int k = 0; k < C::HC; ++k)
+                if (k == at) mine = v[k];
+              if ((u32)at < (u32)C::HC && row < p.rows_a) p.hot[row] = mine;
+            }
+          }
           if (col0 + C::HC > p.rows_b) {
 #pragma unroll
             for (int k = 0; k < C::HC; ++k)
@@ -347,13 +432,20 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
       ok = __all_sync(0xffffffffu, ok);
       if (ok && warp_live) {
         tc_after();
-        const float f = C::MODE == TC_GRAD_W ? p.out_scale * __uint_as_float(*p.top) : 1.f;
+        const float f = C::MODE == TC_PULL ? 1.f : p.out_scale * __uint_as_float(*p.top);
         for (int k = half * 32; k < p.D; k += 32 * C::HV) {
           float o[32];
           tc_ld32(o, tmem + C::O_COL + a * C::DP + k + lanes);
           tc_wait_ld();
           if (row < p.rows_a) {
-            const bool slab = C::MODE == TC_PULL || gridDim.y > 1;
+            const bool slab = C::MODE == TC_PULL || (C::MODE == TC_GRAD_W && gridDim.y > 1);
+            if (C::MODE == TC_GRAD_X) {
+              // the target's own row, taken off in 32 bits; a row that does not count is zero
+              Pack<T, 32> wt;
+              row_piece(wt, (const T*)p.w + (i64)(hot < 0 ? 0 : hot) * p.ldw + k, row_live ? p.D - k : 0, p.w_bytes);
+#pragma unroll
+              for (int q = 0; q < 32; ++q) o[q] = row_live ? fmaf(-gs, to_float(wt.v[q]), o[q]) : 0.f;
+            }
             if (slab) {
               float* to = p.part_o + ((i64)blockIdx.y * p.rows_a + row) * p.D + k;
               if ((p.D & 3) == 0) {
@@ -367,16 +459,25 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
               }
             } else {
               T* to = (T*)p.out + (i64)row * p.D + k;
+              u32 h[16];
+#pragma unroll
+              for (int q = 0; q < 16; ++q) h[q] = pack2<T>(o[2 * q] * f, o[2 * q + 1] * f);
               if ((p.D & 7) == 0) {
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                  if (k + 8 * q < p.D)
-                    reinterpret_cast<uint4*>(to)[q] = make_uint4(pack2<T>(o[8 * q] * f, o[8 * q + 1] * f), pack2<T>(o[8 * q + 2] * f, o[8 * q + 3] * f),
-                                                                 pack2<T>(o[8 * q + 4] * f, o[8 * q + 5] * f), pack2<T>(o[8 * q + 6] * f, o[8 * q + 7] * f));
+                  if (k + 8 * q < p.D) reinterpret_cast<uint4*>(to)[q] = make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]);
+              } else if ((p.D & 3) == 0) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                  if (k + 4 * q < p.D) reinterpret_cast<uint2*>(to)[q] = make_uint2(h[2 * q], h[2 * q + 1]);
+              } else if ((p.D & 1) == 0) {
+#pragma unroll
+                for (int q = 0; q < 16; ++q)
+                  if (k + 2 * q < p.D) reinterpret_cast<u32*>(to)[q] = h[q];
               } else {
 #pragma unroll
                 for (int q = 0; q < 32; ++q)
-                  if (k + q < p.D) to[q] = from_float<T>(o[q] * f);
+                  if (k + q < p.D) to[q] = reinterpret_cast<const T*>(h)[q];
               }
             }
           }
@@ -393,26 +494,18 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
 }
 
 // ---------------------------------------------------------------- preparation and joins
-// dst[r, :] = +-src[r, :] with rows of ldp elements (16-byte multiples, zeros behind D); rows whose
-// g is zero become zeros, so that nothing they hold reaches a product.
+// dst[r, :] = src[r, :] with rows of ldp elements (16-byte multiples, zeros behind D), for a matrix
+// whose address or row step TMA does not take
 template <typename T>
-__global__ void loss_pack_kernel(const T* __restrict__ src, i64 ld, i64 rows, int D, int ldp, bool negate,
-                                 const float* __restrict__ g, T* __restrict__ dst) {
+__global__ void loss_pack_kernel(const T* __restrict__ src, i64 ld, i64 rows, int D, int ldp, T* __restrict__ dst) {
   const int chunks = ldp / 8;
   const i64 total = rows * chunks;
   for (i64 e = (i64)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (i64)gridDim.x * blockDim.x) {
     const i64 r = e / chunks;
     const int c = (int)(e - r * chunks) * 8;
-    const bool live = !g || g[r] != 0.f;
     Pack<T, 8> v;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      v.v[q] = from_float<T>(0.f);
-      if (live && c + q < D) {
-        v.v[q] = src[r * ld + c + q];
-        if (negate) v.v[q] = -v.v[q];
-      }
-    }
+    for (int q = 0; q < 8; ++q) v.v[q] = c + q < D ? src[r * ld + c + q] : from_float<T>(0.f);
     v.store(dst + r * ldp + c);
   }
 }
@@ -442,7 +535,47 @@ __global__ void loss_meta_kernel(const float* __restrict__ lse2, const i64* __re
   reinterpret_cast<unsigned short*>(tile + 12 * BT)[k] = (unsigned short)sign;
 }
 
-// A warp per row: joins the parts' statistics (and pulls), adds the target's logit.
+// The statistics of a row's parts joined: the log-sum-exp in base 2 (of values held at 2^FWD_SHIFT).
+__device__ __forceinline__ float join_parts(const float2* __restrict__ part, int parts, i64 N, i64 r, int first, int step, float& m, float& s) {
+  m = -INFINITY;
+  for (int k = first; k < parts; k += step) m = max_nan(m, part[(i64)k * N + r].x);
+  if (step == 32) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+  }
+  s = 0.f;
+  for (int k = first; k < parts; k += step) {
+    const float2 q = part[(i64)k * N + r];
+    // a part without a reference has either no finite logit (sum 0) or a NaN
+    s += q.x == -INFINITY ? q.y : q.y * exp2f(q.x - m);
+  }
+  if (step == 32) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  }
+  return m - (float)FWD_SHIFT + log2f(s);
+}
+constexpr float LN2 = 0.6931471805599453f;
+
+// Losses from the parts and the targets' products that went past (hot): a thread a row, or a warp
+// where there are many parts.
+__global__ void __launch_bounds__(256)
+loss_finish_kernel(const float2* __restrict__ part, int parts, int lanes, const float* __restrict__ hot, i64 N, i64 V, float scale,
+                   const i64* __restrict__ target, i64 ignore, float* __restrict__ loss, float* __restrict__ lse2, int* err) {
+  const i64 e = (i64)blockIdx.x * blockDim.x + threadIdx.x;
+  const i64 r = lanes == 32 ? e >> 5 : e;
+  if (r >= N) return;
+  float m, s;
+  const float total = join_parts(part, parts, N, r, lanes == 32 ? (int)(e & 31) : 0, lanes, m, s);
+  if (lanes == 32 && (e & 31) != 0) return;
+  const i64 t = target[r];
+  const bool counts = t != ignore && t >= 0 && t < V;
+  if (t != ignore && !counts) raise(err, ERRBIT_BAD_INPUT);
+  lse2[r] = total;
+  loss[r] = counts ? total * LN2 - hot[r] * scale : 0.f;
+}
+
+// A warp per row: joins the parts' statistics (and pulls), makes the target's logit.
 //   pull_i = sum_j p_ij w_j - w_{t_i}      (zeros for a row that does not count)
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -452,19 +585,8 @@ loss_join_kernel(const float2* __restrict__ part, int parts, const float* __rest
   const i64 r = ((i64)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (r >= N) return;
-  float m = -INFINITY;
-  for (int k = lane; k < parts; k += 32) m = max_nan(m, part[(i64)k * N + r].x);
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
-  float s = 0.f;
-  for (int k = lane; k < parts; k += 32) {
-    const float2 q = part[(i64)k * N + r];
-    // a part without a reference has either no finite logit (sum 0) or a NaN
-    s += q.x == -INFINITY ? q.y : q.y * exp2f(q.x - m);
-  }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-  const float total = m - (float)FWD_SHIFT + log2f(s);
+  float m, s;
+  const float total = join_parts(part, parts, N, r, lane, 32, m, s);
   const i64 t = target[r];
   const bool counts = t != ignore && t >= 0 && t < V;
   if (t != ignore && !counts && lane == 0) raise(err, ERRBIT_BAD_INPUT);
@@ -475,7 +597,7 @@ loss_join_kernel(const float2* __restrict__ part, int parts, const float* __rest
   for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
   if (lane == 0) {
     lse2[r] = total;
-    loss[r] = counts ? total * 0.6931471805599453f - dot * scale : 0.f;
+    loss[r] = counts ? total * LN2 - dot * scale : 0.f;
   }
   if (pull) {
     const float inv = 1.f / s;
@@ -516,8 +638,6 @@ struct TcPlan {
   int NA, BT, ctas, splits, per, parts;
   i64 groups;
 };
-// Few rows on the streaming side's partner make the pass a stream of B (forward, N <= 128) or of A (dW, N <= 256):
-// then two small CTAs an SM overlap one's loads with the other's products.  Otherwise one large CTA.
 template <typename C>
 static TcPlan plan_of(i64 rows_a, i64 rows_b) {
   TcPlan p;
@@ -541,56 +661,64 @@ typedef TcShape<TC_STATS, 128, 2, 3, 128, 5, 1, 2, true> Stats128;
 typedef TcShape<TC_STATS, 256, 2, 2, 128, 3, 1, 2, true> Stats256;
 typedef TcShape<TC_STATS, 64, 1, 3, 64, 8, 2, 2, true> StatsFew64;
 typedef TcShape<TC_STATS, 128, 1, 3, 64, 6, 2, 2, true> StatsFew128;
+typedef TcShape<TC_STATS, 256, 1, 2, 64, 3, 2, 2, true> StatsFew256;
 typedef TcShape<TC_PULL, 64, 2, 2, 128, 6, 1, 1, true> Pull64;
 typedef TcShape<TC_PULL, 128, 2, 2, 128, 4, 1, 1, false> Pull128;
 typedef TcShape<TC_PULL, 256, 1, 2, 64, 5, 1, 1, true> Pull256;
 typedef TcShape<TC_PULL, 64, 1, 2, 64, 8, 2, 1, true> PullFew64;
 typedef TcShape<TC_PULL, 128, 1, 1, 64, 6, 2, 1, true> PullFew128;
+typedef TcShape<TC_GRAD_X, 64, 1, 2, 64, 4, 2, 2, true> GradX64;
+typedef TcShape<TC_GRAD_X, 128, 1, 1, 64, 4, 2, 2, true> GradX128;
+typedef TcShape<TC_GRAD_X, 256, 1, 2, 64, 3, 1, 2, true> GradX256;
 typedef TcShape<TC_GRAD_W, 64, 2, 2, 128, 6, 1, 2, true> Grad64;
 typedef TcShape<TC_GRAD_W, 128, 1, 2, 128, 4, 1, 2, true> Grad128;
 typedef TcShape<TC_GRAD_W, 256, 1, 2, 64, 5, 1, 2, true> Grad256;
 typedef TcShape<TC_GRAD_W, 64, 1, 2, 64, 8, 2, 2, true> GradFew64;
 typedef TcShape<TC_GRAD_W, 128, 1, 1, 64, 6, 2, 2, true> GradFew128;
 
-// f(shape) for the shape that the sizes ask for
+// A vocabulary of up to this many rows: dx by making the logits again (2 V multiply-adds an element of
+// x more at 1.3 PFLOP/s, against writing and reading 16 bytes of pull at 5 TB/s: equal near 2080).
+constexpr i64 SMALL_V = 2048;
+
+// f(shape) for the shape that the sizes ask for.  Where the pass is a stream of loads or stores (few
+// rows against the vocabulary; a small vocabulary under many rows), two small CTAs an SM overlap one's
+// loads with the other's products; else one large CTA keeps the tensor cores busier.  dW, 1024 x
+// 232965 x 112: 0.154 ms with two, 0.182 with one; 8192 x 300000 x 128: 1.043 and 0.949.
 template <typename F>
-static auto with_shape(int mode, i64 N, i64 D, F f) {
+static auto with_shape(int mode, i64 N, i64 V, i64 D, F f) {
   if (mode == TC_STATS) {
-    if (D > 128) return f(Stats256());
-    if (N <= 128) return D > 64 ? f(StatsFew128()) : f(StatsFew64());
-    return D > 64 ? f(Stats128()) : f(Stats64());
+    if (N <= 128 || V <= SMALL_V) return D > 128 ? f(StatsFew256()) : D > 64 ? f(StatsFew128()) : f(StatsFew64());
+    return D > 128 ? f(Stats256()) : D > 64 ? f(Stats128()) : f(Stats64());
   }
   if (mode == TC_PULL) {
     if (D > 128) return f(Pull256());
     if (N <= 128) return D > 64 ? f(PullFew128()) : f(PullFew64());
     return D > 64 ? f(Pull128()) : f(Pull64());
   }
+  if (mode == TC_GRAD_X) return D > 128 ? f(GradX256()) : D > 64 ? f(GradX128()) : f(GradX64());
   if (D > 128) return f(Grad256());
-  if (N <= 256) return D > 64 ? f(GradFew128()) : f(GradFew64());
+  if (N <= 2048) return D > 64 ? f(GradFew128()) : f(GradFew64());
   return D > 64 ? f(Grad128()) : f(Grad64());
 }
 
 static TcPlan tc_plan(int mode, i64 N, i64 V, i64 D) {
-  return with_shape(mode, N, D, [&](auto shape) {
+  return with_shape(mode, N, V, D, [&](auto shape) {
     return mode == TC_GRAD_W ? plan_of<decltype(shape)>(V, N) : plan_of<decltype(shape)>(N, V);
   });
 }
 
-bool tc_loss_takes(int dtype, i64 N, i64 V, i64 D) {
-  (void)N;
-  (void)V;
-  return dtype != GSB_F32 && D <= 256;
-}
+bool tc_loss_takes(int dtype, i64 D) { return dtype != GSB_F32 && D <= 256; }
+bool tc_loss_pulls(i64 V) { return V > SMALL_V; }
 
-struct TcFwdLayout { size_t ms, o, x, w, bytes; };
+struct TcFwdLayout { size_t ms, hot, o, w, bytes; };
 static TcFwdLayout fwd_layout(i64 N, i64 V, i64 D, bool pull) {
   TcFwdLayout L;
   size_t o = 0;
   auto take = [&](size_t b) { const size_t at = o; o += up256(b); return at; };
   const TcPlan p = tc_plan(pull ? TC_PULL : TC_STATS, N, V, D);
   L.ms = take(8 * (size_t)p.parts * N);
+  L.hot = take(pull ? 0 : 4 * (size_t)N);
   L.o = take(pull ? 4 * (size_t)p.splits * N * D : 0);
-  L.x = take(2 * (size_t)N * packed_ld(D));
   // whether the rows of W have to be copied depends on its address and row step
   L.w = take(2 * (size_t)V * packed_ld(D));
   L.bytes = o;
@@ -601,31 +729,31 @@ size_t tc_loss_workspace(i64 N, i64 V, i64 D, bool pull, bool pack_w) {
   return pack_w ? L.bytes : L.w;
 }
 
-struct TcGradLayout { size_t meta, x, slab, w, bytes; };
-static TcGradLayout grad_layout(i64 N, i64 V, i64 D) {
+struct TcGradLayout { size_t meta, slab, x, w, bytes; };
+static TcGradLayout grad_layout(i64 N, i64 V, i64 D, bool dx, bool dw) {
   TcGradLayout L;
   size_t o = 0;
   auto take = [&](size_t b) { const size_t at = o; o += up256(b); return at; };
   const TcPlan p = tc_plan(TC_GRAD_W, N, V, D);
-  L.meta = take((size_t)((N + p.BT - 1) / p.BT) * p.BT * 14);
-  L.x = take(2 * (size_t)N * packed_ld(D));
-  L.slab = take(p.splits > 1 ? 4 * (size_t)p.splits * V * D : 0);
-  L.w = take(2 * (size_t)V * packed_ld(D));
+  L.meta = take(dw ? (size_t)((N + p.BT - 1) / p.BT) * p.BT * 14 : 0);
+  L.slab = take(dw && p.splits > 1 ? 4 * (size_t)p.splits * V * D : 0);
+  L.x = take(dw ? 2 * (size_t)N * packed_ld(D) : 0);
+  L.w = take(dx ? 2 * (size_t)V * packed_ld(D) : 0);
   L.bytes = o;
   return L;
 }
-size_t tc_loss_grad_workspace(i64 N, i64 V, i64 D, bool pack_w) {
-  const TcGradLayout L = grad_layout(N, V, D);
-  return pack_w ? L.bytes : L.w;
-}
+size_t tc_loss_grad_workspace(i64 N, i64 V, i64 D, bool dx, bool dw) { return grad_layout(N, V, D, dx, dw).bytes; }
 bool tc_loss_packs(const void* w, i64 ldw) { return !tma_ready(w, ldw); }
 
 template <typename T>
-static const T* pack_rows(const void* src, i64 ld, i64 rows, i64 D, bool negate, const float* g, void* dst, cudaStream_t st) {
+static const T* pack_rows(const T* src, i64 ld, i64 rows, i64 D, void* dst, cudaStream_t st) {
   LaunchScope ls(KID_LOSS_JOIN, st);
-  loss_pack_kernel<T><<<blocks_for(rows * packed_ld(D) / 8), 256, 0, st>>>((const T*)src, ld, rows, (int)D, (int)packed_ld(D), negate, g,
-                                                                          (T*)dst);
+  loss_pack_kernel<T><<<blocks_for(rows * packed_ld(D) / 8), 256, 0, st>>>(src, ld, rows, (int)D, (int)packed_ld(D), (T*)dst);
   return (const T*)dst;
+}
+static int row_bytes(const void* p, i64 ld) {
+  const uintptr_t m = (uintptr_t)p | (uintptr_t)(ld * 2);
+  return m & 2 ? 2 : m & 4 ? 4 : m & 8 ? 8 : 16;
 }
 
 template <typename T, typename C>
@@ -644,76 +772,101 @@ void launch_loss_join(const LossArgs& a, const float2* part_ms, int parts, const
                                                             (int)a.D, a.scale, a.target, a.ignore, a.loss, a.lse2, pull, a.err);
 }
 
+// what the forward pass and both gradients have in common
+template <typename T>
+static TcParams base_params(const LossArgs& a, const TcPlan& plan, bool vocabulary_side) {
+  TcParams p = {};
+  p.a = vocabulary_side ? a.w : a.x;
+  p.lda = vocabulary_side ? a.ldw : a.ldx;
+  p.a_bytes = row_bytes(p.a, p.lda);
+  // l = |scale| (+-A) . B: the running maximum needs a factor that is not negative
+  p.a_sign = a.scale < 0.f ? 0x80008000u : 0u;
+  p.rows_a = (int)(vocabulary_side ? a.V : a.N);
+  p.rows_b = (int)(vocabulary_side ? a.N : a.V);
+  p.D = (int)a.D;
+  p.tiles_per_split = plan.per;
+  p.c = logit_factor(a.scale);
+  p.target = a.target;
+  p.lse2 = a.lse2;
+  p.g = a.g;
+  p.top = a.top;
+  p.out_scale = a.scale / (float)(1 << GRAD_SHIFT);
+  p.err = a.err;
+  return p;
+}
+// the map of the streamed matrix; rows that TMA does not take as they lie are copied to `copy` first
+template <typename T>
+static bool stream_map(CUtensorMap* map, const void* src, i64 ld, i64 rows, i64 D, int box_rows, void* copy, cudaStream_t st) {
+  if (!tma_ready(src, ld)) { src = pack_rows<T>((const T*)src, ld, rows, D, copy, st); ld = packed_ld(D); }
+  return tc_map(map, src, IsBf16<T>::value, rows, D, ld, 1, 64, box_rows);
+}
+
 template <typename T>
 int tc_loss_forward(const LossArgs& a, float* pull) {
   const int mode = pull ? TC_PULL : TC_STATS;
   const TcPlan plan = tc_plan(mode, a.N, a.V, a.D);
   const TcFwdLayout L = fwd_layout(a.N, a.V, a.D, pull != nullptr);
   char* ws = (char*)a.ws;
-  // l = |scale| (+-x) . w: the running maximum needs a factor that is not negative
-  const bool negate = a.scale < 0.f;
-  const T* x = (const T*)a.x;
-  const T* w = (const T*)a.w;
-  i64 ldx = a.ldx, ldw = a.ldw;
-  if (negate || !tma_ready(x, ldx)) { x = pack_rows<T>(x, ldx, a.N, a.D, negate, nullptr, ws + L.x, a.st); ldx = packed_ld(a.D); }
-  if (!tma_ready(w, ldw)) { w = pack_rows<T>(w, ldw, a.V, a.D, false, nullptr, ws + L.w, a.st); ldw = packed_ld(a.D); }
   CUtensorMap mb;
-  if (!tc_map(&mb, w, IsBf16<T>::value, a.V, a.D, ldw, 1, 64, plan.BT)) return GSB_ERR_CUDA;
-  TcParams p = {};
-  p.a = x;
-  p.lda = ldx;
-  p.rows_a = (int)a.N;
-  p.rows_b = (int)a.V;
-  p.D = (int)a.D;
-  p.tiles_per_split = plan.per;
-  p.c = logit_factor(a.scale);
+  if (!stream_map<T>(&mb, a.w, a.ldw, a.V, a.D, plan.BT, ws + L.w, a.st)) return GSB_ERR_CUDA;
+  TcParams p = base_params<T>(a, plan, false);
   p.part_ms = (float2*)(ws + L.ms);
   p.part_o = (float*)(ws + L.o);
-  p.err = a.err;
-  const int rc = with_shape(mode, a.N, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS, a.st); });
+  p.hot = (float*)(ws + L.hot);
+  const int rc = with_shape(mode, a.N, a.V, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS, a.st); });
   if (rc != GSB_OK) return rc;
-  launch_loss_join<T>(a, p.part_ms, plan.parts, p.part_o, pull);
+  if (pull) {
+    launch_loss_join<T>(a, p.part_ms, plan.parts, p.part_o, pull);
+    return GSB_OK;
+  }
+  const int lanes = plan.parts > 8 ? 32 : 1;
+  LaunchScope ls(KID_LOSS_JOIN, a.st);
+  // hot holds products of +-x; loss takes them times |scale|
+  loss_finish_kernel<<<ceil_div_i(a.N * lanes, 256), 256, 0, a.st>>>(p.part_ms, plan.parts, lanes, p.hot, a.N, a.V, fabsf(a.scale), a.target,
+                                                                    a.ignore, a.loss, a.lse2, a.err);
   return GSB_OK;
 }
 
 template <typename T>
 int tc_loss_grad_w(const LossArgs& a) {
   const TcPlan plan = tc_plan(TC_GRAD_W, a.N, a.V, a.D);
-  const TcGradLayout L = grad_layout(a.N, a.V, a.D);
+  const TcGradLayout L = grad_layout(a.N, a.V, a.D, a.dx != nullptr, true);
   char* ws = (char*)a.ws;
-  const T* x = pack_rows<T>(a.x, a.ldx, a.N, a.D, a.scale < 0.f, a.g, ws + L.x, a.st);
-  const T* w = (const T*)a.w;
-  i64 ldw = a.ldw;
-  if (!tma_ready(w, ldw)) { w = pack_rows<T>(w, ldw, a.V, a.D, false, nullptr, ws + L.w, a.st); ldw = packed_ld(a.D); }
   {
     const i64 npad = (a.N + plan.BT - 1) / plan.BT * plan.BT;
     LaunchScope ls(KID_LOSS_JOIN, a.st);
     loss_meta_kernel<<<ceil_div_i(npad, 256), 256, 0, a.st>>>(a.lse2, a.target, a.g, a.top, a.N, npad, plan.BT, (unsigned char*)(ws + L.meta));
   }
   CUtensorMap mb;
-  if (!tc_map(&mb, x, IsBf16<T>::value, a.N, a.D, packed_ld(a.D), 1, 64, plan.BT))
-    return GSB_ERR_CUDA;
-  TcParams p = {};
-  p.a = w;
-  p.lda = ldw;
-  p.rows_a = (int)a.V;
-  p.rows_b = (int)a.N;
-  p.D = (int)a.D;
-  p.tiles_per_split = plan.per;
-  p.c = logit_factor(a.scale);
+  if (!stream_map<T>(&mb, a.x, a.ldx, a.N, a.D, plan.BT, ws + L.x, a.st)) return GSB_ERR_CUDA;
+  TcParams p = base_params<T>(a, plan, true);
   p.meta = (const unsigned char*)(ws + L.meta);
   p.part_o = (float*)(ws + L.slab);
   p.out = a.dw;
-  p.top = a.top;
-  p.out_scale = fabsf(a.scale) / (float)(1 << GRAD_SHIFT);
-  p.err = a.err;
-  const int rc = with_shape(TC_GRAD_W, a.N, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS_GRAD, a.st); });
+  const int rc = with_shape(TC_GRAD_W, a.N, a.V, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS_GRAD, a.st); });
   if (rc != GSB_OK) return rc;
   if (plan.splits > 1) {
     LaunchScope ls(KID_LOSS_JOIN, a.st);
     loss_join_dw_kernel<T><<<blocks_for(a.V * a.D), 256, 0, a.st>>>(p.part_o, a.V * a.D, plan.splits, (T*)a.dw);
   }
   return GSB_OK;
+}
+
+// dx of a small vocabulary
+template <typename T>
+int tc_loss_grad_x(const LossArgs& a) {
+  TcPlan plan = tc_plan(TC_GRAD_X, a.N, a.V, a.D);
+  plan.splits = 1;  // a CTA sees the whole vocabulary
+  plan.per = (int)((a.V + plan.BT - 1) / plan.BT);
+  const TcGradLayout L = grad_layout(a.N, a.V, a.D, true, a.dw != nullptr);
+  CUtensorMap mb;
+  if (!stream_map<T>(&mb, a.w, a.ldw, a.V, a.D, plan.BT, (char*)a.ws + L.w, a.st)) return GSB_ERR_CUDA;
+  TcParams p = base_params<T>(a, plan, false);
+  p.w = a.w;
+  p.ldw = a.ldw;
+  p.w_bytes = row_bytes(a.w, a.ldw);
+  p.out = a.dx;
+  return with_shape(TC_GRAD_X, a.N, a.V, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS_GRAD, a.st); });
 }
 
 template <typename T>
@@ -729,6 +882,8 @@ template int tc_loss_forward<__half>(const LossArgs&, float*);
 template int tc_loss_forward<__nv_bfloat16>(const LossArgs&, float*);
 template int tc_loss_grad_w<__half>(const LossArgs&);
 template int tc_loss_grad_w<__nv_bfloat16>(const LossArgs&);
+template int tc_loss_grad_x<__half>(const LossArgs&);
+template int tc_loss_grad_x<__nv_bfloat16>(const LossArgs&);
 template void tc_loss_dx<__half>(const LossArgs&, const float*);
 template void tc_loss_dx<__nv_bfloat16>(const LossArgs&, const float*);
 

@@ -56,15 +56,6 @@ __device__ __forceinline__ void tma_tile(u32 dst, const CUtensorMap* map, int x,
                "l"(map), "r"(x), "r"(y), "r"(plane), "r"(bar)
                : "memory");
 }
-// a tile from shared memory to the tensor; what lies outside the tensor is not written
-__device__ __forceinline__ void tma_store(const CUtensorMap* map, int x, int y, int plane, u32 src) {
-  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x), "r"(y), "r"(plane),
-               "r"(src)
-               : "memory");
-  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-}
-__device__ __forceinline__ void tma_store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void tma_store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_copy(u32 dst, const void* src, u32 bytes, u32 bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
                "r"(bytes), "r"(bar)

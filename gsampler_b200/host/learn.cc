@@ -174,7 +174,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> LinearCrossEntropy(torch
   const int64_t N = x.size(0), V = weight.size(0), D = x.size(1);
   auto f32 = x.options().dtype(torch::kFloat32);
   auto loss = torch::empty({N}, f32), lse2 = torch::empty({N}, f32);
-  const bool want_pull = want_dx && gsb_linear_ce_has_pull(dt, N, V, D);
+  const bool want_pull = want_dx && gsb_linear_ce_has_pull(dt, V, D);
   auto pull = torch::empty(want_pull ? std::vector<int64_t>{N, D} : std::vector<int64_t>{0}, f32);
   auto ws = NewWorkspace(gsb_linear_ce_workspace_bytes(dt, weight.data_ptr(), RowStep(weight), N, V, D, want_pull), x.device());
   CheckStatus(gsb_linear_ce(x.data_ptr(), dt, RowStep(x), N, weight.data_ptr(), RowStep(weight), V, D,
@@ -194,8 +194,10 @@ std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyTotal(torch::Tensor l
   c10::cuda::CUDAGuard guard(loss.device());
   target = target.contiguous();
   auto total = torch::empty({}, loss.options()), count = torch::empty({}, loss.options());
+  auto ws = NewWorkspace(gsb_linear_ce_total_workspace_bytes(loss.numel()), loss.device());
   CheckStatus(gsb_linear_ce_total(loss.data_ptr<float>(), target.data_ptr<int64_t>(), ignore, vocabulary, loss.numel(),
-                                  mean, total.data_ptr<float>(), count.data_ptr<float>(), CurrentStream()),
+                                  mean, total.data_ptr<float>(), count.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(),
+                                  CurrentStream()),
               "linear_ce_total");
   return {total, count};
 }

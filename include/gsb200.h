@@ -278,18 +278,20 @@ GSB_API int gsb_dropout(const void* x, int dtype, int64_t n, double p, uint64_t 
  * count, 0 when there are none) of the rows' losses, *count = max(that number, 1).
  * gsb_linear_ce_grad: dx[N, D] and / or dw[V, D] (either may be NULL) from the
  * upstream gradient: upstream[N] when per_row, else one value, divided by *count
- * when count is given.  Sums are made in an order that depends on the sizes
- * alone.  N, V <= 2^30.  A workspace is sized for the device that is current. */
+ * when count is given.  Sums are made in an order that depends on the sizes and
+ * on which results are asked for, nothing else.  N, V <= 2^30.  A workspace is sized for the device that is current. */
 #define GSB_LOSS_MAX_D 65536
-GSB_API int gsb_linear_ce_has_pull(int dtype, int64_t N, int64_t V, int64_t D);
+GSB_API int gsb_linear_ce_has_pull(int dtype, int64_t V, int64_t D);
 GSB_API size_t gsb_linear_ce_workspace_bytes(int dtype, const void* weight, int64_t ldw, int64_t N, int64_t V,
                                              int64_t D, int want_pull);
 GSB_API int gsb_linear_ce(const void* x, int dtype, int64_t ldx, int64_t N, const void* weight, int64_t ldw,
                           int64_t V, int64_t D, const int64_t* target, int64_t ignore, float scale, float* loss,
                           float* lse2, float* pull, void* workspace, size_t workspace_bytes, int* d_err,
                           void* cuda_stream);
+GSB_API size_t gsb_linear_ce_total_workspace_bytes(int64_t N);
 GSB_API int gsb_linear_ce_total(const float* loss, const int64_t* target, int64_t ignore, int64_t V, int64_t N,
-                                int mean, float* total, float* count, void* cuda_stream);
+                                int mean, float* total, float* count, void* workspace, size_t workspace_bytes,
+                                void* cuda_stream);
 GSB_API size_t gsb_linear_ce_grad_workspace_bytes(int dtype, const void* weight, int64_t ldw, int64_t N, int64_t V,
                                                   int64_t D, int have_pull, int want_dx, int want_dw);
 GSB_API int gsb_linear_ce_grad(const void* x, int dtype, int64_t ldx, int64_t N, const void* weight, int64_t ldw,

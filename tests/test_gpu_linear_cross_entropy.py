@@ -101,7 +101,9 @@ def check(gsb, x, w, t, scale=1.0, reduction="mean", up=None):
 
 
 SIZES = [(1, 1, 1), (1, 2, 16), (3, 47, 24), (1, 1000, 128), (2, 129, 64), (127, 128, 100), (128, 257, 128), (129, 255, 65),
-         (130, 300, 256), (257, 1000, 33), (300, 47, 200), (513, 2000, 128), (700, 3, 256), (64, 4099, 72), (40, 700, 300)]
+         (130, 300, 256), (257, 1000, 33), (300, 47, 200), (513, 2000, 128), (700, 3, 256), (64, 4099, 72), (40, 700, 300),
+         (300, 2500, 64), (257, 3001, 128), (130, 2100, 256), (700, 5000, 100), (120, 2049, 16), (90, 2300, 120),
+         (2100, 300, 64), (2100, 260, 128), (2050, 129, 256), (5000, 2060, 50), (9001, 5, 40)]
 
 
 @pytest.mark.parametrize("dt", DTYPES)
@@ -113,17 +115,18 @@ def test_sizes_and_types(gsb, dt, N, V, D):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("V,scale", [(501, 1.0), (2200, 1.0), (501, -0.5), (2200, -0.5), (70, 0.0)])
 @pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
-def test_reductions_and_upstream_gradients(gsb, dt, reduction):
-    x, w, t = make(200, 501, 96, dt, seed=5, ignored=0.3)
+def test_reductions_upstream_gradients_and_signs(gsb, dt, reduction, V, scale):
+    x, w, t = make(200, V, 96, dt, seed=5, ignored=0.3)
     up = torch.randn(200, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) if reduction == "none" else -2.5
-    check(gsb, x, w, t, reduction=reduction, up=up)
+    check(gsb, x, w, t, scale=scale, reduction=reduction, up=up)
 
 
 @pytest.mark.parametrize("dt", DTYPES)
-@pytest.mark.parametrize("D", [64, 128, 300])
-def test_rows_that_do_not_count_hide_what_they_hold(gsb, dt, D):
-    x, w, t = make(300, 400, D, dt, seed=6, ignored=0.5)
+@pytest.mark.parametrize("N,V,D", [(300, 400, 64), (300, 400, 128), (300, 400, 300), (2100, 2100, 100), (200, 2100, 256)])
+def test_rows_that_do_not_count_hide_what_they_hold(gsb, dt, N, V, D):
+    x, w, t = make(N, V, D, dt, seed=6, ignored=0.5)
     clean = check(gsb, x, w, t)
     dirty = x.clone()
     dirty[t < 0] = float("nan")
@@ -194,7 +197,13 @@ def test_values_that_are_not_finite_reach_the_loss(gsb, dt):
 def test_views(gsb, dt):
     """Column slices, transposed tables, strided rows and leading dimensions give what their copies give."""
     x, w, t = make(96, 260, 72, dt, seed=10)
-    want = gsb.ops.linear_cross_entropy(x, w, t, reduction="none")
+
+    def value(x, w, t):
+        x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+        loss = gsb.ops.linear_cross_entropy(x, w, t, reduction="none")
+        return (loss.detach(),) + torch.autograd.grad(loss.sum(), [x, w])
+
+    want = value(x, w, t)
     wide_x = torch.randn(96, 100, device="cuda").to(dt)
     wide_x[:, 13:85] = x
     wide_w = torch.randn(260, 75, device="cuda").to(dt)
@@ -202,8 +211,10 @@ def test_views(gsb, dt):
     off = torch.empty(96 * 72 + 1, device="cuda", dtype=dt)[1:].view(96, 72).copy_(x)
     for xx, ww in ((wide_x[:, 13:85], w), (x, wide_w[:, 1:73]), (x.t().contiguous().t(), w), (off, w),
                    (x, w.t().contiguous().t()), (x.repeat_interleave(2, 0)[::2], w.repeat_interleave(3, 0)[::3])):
-        assert torch.equal(gsb.ops.linear_cross_entropy(xx, ww, t, reduction="none"), want)
-    assert torch.equal(gsb.ops.linear_cross_entropy(x.view(8, 12, 72), w, t.view(8, 12), reduction="none"), want.view(8, 12))
+        for a, b in zip(value(xx, ww, t), want):
+            assert torch.equal(a, b)
+    got = value(x.view(8, 12, 72), w, t.view(8, 12))
+    assert torch.equal(got[0], want[0].view(8, 12)) and torch.equal(got[1], want[1].view(8, 12, 72)) and torch.equal(got[2], want[2])
 
 
 @pytest.mark.parametrize("dt", DTYPES)
