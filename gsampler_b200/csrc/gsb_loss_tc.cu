@@ -27,6 +27,8 @@
 
 namespace gsb {
 
+constexpr int WIPE = -2;  // in the place of a target: the row must be zeroed
+
 enum { TC_STATS = 0, TC_PULL = 1, TC_GRAD_W = 2, TC_GRAD_X = 3 };
 
 // ---------------------------------------------------------------- shapes of the kernel
@@ -86,26 +88,43 @@ struct TcParams {
   int* err;
 };
 
-// 32 elements of a row of which `left` are there (zeros behind them); rows start at multiples of `bytes`
-template <typename T>
-__device__ __forceinline__ void row_piece(Pack<T, 32>& piece, const T* from, int left, int bytes) {
+// PIECES times 32 elements of a row, `step` elements apart, of which `left` are there (zeros behind
+// them); rows start at multiples of `bytes`.  All loads are requested before the first is used.
+template <typename T, int PIECES>
+__device__ __forceinline__ void row_pieces(Pack<T, 32> (&to)[PIECES], const T* from, int step, int left, int bytes) {
 #pragma unroll
-  for (int q = 0; q < 32; q += 8) {
-    Pack<T, 8>* to = reinterpret_cast<Pack<T, 8>*>(piece.v + q);
-    if (q + 8 <= left && bytes >= 4) {
-      if (bytes == 16) {
-        to->load(from + q);
-      } else if (bytes == 8) {
+  for (int i = 0; i < PIECES; ++i) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) reinterpret_cast<uint2*>(to)[e] = __ldg(reinterpret_cast<const uint2*>(from + q) + e);
-      } else {
+    for (int q = 0; q < 16; ++q) reinterpret_cast<u32*>(to[i].v)[q] = 0;
+  }
+  if (bytes == 16) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) reinterpret_cast<u32*>(to)[e] = __ldg(reinterpret_cast<const u32*>(from + q) + e);
-      }
-    } else {
+    for (int i = 0; i < PIECES; ++i) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) piece.v[q + e] = q + e < left ? from[q + e] : from_float<T>(0.f);
+      for (int q = 0; q < 32; q += 8)
+        if (i * step + q + 8 <= left) reinterpret_cast<Pack<T, 8>*>(to[i].v + q)->load(from + i * step + q);
     }
+  } else if (bytes >= 4) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+#pragma unroll
+      for (int q = 0; q < 32; q += 8)
+        if (i * step + q + 8 <= left) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) reinterpret_cast<u32*>(to[i].v + q)[e] = __ldg(reinterpret_cast<const u32*>(from + i * step + q) + e);
+        }
+    }
+  }
+  // what no whole piece of 8 covers
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+#pragma unroll
+    for (int q = 0; q < 32; q += 8)
+      if (i * step + q < left && (bytes < 4 || i * step + q + 8 > left)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (i * step + q + e < left) to[i].v[q + e] = from[i * step + q + e];
+      }
   }
 }
 
@@ -226,15 +245,17 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
       for (int k = 0; k < (1 << 16) && !bar_try(o_full, 0); ++k) __nanosleep(32);
     }
   } else if (C::MODE == TC_GRAD_W && warp == C::WG * 4 + 2) {
-    // ------------------------------------------------ rows that do not count become zeros, whatever they hold
+    // ------------------------------------------------ rows that do not count must not reach a product with a NaN
+    // P is zero there, which is enough unless the row holds an infinity or a NaN, and then its
+    // log-sum-exp is not finite either (every logit has a term that is not): only those are wiped.
     for (int j = 0; j < my_tiles; ++j) {
       const int st = j % C::ST;
       const bool ok = __all_sync(0xffffffffu, bar_wait(full(st), (j / C::ST) & 1, gave_up, p.err));
       if (!ok) break;
-      const float* bias = reinterpret_cast<const float*>(smem + C::OFF_META + st * C::META);
+      const int* tgt = reinterpret_cast<const int*>(smem + C::OFF_META + st * C::META + 4 * C::BT);
       bool wiped = false;
       for (int r0 = 0; r0 < C::BT; r0 += 32) {
-        u32 dead = __ballot_sync(0xffffffffu, bias[r0 + lane] == -INFINITY);
+        u32 dead = __ballot_sync(0xffffffffu, tgt[r0 + lane] == WIPE);
         wiped |= dead != 0;
         for (; dead; dead &= dead - 1) {
           const int r = r0 + __ffs(dead) - 1;
@@ -255,19 +276,26 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
     // the rows of A into TMEM: a thread its row, pairs of elements a column; zeros behind the last
     // column (nothing there may meet the zeros of B as a NaN) and row
     const bool row_live = row < p.rows_a && (C::MODE != TC_GRAD_X || p.g[row < p.rows_a ? row : 0] != 0.f);
-    for (int k = half * 32; k < ksteps * 16; k += 32 * C::HV) {
-      Pack<T, 32> piece;
-      row_piece(piece, (const T*)p.a + (i64)row * p.lda + k, row_live ? p.D - k : 0, p.a_bytes);
+    constexpr int PIECES = C::DP / (32 * C::HV);
+    {
+      Pack<T, 32> piece[PIECES];
+      row_pieces(piece, (const T*)p.a + (i64)row * p.lda + half * 32, 32 * C::HV, row_live ? p.D - half * 32 : 0, p.a_bytes);
 #pragma unroll
-      for (int q = 0; q < 16; ++q) reinterpret_cast<u32*>(piece.v)[q] ^= p.a_sign;
-      if constexpr (C::ATM) {
-        tc_st16(tmem + C::A_COL + a * (C::DP / 2) + k / 2 + lanes, reinterpret_cast<const u32*>(piece.v));
-      } else {  // as a swizzled tile: 16-byte piece c of row r lies at c ^ (r & 7)
-        const int r = quarter * 32 + lane;
-        unsigned char* to = smem + a * C::A_BYTES + (k >> 6) * 16384 + r * 128;
+      for (int i = 0; i < PIECES; ++i) {
+        const int k = half * 32 + i * (32 * C::HV);
+        if (k < ksteps * 16) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<uint4*>(to + ((((k & 63) >> 3) + q) ^ (r & 7)) * 16) = reinterpret_cast<const uint4*>(piece.v)[q];
+          for (int q = 0; q < 16; ++q) reinterpret_cast<u32*>(piece[i].v)[q] ^= p.a_sign;
+          if constexpr (C::ATM) {
+            tc_st16(tmem + C::A_COL + a * (C::DP / 2) + k / 2 + lanes, reinterpret_cast<const u32*>(piece[i].v));
+          } else {  // as a swizzled tile: 16-byte piece c of row r lies at c ^ (r & 7)
+            const int r = quarter * 32 + lane;
+            unsigned char* to = smem + a * C::A_BYTES + (k >> 6) * 16384 + r * 128;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<uint4*>(to + ((((k & 63) >> 3) + q) ^ (r & 7)) * 16) = reinterpret_cast<const uint4*>(piece[i].v)[q];
+          }
+        }
       }
     }
     if (C::ATM) tc_wait_st();
@@ -427,24 +455,29 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
     if (C::MODE == TC_STATS && row < p.rows_a && ok)
       p.part_ms[(i64)(blockIdx.y * C::HV + half) * p.rows_a + row] = make_float2(m, sum);
     if (C::MODE == TC_PULL && row < p.rows_a && ok) p.part_ms[(i64)blockIdx.y * p.rows_a + row] = make_float2(m, sum);
+    // dx: the target's own row is taken off in 32 bits
+    Pack<T, 32> target_row[C::MODE == TC_GRAD_X ? PIECES : 1];
+    if constexpr (C::MODE == TC_GRAD_X)
+      row_pieces(target_row, (const T*)p.w + (i64)(hot < 0 ? 0 : hot) * p.ldw + half * 32, 32 * C::HV, row_live ? p.D - half * 32 : 0, p.w_bytes);
     if (C::SECOND && my_tiles > 0) {
       ok = ok && bar_wait(o_full, 0, gave_up, p.err);
       ok = __all_sync(0xffffffffu, ok);
       if (ok && warp_live) {
         tc_after();
         const float f = C::MODE == TC_PULL ? 1.f : p.out_scale * __uint_as_float(*p.top);
-        for (int k = half * 32; k < p.D; k += 32 * C::HV) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          const int k = half * 32 + i * (32 * C::HV);
+          if (k >= p.D) break;
           float o[32];
           tc_ld32(o, tmem + C::O_COL + a * C::DP + k + lanes);
           tc_wait_ld();
           if (row < p.rows_a) {
             const bool slab = C::MODE == TC_PULL || (C::MODE == TC_GRAD_W && gridDim.y > 1);
             if (C::MODE == TC_GRAD_X) {
-              // the target's own row, taken off in 32 bits; a row that does not count is zero
-              Pack<T, 32> wt;
-              row_piece(wt, (const T*)p.w + (i64)(hot < 0 ? 0 : hot) * p.ldw + k, row_live ? p.D - k : 0, p.w_bytes);
+              // a row that does not count is zero
 #pragma unroll
-              for (int q = 0; q < 32; ++q) o[q] = row_live ? fmaf(-gs, to_float(wt.v[q]), o[q]) : 0.f;
+              for (int q = 0; q < 32; ++q) o[q] = row_live ? fmaf(-gs, to_float(target_row[C::MODE == TC_GRAD_X ? i : 0].v[q]), o[q]) : 0.f;
             }
             if (slab) {
               float* to = p.part_o + ((i64)blockIdx.y * p.rows_a + row) * p.D + k;
@@ -522,6 +555,7 @@ __global__ void loss_meta_kernel(const float* __restrict__ lse2, const i64* __re
   float bias = INFINITY, gs = 0.f;
   int t = -1;
   u32 sign = 0;
+  if (r < N && g[r] == 0.f && !(fabsf(lse2[r]) < INFINITY)) t = WIPE;
   if (r < N && g[r] != 0.f) {
     const float rel = fabsf(g[r]) / __uint_as_float(*top);
     gs = rel * (float)(1 << GRAD_SHIFT);
@@ -624,12 +658,23 @@ __global__ void loss_dx_kernel(const float* __restrict__ pull, const float* __re
   }
 }
 
+// out[e] = sum over the slabs: 32 elements a CTA, eight runs of slabs each, joined in order
 template <typename T>
-__global__ void loss_join_dw_kernel(const float* __restrict__ slab, i64 size, int slabs, T* __restrict__ out) {
-  for (i64 e = (i64)blockIdx.x * blockDim.x + threadIdx.x; e < size; e += (i64)gridDim.x * blockDim.x) {
+__global__ void __launch_bounds__(256) loss_join_dw_kernel(const float* __restrict__ slab, i64 size, int slabs, T* __restrict__ out) {
+  __shared__ float part[8][32];
+  const int lane = threadIdx.x & 31, run = threadIdx.x >> 5, per = (slabs + 7) / 8;
+  for (i64 e0 = (i64)blockIdx.x * 32; e0 < size; e0 += (i64)gridDim.x * 32) {
+    const i64 e = e0 + lane;
     float v = 0.f;
-    for (int z = 0; z < slabs; ++z) v += slab[z * size + e];
-    out[e] = from_float<T>(v);
+    if (e < size)
+      for (int z = run * per; z < slabs && z < (run + 1) * per; ++z) v += slab[z * size + e];
+    part[run][lane] = v;
+    __syncthreads();
+    if (run == 0 && e < size) {
+      for (int q = 1; q < 8; ++q) v += part[q][lane];
+      out[e] = from_float<T>(v);
+    }
+    __syncthreads();
   }
 }
 
@@ -847,7 +892,7 @@ int tc_loss_grad_w(const LossArgs& a) {
   if (rc != GSB_OK) return rc;
   if (plan.splits > 1) {
     LaunchScope ls(KID_LOSS_JOIN, a.st);
-    loss_join_dw_kernel<T><<<blocks_for(a.V * a.D), 256, 0, a.st>>>(p.part_o, a.V * a.D, plan.splits, (T*)a.dw);
+    loss_join_dw_kernel<T><<<blocks_for(a.V * a.D * 8), 256, 0, a.st>>>(p.part_o, a.V * a.D, plan.splits, (T*)a.dw);
   }
   return GSB_OK;
 }
