@@ -68,12 +68,12 @@ embed_rows_kernel(const T* __restrict__ w, i64 ld, i64 rows, u32 chunks, const i
 }
 
 // ---------------------------------------------------------------- sort of (id, position)
-// Least significant digit first, 8 bits at most a pass, one kernel a pass: a tile of 4096 items
-// ranks its items (warp by warp in item order, so the sort is stable), learns from its
-// predecessors where its run of each digit starts (one look-back chain per digit, a thread each;
-// the tiles take tickets so that a predecessor is always running or done), orders the tile in
-// shared memory and writes it out in runs.  One kernel before all passes counts every digit.
-constexpr int ST_THREADS = 256, ST_ITEMS = 16, ST_TILE = ST_THREADS * ST_ITEMS, ST_WARPS = ST_THREADS / 32;
+// Least significant digit first, 8 bits at most a pass, three kernels a pass: every tile of 4096 items
+// counts its digits; one CTA a digit turns the tiles' counts into places; every tile ranks its items
+// (warp by warp in item order, so the sort is stable), orders itself in shared memory and writes
+// itself out in runs.  A pass in one kernel, the tiles passing their sums down a look-back chain, took
+// 86 us for 4 M items against 33: the chain is hundreds of tiles long, a trip to L2 each sixteen.
+constexpr int ST_THREADS = 512, ST_ITEMS = 8, ST_TILE = ST_THREADS * ST_ITEMS, ST_WARPS = ST_THREADS / 32;
 
 __device__ __forceinline__ u32 key_of(i64 id, i64 rows, i64 padding, int* err) {
   if (id != padding) {
@@ -88,31 +88,73 @@ struct SortPlan {
   int shift[4], bits[4];
 };
 
-__global__ void __launch_bounds__(256)
-embed_digits_kernel(const i64* __restrict__ idx, i64 n, i64 rows, i64 padding, SortPlan plan,
+// counts[digit * tiles + tile]
+__global__ void __launch_bounds__(ST_THREADS)
+embed_digits_kernel(const i64* __restrict__ idx, i64 rows, i64 padding, const u32* __restrict__ key_in, i64 n, int shift, int bits,
                     u32* __restrict__ counts, int* err) {
-  __shared__ u32 hist[4][256];
-  for (int j = threadIdx.x; j < 1024; j += 256) (&hist[0][0])[j] = 0;
+  __shared__ u32 hist[256];
+  const int tid = threadIdx.x;
+  if (tid < 256) hist[tid] = 0;
   __syncthreads();
-  for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < n; i += (i64)gridDim.x * 256) {
-    const u32 k = key_of(__ldg(idx + i), rows, padding, err);
-    for (int p = 0; p < plan.passes; ++p)
-      atomicAdd(&hist[p][(k >> plan.shift[p]) & ((1u << plan.bits[p]) - 1)], 1u);
+  const i64 base = (i64)blockIdx.x * ST_TILE;
+  u32 digit[ST_ITEMS];
+#pragma unroll
+  for (int k = 0; k < ST_ITEMS; ++k) {
+    const i64 i = base + k * ST_THREADS + tid;
+    digit[k] = 256;
+    if (i < n) digit[k] = ((idx ? key_of(__ldg(idx + i), rows, padding, err) : key_in[i]) >> shift) & ((1u << bits) - 1);
   }
+#pragma unroll
+  for (int k = 0; k < ST_ITEMS; ++k)
+    if (digit[k] < 256) atomicAdd(&hist[digit[k]], 1u);
   __syncthreads();
-  for (int j = threadIdx.x; j < plan.passes * 256; j += 256) {
-    const u32 c = (&hist[0][0])[j];
-    if (c) atomicAdd(counts + j, c);
+  if (tid < 256) counts[(i64)tid * gridDim.x + blockIdx.x] = hist[tid];
+}
+
+// a CTA per digit: its tiles' counts become the sum of those before; totals[digit] = all of them
+__global__ void __launch_bounds__(256)
+embed_places_kernel(u32* __restrict__ counts, i64 tiles, u32* __restrict__ totals) {
+  __shared__ u32 warp_tot[8];
+  u32* mine = counts + (i64)blockIdx.x * tiles;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  u32 before = 0;
+  for (i64 t0 = 0; t0 < tiles; t0 += 1024) {
+    u32 v[4], sum = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const i64 t = t0 + threadIdx.x * 4 + q;
+      v[q] = t < tiles ? mine[t] : 0;
+      sum += v[q];
+    }
+    u32 inc = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const u32 o = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += o;
+    }
+    if (lane == 31) warp_tot[wid] = inc;
+    __syncthreads();
+    u32 at = before + inc - sum;
+    for (int w = 0; w < wid; ++w) at += warp_tot[w];
+    for (int w = 0; w < 8; ++w) before += warp_tot[w];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const i64 t = t0 + threadIdx.x * 4 + q;
+      if (t < tiles) mine[t] = at;
+      at += v[q];
+    }
+    __syncthreads();
   }
+  if (threadIdx.x == 0) totals[blockIdx.x] = before;
 }
 
 struct RankShared {
-  u32 warp_hist[ST_WARPS][256];
-  u32 local[256];  // first place of the digit in the tile
-  u32 warp_tot[33];
+  unsigned short warp_hist[ST_WARPS][256];  // a warp has 256 items
+  u32 local[256];                           // first place of the digit in the tile
+  u32 warp_tot[9];
 };
 
-// exclusive scan of one u32 a thread over 256 threads
+// exclusive scan of one value of each of the first 256 threads (all threads call it)
 __device__ __forceinline__ u32 scan256(u32 v, u32* warp_tot) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   u32 inc = v;
@@ -122,64 +164,67 @@ __device__ __forceinline__ u32 scan256(u32 v, u32* warp_tot) {
     if (lane >= d) inc += t;
   }
   __syncthreads();
-  if (lane == 31) warp_tot[wid] = inc;
+  if (lane == 31 && wid < 8) warp_tot[wid] = inc;
   __syncthreads();
   u32 before = 0;
-  for (int w = 0; w < wid; ++w) before += warp_tot[w];
+#pragma unroll
+  for (int w = 0; w < 7; ++w) before += w < wid ? warp_tot[w] : 0;
   return before + inc - v;
 }
 
 // Ranks the tile's items by `digit` (256 = no item).  On return place[k] is the item's place in
-// the digit-ordered tile and sh.local the first place of each digit; returns the count of digit
-// threadIdx.x.
-__device__ __forceinline__ u32 rank_tile(const u32 (&digit)[ST_ITEMS], u32 (&place)[ST_ITEMS], RankShared& sh) {
+// the digit-ordered tile and sh.local the first place of each digit.
+__device__ __forceinline__ void rank_tile(const u32 (&digit)[ST_ITEMS], u32 (&place)[ST_ITEMS], RankShared& sh) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, tid = threadIdx.x;
-  for (int w = 0; w < ST_WARPS; ++w) sh.warp_hist[w][tid] = 0;
-  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < 4; ++q) reinterpret_cast<u32*>(sh.warp_hist[wid])[q * 32 + lane] = 0;
+  __syncwarp();
 #pragma unroll
   for (int k = 0; k < ST_ITEMS; ++k) {
     const u32 d = digit[k];
+    // the lanes with the same digit, a vote a bit (the match instruction took 4 times as long)
     unsigned same = __ballot_sync(0xffffffffu, d < 256);
 #pragma unroll
     for (int b = 0; b < 8; ++b) {
-      const unsigned m = __ballot_sync(0xffffffffu, (d >> b) & 1);
-      same &= ((d >> b) & 1) ? m : ~m;
+      const bool set = (d >> b) & 1;
+      const unsigned m = __ballot_sync(0xffffffffu, set);
+      same &= set ? m : ~m;
     }
     if (d < 256) place[k] = sh.warp_hist[wid][d] + __popc(same & ((1u << lane) - 1));
     __syncwarp();
-    if (d < 256 && (same >> lane) == 1u) sh.warp_hist[wid][d] = place[k] + 1;  // the last lane of the group
+    if (d < 256 && (same >> lane) == 1u) sh.warp_hist[wid][d] = (unsigned short)(place[k] + 1);  // the last lane of the group
     __syncwarp();
   }
   __syncthreads();
   u32 total = 0;
-  for (int w = 0; w < ST_WARPS; ++w) {
-    const u32 c = sh.warp_hist[w][tid];
-    sh.warp_hist[w][tid] = total;
-    total += c;
+  if (tid < 256) {
+#pragma unroll
+    for (int w = 0; w < ST_WARPS; ++w) {
+      const u32 c = sh.warp_hist[w][tid];
+      sh.warp_hist[w][tid] = (unsigned short)total;
+      total += c;
+    }
   }
   const u32 first = scan256(total, sh.warp_tot);
-  sh.local[tid] = first;
+  if (tid < 256) sh.local[tid] = first;
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < ST_ITEMS; ++k)
     if (digit[k] < 256) place[k] += sh.local[digit[k]] + sh.warp_hist[wid][digit[k]];
-  return total;
 }
 
 __global__ void __launch_bounds__(ST_THREADS)
 embed_sort_pass_kernel(const i64* __restrict__ idx, i64 rows, i64 padding, const u32* __restrict__ key_in,
                        const u32* __restrict__ pos_in, u32* __restrict__ key_out, u32* __restrict__ pos_out,
-                       i64 n, int shift, int bits, const u32* __restrict__ counts, u64* status, u32* ticket,
-                       int* err) {
+                       i64 n, int shift, int bits, const u32* __restrict__ counts, const u32* __restrict__ totals) {
   __shared__ RankShared sh;
   __shared__ u32 skey[ST_TILE], spos[ST_TILE];
   __shared__ u32 start[256];  // global place of the digit's run minus its place in the tile
-  __shared__ u32 tile_s;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  if (tid == 0) tile_s = atomicAdd(ticket, 1u);
-  __syncthreads();
-  const i64 tile = tile_s, base = tile * ST_TILE;
+  const i64 base = (i64)blockIdx.x * ST_TILE;
   u32 key[ST_ITEMS], pos[ST_ITEMS], digit[ST_ITEMS], place[ST_ITEMS];
+  const u32 digit_base = scan256(tid < 256 ? totals[tid] : 0, sh.warp_tot);
+  const u32 before = tid < 256 ? counts[(i64)tid * gridDim.x + blockIdx.x] : 0;
 #pragma unroll
   for (int k = 0; k < ST_ITEMS; ++k) {
     const i64 i = base + wid * (32 * ST_ITEMS) + k * 32 + lane;
@@ -190,33 +235,8 @@ embed_sort_pass_kernel(const i64* __restrict__ idx, i64 rows, i64 padding, const
       digit[k] = (key[k] >> shift) & ((1u << bits) - 1);
     }
   }
-  const u32 mine = rank_tile(digit, place, sh);
-  // look-back: one chain per digit
-  u64* st = status + tile * 256 + tid;
-  u64 before = 0;
-  if (tile == 0) {
-    st_relaxed(st, LB_PREFIX | mine);
-  } else {
-    st_relaxed(st, LB_AGG | mine);
-    for (i64 t = tile - 1; t >= 0; --t) {
-      const u64* p = status + t * 256 + tid;
-      u64 w = ld_relaxed(p);
-      int spins = 0;
-      while ((w >> 62) == 0 && ++spins < LB_SPIN_LIMIT) {
-        __nanosleep(20);
-        w = ld_relaxed(p);
-      }
-      if ((w >> 62) == 0) {  // every place is still below n: nothing is written out of range
-        raise(err, ERRBIT_LOOKBACK_TIMEOUT);
-        break;
-      }
-      before += w & LB_MASK;
-      if ((w >> 62) == 2) break;
-    }
-    st_relaxed(st, LB_PREFIX | (before + mine));
-  }
-  const u32 digit_base = scan256(counts[tid], sh.warp_tot);
-  start[tid] = digit_base + (u32)before - sh.local[tid];
+  rank_tile(digit, place, sh);
+  if (tid < 256) start[tid] = digit_base + before - sh.local[tid];
 #pragma unroll
   for (int k = 0; k < ST_ITEMS; ++k)
     if (digit[k] < 256) {
@@ -228,10 +248,8 @@ embed_sort_pass_kernel(const i64* __restrict__ idx, i64 rows, i64 padding, const
   for (int j = tid; j < live; j += ST_THREADS) {
     const u32 k = skey[j];
     const u32 to = start[(k >> shift) & ((1u << bits) - 1)] + j;
-    if (to < n) {
-      key_out[to] = k;
-      pos_out[to] = spos[j];
-    }
+    key_out[to] = k;
+    pos_out[to] = spos[j];
   }
 }
 
@@ -321,16 +339,14 @@ embed_segments_kernel(const u32* __restrict__ key, i64 n, u32 rows, u32* __restr
 // A group of lanes owns `chunk` consecutive sorted items and walks them with the running sum of
 // its columns in registers.  A segment that lies inside the chunk is finished: one rounding,
 // one store.  What reaches beyond the chunk becomes a 32-bit partial row: slot 2c for a segment
-// that began before chunk c, slot 2c + 1 for one that began in it and goes on (for one that does
-// both, slot 2c has the sum and slot 2c + 1 zeros, so that a segment's partials are neighbours).
-// The next level runs the same kernel over the slots, until one chunk holds them all: a hub that
-// fills half the batch is summed by thousands of groups, and in an order that is always the same.
-// Eight rows are requested before the first is added.
-template <typename Tin, typename Tout, int VEC, bool FIRST>
+// that began before chunk c, slot 2c + 1 for one that begins in it and goes on.  A second kernel adds
+// the partials of a segment in the order of its chunks.  Eight rows are requested before the first is
+// added.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
-embed_segsum_kernel(const u32* __restrict__ key, const u32* __restrict__ pos, i64 n, const Tin* __restrict__ src,
-                    i64 ld, int D, int log_group, int chunk, u32 limit, float scale, Tout* __restrict__ out,
-                    float* __restrict__ part, i64 part_ld, u32* __restrict__ part_key) {
+embed_segsum_kernel(const u32* __restrict__ key, const u32* __restrict__ pos, i64 n, const T* __restrict__ grad, int D,
+                    int log_group, int chunk, u32 limit, float scale, T* __restrict__ out, float* __restrict__ part,
+                    i64 part_ld, u32* __restrict__ part_key) {
   constexpr int U = 8;
   const int lane = threadIdx.x & ((1 << log_group) - 1);
   const i64 c = ((i64)blockIdx.x * blockDim.x + threadIdx.x) >> log_group;
@@ -339,7 +355,6 @@ embed_segsum_kernel(const u32* __restrict__ key, const u32* __restrict__ pos, i6
   const i64 end = begin + chunk < n ? begin + chunk : n;
   const int col = (((int)blockIdx.y << log_group) + lane) * VEC;
   const bool live = col < D;
-  const bool scribe = blockIdx.y == 0 && lane == 0;
   auto key_at = [&](i64 i) {
     const u32 k = key[i];
     return k < limit ? k : NO_KEY;
@@ -350,38 +365,43 @@ embed_segsum_kernel(const u32* __restrict__ key, const u32* __restrict__ pos, i6
   u32 cur = key_at(begin);
   bool began_before = cur != NO_KEY && begin > 0 && key_at(begin - 1) == cur;
   const bool goes_on_at_end = end < n && key_at(end) != NO_KEY && key_at(end) == key_at(end - 1);
-  u32 slot_key0 = NO_KEY, slot_key1 = NO_KEY;
+  u32 from_before = NO_KEY, to_after = NO_KEY;
 
-  auto partial = [&](int which, bool zeros) {
+  auto partial = [&](int which) {
     if (!live) return;
     float* to = part + (2 * c + which) * part_ld + col;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) to[j] = zeros ? 0.f : acc[j];
+    for (int j = 0; j < VEC; ++j) to[j] = acc[j];
   };
-  auto finish = [&]() {
-    if (!live) return;
-    Pack<Tout, VEC> r;
+  auto close = [&](bool goes_on) {
+    if (cur == NO_KEY) return;
+    if (began_before) {
+      partial(0);
+      from_before = cur;
+    } else if (goes_on) {
+      partial(1);
+      to_after = cur;
+    } else if (live) {
+      Pack<T, VEC> r;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) r.v[j] = from_float<Tout>(acc[j] * scale);
-    r.store(out + (i64)cur * D + col);
+      for (int j = 0; j < VEC; ++j) r.v[j] = from_float<T>(acc[j] * scale);
+      r.store(out + (i64)cur * D + col);
+    }
   };
 
   for (i64 i = begin; i < end; i += U) {
     u32 k[U];
-    Pack<Tin, VEC> row[U];
+    Pack<T, VEC> row[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) k[u] = i + u < end ? key_at(i + u) : NO_KEY;
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (k[u] != NO_KEY && live) row[u].load(src + (FIRST ? (i64)pos[i + u] : i + u) * ld + col);
+      if (k[u] != NO_KEY && live) row[u].load(grad + (i64)pos[i + u] * D + col);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (i + u >= end) break;
       if (k[u] != cur) {
-        if (cur != NO_KEY) {
-          if (began_before) { partial(0, false); slot_key0 = cur; }
-          else finish();
-        }
+        close(false);
         cur = k[u];
         began_before = false;
 #pragma unroll
@@ -393,21 +413,110 @@ embed_segsum_kernel(const u32* __restrict__ key, const u32* __restrict__ pos, i6
       }
     }
   }
-  if (cur != NO_KEY) {
-    if (began_before) {
-      partial(0, false);
-      slot_key0 = cur;
-      if (goes_on_at_end) { partial(1, true); slot_key1 = cur; }
-    } else if (goes_on_at_end) {
-      partial(1, false);
-      slot_key1 = cur;
+  close(goes_on_at_end);
+  if (blockIdx.y == 0 && lane == 0) {
+    part_key[2 * c] = from_before;
+    part_key[2 * c + 1] = to_after;
+  }
+}
+
+// A group per chunk in which a segment begins and goes on: adds the partials of the chunks behind it.
+// Nearly all runs end within a chunk or two; a hub that fills thousands of chunks is left to the
+// whole CTA, whose groups take equal shares of it that are then added in order.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256)
+embed_join_kernel(const u32* __restrict__ part_key, const float* __restrict__ part, i64 part_ld, i64 chunks, int D, int log_group,
+                  float scale, T* __restrict__ out) {
+  constexpr int U = 8, SHORT = 32;
+  __shared__ i64 long_run[256];
+  __shared__ int longs;
+  __shared__ i64 lo_s, hi_s;
+  __shared__ float sums[256 * VEC];
+  const int lane = threadIdx.x & ((1 << log_group) - 1), group = threadIdx.x >> log_group, groups = 256 >> log_group;
+  const i64 c = (i64)blockIdx.x * groups + group;
+  const int col = (((int)blockIdx.y << log_group) + lane) * VEC;
+  const bool live = col < D;
+  if (threadIdx.x == 0) longs = 0;
+  __syncthreads();
+  auto write = [&](u32 key, const float (&acc)[VEC]) {
+    Pack<T, VEC> r;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) r.v[j] = from_float<T>(acc[j] * scale);
+    r.store(out + (i64)key * D + col);
+  };
+  auto add_run = [&](float (&acc)[VEC], i64 from, i64 to, u32 key, bool look) {  // stops at another key when it has to look
+    for (i64 k = from; k < to; k += U) {
+      bool mine[U];
+      float row[U][VEC];
+#pragma unroll
+      for (int u = 0; u < U; ++u) mine[u] = k + u < to && (!look || part_key[2 * (k + u)] == key);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (mine[u] && live) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) row[u][j] = part[2 * (k + u) * part_ld + col + j];
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (!mine[u]) return;
+        if (live) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) acc[j] += row[u][j];
+        }
+      }
+    }
+  };
+  const u32 key = c < chunks ? part_key[2 * c + 1] : NO_KEY;
+  if (key != NO_KEY) {
+    if (c + SHORT < chunks && part_key[2 * (c + SHORT)] == key) {
+      if (lane == 0) long_run[atomicAdd(&longs, 1)] = c;  // any order: every run has its own row
     } else {
-      finish();
+      float acc[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[j] = live ? part[(2 * c + 1) * part_ld + col + j] : 0.f;
+      add_run(acc, c + 1, c + SHORT < chunks ? c + SHORT : chunks, key, true);
+      if (live) write(key, acc);
     }
   }
-  if (scribe && part_key) {
-    part_key[2 * c] = slot_key0;
-    part_key[2 * c + 1] = slot_key1;
+  __syncthreads();
+  const int todo = longs;
+  for (int q = 0; q < todo; ++q) {
+    const i64 at = long_run[q];
+    const u32 k0 = part_key[2 * at + 1];
+    // the run's chunks are neighbours: its end by cutting the range into 256 until it is found
+    i64 lo = at + 1, hi = chunks;  // chunk lo belongs to the run; hi does not, or is behind the last
+    while (hi - lo > 1) {
+      const i64 step = (hi - lo + 255) / 256, probe = lo + step * threadIdx.x;
+      const int in = probe < hi && part_key[2 * probe] == k0;
+      const int count = __syncthreads_count(in);  // threads 0 .. count - 1 are in
+      if (threadIdx.x == 0) {
+        lo_s = lo + step * (count - 1);
+        hi_s = lo + step * count < hi ? lo + step * count : hi;
+      }
+      __syncthreads();
+      lo = lo_s;
+      hi = hi_s;
+      __syncthreads();
+    }
+    const i64 len = hi - (at + 1), per = (len + groups - 1) / groups;
+    float acc[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+    const i64 from = at + 1 + group * per;
+    add_run(acc, from, from + per < hi ? from + per : hi, k0, false);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sums[threadIdx.x * VEC + j] = acc[j];
+    __syncthreads();
+    if (group == 0 && live) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[j] = part[(2 * at + 1) * part_ld + col + j];
+      for (int g = 0; g < groups; ++g) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] += sums[((g << log_group) + lane) * VEC + j];
+      }
+      write(k0, acc);
+    }
+    __syncthreads();
   }
 }
 
@@ -436,10 +545,9 @@ static int first_chunk(i64 n) {
   while (chunk > 8 && n / chunk < (i64)sm_count() * 64) chunk >>= 1;
   return chunk;
 }
-constexpr int NEXT_CHUNK = 64;
 
 struct EmbedLayout {
-  size_t key[2], pos[2], counts, status, ticket, zero_begin, zero_bytes, part[2], part_key[2], bytes;
+  size_t key[2], pos[2], counts, totals, status, ticket, zero_bytes, part, part_key, bytes;
   i64 tiles, part_ld;
 };
 
@@ -449,21 +557,15 @@ static EmbedLayout embed_layout(i64 n, i64 D, i64 rows) {
   auto take = [&](size_t b) { const size_t at = o; o += up256(b); return at; };
   for (int k = 0; k < 2; ++k) { L.key[k] = take(4 * (size_t)n); L.pos[k] = take(4 * (size_t)n); }
   L.tiles = (n + ST_TILE - 1) / ST_TILE;
-  const int passes = sort_plan(rows).passes;
-  L.zero_begin = o;
-  L.counts = take(4 * 1024);
-  L.ticket = take(4 * 8);
-  // the sort's look-back words; the distinct-id pass has its own behind them
-  L.status = take(8 * ((size_t)passes * L.tiles * 256 + (size_t)(n + 2047) / 2048));
-  L.zero_bytes = o - L.zero_begin;
+  L.counts = take(4 * 256 * (size_t)L.tiles);
+  L.totals = take(4 * 256);
+  L.ticket = take(4);
+  L.status = take(8 * (size_t)((n + 2047) / 2048));  // look-back words of the distinct-id pass
+  L.zero_bytes = o - L.ticket;
   L.part_ld = (D + 7) / 8 * 8;
-  const i64 chunks0 = (n + first_chunk(n) - 1) / first_chunk(n);
-  const i64 slots0 = 2 * chunks0, slots1 = 2 * ((slots0 + NEXT_CHUNK - 1) / NEXT_CHUNK);
-  const i64 slots[2] = {slots0, slots1};
-  for (int k = 0; k < 2; ++k) {
-    L.part[k] = take(4 * (size_t)slots[k] * L.part_ld);
-    L.part_key[k] = take(4 * (size_t)slots[k]);
-  }
+  const i64 chunks = (n + first_chunk(n) - 1) / first_chunk(n);
+  L.part = take(4 * (size_t)(2 * chunks) * L.part_ld);
+  L.part_key = take(4 * (size_t)(2 * chunks));
   L.bytes = o;
   return L;
 }
@@ -481,54 +583,44 @@ static int launch_embed_sort(const i64* idx, i64 n, i64 rows, i64 padding, char*
     return GSB_OK;
   }
   u32* counts = (u32*)(ws + L.counts);
-  u32* ticket = (u32*)(ws + L.ticket);
-  u64* status = (u64*)(ws + L.status);
-  {
-    i64 blocks = (n + 2047) / 2048;
-    if (blocks > sm_count() * 8) blocks = sm_count() * 8;
-    LaunchScope ls(KID_EMBED_SORT, st);
-    embed_digits_kernel<<<(int)blocks, 256, 0, st>>>(idx, n, rows, padding, plan, counts, d_err);
-  }
+  u32* totals = (u32*)(ws + L.totals);
   for (int p = 0; p < plan.passes; ++p) {
+    const i64* ids = p == 0 ? idx : nullptr;
+    const u32 *key_in = key[(p + 1) & 1], *pos_in = pos[(p + 1) & 1];
+    {
+      LaunchScope ls(KID_EMBED_SORT, st);
+      embed_digits_kernel<<<(int)L.tiles, ST_THREADS, 0, st>>>(ids, rows, padding, key_in, n, plan.shift[p], plan.bits[p], counts, d_err);
+    }
+    {
+      LaunchScope ls(KID_EMBED_SORT, st);
+      embed_places_kernel<<<256, 256, 0, st>>>(counts, L.tiles, totals);
+    }
     LaunchScope ls(KID_EMBED_SORT, st);
-    embed_sort_pass_kernel<<<(int)L.tiles, ST_THREADS, 0, st>>>(
-        p == 0 ? idx : nullptr, rows, padding, key[(p + 1) & 1], pos[(p + 1) & 1], key[p & 1], pos[p & 1], n,
-        plan.shift[p], plan.bits[p], counts + 256 * p, status + (size_t)p * L.tiles * 256, ticket + p, d_err);
+    embed_sort_pass_kernel<<<(int)L.tiles, ST_THREADS, 0, st>>>(ids, rows, padding, key_in, pos_in, key[p & 1], pos[p & 1], n,
+                                                                plan.shift[p], plan.bits[p], counts, totals);
   }
   *which = (plan.passes - 1) & 1;
   return GSB_OK;
 }
 
-template <typename Tin, typename Tout, int VEC, bool FIRST>
-static void launch_level(const u32* key, const u32* pos, i64 n, const void* src, i64 ld, i64 D, int chunk,
-                         u32 limit, float scale, void* out, float* part, i64 part_ld, u32* part_key,
-                         cudaStream_t st) {
-  const i64 per_row = D / VEC;
-  int lg = 0;
-  while (lg < 5 && (1 << lg) < per_row) ++lg;
-  const i64 groups = (n + chunk - 1) / chunk, threads = groups << lg;
-  dim3 grid((unsigned)((threads + 255) / 256), (unsigned)((per_row + (1 << lg) - 1) >> lg));
-  LaunchScope ls(KID_EMBED_GRAD, st);
-  embed_segsum_kernel<Tin, Tout, VEC, FIRST><<<grid, 256, 0, st>>>(key, pos, n, (const Tin*)src, ld, (int)D, lg,
-                                                                   chunk, limit, scale, (Tout*)out, part, part_ld,
-                                                                   part_key);
-}
-
 template <typename T, int VEC>
 static void launch_segsum(const u32* key, const u32* pos, i64 n, const void* grad, i64 D, u32 limit, float scale,
                           void* out, char* ws, const EmbedLayout& L, cudaStream_t st) {
-  float* part[2] = {(float*)(ws + L.part[0]), (float*)(ws + L.part[1])};
-  u32* pkey[2] = {(u32*)(ws + L.part_key[0]), (u32*)(ws + L.part_key[1])};
-  const int c0 = first_chunk(n);
-  i64 groups = (n + c0 - 1) / c0;
-  launch_level<T, T, VEC, true>(key, pos, n, grad, D, D, c0, limit, scale, out, part[0], L.part_ld, pkey[0], st);
-  int at = 0;
-  while (groups > 1) {
-    const i64 items = 2 * groups;
-    groups = (items + NEXT_CHUNK - 1) / NEXT_CHUNK;
-    launch_level<float, T, VEC, false>(pkey[at], nullptr, items, part[at], L.part_ld, D, NEXT_CHUNK, limit, scale,
-                                       out, part[at ^ 1], L.part_ld, pkey[at ^ 1], st);
-    at ^= 1;
+  float* part = (float*)(ws + L.part);
+  u32* part_key = (u32*)(ws + L.part_key);
+  const int chunk = first_chunk(n);
+  const i64 chunks = (n + chunk - 1) / chunk, per_row = D / VEC;
+  int lg = 0;
+  while (lg < 5 && (1 << lg) < per_row) ++lg;
+  const dim3 grid((unsigned)(((chunks << lg) + 255) / 256), (unsigned)((per_row + (1 << lg) - 1) >> lg));
+  {
+    LaunchScope ls(KID_EMBED_GRAD, st);
+    embed_segsum_kernel<T, VEC><<<grid, 256, 0, st>>>(key, pos, n, (const T*)grad, (int)D, lg, chunk, limit, scale, (T*)out, part,
+                                                      L.part_ld, part_key);
+  }
+  if (chunks > 1) {
+    LaunchScope ls(KID_EMBED_GRAD, st);
+    embed_join_kernel<T, VEC><<<grid, 256, 0, st>>>(part_key, part, L.part_ld, chunks, (int)D, lg, scale, (T*)out);
   }
 }
 
@@ -611,7 +703,6 @@ extern "C" int gsb_embedding_grad(const void* grad, int dtype, int64_t D, const 
   const EmbedLayout L = embed_layout(n, D, rows);
   if (!workspace || workspace_bytes < L.bytes) return GSB_ERR_WORKSPACE;
   char* ws = (char*)workspace;
-  if (n > ST_TILE) GSB_CUDA_OK(cudaMemsetAsync(ws + L.zero_begin, 0, L.zero_bytes, st));
   int which = 0;
   launch_embed_sort((const i64*)idx, n, rows, padding, ws, L, d_err, st, &which);
   segsum_any(dtype, (u32*)(ws + L.key[which]), (u32*)(ws + L.pos[which]), n, grad, D, (u32)rows, scale, out, ws, L, st);
@@ -627,16 +718,16 @@ extern "C" int gsb_embedding_sort(const int64_t* idx, int64_t n, int64_t rows, i
   if (!workspace || workspace_bytes < L.bytes) return GSB_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)cuda_stream;
   char* ws = (char*)workspace;
-  GSB_CUDA_OK(cudaMemsetAsync(ws + L.zero_begin, 0, L.zero_bytes, st));
+  GSB_CUDA_OK(cudaMemsetAsync(ws + L.ticket, 0, L.zero_bytes, st));
   int which = 0;
   launch_embed_sort((const i64*)idx, n, rows, padding, ws, L, d_err, st, &which);
-  u64* status = (u64*)(ws + L.status) + (size_t)sort_plan(rows).passes * L.tiles * 256;
+  u64* status = (u64*)(ws + L.status);
   {
     LaunchScope ls(KID_EMBED_SORT, st);
     // the ranks take the place of the other key buffer
     embed_segments_kernel<<<(int)((n + 2047) / 2048), 256, 0, st>>>(
         (u32*)(ws + L.key[which]), n, (u32)rows, (u32*)(ws + L.key[which ^ 1]), (i64*)ids, (i64*)d_num, status,
-        (u32*)(ws + L.ticket) + 4, d_err);
+        (u32*)(ws + L.ticket), d_err);
   }
   GSB_CUDA_OK(cudaGetLastError());
   return GSB_OK;

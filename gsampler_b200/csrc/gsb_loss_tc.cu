@@ -705,7 +705,7 @@ typedef TcShape<TC_STATS, 64, 2, 3, 128, 6, 1, 2, true> Stats64;
 typedef TcShape<TC_STATS, 128, 2, 3, 128, 5, 1, 2, true> Stats128;
 typedef TcShape<TC_STATS, 256, 2, 2, 128, 3, 1, 2, true> Stats256;
 typedef TcShape<TC_STATS, 64, 1, 3, 64, 8, 2, 2, true> StatsFew64;
-typedef TcShape<TC_STATS, 128, 1, 3, 64, 6, 2, 2, true> StatsFew128;
+typedef TcShape<TC_STATS, 128, 1, 2, 128, 2, 2, 2, false> StatsFew128;
 typedef TcShape<TC_STATS, 256, 1, 2, 64, 3, 2, 2, true> StatsFew256;
 typedef TcShape<TC_PULL, 64, 2, 2, 128, 6, 1, 1, true> Pull64;
 typedef TcShape<TC_PULL, 128, 2, 2, 128, 4, 1, 1, false> Pull128;
