@@ -14,31 +14,71 @@
 
 namespace gsb {
 
-template <typename T, bool VECTOR>
+__device__ __forceinline__ u32 scale_pair(u32 v, float scale, const __half*) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+  const __half2 r = __floats2half2_rn(f.x * scale, f.y * scale);
+  return *reinterpret_cast<const u32*>(&r);
+}
+__device__ __forceinline__ u32 scale_pair(u32 v, float scale, const __nv_bfloat16*) {
+  const __nv_bfloat162 r = __floats2bfloat162_rn(__uint_as_float(v << 16) * scale, __uint_as_float(v & 0xFFFF0000u) * scale);
+  return *reinterpret_cast<const u32*>(&r);
+}
+
+// the eight elements of block g; a selection, not a product: what is dropped is zero even where x is
+// not finite
+template <typename T>
+__device__ __forceinline__ void drop_block(Pack<T, 8>& v, i64 g, u32 threshold, float scale, u64 seed, u32 stream) {
+  const Philox4 r = stream_block(seed, stream, (u64)g, 0);
+  const u32 w[4] = {r.x, r.y, r.z, r.w};
+  // threshold 65536 drops everything: its comparisons would wrap
+  const u32 high = threshold < 65536u ? threshold << 16 : 0xFFFFFFFFu;
+  const bool none = threshold >= 65536u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const bool keep_lo = (w[j] << 16) >= high && !none, keep_hi = w[j] >= high && !none;
+    if constexpr (sizeof(T) == 2) {  // two elements a word
+      u32* p = reinterpret_cast<u32*>(v.v) + j;
+      *p = scale_pair(*p, scale, (const T*)nullptr) & ((keep_lo ? 0xFFFFu : 0u) | (keep_hi ? 0xFFFF0000u : 0u));
+    } else {
+      v.v[2 * j] = keep_lo ? v.v[2 * j] * scale : 0.f;
+      v.v[2 * j + 1] = keep_hi ? v.v[2 * j + 1] * scale : 0.f;
+    }
+  }
+}
+
+// U blocks of eight a thread, all requested first; no grid-stride loop, whose last round leaves most of
+// a launch of a few rounds idle.  The copy needs about 35 KB in flight an SM: 4 M x 100 bf16 in 319 us
+// with U = 1, 267 with 2, 253 with 4 (6.3 TB/s); a small tensor has more CTAs with U = 1.
+template <typename T, bool VECTOR, int U>
 __global__ void __launch_bounds__(256)
 dropout_kernel(const T* __restrict__ x, i64 n, u32 threshold, float scale, u64 seed, u32 stream,
                const i64* __restrict__ stream_dev, T* __restrict__ y) {
+  const i64 g0 = (i64)blockIdx.x * (256 * U) + threadIdx.x;
+  if (VECTOR && ((i64)blockIdx.x + 1) * (256 * U) * 8 <= n) {  // whole blocks only
+    Pack<T, 8> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u].load(x + (g0 + u * 256) * 8);
+    if (stream_dev) stream += (u32)__ldg(stream_dev);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      drop_block(v[u], g0 + u * 256, threshold, scale, seed, stream);
+      v[u].store(y + (g0 + u * 256) * 8);
+    }
+    return;
+  }
   if (stream_dev) stream += (u32)__ldg(stream_dev);
-  const i64 blocks = (n + 7) / 8, step = (i64)gridDim.x * blockDim.x;
-  for (i64 g = (i64)blockIdx.x * blockDim.x + threadIdx.x; g < blocks; g += step) {
+  for (int u = 0; u < U; ++u) {
+    const i64 g = g0 + u * 256, e = g * 8;
+    if (e >= n) return;
     Pack<T, 8> v;
-    const i64 e = g * 8;
     const bool whole = VECTOR && e + 8 <= n;
     if (whole) {
       v.load(x + e);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (e + j < n) v.v[j] = x[e + j];
+      for (int j = 0; j < 8; ++j) v.v[j] = e + j < n ? x[e + j] : from_float<T>(0.f);
     }
-    const Philox4 r = stream_block(seed, stream, (u64)g, 0);
-    const u32 w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const u32 u = (j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xFFFFu;
-      // a selection, not a product: what is dropped is zero even where x is not finite
-      v.v[j] = u >= threshold ? from_float<T>(to_float(v.v[j]) * scale) : from_float<T>(0.f);
-    }
+    drop_block(v, g, threshold, scale, seed, stream);
     if (whole) {
       v.store(y + e);
     } else {
@@ -49,16 +89,19 @@ dropout_kernel(const T* __restrict__ x, i64 n, u32 threshold, float scale, u64 s
   }
 }
 
-template <typename T>
-static void launch_dropout(const void* x, i64 n, u32 threshold, float scale, u64 seed, u32 stream,
-                           const i64* stream_dev, void* y, cudaStream_t st) {
-  i64 blocks = ((n + 7) / 8 + 255) / 256;
-  if (blocks > (i64)sm_count() * 32) blocks = (i64)sm_count() * 32;
+template <typename T, bool VECTOR, int U>
+static void launch_dropout_u(const void* x, i64 n, u32 threshold, float scale, u64 seed, u32 stream, const i64* stream_dev,
+                             void* y, cudaStream_t st) {
+  const i64 blocks = ((n + 7) / 8 + 256 * U - 1) / (256 * U);
   LaunchScope ls(KID_DROPOUT, st);
-  if ((((uintptr_t)x | (uintptr_t)y) & 15) == 0)
-    dropout_kernel<T, true><<<(int)blocks, 256, 0, st>>>((const T*)x, n, threshold, scale, seed, stream, stream_dev, (T*)y);
-  else
-    dropout_kernel<T, false><<<(int)blocks, 256, 0, st>>>((const T*)x, n, threshold, scale, seed, stream, stream_dev, (T*)y);
+  dropout_kernel<T, VECTOR, U><<<(unsigned)blocks, 256, 0, st>>>((const T*)x, n, threshold, scale, seed, stream, stream_dev, (T*)y);
+}
+template <typename T>
+static void launch_dropout(const void* x, i64 n, u32 threshold, float scale, u64 seed, u32 stream, const i64* stream_dev, void* y,
+                           cudaStream_t st) {
+  if ((((uintptr_t)x | (uintptr_t)y) & 15) != 0) launch_dropout_u<T, false, 1>(x, n, threshold, scale, seed, stream, stream_dev, y, st);
+  else if (n >= (i64)sm_count() * 8 * 8192) launch_dropout_u<T, true, 4>(x, n, threshold, scale, seed, stream, stream_dev, y, st);
+  else launch_dropout_u<T, true, 1>(x, n, threshold, scale, seed, stream, stream_dev, y, st);
 }
 
 }  // namespace gsb
@@ -67,7 +110,7 @@ using namespace gsb;
 
 extern "C" int gsb_dropout(const void* x, int dtype, int64_t n, double p, uint64_t seed, uint32_t stream,
                            const int64_t* stream_dev, void* y, void* cuda_stream) {
-  if (n < 0 || !(p >= 0.0 && p <= 1.0)) return GSB_ERR_INVALID;
+  if (n < 0 || n > (1ll << 40) || !(p >= 0.0 && p <= 1.0)) return GSB_ERR_INVALID;  // the grid's limit
   if (n == 0) return GSB_OK;
   if (!x || !y) return GSB_ERR_INVALID;
   const u32 threshold = (u32)(p * 65536.0 + 0.5);

@@ -1,6 +1,7 @@
 #include "learn.h"
 
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 
 #include <atomic>
 #include <cmath>
@@ -235,6 +236,105 @@ std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyGrad(torch::Tensor x,
                                  (size_t)ws.numel(), ErrorWord(x.device()), CurrentStream()),
               "linear_ce_grad");
   return {dx, dw};
+}
+
+// ------------------------------------------------------------------ autograd
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+static bool Tracked(const torch::Tensor& t) { return at::GradMode::is_enabled() && t.defined() && t.requires_grad(); }
+
+struct EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
+  static torch::Tensor forward(AutogradContext* ctx, torch::Tensor weight, torch::Tensor index, double scale,
+                               int64_t padding, bool sparse) {
+    auto out = Embedding(weight, index, scale, padding);
+    ctx->save_for_backward({index});
+    ctx->saved_data["rows"] = weight.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    ctx->saved_data["sparse"] = sparse;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto index = ctx->get_saved_variables()[0];
+    const int64_t rows = ctx->saved_data["rows"].toInt(), padding = ctx->saved_data["padding"].toInt();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    torch::Tensor dw;
+    if (ctx->saved_data["sparse"].toBool()) {
+      torch::Tensor ids, values;
+      std::tie(ids, values) = EmbeddingSparseGrad(grads[0], index, rows, scale, padding);
+      dw = at::_sparse_coo_tensor_unsafe(ids.unsqueeze(0), values, {rows, values.size(1)},
+                                         values.options().layout(at::kSparse), /*is_coalesced=*/true);
+    } else {
+      dw = EmbeddingGrad(grads[0], index, rows, scale, padding);
+    }
+    return {dw, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()};
+  }
+};
+
+torch::Tensor EmbeddingLookup(torch::Tensor weight, torch::Tensor index, double scale, int64_t padding, bool sparse) {
+  if (!Tracked(weight)) return Embedding(weight, index, scale, padding);
+  return EmbeddingFn::apply(weight, index, scale, padding, sparse);
+}
+
+struct DropoutFn : public torch::autograd::Function<DropoutFn> {
+  static torch::Tensor forward(AutogradContext* ctx, torch::Tensor data, double p, int64_t seed, int64_t stream,
+                               c10::optional<torch::Tensor> step) {
+    if (step.has_value()) ctx->save_for_backward({*step});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed;
+    ctx->saved_data["stream"] = stream;
+    return Dropout(data, p, seed, stream, step);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    c10::optional<torch::Tensor> step;
+    if (!saved.empty()) step = saved[0];
+    auto dx = Dropout(grads[0], ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(),
+                      ctx->saved_data["stream"].toInt(), step);
+    return {dx, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()};
+  }
+};
+
+torch::Tensor DropoutApply(torch::Tensor data, double p, int64_t seed, int64_t stream, c10::optional<torch::Tensor> step) {
+  if (!Tracked(data)) return Dropout(data, p, seed, stream, step);
+  return DropoutFn::apply(data, p, seed, stream, step);
+}
+
+struct LinearCrossEntropyFn : public torch::autograd::Function<LinearCrossEntropyFn> {
+  static torch::Tensor forward(AutogradContext* ctx, torch::Tensor x, torch::Tensor weight, torch::Tensor target,
+                               double scale, int64_t ignore, int64_t reduction, bool want_dx) {
+    torch::Tensor loss, lse2, pull, count;
+    std::tie(loss, lse2, pull) = LinearCrossEntropy(x, weight, target, scale, ignore, want_dx);
+    if (reduction != 0)
+      std::tie(loss, count) = LinearCrossEntropyTotal(loss, target, weight.size(0), ignore, reduction == 2);
+    if (reduction != 2) count = torch::Tensor();
+    ctx->save_for_backward({x, weight, target, lse2, pull, count});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["ignore"] = ignore;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const bool want_dx = ctx->needs_input_grad(0), want_dw = ctx->needs_input_grad(1);
+    c10::optional<torch::Tensor> count;
+    if (s[5].defined()) count = s[5];
+    torch::Tensor dx, dw;
+    std::tie(dx, dw) = LinearCrossEntropyGrad(s[0], s[1], s[2], s[3], s[4], grads[0], count, ctx->saved_data["scale"].toDouble(),
+                                              ctx->saved_data["ignore"].toInt(), want_dx, want_dw);
+    return {want_dx ? dx : torch::Tensor(), want_dw ? dw : torch::Tensor(), torch::Tensor(), torch::Tensor(),
+            torch::Tensor(), torch::Tensor(), torch::Tensor()};
+  }
+};
+
+torch::Tensor LinearCrossEntropyLoss(torch::Tensor x, torch::Tensor weight, torch::Tensor target, double scale,
+                                     int64_t ignore, int64_t reduction) {
+  TORCH_CHECK(reduction >= 0 && reduction <= 2, "LinearCrossEntropy: reduction must be 0, 1 or 2");
+  if (Tracked(x) || Tracked(weight))
+    return LinearCrossEntropyFn::apply(x, weight, target, scale, ignore, reduction, Tracked(x));
+  auto loss = std::get<0>(LinearCrossEntropy(x, weight, target, scale, ignore, false));
+  if (reduction == 0) return loss;
+  return std::get<0>(LinearCrossEntropyTotal(loss, target, weight.size(0), ignore, reduction == 2));
 }
 
 }  // namespace gsb_host

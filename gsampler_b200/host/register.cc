@@ -101,4 +101,8 @@ TORCH_LIBRARY(gs_ops, m) {
   m.def("_CAPI_LinearCrossEntropy", &gsb_host::LinearCrossEntropy);
   m.def("_CAPI_LinearCrossEntropyTotal", &gsb_host::LinearCrossEntropyTotal);
   m.def("_CAPI_LinearCrossEntropyGrad", &gsb_host::LinearCrossEntropyGrad);
+  // the same, differentiable
+  m.def("_CAPI_EmbeddingLookup", &gsb_host::EmbeddingLookup);
+  m.def("_CAPI_DropoutApply", &gsb_host::DropoutApply);
+  m.def("_CAPI_LinearCrossEntropyLoss", &gsb_host::LinearCrossEntropyLoss);
 }

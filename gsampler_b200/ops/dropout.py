@@ -5,20 +5,6 @@ import torch
 __all__ = ["dropout"]
 
 
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, data, p, seed, stream, step):
-        ctx.p, ctx.seed, ctx.stream = p, seed, stream
-        ctx.save_for_backward(*([] if step is None else [step]))
-        return torch.ops.gs_ops._CAPI_Dropout(data, p, seed, stream, step)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        step = ctx.saved_tensors[0] if ctx.saved_tensors else None
-        return torch.ops.gs_ops._CAPI_Dropout(grad, ctx.p, ctx.seed, ctx.stream, step), None, None, None, None
-
-
 def dropout(data: torch.Tensor, p: float = 0.5, training: bool = True, seed: int = None, stream: int = None,
             step: torch.Tensor = None) -> torch.Tensor:
     """Zeroes each element of ``data`` (fp32, fp16 or bf16) with probability ``p`` and multiplies the
@@ -39,4 +25,4 @@ def dropout(data: torch.Tensor, p: float = 0.5, training: bool = True, seed: int
         return data
     if seed is None:
         seed, stream = torch.ops.gs_ops._CAPI_NextDropoutStream()
-    return _Dropout.apply(data, float(p), int(seed), int(stream), step)
+    return torch.ops.gs_ops._CAPI_DropoutApply(data, float(p), int(seed), int(stream), step)

@@ -8,27 +8,6 @@ import torch
 __all__ = ["embedding"]
 
 
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, weight, index, scale, padding_idx, sparse):
-        ctx.save_for_backward(index)
-        ctx.num_rows, ctx.scale, ctx.padding_idx, ctx.sparse = weight.shape[0], scale, padding_idx, sparse
-        return torch.ops.gs_ops._CAPI_Embedding(weight, index, scale, padding_idx)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        (index,) = ctx.saved_tensors
-        if not ctx.sparse:
-            dw = torch.ops.gs_ops._CAPI_EmbeddingGrad(grad, index, ctx.num_rows, ctx.scale, ctx.padding_idx)
-        else:
-            ids, rows = torch.ops.gs_ops._CAPI_EmbeddingSparseGrad(grad, index, ctx.num_rows, ctx.scale,
-                                                                   ctx.padding_idx)
-            dw = torch.sparse_coo_tensor(ids.unsqueeze(0), rows, (ctx.num_rows, rows.shape[1]),
-                                         is_coalesced=True, check_invariants=False)
-        return dw, None, None, None, None
-
-
 def embedding(weight: torch.Tensor, index: torch.Tensor, scale: float = 1.0, padding_idx: int = -1,
               sparse: bool = False) -> torch.Tensor:
     """``scale * weight[index]`` for a table ``weight`` [rows, D] (fp32, fp16 or bf16) and int64 ids
@@ -41,4 +20,4 @@ def embedding(weight: torch.Tensor, index: torch.Tensor, scale: float = 1.0, pad
     inputs give the same bits), and rounds once.  ``sparse=True`` returns it as a coalesced sparse
     tensor over the touched rows, which costs one read-back of their number (so it cannot be
     recorded into a CUDA graph); the dense form writes the whole table."""
-    return _Embedding.apply(weight, index, float(scale), int(padding_idx), bool(sparse))
+    return torch.ops.gs_ops._CAPI_EmbeddingLookup(weight, index, float(scale), int(padding_idx), bool(sparse))

@@ -5,27 +5,7 @@ import torch
 __all__ = ["linear_cross_entropy"]
 
 
-class _LinearCrossEntropy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, target, scale, ignore_index, reduction):
-        loss, lse2, pull = torch.ops.gs_ops._CAPI_LinearCrossEntropy(x, weight, target, scale, ignore_index,
-                                                                     ctx.needs_input_grad[0])
-        count = None
-        if reduction != "none":
-            loss, count = torch.ops.gs_ops._CAPI_LinearCrossEntropyTotal(loss, target, weight.shape[0], ignore_index,
-                                                                         reduction == "mean")
-        ctx.save_for_backward(x, weight, target, lse2, pull, count if reduction == "mean" else None)
-        ctx.scale, ctx.ignore_index = scale, ignore_index
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        x, weight, target, lse2, pull, count = ctx.saved_tensors
-        want_dx, want_dw = ctx.needs_input_grad[:2]
-        dx, dw = torch.ops.gs_ops._CAPI_LinearCrossEntropyGrad(x, weight, target, lse2, pull, grad, count, ctx.scale,
-                                                               ctx.ignore_index, want_dx, want_dw)
-        return dx if want_dx else None, dw if want_dw else None, None, None, None, None
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, scale: float = 1.0,
@@ -39,10 +19,13 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     loss and gradients are zero, whatever ``x`` holds there; "mean" over no rows is zero.  A target
     outside the vocabulary does not count either and is reported by ``check_async_errors()``.
     Nothing here synchronises."""
-    if reduction not in ("mean", "sum", "none"):
+    how = _REDUCTIONS.get(reduction)
+    if how is None:
         raise ValueError("linear_cross_entropy: reduction must be mean, sum or none, got %r" % (reduction,))
-    if x.dim() < 1 or x.shape[:-1] != target.shape:
+    shape = target.shape
+    if x.dim() < 1 or x.shape[:-1] != shape:
         raise ValueError("linear_cross_entropy: target must have the shape of x without its last dimension")
-    loss = _LinearCrossEntropy.apply(x.reshape(-1, x.shape[-1]), weight, target.reshape(-1), float(scale),
-                                     int(ignore_index), reduction)
-    return loss.view(target.shape) if reduction == "none" else loss
+    if x.dim() != 2:
+        x, target = x.reshape(-1, x.shape[-1]), target.reshape(-1)
+    loss = torch.ops.gs_ops._CAPI_LinearCrossEntropyLoss(x, weight, target, float(scale), int(ignore_index), how)
+    return loss.view(shape) if how == 0 else loss
