@@ -5,7 +5,7 @@
 //   p_ij = exp(l_ij - lse_i)
 //
 // Entry points, and the small kernels around two forms of the products: gsb_loss_tc.cu for 16-bit
-// types of up to 256 columns, gsb_loss_gemm.cu for fp32 and for wider rows.
+// types of up to 256 columns and fp32 of up to 128, gsb_loss_gemm.cu for wider rows.
 #include "gsb_common.cuh"
 #include "gsb_loss.cuh"
 #include "gsb_types.cuh"
@@ -89,12 +89,12 @@ static bool loss_sizes_ok(i64 N, i64 V, i64 D, i64 ldx, i64 ldw) {
          (V < 2 || ldw >= D);
 }
 
-extern "C" int gsb_linear_ce_has_pull(int dtype, int64_t V, int64_t D) { return tc_loss_takes(dtype, D) && tc_loss_pulls(V); }
+extern "C" int gsb_linear_ce_has_pull(int dtype, int64_t V, int64_t D) { return tc_loss_takes(dtype, D) && tc_loss_pulls(dtype, V); }
 
 extern "C" size_t gsb_linear_ce_workspace_bytes(int dtype, const void* weight, int64_t ldw, int64_t N, int64_t V, int64_t D,
                                                 int want_pull) {
   if (!loss_sizes_ok(N, V, D, D, D)) return 0;
-  if (tc_loss_takes(dtype, D)) return tc_loss_workspace(N, V, D, want_pull != 0, tc_loss_packs(weight, ldw));
+  if (tc_loss_takes(dtype, D)) return tc_loss_workspace(dtype, N, V, D, want_pull != 0, tc_loss_packs(weight, ldw));
   return gemm_loss_workspace(dtype, N, V, D, tc_loss_packs(weight, ldw));
 }
 
@@ -114,7 +114,8 @@ extern "C" int gsb_linear_ce(const void* x, int dtype, int64_t ldx, int64_t N, c
   a.ws = workspace; a.err = d_err; a.st = (cudaStream_t)cuda_stream;
   int rc = GSB_OK;
   if (tc_loss_takes(dtype, D))
-    rc = dtype == GSB_F16 ? tc_loss_forward<__half>(a, pull) : tc_loss_forward<__nv_bfloat16>(a, pull);
+    rc = dtype == GSB_F32 ? tc_loss_forward<float>(a, pull)
+         : dtype == GSB_F16 ? tc_loss_forward<__half>(a, pull) : tc_loss_forward<__nv_bfloat16>(a, pull);
   else
     rc = dtype == GSB_F32 ? gemm_loss_forward<float>(a)
          : dtype == GSB_F16 ? gemm_loss_forward<__half>(a) : gemm_loss_forward<__nv_bfloat16>(a);
@@ -150,7 +151,7 @@ extern "C" size_t gsb_linear_ce_grad_workspace_bytes(int dtype, const void* weig
   const size_t head = up256(4 * (size_t)N) + 256;
   if (!tc_loss_takes(dtype, D))
     return head + gemm_loss_grad_workspace(dtype, N, V, D, want_dx != 0, want_dw != 0, tc_loss_packs(weight, ldw));
-  return head + tc_loss_grad_workspace(N, V, D, want_dx && !have_pull, want_dw != 0);
+  return head + tc_loss_grad_workspace(dtype, N, V, D, want_dx && !have_pull, want_dw != 0);
 }
 
 extern "C" int gsb_linear_ce_grad(const void* x, int dtype, int64_t ldx, int64_t N, const void* weight, int64_t ldw,
@@ -189,15 +190,17 @@ extern "C" int gsb_linear_ce_grad(const void* x, int dtype, int64_t ldx, int64_t
     rc = dtype == GSB_F32 ? gemm_loss_backward<float>(a)
          : dtype == GSB_F16 ? gemm_loss_backward<__half>(a) : gemm_loss_backward<__nv_bfloat16>(a);
   } else {
-    const bool half = dtype == GSB_F16;
     if (a.dx && pull) {
-      if (half) tc_loss_dx<__half>(a, pull);
+      if (dtype == GSB_F16) tc_loss_dx<__half>(a, pull);
       else tc_loss_dx<__nv_bfloat16>(a, pull);
       a.dx = nullptr;  // what is left below
     } else if (a.dx) {
-      rc = half ? tc_loss_grad_x<__half>(a) : tc_loss_grad_x<__nv_bfloat16>(a);
+      rc = dtype == GSB_F32 ? tc_loss_grad_x<float>(a)
+           : dtype == GSB_F16 ? tc_loss_grad_x<__half>(a) : tc_loss_grad_x<__nv_bfloat16>(a);
     }
-    if (rc == GSB_OK && a.dw) rc = half ? tc_loss_grad_w<__half>(a) : tc_loss_grad_w<__nv_bfloat16>(a);
+    if (rc == GSB_OK && a.dw)
+      rc = dtype == GSB_F32 ? tc_loss_grad_w<float>(a)
+           : dtype == GSB_F16 ? tc_loss_grad_w<__half>(a) : tc_loss_grad_w<__nv_bfloat16>(a);
   }
   if (rc != GSB_OK) return rc;
   GSB_CUDA_OK(cudaGetLastError());

@@ -1,6 +1,7 @@
 // Shared by the two forms of the vocabulary cross entropy (gsb_loss.cu, gsb_loss_tc.cu).
 #pragma once
 #include "gsb_common.cuh"
+#include "gsb_types.cuh"
 
 namespace gsb {
 
@@ -52,12 +53,19 @@ struct LossArgs {
   cudaStream_t st;
 };
 
-// The tensor-core form (gsb_loss_tc.cu): 16-bit types, up to 256 columns.
+// How a type reaches the tensor cores: as it is, or as three bf16 planes (h + m + l, 8 bits each).
+template <typename S> struct Planes { typedef S type; static constexpr int count = 1; };
+template <> struct Planes<float> { typedef __nv_bfloat16 type; static constexpr int count = 3; };
+// dst[plane][r, :] = the planes of +-src[r, :], rows of packed_ld(D) elements; rows whose g is zero as zeros (gsb_loss_gemm.cu)
+template <typename S>
+void make_planes(const void* src, i64 ld, i64 rows, i64 D, bool negate, const float* g, void* dst, cudaStream_t st);
+
+// The streamed form (gsb_loss_tc.cu): 16-bit types of up to 256 columns, fp32 of up to 128.
 bool tc_loss_takes(int dtype, i64 D);
-bool tc_loss_pulls(i64 V);  // whether the forward pass delivers what dx is made from, or dx makes the logits again
+bool tc_loss_pulls(int dtype, i64 V);  // whether the forward pass delivers what dx is made from, or dx makes the logits again
 bool tc_loss_packs(const void* w, i64 ldw);  // whether the rows of W have to be copied for it
-size_t tc_loss_workspace(i64 N, i64 V, i64 D, bool pull, bool pack_w);
-size_t tc_loss_grad_workspace(i64 N, i64 V, i64 D, bool dx, bool dw);
+size_t tc_loss_workspace(int dtype, i64 N, i64 V, i64 D, bool pull, bool pack_w);
+size_t tc_loss_grad_workspace(int dtype, i64 N, i64 V, i64 D, bool dx, bool dw);
 // The general form (gsb_loss_gemm.cu).
 size_t gemm_loss_workspace(int dtype, i64 N, i64 V, i64 D, bool pack_w);
 size_t gemm_loss_grad_workspace(int dtype, i64 N, i64 V, i64 D, bool dx, bool dw, bool pack_w);

@@ -1,4 +1,4 @@
-// The vocabulary cross entropy for fp32 and for more than 256 columns: tiled products on the tensor
+// The vocabulary cross entropy for more columns than gsb_loss_tc.cu takes: tiled products on the tensor
 // cores, with the vocabulary taken in pieces in the backward pass.
 //
 //   statistics  tiles of x W^T whose epilogue keeps the running maximum and sum of every row
@@ -440,11 +440,8 @@ size_t gemm_loss_grad_workspace(int dtype, i64 N, i64 V, i64 D, bool dx, bool dw
   return dtype == GSB_F32 || pack_w ? L.bytes : L.w;
 }
 
-template <typename S> struct Planes { typedef S type; static constexpr int count = 1; };
-template <> struct Planes<float> { typedef __nv_bfloat16 type; static constexpr int count = 3; };
-
 template <typename S>
-static void make_planes(const void* src, i64 ld, i64 rows, i64 D, bool negate, const float* g, void* dst, cudaStream_t st) {
+void make_planes(const void* src, i64 ld, i64 rows, i64 D, bool negate, const float* g, void* dst, cudaStream_t st) {
   typedef typename Planes<S>::type T;
   LaunchScope ls(KID_LOSS_JOIN, st);
   loss_planes_kernel<S, T, Planes<S>::count><<<blocks_for(rows * packed_ld(D) / 8), 256, 0, st>>>(
@@ -593,6 +590,7 @@ int gemm_loss_backward(const LossArgs& a) {
   return GSB_OK;
 }
 
+template void make_planes<float>(const void*, i64, i64, i64, bool, const float*, void*, cudaStream_t);
 template int gemm_loss_forward<float>(const LossArgs&);
 template int gemm_loss_forward<__half>(const LossArgs&);
 template int gemm_loss_forward<__nv_bfloat16>(const LossArgs&);

@@ -36,10 +36,12 @@ enum { TC_STATS = 0, TC_PULL = 1, TC_GRAD_W = 2, TC_GRAD_X = 3 };
 // NA    tiles A a CTA works on at once
 // NB    S buffers, BT  rows of a tile B, ST  stages of the B pipeline, CTAS  CTAs an SM
 // HV    warpgroups that turn an item's S into P, each an equal share of its columns
+// PL    planes: 1 for 16-bit values, 3 for fp32 as three bf16 planes and six plane products (see gsb_loss_gemm.cu)
 // ATM   tiles A in TMEM, where there is room beside O and two S buffers; else in shared memory
 // An item is (tile B j, tile A a), numbered w = j NA + a; it uses buffer w % NB.
-template <int MODE_, int DP_, int NA_, int NB_, int BT_, int ST_, int CTAS_, int HV_, bool ATM_>
+template <int MODE_, int DP_, int NA_, int NB_, int BT_, int ST_, int CTAS_, int HV_, bool ATM_, int PL_ = 1>
 struct TcShape {
+  static constexpr int PL = PL_, ACCS = PL == 3 ? 2 : 1, SB = BT_ * ACCS;  // planes, accumulators, columns of an S buffer
   static constexpr int MODE = MODE_, DP = DP_, NA = NA_, NB = NB_, BT = BT_, ST = ST_, CTAS = CTAS_;
   static constexpr int HV = HV_;
   static constexpr int POLY = MODE == TC_STATS ? 8 : 0;
@@ -47,13 +49,21 @@ struct TcShape {
   static constexpr bool SECOND = MODE != TC_STATS;  // the product with P
   static constexpr int WG = NA * HV, HC = BT / HV;
   static constexpr int SUBS = DP / 64;
-  static constexpr int B_BYTES = SUBS * BT * 128;
+  static constexpr int B_BYTES = PL * SUBS * BT * 128;
   static constexpr int META = MODE == TC_GRAD_W ? BT * 14 : 0;
-  static constexpr int A_COL = NB * BT, O_COL = A_COL + (ATM ? NA * (DP / 2) : 0);
-  static constexpr int USED = O_COL + (SECOND ? NA * DP : 0);
+  static constexpr int A_COL = NB * SB, O_COL = A_COL + (ATM ? NA * PL * (DP / 2) : 0);
+  static constexpr int USED = O_COL + (SECOND ? NA * DP * ACCS : 0);
   static constexpr int COLS = USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
-  static constexpr int THREADS = WG * 128 + 64 + (MODE == TC_GRAD_W ? 32 : 0);
-  static constexpr int A_BYTES = ATM ? 0 : SUBS * 128 * 128;
+  // columns of an S buffer that plane pl of a half's P takes: the half's own, which its warp has read
+  __host__ __device__ static constexpr int p_at(int pl, int half) {
+    return pl < 2 ? half * HC + pl * (HC / 2) : BT + half * HC;
+  }
+  static constexpr int THREADS = WG * 128 + 64 + (MODE == TC_GRAD_W && PL == 1 ? 32 : 0);
+  static constexpr int A_BYTES = ATM ? 0 : PL * SUBS * 128 * 128;
+  static constexpr bool WIPES = MODE == TC_GRAD_W && PL == 1;
+  // tiles B after which O is added to sums in registers: every addition to an accumulator in TMEM
+  // truncates, which over hundreds of tiles is more than 32-bit values may lose
+  static constexpr int FLUSH = PL == 3 ? 16 : 0;
   static constexpr int OFF_B = NA * A_BYTES, OFF_META = OFF_B + ST * B_BYTES;
   static constexpr int OFF_BAR = OFF_META + ST * META;
   static constexpr int BARS = 3 * ST + 2 * NB + 3;
@@ -61,6 +71,7 @@ struct TcShape {
   static_assert(USED <= 512 && COLS * CTAS <= 512, "TMEM");
   static_assert(BYTES * CTAS <= 226 * 1024, "shared memory");
   static_assert(MODE != TC_PULL || HV == 1, "a row's running state has one owner");
+  static_assert(PL == 1 || (MODE != TC_PULL && NA == 1), "");
   static_assert(HC % 32 == 0 && META % 16 == 0 && OFF_BAR % 8 == 0, "");
 };
 
@@ -90,45 +101,62 @@ struct TcParams {
 
 // PIECES times 32 elements of a row, `step` elements apart, of which `left` are there (zeros behind
 // them); rows start at multiples of `bytes`.  All loads are requested before the first is used.
-template <typename T, int PIECES>
-__device__ __forceinline__ void row_pieces(Pack<T, 32> (&to)[PIECES], const T* from, int step, int left, int bytes) {
+template <typename V, int PIECES>
+__device__ __forceinline__ void row_pieces(Pack<V, 32> (&to)[PIECES], const V* from, int step, int left, int bytes) {
+  constexpr int E = 16 / sizeof(V);
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
 #pragma unroll
-    for (int q = 0; q < 16; ++q) reinterpret_cast<u32*>(to[i].v)[q] = 0;
+    for (int q = 0; q < 32 * (int)sizeof(V) / 4; ++q) reinterpret_cast<u32*>(to[i].v)[q] = 0;
   }
   if (bytes == 16) {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
 #pragma unroll
-      for (int q = 0; q < 32; q += 8)
-        if (i * step + q + 8 <= left) reinterpret_cast<Pack<T, 8>*>(to[i].v + q)->load(from + i * step + q);
+      for (int q = 0; q < 32; q += E)
+        if (i * step + q + E <= left) reinterpret_cast<Pack<V, E>*>(to[i].v + q)->load(from + i * step + q);
     }
   } else if (bytes >= 4) {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
 #pragma unroll
-      for (int q = 0; q < 32; q += 8)
-        if (i * step + q + 8 <= left) {
+      for (int q = 0; q < 32; q += E)
+        if (i * step + q + E <= left) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) reinterpret_cast<u32*>(to[i].v + q)[e] = __ldg(reinterpret_cast<const u32*>(from + i * step + q) + e);
         }
     }
   }
-  // what no whole piece of 8 covers
+  // what no whole piece of 16 bytes covers
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
 #pragma unroll
-    for (int q = 0; q < 32; q += 8)
-      if (i * step + q < left && (bytes < 4 || i * step + q + 8 > left)) {
+    for (int q = 0; q < 32; q += E)
+      if (i * step + q < left && (bytes < 4 || i * step + q + E > left)) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < E; ++e)
           if (i * step + q + e < left) to[i].v[q + e] = from[i * step + q + e];
       }
   }
 }
 
-template <typename T, typename C>
+// Pairs of values as packed 16-bit elements; with more planes to come, the values become what this
+// plane does not hold.
+template <typename T, int N>
+__device__ __forceinline__ void take_plane(u32 (&h)[N], float* v, bool more) {
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    h[q] = pack2<T>(v[2 * q], v[2 * q + 1]);
+    if (more) {
+      const T* t = reinterpret_cast<const T*>(h + q);
+      v[2 * q] -= to_float(t[0]);
+      v[2 * q + 1] -= to_float(t[1]);
+    }
+  }
+}
+
+// T: type of the planes, V: of the values in memory
+template <typename T, typename V, typename C>
 __global__ void __launch_bounds__(C::THREADS, C::CTAS)
 loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
   extern __shared__ unsigned char smem_raw[];
@@ -141,7 +169,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
   auto p_full = [&](int b) { return bar0 + 8 * (2 * C::ST + C::NB + b); };
   const u32 a_full = bar0 + 8 * (2 * C::ST + 2 * C::NB), o_full = a_full + 8, pv_done = a_full + 16;
   // a tile of B may be read: with dW, after the rows that do not count were wiped
-  auto ready = [&](int s) { return C::MODE == TC_GRAD_W ? a_full + 24 + 8 * s : full(s); };
+  auto ready = [&](int s) { return C::WIPES ? a_full + 24 + 8 * s : full(s); };
   u32* tmem_slot = reinterpret_cast<u32*>(smem + C::OFF_BAR + 8 * C::BARS);
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -157,7 +185,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
     for (int s = 0; s < C::ST; ++s) {
       bar_init(full(s), 1);
       bar_init(empty(s), 1);
-      if (C::MODE == TC_GRAD_W) bar_init(ready(s), 1);
+      if (C::WIPES) bar_init(ready(s), 1);
     }
     for (int b = 0; b < C::NB; ++b) { bar_init(s_full(b), 1); bar_init(p_full(b), 4 * C::HV); }
     bar_init(a_full, 4 * C::WG);
@@ -184,9 +212,10 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
       for (int j = 0; j < my_tiles; ++j) {
         const int st = j % C::ST;
         if (j >= C::ST && !bar_wait(empty(st), ((j / C::ST) - 1) & 1, gave_up, p.err)) break;
-        bar_expect(full(st), (u32)(subs * C::BT * 128 + C::META));
-        for (int s = 0; s < subs; ++s)
-          tma_tile(base + C::OFF_B + st * C::B_BYTES + s * (C::BT * 128), &map_b, s * 64, (t0 + j) * C::BT, 0, full(st));
+        bar_expect(full(st), (u32)(C::PL * subs * C::BT * 128 + C::META));
+        for (int pl = 0; pl < C::PL; ++pl)
+          for (int s = 0; s < subs; ++s)
+            tma_tile(base + C::OFF_B + st * C::B_BYTES + (pl * C::SUBS + s) * (C::BT * 128), &map_b, s * 64, (t0 + j) * C::BT, pl, full(st));
         if (C::META) bulk_copy(base + C::OFF_META + st * C::META, p.meta + (i64)(t0 + j) * C::META, C::META, full(st));
         ++issued;
       }
@@ -202,6 +231,8 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
     if (my_tiles > 0) {
       const bool bf = IsBf16<T>::value;
       const u32 id_s = tc_idesc(bf, C::BT, false, false), id_o = tc_idesc(bf, (u32)ksteps * 16, false, true);
+      constexpr int PAIRS = C::PL == 3 ? 6 : 1;
+      constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
       const bool leader = elect_one();
       bool ok = bar_wait(a_full, 0, gave_up, p.err);
       tc_after();
@@ -210,13 +241,22 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
         if (a == 0) ok = ok && bar_wait(ready(st), (j / C::ST) & 1, gave_up, p.err);
         if (!ok) return;
         tc_after();
-        const u32 A = tmem + C::A_COL + a * (C::DP / 2), d = tmem + (w % C::NB) * C::BT;
+        const u32 A = tmem + C::A_COL + a * (C::DP / 2), d = tmem + (w % C::NB) * C::SB;
         const u64 B = tc_desc(base + C::OFF_B + st * C::B_BYTES, 16), As = tc_desc(base + a * C::A_BYTES, 16);
         if (leader) {
 #pragma unroll
-          for (int k = 0; k < C::DP / 16; ++k)
-            if (k < ksteps && C::ATM) tc_mma_ta(d, A + k * 8, B + ((k >> 2) * (C::BT * 128) + (k & 3) * 32) / 16, id_s, k > 0);
-            else if (k < ksteps) tc_mma(d, As + ((k >> 2) * 16384 + (k & 3) * 32) / 16, B + ((k >> 2) * (C::BT * 128) + (k & 3) * 32) / 16, id_s, k > 0);
+          for (int q = 0; q < PAIRS; ++q) {
+            const int pa = C::PL == 3 ? PA[q] : 0, pb = C::PL == 3 ? PB[q] : 0;
+            const bool high = q == PAIRS - 1;  // the largest products have an accumulator of their own
+            const u32 to = d + (high ? (C::ACCS - 1) * C::BT : 0);
+#pragma unroll
+            for (int k = 0; k < C::DP / 16; ++k) {
+              const u64 b = B + ((pb * C::SUBS + (k >> 2)) * (C::BT * 128) + (k & 3) * 32) / 16;
+              const bool add = k > 0 || (q > 0 && !high);
+              if (k < ksteps && C::ATM) tc_mma_ta(to, A + pa * (C::DP / 2) + k * 8, b, id_s, add);
+              else if (k < ksteps) tc_mma(to, As + ((pa * C::SUBS + (k >> 2)) * 16384 + (k & 3) * 32) / 16, b, id_s, add);
+            }
+          }
           tc_commit(s_full(w % C::NB));
           if (!C::SECOND && a == C::NA - 1) tc_commit(empty(st));
         }
@@ -228,14 +268,21 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
         if (!ok) break;
         if (C::SECOND) {
           tc_after();
-          const u32 P = tmem + b * C::BT, d = tmem + C::O_COL + a * C::DP;
+          const u32 P = tmem + b * C::SB, d = tmem + C::O_COL + a * C::DP;
           const u64 B = tc_desc(base + C::OFF_B + st * C::B_BYTES, C::BT * 128);
+          const bool fresh = C::FLUSH ? j % (C::FLUSH ? C::FLUSH : 1) == 0 : j == 0;
           if (leader) {
 #pragma unroll
-            for (int k = 0; k < C::BT / 16; ++k)
-              tc_mma_ta(d, P + (k / (C::HC / 16)) * C::HC + (k % (C::HC / 16)) * 8, B + k * (2048 / 16), id_o, j > 0 || k > 0);
+            for (int q = 0; q < PAIRS; ++q) {
+              const int pa = C::PL == 3 ? PA[q] : 0, pb = C::PL == 3 ? PB[q] : 0;
+              const bool high = q == PAIRS - 1;
+#pragma unroll
+              for (int k = 0; k < C::BT / 16; ++k)
+                tc_mma_ta(d + (high ? (C::ACCS - 1) * C::DP : 0), P + C::p_at(pa, k / (C::HC / 16)) + (k % (C::HC / 16)) * 8,
+                          B + (pb * C::SUBS * (C::BT * 128) + k * 2048) / 16, id_o, !fresh || k > 0 || (q > 0 && !high));
+            }
             if (a == C::NA - 1) tc_commit(empty(st));
-            if (C::MODE == TC_PULL && C::NA == 1 && C::NB > 1) tc_commit(pv_done);
+            if (C::FLUSH || (C::MODE == TC_PULL && C::NA == 1 && C::NB > 1)) tc_commit(pv_done);
           }
         }
         if (w + C::NB < items) product_s(w + C::NB);
@@ -244,7 +291,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
       // the products that were issued end by themselves; a bounded look keeps the order when a wait gave up
       for (int k = 0; k < (1 << 16) && !bar_try(o_full, 0); ++k) __nanosleep(32);
     }
-  } else if (C::MODE == TC_GRAD_W && warp == C::WG * 4 + 2) {
+  } else if (C::WIPES && warp == C::WG * 4 + 2) {
     // ------------------------------------------------ rows that do not count must not reach a product with a NaN
     // P is zero there, which is enough unless the row holds an infinity or a NaN, and then its
     // log-sum-exp is not finite either (every logit has a term that is not): only those are wiped.
@@ -278,22 +325,32 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
     const bool row_live = row < p.rows_a && (C::MODE != TC_GRAD_X || p.g[row < p.rows_a ? row : 0] != 0.f);
     constexpr int PIECES = C::DP / (32 * C::HV);
     {
-      Pack<T, 32> piece[PIECES];
-      row_pieces(piece, (const T*)p.a + (i64)row * p.lda + half * 32, 32 * C::HV, row_live ? p.D - half * 32 : 0, p.a_bytes);
+      Pack<V, 32> piece[PIECES];
+      row_pieces(piece, (const V*)p.a + (i64)row * p.lda + half * 32, 32 * C::HV, row_live ? p.D - half * 32 : 0, p.a_bytes);
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
         const int k = half * 32 + i * (32 * C::HV);
         if (k < ksteps * 16) {
 #pragma unroll
-          for (int q = 0; q < 16; ++q) reinterpret_cast<u32*>(piece[i].v)[q] ^= p.a_sign;
-          if constexpr (C::ATM) {
-            tc_st16(tmem + C::A_COL + a * (C::DP / 2) + k / 2 + lanes, reinterpret_cast<const u32*>(piece[i].v));
-          } else {  // as a swizzled tile: 16-byte piece c of row r lies at c ^ (r & 7)
-            const int r = quarter * 32 + lane;
-            unsigned char* to = smem + a * C::A_BYTES + (k >> 6) * 16384 + r * 128;
+          for (int pl = 0; pl < C::PL; ++pl) {
+            u32 h[16];
+            if constexpr (C::PL == 1) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              *reinterpret_cast<uint4*>(to + ((((k & 63) >> 3) + q) ^ (r & 7)) * 16) = reinterpret_cast<const uint4*>(piece[i].v)[q];
+              for (int q = 0; q < 16; ++q) h[q] = reinterpret_cast<const u32*>(piece[i].v)[q];
+            } else {
+              take_plane<T>(h, reinterpret_cast<float*>(piece[i].v), pl + 1 < C::PL);
+            }
+#pragma unroll
+            for (int q = 0; q < 16; ++q) h[q] ^= p.a_sign;
+            if constexpr (C::ATM) {
+              tc_st16(tmem + C::A_COL + (a * C::PL + pl) * (C::DP / 2) + k / 2 + lanes, h);
+            } else {  // as a swizzled tile: 16-byte piece c of row r lies at c ^ (r & 7)
+              const int r = quarter * 32 + lane;
+              unsigned char* to = smem + a * C::A_BYTES + (pl * C::SUBS + (k >> 6)) * 16384 + r * 128;
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<uint4*>(to + ((((k & 63) >> 3) + q) ^ (r & 7)) * 16) = reinterpret_cast<const uint4*>(h)[q];
+            }
           }
         }
       }
@@ -327,6 +384,25 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
       row_bias = -p.lse2[row];
     }
     bool ok = true;
+    float kept[C::FLUSH ? PIECES * 32 : 1];  // O of the tiles before the last flush, this warp's columns of it
+    if constexpr (C::FLUSH != 0) {
+#pragma unroll
+      for (int q = 0; q < PIECES * 32; ++q) kept[q] = 0.f;
+    }
+    auto keep = [&]() {  // both accumulators of O into the sums
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int k = half * 32 + i * (32 * C::HV);
+        if (k < ksteps * 16) {
+          float o[32], u[32];
+          tc_ld32(o, tmem + C::O_COL + k + lanes);
+          tc_ld32(u, tmem + C::O_COL + C::DP + k + lanes);
+          tc_wait_ld();
+#pragma unroll
+          for (int q = 0; q < 32; ++q) kept[i * 32 + q] += o[q] + u[q];
+        }
+      }
+    };
     for (int w = a; w < items; w += C::NA) {
       const int j = w / C::NA, st = j % C::ST, b = w % C::NB;
       ok = bar_wait(s_full(b), (w / C::NB) & 1, gave_up, p.err);
@@ -334,11 +410,28 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_after();
+      if constexpr (C::SECOND && C::FLUSH != 0) {
+        if (j > 0 && j % C::FLUSH == 0) {
+          ok = __all_sync(0xffffffffu, bar_wait(pv_done, (w - 1) & 1, gave_up, p.err));
+          if (!ok) break;
+          tc_after();
+          if (warp_live) keep();
+        }
+      }
       if (warp_live) {
-        const u32 S = tmem + b * C::BT + half * C::HC + lanes;
+        const u32 S = tmem + b * C::SB + half * C::HC + lanes;
         float v[C::HC];
 #pragma unroll
-        for (int k = 0; k < C::HC; k += 32) tc_ld32(v + k, S + k);
+        for (int k = 0; k < C::HC; k += 32) {
+          tc_ld32(v + k, S + k);
+          if constexpr (C::ACCS == 2) {
+            float u[32];
+            tc_ld32(u, S + C::BT + k);
+            tc_wait_ld();
+#pragma unroll
+            for (int q = 0; q < 32; ++q) v[k + q] += u[q];
+          }
+        }
         tc_wait_ld();
         if constexpr (C::MODE == TC_GRAD_W) {
           const unsigned char* meta = smem + C::OFF_META + st * C::META + half * C::HC * 4;
@@ -362,6 +455,12 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
               if (tgt[k] == row) v[k] -= gs[k];
           }
         } else if constexpr (C::MODE == TC_GRAD_X) {
+          const int col0 = (t0 + j) * C::BT + half * C::HC;
+          if (col0 + C::HC > p.rows_b) {  // behind the vocabulary: a logit of 0 may lie far above the row's own
+#pragma unroll
+            for (int k = 0; k < C::HC; ++k)
+              if (col0 + k >= p.rows_b) v[k] = -INFINITY;
+          }
           const u64 bias2 = both(row_bias), gs2 = both(gs);
 #pragma unroll
           for (int k = 0; k < C::HC; k += 2) {
@@ -431,20 +530,22 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
         }
         if constexpr (C::SECOND) {
           // each half's P takes the first columns of the half's own S: a warp overwrites what it has read itself
-          u32 h[C::HC / 2];
 #pragma unroll
-          for (int q = 0; q < C::HC / 2; ++q) h[q] = pack2<T>(v[2 * q], v[2 * q + 1]);
-          if constexpr (C::MODE == TC_GRAD_W) {
-            // rows with a negative upstream gradient: the sign of their whole column
-            const u32* sign = reinterpret_cast<const u32*>(smem + C::OFF_META + st * C::META + 12 * C::BT) + half * (C::HC / 2);
-            const u32 own = sign[lane % (C::HC / 2)];
-            if (__any_sync(0xffffffffu, own != 0)) {
+          for (int pl = 0; pl < C::PL; ++pl) {
+            u32 h[C::HC / 2];
+            take_plane<T>(h, v, pl + 1 < C::PL);
+            if constexpr (C::MODE == TC_GRAD_W) {
+              // rows with a negative upstream gradient: the sign of their whole column
+              const u32* sign = reinterpret_cast<const u32*>(smem + C::OFF_META + st * C::META + 12 * C::BT) + half * (C::HC / 2);
+              const u32 own = sign[lane % (C::HC / 2)];
+              if (__any_sync(0xffffffffu, own != 0)) {
 #pragma unroll
-              for (int q = 0; q < C::HC / 2; ++q) h[q] ^= sign[q];
+                for (int q = 0; q < C::HC / 2; ++q) h[q] ^= sign[q];
+              }
             }
-          }
 #pragma unroll
-          for (int q = 0; q < C::HC / 2; q += 16) tc_st16(S + q, h + q);
+            for (int q = 0; q < C::HC / 2; q += 16) tc_st16(tmem + b * C::SB + C::p_at(pl, half) + lanes + q, h + q);
+          }
           tc_wait_st();
         }
       }
@@ -456,28 +557,36 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
       p.part_ms[(i64)(blockIdx.y * C::HV + half) * p.rows_a + row] = make_float2(m, sum);
     if (C::MODE == TC_PULL && row < p.rows_a && ok) p.part_ms[(i64)blockIdx.y * p.rows_a + row] = make_float2(m, sum);
     // dx: the target's own row is taken off in 32 bits
-    Pack<T, 32> target_row[C::MODE == TC_GRAD_X ? PIECES : 1];
-    if constexpr (C::MODE == TC_GRAD_X)
-      row_pieces(target_row, (const T*)p.w + (i64)(hot < 0 ? 0 : hot) * p.ldw + half * 32, 32 * C::HV, row_live ? p.D - half * 32 : 0, p.w_bytes);
+    constexpr int AHEAD = C::MODE == TC_GRAD_X && C::PL == 1 ? PIECES : 1;  // pieces of it requested before the wait
+    Pack<V, 32> target_row[AHEAD];
+    if (C::MODE == TC_GRAD_X && C::PL == 1 && gridDim.y == 1)
+      row_pieces(target_row, (const V*)p.w + (i64)(hot < 0 ? 0 : hot) * p.ldw + half * 32, 32 * C::HV, row_live ? p.D - half * 32 : 0, p.w_bytes);
     if (C::SECOND && my_tiles > 0) {
       ok = ok && bar_wait(o_full, 0, gave_up, p.err);
       ok = __all_sync(0xffffffffu, ok);
       if (ok && warp_live) {
         tc_after();
+        if constexpr (C::FLUSH != 0) keep();
         const float f = C::MODE == TC_PULL ? 1.f : p.out_scale * __uint_as_float(*p.top);
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
           const int k = half * 32 + i * (32 * C::HV);
           if (k >= p.D) break;
           float o[32];
-          tc_ld32(o, tmem + C::O_COL + a * C::DP + k + lanes);
-          tc_wait_ld();
+          if constexpr (C::FLUSH != 0) {
+#pragma unroll
+            for (int q = 0; q < 32; ++q) o[q] = kept[i * 32 + q];
+          } else {
+            tc_ld32(o, tmem + C::O_COL + a * C::DP + k + lanes);
+            tc_wait_ld();
+          }
           if (row < p.rows_a) {
-            const bool slab = C::MODE == TC_PULL || (C::MODE == TC_GRAD_W && gridDim.y > 1);
-            if (C::MODE == TC_GRAD_X) {
+            const bool slab = C::MODE == TC_PULL || gridDim.y > 1;
+            if (C::MODE == TC_GRAD_X && !slab) {
+              if (C::PL == 3) row_pieces(target_row, (const V*)p.w + (i64)(hot < 0 ? 0 : hot) * p.ldw + k, 0, row_live ? p.D - k : 0, p.w_bytes);
               // a row that does not count is zero
 #pragma unroll
-              for (int q = 0; q < 32; ++q) o[q] = row_live ? fmaf(-gs, to_float(target_row[C::MODE == TC_GRAD_X ? i : 0].v[q]), o[q]) : 0.f;
+              for (int q = 0; q < 32; ++q) o[q] = row_live ? fmaf(-gs, to_float(target_row[AHEAD == 1 ? 0 : i].v[q]), o[q]) : 0.f;
             }
             if (slab) {
               float* to = p.part_o + ((i64)blockIdx.y * p.rows_a + row) * p.D + k;
@@ -491,7 +600,18 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
                   if (k + q < p.D) to[q] = o[q] * f;
               }
             } else {
-              T* to = (T*)p.out + (i64)row * p.D + k;
+              V* to = (V*)p.out + (i64)row * p.D + k;
+              if constexpr (C::PL == 3) {
+                if ((p.D & 3) == 0) {
+#pragma unroll
+                  for (int q = 0; q < 8; ++q)
+                    if (k + 4 * q < p.D) reinterpret_cast<float4*>(to)[q] = make_float4(o[4 * q] * f, o[4 * q + 1] * f, o[4 * q + 2] * f, o[4 * q + 3] * f);
+                } else {
+#pragma unroll
+                  for (int q = 0; q < 32; ++q)
+                    if (k + q < p.D) to[q] = o[q] * f;
+                }
+              } else {
               u32 h[16];
 #pragma unroll
               for (int q = 0; q < 16; ++q) h[q] = pack2<T>(o[2 * q] * f, o[2 * q + 1] * f);
@@ -510,7 +630,8 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
               } else {
 #pragma unroll
                 for (int q = 0; q < 32; ++q)
-                  if (k + q < p.D) to[q] = reinterpret_cast<const T*>(h)[q];
+                  if (k + q < p.D) to[q] = reinterpret_cast<const V*>(h)[q];
+              }
               }
             }
           }
@@ -658,6 +779,21 @@ __global__ void loss_dx_kernel(const float* __restrict__ pull, const float* __re
   }
 }
 
+// dx[i] = sum over the slabs, less the target's row; zeros for a row that does not count
+template <typename T>
+__global__ void loss_join_dx_kernel(const float* __restrict__ slab, i64 N, int D, int slabs, const float* __restrict__ g, float scale,
+                                    const i64* __restrict__ target, const T* __restrict__ w, i64 ldw, T* __restrict__ dx) {
+  for (i64 e = (i64)blockIdx.x * blockDim.x + threadIdx.x; e < N * D; e += (i64)gridDim.x * blockDim.x) {
+    const i64 r = e / D;
+    float v = 0.f;
+    if (g[r] != 0.f) {
+      for (int z = 0; z < slabs; ++z) v += slab[z * (N * D) + e];
+      v = fmaf(-g[r] * scale, to_float(w[target[r] * ldw + (e - r * D)]), v);
+    }
+    dx[e] = from_float<T>(v);
+  }
+}
+
 // out[e] = sum over the slabs: 32 elements a CTA, eight runs of slabs each, joined in order
 template <typename T>
 __global__ void __launch_bounds__(256) loss_join_dw_kernel(const float* __restrict__ slab, i64 size, int slabs, T* __restrict__ out) {
@@ -715,6 +851,13 @@ typedef TcShape<TC_PULL, 128, 1, 1, 64, 6, 2, 1, true> PullFew128;
 typedef TcShape<TC_GRAD_X, 64, 1, 2, 64, 4, 2, 2, true> GradX64;
 typedef TcShape<TC_GRAD_X, 128, 1, 1, 64, 4, 2, 2, true> GradX128;
 typedef TcShape<TC_GRAD_X, 256, 1, 2, 64, 3, 1, 2, true> GradX256;
+// fp32: the products are six times as many, so one tile A and small tiles B are enough to hide the rest
+typedef TcShape<TC_STATS, 64, 1, 3, 64, 5, 1, 2, true, 3> StatsF64;
+typedef TcShape<TC_STATS, 128, 1, 2, 64, 2, 1, 2, false, 3> StatsF128;
+typedef TcShape<TC_GRAD_X, 64, 1, 2, 64, 5, 1, 2, true, 3> GradXF64;
+typedef TcShape<TC_GRAD_X, 128, 1, 1, 64, 2, 1, 2, false, 3> GradXF128;
+typedef TcShape<TC_GRAD_W, 64, 1, 2, 64, 5, 1, 2, true, 3> GradF64;
+typedef TcShape<TC_GRAD_W, 128, 1, 1, 64, 2, 1, 2, false, 3> GradF128;
 typedef TcShape<TC_GRAD_W, 64, 2, 2, 128, 6, 1, 2, true> Grad64;
 typedef TcShape<TC_GRAD_W, 128, 1, 2, 128, 4, 1, 2, true> Grad128;
 typedef TcShape<TC_GRAD_W, 256, 1, 2, 64, 5, 1, 2, true> Grad256;
@@ -729,8 +872,13 @@ constexpr i64 SMALL_V = 2048;
 // rows against the vocabulary; a small vocabulary under many rows), two small CTAs an SM overlap one's
 // loads with the other's products; else one large CTA keeps the tensor cores busier.  dW, 1024 x
 // 232965 x 112: 0.154 ms with two, 0.182 with one; 8192 x 300000 x 128: 1.043 and 0.949.
-template <typename F>
+template <int PL, typename F>
 static auto with_shape(int mode, i64 N, i64 V, i64 D, F f) {
+  if constexpr (PL == 3) {
+    if (mode == TC_STATS) return D > 64 ? f(StatsF128()) : f(StatsF64());
+    if (mode == TC_GRAD_X) return D > 64 ? f(GradXF128()) : f(GradXF64());
+    return D > 64 ? f(GradF128()) : f(GradF64());
+  } else {
   if (mode == TC_STATS) {
     if (N <= 128 || V <= SMALL_V) return D > 128 ? f(StatsFew256()) : D > 64 ? f(StatsFew128()) : f(StatsFew64());
     return D > 128 ? f(Stats256()) : D > 64 ? f(Stats128()) : f(Stats64());
@@ -744,50 +892,63 @@ static auto with_shape(int mode, i64 N, i64 V, i64 D, F f) {
   if (D > 128) return f(Grad256());
   if (N <= 2048) return D > 64 ? f(GradFew128()) : f(GradFew64());
   return D > 64 ? f(Grad128()) : f(Grad64());
+  }
 }
 
+template <int PL>
 static TcPlan tc_plan(int mode, i64 N, i64 V, i64 D) {
-  return with_shape(mode, N, V, D, [&](auto shape) {
+  return with_shape<PL>(mode, N, V, D, [&](auto shape) {
     return mode == TC_GRAD_W ? plan_of<decltype(shape)>(V, N) : plan_of<decltype(shape)>(N, V);
   });
 }
 
-bool tc_loss_takes(int dtype, i64 D) { return dtype != GSB_F32 && D <= 256; }
-bool tc_loss_pulls(i64 V) { return V > SMALL_V; }
+static TcPlan tc_plan(int planes, int mode, i64 N, i64 V, i64 D) {
+  return planes == 3 ? tc_plan<3>(mode, N, V, D) : tc_plan<1>(mode, N, V, D);
+}
+
+bool tc_loss_takes(int dtype, i64 D) { return D <= (dtype == GSB_F32 ? 128 : 256); }
+// fp32 makes the logits once more instead (a row's state and its sums of O would not fit beside one another)
+bool tc_loss_pulls(int dtype, i64 V) { return dtype != GSB_F32 && V > SMALL_V; }
+
+// rows of a streamed matrix as TMA takes them: a copy where its address or row step does not do, planes for fp32
+static size_t copy_bytes(int planes, i64 rows, i64 D) { return 2 * (size_t)planes * rows * packed_ld(D); }
 
 struct TcFwdLayout { size_t ms, hot, o, w, bytes; };
-static TcFwdLayout fwd_layout(i64 N, i64 V, i64 D, bool pull) {
+static TcFwdLayout fwd_layout(int planes, i64 N, i64 V, i64 D, bool pull) {
   TcFwdLayout L;
   size_t o = 0;
   auto take = [&](size_t b) { const size_t at = o; o += up256(b); return at; };
-  const TcPlan p = tc_plan(pull ? TC_PULL : TC_STATS, N, V, D);
+  const TcPlan p = tc_plan(planes, pull ? TC_PULL : TC_STATS, N, V, D);
   L.ms = take(8 * (size_t)p.parts * N);
   L.hot = take(pull ? 0 : 4 * (size_t)N);
   L.o = take(pull ? 4 * (size_t)p.splits * N * D : 0);
-  // whether the rows of W have to be copied depends on its address and row step
-  L.w = take(2 * (size_t)V * packed_ld(D));
+  L.w = take(copy_bytes(planes, V, D));
   L.bytes = o;
   return L;
 }
-size_t tc_loss_workspace(i64 N, i64 V, i64 D, bool pull, bool pack_w) {
-  const TcFwdLayout L = fwd_layout(N, V, D, pull);
-  return pack_w ? L.bytes : L.w;
+size_t tc_loss_workspace(int dtype, i64 N, i64 V, i64 D, bool pull, bool pack_w) {
+  const int planes = dtype == GSB_F32 ? 3 : 1;
+  const TcFwdLayout L = fwd_layout(planes, N, V, D, pull);
+  return pack_w || planes == 3 ? L.bytes : L.w;
 }
 
-struct TcGradLayout { size_t meta, slab, x, w, bytes; };
-static TcGradLayout grad_layout(i64 N, i64 V, i64 D, bool dx, bool dw) {
+struct TcGradLayout { size_t meta, dw_slab, dx_slab, x, w, bytes; };
+static TcGradLayout grad_layout(int planes, i64 N, i64 V, i64 D, bool dx, bool dw) {
   TcGradLayout L;
   size_t o = 0;
   auto take = [&](size_t b) { const size_t at = o; o += up256(b); return at; };
-  const TcPlan p = tc_plan(TC_GRAD_W, N, V, D);
-  L.meta = take(dw ? (size_t)((N + p.BT - 1) / p.BT) * p.BT * 14 : 0);
-  L.slab = take(dw && p.splits > 1 ? 4 * (size_t)p.splits * V * D : 0);
-  L.x = take(dw ? 2 * (size_t)N * packed_ld(D) : 0);
-  L.w = take(dx ? 2 * (size_t)V * packed_ld(D) : 0);
+  const TcPlan w = tc_plan(planes, TC_GRAD_W, N, V, D), x = tc_plan(planes, TC_GRAD_X, N, V, D);
+  L.meta = take(dw ? (size_t)((N + w.BT - 1) / w.BT) * w.BT * 14 : 0);
+  L.dw_slab = take(dw && w.splits > 1 ? 4 * (size_t)w.splits * V * D : 0);
+  L.dx_slab = take(dx && x.splits > 1 ? 4 * (size_t)x.splits * N * D : 0);
+  L.x = take(dw ? copy_bytes(planes, N, D) : 0);
+  L.w = take(dx ? copy_bytes(planes, V, D) : 0);
   L.bytes = o;
   return L;
 }
-size_t tc_loss_grad_workspace(i64 N, i64 V, i64 D, bool dx, bool dw) { return grad_layout(N, V, D, dx, dw).bytes; }
+size_t tc_loss_grad_workspace(int dtype, i64 N, i64 V, i64 D, bool dx, bool dw) {
+  return grad_layout(dtype == GSB_F32 ? 3 : 1, N, V, D, dx, dw).bytes;
+}
 bool tc_loss_packs(const void* w, i64 ldw) { return !tma_ready(w, ldw); }
 
 template <typename T>
@@ -796,17 +957,18 @@ static const T* pack_rows(const T* src, i64 ld, i64 rows, i64 D, void* dst, cuda
   loss_pack_kernel<T><<<blocks_for(rows * packed_ld(D) / 8), 256, 0, st>>>(src, ld, rows, (int)D, (int)packed_ld(D), (T*)dst);
   return (const T*)dst;
 }
-static int row_bytes(const void* p, i64 ld) {
-  const uintptr_t m = (uintptr_t)p | (uintptr_t)(ld * 2);
+static int row_bytes(const void* p, i64 ld, int size) {
+  const uintptr_t m = (uintptr_t)p | (uintptr_t)(ld * size);
   return m & 2 ? 2 : m & 4 ? 4 : m & 8 ? 8 : 16;
 }
 
-template <typename T, typename C>
+template <typename V, typename C>
 static int launch_tc(const CUtensorMap& b, const TcPlan& plan, const TcParams& p, int kid, cudaStream_t st) {
+  typedef typename Planes<V>::type T;
   // the attribute belongs to the device's copy of the kernel; setting it is cheap and not a stream operation
-  GSB_CUDA_OK(cudaFuncSetAttribute(loss_tc_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
+  GSB_CUDA_OK(cudaFuncSetAttribute(loss_tc_kernel<T, V, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
   LaunchScope ls(kid, st);
-  loss_tc_kernel<T, C><<<dim3((unsigned)plan.groups, (unsigned)plan.splits), C::THREADS, C::BYTES, st>>>(b, p);
+  loss_tc_kernel<T, V, C><<<dim3((unsigned)plan.groups, (unsigned)plan.splits), C::THREADS, C::BYTES, st>>>(b, p);
   return GSB_OK;
 }
 
@@ -823,7 +985,7 @@ static TcParams base_params(const LossArgs& a, const TcPlan& plan, bool vocabula
   TcParams p = {};
   p.a = vocabulary_side ? a.w : a.x;
   p.lda = vocabulary_side ? a.ldw : a.ldx;
-  p.a_bytes = row_bytes(p.a, p.lda);
+  p.a_bytes = row_bytes(p.a, p.lda, sizeof(T));
   // l = |scale| (+-A) . B: the running maximum needs a factor that is not negative
   p.a_sign = a.scale < 0.f ? 0x80008000u : 0u;
   p.rows_a = (int)(vocabulary_side ? a.V : a.N);
@@ -839,26 +1001,35 @@ static TcParams base_params(const LossArgs& a, const TcPlan& plan, bool vocabula
   p.err = a.err;
   return p;
 }
-// the map of the streamed matrix; rows that TMA does not take as they lie are copied to `copy` first
+// The map of the streamed matrix; rows that TMA does not take as they lie are copied to `copy` first.
+// fp32 rows go there as planes, those whose g is zero as zeros.
 template <typename T>
-static bool stream_map(CUtensorMap* map, const void* src, i64 ld, i64 rows, i64 D, int box_rows, void* copy, cudaStream_t st) {
-  if (!tma_ready(src, ld)) { src = pack_rows<T>((const T*)src, ld, rows, D, copy, st); ld = packed_ld(D); }
-  return tc_map(map, src, IsBf16<T>::value, rows, D, ld, 1, 64, box_rows);
+static bool stream_map(CUtensorMap* map, const void* src, i64 ld, i64 rows, i64 D, int box_rows, const float* g, void* copy, cudaStream_t st) {
+  constexpr int planes = Planes<T>::count;
+  if constexpr (planes == 3) {
+    make_planes<T>(src, ld, rows, D, false, g, copy, st);
+    src = copy;
+    ld = packed_ld(D);
+  } else if (!tma_ready(src, ld)) {
+    src = pack_rows<T>((const T*)src, ld, rows, D, copy, st);
+    ld = packed_ld(D);
+  }
+  return tc_map(map, src, IsBf16<typename Planes<T>::type>::value, rows, D, ld, planes, 64, box_rows);
 }
 
 template <typename T>
 int tc_loss_forward(const LossArgs& a, float* pull) {
   const int mode = pull ? TC_PULL : TC_STATS;
-  const TcPlan plan = tc_plan(mode, a.N, a.V, a.D);
-  const TcFwdLayout L = fwd_layout(a.N, a.V, a.D, pull != nullptr);
+  const TcPlan plan = tc_plan(Planes<T>::count, mode, a.N, a.V, a.D);
+  const TcFwdLayout L = fwd_layout(Planes<T>::count, a.N, a.V, a.D, pull != nullptr);
   char* ws = (char*)a.ws;
   CUtensorMap mb;
-  if (!stream_map<T>(&mb, a.w, a.ldw, a.V, a.D, plan.BT, ws + L.w, a.st)) return GSB_ERR_CUDA;
+  if (!stream_map<T>(&mb, a.w, a.ldw, a.V, a.D, plan.BT, nullptr, ws + L.w, a.st)) return GSB_ERR_CUDA;
   TcParams p = base_params<T>(a, plan, false);
   p.part_ms = (float2*)(ws + L.ms);
   p.part_o = (float*)(ws + L.o);
   p.hot = (float*)(ws + L.hot);
-  const int rc = with_shape(mode, a.N, a.V, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS, a.st); });
+  const int rc = with_shape<Planes<T>::count>(mode, a.N, a.V, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS, a.st); });
   if (rc != GSB_OK) return rc;
   if (pull) {
     launch_loss_join<T>(a, p.part_ms, plan.parts, p.part_o, pull);
@@ -874,8 +1045,8 @@ int tc_loss_forward(const LossArgs& a, float* pull) {
 
 template <typename T>
 int tc_loss_grad_w(const LossArgs& a) {
-  const TcPlan plan = tc_plan(TC_GRAD_W, a.N, a.V, a.D);
-  const TcGradLayout L = grad_layout(a.N, a.V, a.D, a.dx != nullptr, true);
+  const TcPlan plan = tc_plan(Planes<T>::count, TC_GRAD_W, a.N, a.V, a.D);
+  const TcGradLayout L = grad_layout(Planes<T>::count, a.N, a.V, a.D, a.dx != nullptr, true);
   char* ws = (char*)a.ws;
   {
     const i64 npad = (a.N + plan.BT - 1) / plan.BT * plan.BT;
@@ -883,12 +1054,12 @@ int tc_loss_grad_w(const LossArgs& a) {
     loss_meta_kernel<<<ceil_div_i(npad, 256), 256, 0, a.st>>>(a.lse2, a.target, a.g, a.top, a.N, npad, plan.BT, (unsigned char*)(ws + L.meta));
   }
   CUtensorMap mb;
-  if (!stream_map<T>(&mb, a.x, a.ldx, a.N, a.D, plan.BT, ws + L.x, a.st)) return GSB_ERR_CUDA;
+  if (!stream_map<T>(&mb, a.x, a.ldx, a.N, a.D, plan.BT, a.g, ws + L.x, a.st)) return GSB_ERR_CUDA;
   TcParams p = base_params<T>(a, plan, true);
   p.meta = (const unsigned char*)(ws + L.meta);
-  p.part_o = (float*)(ws + L.slab);
+  p.part_o = (float*)(ws + L.dw_slab);
   p.out = a.dw;
-  const int rc = with_shape(TC_GRAD_W, a.N, a.V, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS_GRAD, a.st); });
+  const int rc = with_shape<Planes<T>::count>(TC_GRAD_W, a.N, a.V, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS_GRAD, a.st); });
   if (rc != GSB_OK) return rc;
   if (plan.splits > 1) {
     LaunchScope ls(KID_LOSS_JOIN, a.st);
@@ -897,21 +1068,27 @@ int tc_loss_grad_w(const LossArgs& a) {
   return GSB_OK;
 }
 
-// dx of a small vocabulary
+// dx by making the logits again
 template <typename T>
 int tc_loss_grad_x(const LossArgs& a) {
-  TcPlan plan = tc_plan(TC_GRAD_X, a.N, a.V, a.D);
-  plan.splits = 1;  // a CTA sees the whole vocabulary
-  plan.per = (int)((a.V + plan.BT - 1) / plan.BT);
-  const TcGradLayout L = grad_layout(a.N, a.V, a.D, true, a.dw != nullptr);
+  const TcPlan plan = tc_plan(Planes<T>::count, TC_GRAD_X, a.N, a.V, a.D);
+  const TcGradLayout L = grad_layout(Planes<T>::count, a.N, a.V, a.D, true, a.dw != nullptr);
+  char* ws = (char*)a.ws;
   CUtensorMap mb;
-  if (!stream_map<T>(&mb, a.w, a.ldw, a.V, a.D, plan.BT, (char*)a.ws + L.w, a.st)) return GSB_ERR_CUDA;
+  if (!stream_map<T>(&mb, a.w, a.ldw, a.V, a.D, plan.BT, nullptr, ws + L.w, a.st)) return GSB_ERR_CUDA;
   TcParams p = base_params<T>(a, plan, false);
   p.w = a.w;
   p.ldw = a.ldw;
-  p.w_bytes = row_bytes(a.w, a.ldw);
+  p.w_bytes = row_bytes(a.w, a.ldw, sizeof(T));
   p.out = a.dx;
-  return with_shape(TC_GRAD_X, a.N, a.V, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS_GRAD, a.st); });
+  p.part_o = (float*)(ws + L.dx_slab);
+  const int rc = with_shape<Planes<T>::count>(TC_GRAD_X, a.N, a.V, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS_GRAD, a.st); });
+  if (rc != GSB_OK) return rc;
+  if (plan.splits > 1) {
+    LaunchScope ls(KID_LOSS_JOIN, a.st);
+    loss_join_dx_kernel<T><<<blocks_for(a.N * a.D), 256, 0, a.st>>>(p.part_o, a.N, (int)a.D, plan.splits, a.g, a.scale, a.target, (const T*)a.w, a.ldw, (T*)a.dx);
+  }
+  return GSB_OK;
 }
 
 template <typename T>
@@ -923,10 +1100,13 @@ void tc_loss_dx(const LossArgs& a, const float* pull) {
 template void launch_loss_join<float>(const LossArgs&, const float2*, int, const float*, float*);
 template void launch_loss_join<__half>(const LossArgs&, const float2*, int, const float*, float*);
 template void launch_loss_join<__nv_bfloat16>(const LossArgs&, const float2*, int, const float*, float*);
+template int tc_loss_forward<float>(const LossArgs&, float*);
 template int tc_loss_forward<__half>(const LossArgs&, float*);
 template int tc_loss_forward<__nv_bfloat16>(const LossArgs&, float*);
+template int tc_loss_grad_w<float>(const LossArgs&);
 template int tc_loss_grad_w<__half>(const LossArgs&);
 template int tc_loss_grad_w<__nv_bfloat16>(const LossArgs&);
+template int tc_loss_grad_x<float>(const LossArgs&);
 template int tc_loss_grad_x<__half>(const LossArgs&);
 template int tc_loss_grad_x<__nv_bfloat16>(const LossArgs&);
 template void tc_loss_dx<__half>(const LossArgs&, const float*);
