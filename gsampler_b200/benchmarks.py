@@ -9,6 +9,9 @@ repository root holds the headline one):
                                                   # a 1 M-node / 50 M-edge graph (a profiling shape)
     python -m gsampler_b200.benchmarks weighted   # weighted per-column sampling of a column slice, same
                                                   # 1 M-node graph: 400 000 columns, K = 10 and K = 5
+    python -m gsampler_b200.benchmarks embed      # one training step on node2vec walks: 1024 walkers x 8 steps,
+                                                  # embedding rows, dropout, full softmax over all 2 449 029
+                                                  # nodes (128 columns, bf16), both tables' gradients and update
     python -m gsampler_b200.benchmarks gather     # feature fetch: 4 M rows of 100 fp32 out of 2 449 029
     python -m gsampler_b200.benchmarks cfg5       # the same on the full 111 M nodes / 3.2 G edges (14 GB)
     python -m gsampler_b200.benchmarks cfg5s      # GraphSAGE [15,10,5] on an int32-index R-MAT-like
@@ -318,9 +321,59 @@ def cfg5s(steps=6, warmup=3, n=11105996, e=320000000, large=False):
                                  "mean_SEU_per_layer": c.double().mean(0).tolist()}}))
 
 
+def embed(steps=5, warmup=2, walkers=1024, length=8, D=128, p=0.1):
+    """Walks -> (node, next node) pairs -> embedding -> dropout -> softmax over every node -> gradients ->
+    plain gradient step on both tables."""
+    dev = torch.device("cuda")
+    n, e = 2449029, 123718280
+    indptr, indices = synth.powerlaw_csc(n, e, exponent=2.1, max_degree=20000, seed=2024, device=dev)
+    A = gs.Graph(n, n)
+    A._CAPI_LoadCSC(indptr, indices)
+    A._CAPI_SortCSCIndices()
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(11)
+    table = torch.empty(n, D, dtype=torch.bfloat16, device=dev).normal_(0, 1, generator=gen).requires_grad_()
+    out = torch.empty(n, D, dtype=torch.bfloat16, device=dev).normal_(0, D ** -0.5, generator=gen).requires_grad_()
+
+    def step(i):
+        seeds = torch.randint(0, n, (walkers,), generator=gen, device=dev)
+        walk = A._CAPI_Node2Vec(seeds, length, 2.0, 0.5).view(length + 1, walkers)
+        centre, context = walk[:-1].reshape(-1), walk[1:].reshape(-1)
+        x = gs.ops.dropout(gs.ops.embedding(table, centre, sparse=True), p, seed=5, stream=i)
+        loss = gs.ops.linear_cross_entropy(x, out, context, scale=D ** -0.5)
+        d_table, d_out = torch.autograd.grad(loss, [table, out])
+        with torch.no_grad():
+            table.index_add_(0, d_table.indices()[0], d_table.values(), alpha=-0.1)
+            out.add_(d_out, alpha=-0.1)
+        return loss.detach()
+
+    for i in range(warmup):
+        step(i)
+    torch.cuda.synchronize()
+    e0, e1 = _events()
+    e0.record()
+    for i in range(steps):
+        loss = step(warmup + i)
+    e1.record()
+    torch.cuda.synchronize()
+    ms = e0.elapsed_time(e1) / steps
+    pipeline.timing_enable(True)
+    step(warmup + steps)
+    timed = pipeline.timing_collect()
+    pipeline.timing_enable(False)
+    gs.check_async_errors()
+    pairs = walkers * length
+    print(json.dumps({"metric": "walk_pairs_trained_per_sec", "value": pairs / (ms / 1e3), "unit": "pairs/s",
+                      "ms_per_step": ms, "steps": steps, "loss": float(loss),
+                      "tflops": 6.0 * pairs * n * D / (ms / 1e3) / 1e12,
+                      "config": {"workload": "%d walkers x %d steps, node2vec p=2 q=0.5, full softmax over %d nodes, "
+                                             "%d columns bf16" % (walkers, length, n, D)},
+                      "kernels": _kernel_table(timed)}))
+
+
 if __name__ == "__main__":
     which = sys.argv[1] if len(sys.argv) > 1 else "node2vec"
     t0 = time.time()
     {"ladies": ladies, "node2vec": node2vec, "cfg5s": cfg5s, "cfg5": cfg5, "gather": gather,
-     "limits": limits, "weighted": weighted}[which]()
+     "limits": limits, "weighted": weighted, "embed": embed}[which]()
     print("# %s finished in %.1f s" % (which, time.time() - t0), file=sys.stderr)
