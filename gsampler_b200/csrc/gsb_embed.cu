@@ -340,14 +340,15 @@ embed_segments_kernel(const u32* __restrict__ key, i64 n, u32 rows, u32* __restr
 // its columns in registers.  A segment that lies inside the chunk is finished: one rounding,
 // one store.  What reaches beyond the chunk becomes a 32-bit partial row: slot 2c for a segment
 // that began before chunk c, slot 2c + 1 for one that begins in it and goes on.  A second kernel adds
-// the partials of a segment in the order of its chunks.  Eight rows are requested before the first is
-// added.
+// the partials of a segment in the order of its chunks.  Four rows are requested before the first is
+// added: bound by the latency of id -> position -> row, which the resident warps hide (4 M rows of 128
+// bf16: 322 us with eight rows and fewer warps, 270 with four; ids handed round by shuffles 450).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
 embed_segsum_kernel(const u32* __restrict__ key, const u32* __restrict__ pos, i64 n, const T* __restrict__ grad, int D,
                     int log_group, int chunk, u32 limit, float scale, T* __restrict__ out, float* __restrict__ part,
                     i64 part_ld, u32* __restrict__ part_key) {
-  constexpr int U = 8;
+  constexpr int U = 4;
   const int lane = threadIdx.x & ((1 << log_group) - 1);
   const i64 c = ((i64)blockIdx.x * blockDim.x + threadIdx.x) >> log_group;
   const i64 begin = c * chunk;
@@ -541,7 +542,7 @@ static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 // Sorted items a group takes at the first level: long chunks leave fewer partial rows (2 of
 // `chunk` at worst), short ones give a small batch enough groups for every SM.
 static int first_chunk(i64 n) {
-  int chunk = 64;
+  int chunk = 128;
   while (chunk > 8 && n / chunk < (i64)sm_count() * 64) chunk >>= 1;
   return chunk;
 }
