@@ -18,7 +18,7 @@ void CheckStatus(int status, const char* what) {
 void CheckDeviceError(int err, const char* what) {
   if (err == 0) return;
   std::string msg;
-  if (err & GSB_ERRBIT_LOOKBACK_TIMEOUT) msg += " tile-prefix wait timed out;";
+  if (err & GSB_ERRBIT_LOOKBACK_TIMEOUT) msg += " a wait inside a kernel timed out;";
   if (err & GSB_ERRBIT_TABLE_FULL) msg += " hash table full;";
   if (err & GSB_ERRBIT_KEY_MISSING) msg += " id missing from the node list;";
   if (err & GSB_ERRBIT_CAPACITY) msg += " output capacity exceeded;";

@@ -55,7 +55,7 @@ enum { GSB_F32 = 0, GSB_F16 = 1, GSB_BF16 = 2 };
 /* bits of the device error word (`d_err`, an int in device memory that the
  * caller zeroes once and may poll after synchronising) */
 enum {
-  GSB_ERRBIT_LOOKBACK_TIMEOUT = 1,
+  GSB_ERRBIT_LOOKBACK_TIMEOUT = 1, /* a bounded wait inside a kernel ran out */
   GSB_ERRBIT_TABLE_FULL = 2,
   GSB_ERRBIT_KEY_MISSING = 4,
   GSB_ERRBIT_CAPACITY = 8,
