@@ -754,18 +754,38 @@ loss_join_kernel(const float2* __restrict__ part, int parts, const float* __rest
     lse2[r] = total;
     loss[r] = counts ? total * LN2 - dot * scale : 0.f;
   }
-  if (pull) {
+  if (pull) {  // D <= 256: a lane has every 32nd column; the parts' weights go round the warp
     const float inv = 1.f / s;
-    for (int d = lane; d < D; d += 32) {
-      float v = 0.f;
-      if (counts) {
-        for (int k = 0; k < parts; ++k) {
-          const float mk = part[(i64)k * N + r].x;
-          v += part_o[((i64)k * N + r) * D + d] * (mk == -INFINITY ? 1.f : exp2f(mk - m));
+    float v[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = 0.f;
+    if (counts) {
+      for (int k0 = 0; k0 < parts; k0 += 32) {
+        const float mk = k0 + lane < parts ? part[(i64)(k0 + lane) * N + r].x : -INFINITY;
+        const float weight = mk == -INFINITY ? 1.f : exp2f(mk - m);
+        const int here = parts - k0 < 32 ? parts - k0 : 32;
+        for (int k = 0; k < here; k += 4) {  // four parts requested before the first is added
+          float o[4][8];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const float* from = part_o + ((i64)(k0 + (k + u < here ? k + u : 0)) * N + r) * D;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) o[u][q] = q * 32 + lane < D ? __ldg(from + q * 32 + lane) : 0.f;
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            float f = __shfl_sync(0xffffffffu, weight, (k + u) & 31);
+            if (k + u >= here) break;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = fmaf(o[u][q], f, v[q]);
+          }
         }
-        v = v * inv - to_float(w[t * ldw + d]);
       }
-      pull[r * D + d] = v;
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int d = q * 32 + lane;
+      if (d < D) pull[r * D + d] = counts ? v[q] * inv - to_float(w[t * ldw + d]) : 0.f;
     }
   }
 }
@@ -843,11 +863,9 @@ typedef TcShape<TC_STATS, 256, 2, 2, 128, 3, 1, 2, true> Stats256;
 typedef TcShape<TC_STATS, 64, 1, 3, 64, 8, 2, 2, true> StatsFew64;
 typedef TcShape<TC_STATS, 128, 1, 2, 128, 2, 2, 2, false> StatsFew128;
 typedef TcShape<TC_STATS, 256, 1, 2, 64, 3, 2, 2, true> StatsFew256;
-typedef TcShape<TC_PULL, 64, 2, 2, 128, 6, 1, 1, true> Pull64;
-typedef TcShape<TC_PULL, 128, 2, 2, 128, 4, 1, 1, false> Pull128;
+typedef TcShape<TC_PULL, 64, 1, 2, 64, 8, 2, 1, false> Pull64;
+typedef TcShape<TC_PULL, 128, 1, 2, 64, 4, 2, 1, false> Pull128;
 typedef TcShape<TC_PULL, 256, 1, 2, 64, 5, 1, 1, true> Pull256;
-typedef TcShape<TC_PULL, 64, 1, 2, 64, 8, 2, 1, true> PullFew64;
-typedef TcShape<TC_PULL, 128, 1, 1, 64, 6, 2, 1, true> PullFew128;
 typedef TcShape<TC_GRAD_X, 64, 1, 2, 64, 4, 2, 2, true> GradX64;
 typedef TcShape<TC_GRAD_X, 128, 1, 1, 64, 4, 2, 2, true> GradX128;
 typedef TcShape<TC_GRAD_X, 256, 1, 2, 64, 3, 1, 2, true> GradX256;
@@ -858,20 +876,21 @@ typedef TcShape<TC_GRAD_X, 64, 1, 2, 64, 5, 1, 2, true, 3> GradXF64;
 typedef TcShape<TC_GRAD_X, 128, 1, 1, 64, 2, 1, 2, false, 3> GradXF128;
 typedef TcShape<TC_GRAD_W, 64, 1, 2, 64, 5, 1, 2, true, 3> GradF64;
 typedef TcShape<TC_GRAD_W, 128, 1, 1, 64, 2, 1, 2, false, 3> GradF128;
-typedef TcShape<TC_GRAD_W, 64, 2, 2, 128, 6, 1, 2, true> Grad64;
+typedef TcShape<TC_GRAD_W, 64, 1, 2, 64, 8, 2, 2, true> Grad64;
 typedef TcShape<TC_GRAD_W, 128, 1, 2, 128, 4, 1, 2, true> Grad128;
 typedef TcShape<TC_GRAD_W, 256, 1, 2, 64, 5, 1, 2, true> Grad256;
-typedef TcShape<TC_GRAD_W, 64, 1, 2, 64, 8, 2, 2, true> GradFew64;
-typedef TcShape<TC_GRAD_W, 128, 1, 1, 64, 6, 2, 2, true> GradFew128;
+typedef TcShape<TC_GRAD_W, 128, 1, 2, 64, 4, 2, 2, false> GradFew128;
 
 // A vocabulary of up to this many rows: dx by making the logits again (2 V multiply-adds an element of
 // x more at 1.3 PFLOP/s, against writing and reading 16 bytes of pull at 5 TB/s: equal near 2080).
 constexpr i64 SMALL_V = 2048;
 
-// f(shape) for the shape that the sizes ask for.  Where the pass is a stream of loads or stores (few
-// rows against the vocabulary; a small vocabulary under many rows), two small CTAs an SM overlap one's
-// loads with the other's products; else one large CTA keeps the tensor cores busier.  dW, 1024 x
-// 232965 x 112: 0.154 ms with two, 0.182 with one; 8192 x 300000 x 128: 1.043 and 0.949.
+// f(shape) for the shape that the sizes ask for.  Two small CTAs an SM overlap one's loads and stores
+// with the other's products, and their hand-overs fall out of step by themselves; one large CTA reads B
+// less often.  Measured (bf16, ms): forward with pulls, 128 columns, two small / one large: 1024 x 232965
+// 0.107 / 0.116, 4096 x 100000 0.173 / 0.186, 8192 x 300000 0.956 / 0.975; 64 columns 8192 x 300000
+// 0.886 / 1.040.  dW: 1024 x 232965 x 128 0.149 / 0.182, 8192 x 300000 x 128 0.993 / 0.982, x 64 0.854 / 1.035.
+// Statistics alone: 8192 x 300000 x 128 0.692 / 0.620, but one row against 2.45 M 0.104 / 0.125.
 template <int PL, typename F>
 static auto with_shape(int mode, i64 N, i64 V, i64 D, F f) {
   if constexpr (PL == 3) {
@@ -879,19 +898,12 @@ static auto with_shape(int mode, i64 N, i64 V, i64 D, F f) {
     if (mode == TC_GRAD_X) return D > 64 ? f(GradXF128()) : f(GradXF64());
     return D > 64 ? f(GradF128()) : f(GradF64());
   } else {
-  if (mode == TC_STATS) {
-    if (N <= 128 || V <= SMALL_V) return D > 128 ? f(StatsFew256()) : D > 64 ? f(StatsFew128()) : f(StatsFew64());
-    return D > 128 ? f(Stats256()) : D > 64 ? f(Stats128()) : f(Stats64());
-  }
-  if (mode == TC_PULL) {
-    if (D > 128) return f(Pull256());
-    if (N <= 128) return D > 64 ? f(PullFew128()) : f(PullFew64());
-    return D > 64 ? f(Pull128()) : f(Pull64());
-  }
-  if (mode == TC_GRAD_X) return D > 128 ? f(GradX256()) : D > 64 ? f(GradX128()) : f(GradX64());
-  if (D > 128) return f(Grad256());
-  if (N <= 2048) return D > 64 ? f(GradFew128()) : f(GradFew64());
-  return D > 64 ? f(Grad128()) : f(Grad64());
+    if (mode == TC_STATS && (N <= 128 || V <= SMALL_V)) return D > 128 ? f(StatsFew256()) : D > 64 ? f(StatsFew128()) : f(StatsFew64());
+    if (mode == TC_STATS) return D > 128 ? f(Stats256()) : D > 64 ? f(Stats128()) : f(Stats64());
+    if (mode == TC_PULL) return D > 128 ? f(Pull256()) : D > 64 ? f(Pull128()) : f(Pull64());
+    if (mode == TC_GRAD_X) return D > 128 ? f(GradX256()) : D > 64 ? f(GradX128()) : f(GradX64());
+    if (D > 64 && D <= 128 && N <= 2048) return f(GradFew128());
+    return D > 128 ? f(Grad256()) : D > 64 ? f(Grad128()) : f(Grad64());
   }
 }
 
