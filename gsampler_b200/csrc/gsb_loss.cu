@@ -76,6 +76,10 @@ __global__ void loss_row_grad_kernel(const float* __restrict__ up, int per_row, 
     const u32 b = __float_as_uint(fabsf(v));
     mine = b > mine ? b : mine;
   }
+  if (!per_row) {  // the same for every row that counts
+    if (blockIdx.x == 0 && threadIdx.x == 0) *top = __float_as_uint(fabsf(count ? *up / *count : *up));
+    return;
+  }
   mine = __reduce_max_sync(0xffffffffu, mine);
   if ((threadIdx.x & 31) == 0 && mine) atomicMax(top, mine);
 }
@@ -174,7 +178,7 @@ extern "C" int gsb_linear_ce_grad(const void* x, int dtype, int64_t ldx, int64_t
   char* ws = (char*)workspace;
   float* g = (float*)ws;
   u32* top = (u32*)(ws + up256(4 * (size_t)N));
-  GSB_CUDA_OK(cudaMemsetAsync(top, 0, 4, st));
+  if (per_row) GSB_CUDA_OK(cudaMemsetAsync(top, 0, 4, st));
   {
     LaunchScope ls(KID_LOSS_JOIN, st);
     i64 blocks = (N + 255) / 256;

@@ -115,6 +115,30 @@ def test_sizes_and_types(gsb, dt, N, V, D):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("D", [40, 64, 128, 200, 272])
+def test_long_sums_and_several_pieces(gsb, dt, D):
+    """Every CTA runs over dozens of tiles (fp32 sums leave the accumulators several times), and the wide
+    form takes the vocabulary in more than one piece."""
+    x, w, t = make(5000, 8000, D, dt, seed=D, ignored=0.2)
+    check(gsb, x, w, t)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("N,V,D", [(1, 5000, 128), (3, 129, 40), (200, 2500, 48), (300, 3001, 128), (257, 2100, 256), (140, 9000, 100),
+                                   (70, 3000, 260)])
+def test_scores_without_gradients(gsb, dt, N, V, D):
+    """No gradient is asked for: the pass that only keeps statistics, and with it dW alone."""
+    x, w, t = make(N, V, D, dt, seed=V, ignored=0.1 if N > 4 else 0.0)
+    t[0] = V - 1
+    f = Formula(x, w, t, 0.9, dt)
+    with torch.no_grad():
+        within(gsb.ops.linear_cross_entropy(x, w.requires_grad_(), t, scale=0.9, reduction="none"), f.loss, f.loss_tol, "loss")
+    (dw,) = torch.autograd.grad(gsb.ops.linear_cross_entropy(x, w, t, scale=0.9, reduction="sum"), [w])
+    _, _, want, tol = f.grads(torch.ones(N, device="cuda"), dt)
+    within(dw, want, tol, "dW")
+
+
+@pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("V,scale", [(501, 1.0), (2200, 1.0), (501, -0.5), (2200, -0.5), (70, 0.0)])
 @pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
 def test_reductions_upstream_gradients_and_signs(gsb, dt, reduction, V, scale):
