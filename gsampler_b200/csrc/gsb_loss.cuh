@@ -20,20 +20,23 @@ inline int blocks_for(i64 threads) {
   return (int)(b < 1 ? 1 : b < most ? b : most);
 }
 
-// Tiles B a CTA runs over.  `groups` CTAs cover the rows A; the tiles are split until the CTAs fill
-// the SMs' `slots` evenly: the time is (rounds of CTAs) x (tiles of one + about 3 for its start and end).
+// In how many parts the tiles B are split among the CTAs of one group of rows A.  `groups` CTAs cover
+// the rows; the time is (rounds of CTAs on the SMs' `slots`) x (tiles of one + about 3 for its start and
+// end), so for each number of rounds the split that just fills them is the only one worth a look.
 inline int split_count(i64 groups, i64 tiles, i64 slots) {
+  const i64 first = (groups + slots - 1) / slots;
   int best = 1;
-  double best_t = 1e300;
-  for (i64 s = 1; s <= tiles && s <= 2 * slots && (s == 1 || groups * s <= 3 * slots); ++s) {
-    const i64 per = (tiles + s - 1) / s;
-    if ((tiles + per - 1) / per != s) continue;  // the same as fewer splits
+  double best_t = (double)first * (double)(tiles + 3);
+  for (i64 rounds = first; rounds <= 3; ++rounds) {
+    i64 s = rounds * slots / groups;
+    if (s < 1) continue;
+    const i64 per = tiles <= s ? 1 : (tiles + s - 1) / s;
+    s = (tiles + per - 1) / per;
     const double t = (double)((groups * s + slots - 1) / slots) * (double)(per + 3);
     if (t < best_t * 0.999) { best_t = t; best = (int)s; }
   }
   return best;
 }
-
 
 struct LossArgs {
   const void* x;

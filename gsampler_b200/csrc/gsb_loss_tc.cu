@@ -1,21 +1,24 @@
-// The vocabulary cross entropy of 16-bit types on the tensor cores (tcgen05, TMA, TMEM).
+// The vocabulary cross entropy on the tensor cores (tcgen05, TMA, TMEM): 16-bit types of up to 256
+// columns, fp32 of up to 128 as three bf16 planes.
 //
-// Both passes are one shape of computation: a tile of 128 rows A stays in TMEM, tiles B of the other
+// Every pass is one shape of computation: a tile of 128 rows A stays on chip, tiles B of the other
 // matrix stream past it, and for each
 //     S = A B^T   ->   P = f(S)   ->   O += P B
 // where one copy of the B tile in shared memory serves both products (read along its rows for S,
-// across them for O).  S, P (16-bit, in the place of S) and O live in TMEM too.  A there, and not in
-// shared memory, halves what a product reads from shared memory: S alone ran at 984 TFLOP/s with
-// both operands in shared memory (128 x 128 tiles, 8192 x 300000 x 128), the second product, whose
-// first operand was in TMEM already, at 2000.
+// across them for O).  S, P (16-bit, in the place of S) and O live in TMEM; so does A where there is
+// room, which halves what the first product reads from shared memory.
 //   forward   A = rows of x, B = the vocabulary.  P = exp2(l - m) against a running reference m;
 //             O / sum P is the expected row of W, which is all that dx needs; log2 sum P + m is
 //             the log-sum-exp.  Without a gradient for x there is no second product.
 //   dW        A = rows of W, B = rows of x.  P = g (p - target) with the known log-sum-exp.
-//   dx        (small vocabularies) A = rows of x, B = the vocabulary, P = g p (the target's row is taken off in 32 bits): making the logits
-//             once more costs less than 16 bytes of pull traffic an element of x.
-// So training costs four products of N V D multiply-adds (the logits twice, dx, dW) and no array of
+//   dx        (small vocabularies, fp32) A = rows of x, B = the vocabulary, P = g p; the target's row is
+//             taken off in 32 bits.  Makes the logits once more instead of keeping the expected rows.
+// So training costs four products of N V D multiply-adds (five with dx by itself), and no array of
 // N x V values exists anywhere.
+//
+// Bound by the hand-over from the tensor cores to the exponentials and back: at 128 columns both take
+// 1024 cycles a tile of 128 x 128 and each is busy 56 - 58 % of the time (8192 x 60000, bf16); at 256
+// columns the products are twice as long and run at 1500 TFLOP/s (8192 x 300000).
 //
 // The reference m moves only when a row's maximum passes it by 2^8, because moving it rescales O;
 // P stays below 2^15, which fp16 holds.  Sums and O are 32 bits; P is rounded to the type, half a
@@ -44,8 +47,10 @@ struct TcShape {
   static constexpr int PL = PL_, ACCS = PL == 3 ? 2 : 1, SB = BT_ * ACCS;  // planes, accumulators, columns of an S buffer
   static constexpr int MODE = MODE_, DP = DP_, NA = NA_, NB = NB_, BT = BT_, ST = ST_, CTAS = CTAS_;
   static constexpr int HV = HV_;
+  // one pair of exponentials in POLY by the polynomial, where no second product waits for them (0.667 ->
+  // 0.622 ms for 8192 x 300000 x 128; with a second product, a quarter: 0.992 -> 1.038)
   static constexpr int POLY = MODE == TC_STATS ? 8 : 0;
-  static constexpr bool ATM = ATM_;  // tiles A in TMEM, else in shared memory
+  static constexpr bool ATM = ATM_;
   static constexpr bool SECOND = MODE != TC_STATS;  // the product with P
   static constexpr int WG = NA * HV, HC = BT / HV;
   static constexpr int SUBS = DP / 64;
@@ -58,9 +63,9 @@ struct TcShape {
   __host__ __device__ static constexpr int p_at(int pl, int half) {
     return pl < 2 ? half * HC + pl * (HC / 2) : BT + half * HC;
   }
-  static constexpr int THREADS = WG * 128 + 64 + (MODE == TC_GRAD_W && PL == 1 ? 32 : 0);
-  static constexpr int A_BYTES = ATM ? 0 : PL * SUBS * 128 * 128;
   static constexpr bool WIPES = MODE == TC_GRAD_W && PL == 1;
+  static constexpr int THREADS = WG * 128 + 64 + (WIPES ? 32 : 0);
+  static constexpr int A_BYTES = ATM ? 0 : PL * SUBS * 128 * 128;
   // tiles B after which O is added to sums in registers: every addition to an accumulator in TMEM
   // truncates, which over hundreds of tiles is more than 32-bit values may lose
   static constexpr int FLUSH = PL == 3 ? 16 : 0;
@@ -92,8 +97,8 @@ struct TcParams {
   const i64* target;        // TC_STATS, TC_GRAD_X
   float* hot;               // TC_STATS: [rows_a] the target's product, where the target lies in the vocabulary
   float2* part_ms;          // TC_STATS / TC_PULL: [parts][rows_a] reference and sum
-  float* part_o;            // TC_PULL: [splits][rows_a][D]; TC_GRAD_W with splits: the same
-  void* out;                // TC_GRAD_W without splits, TC_GRAD_X: [rows_a][D]
+  float* part_o;            // TC_PULL, gradients with splits: [splits][rows_a][D]
+  void* out;                // gradients without splits: [rows_a][D]
   const u32* top;           // gradients: bits of max |g|
   float out_scale;          // scale 2^-GRAD_SHIFT
   int* err;
@@ -227,7 +232,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
     // ------------------------------------------------ products
     // The whole warp walks the items and one lane issues: unrolled, with descriptors that differ by
     // constants.  A product of 128 x 128 x 16 takes 64 cycles; issued from a divergent lane with its
-    // descriptors made one by one it took 130.
+    // descriptors made one by one it took 130 (8192 x 300000 x 256: 2.84 -> 1.81 ms).
     if (my_tiles > 0) {
       const bool bf = IsBf16<T>::value;
       const u32 id_s = tc_idesc(bf, C::BT, false, false), id_o = tc_idesc(bf, (u32)ksteps * 16, false, true);
@@ -836,7 +841,7 @@ __global__ void __launch_bounds__(256) loss_join_dw_kernel(const float* __restri
 
 // ---------------------------------------------------------------- host side
 struct TcPlan {
-  int NA, BT, ctas, splits, per, parts;
+  int BT, splits, per, parts;
   i64 groups;
 };
 template <typename C>
@@ -844,9 +849,7 @@ static TcPlan plan_of(i64 rows_a, i64 rows_b) {
   TcPlan p;
   if (rows_a < 1) rows_a = 1;  // sizes are asked for empty batches too
   if (rows_b < 1) rows_b = 1;
-  p.NA = C::NA;
   p.BT = C::BT;
-  p.ctas = C::CTAS;
   p.groups = (rows_a + 128 * C::NA - 1) / (128 * C::NA);
   const i64 tiles = (rows_b + C::BT - 1) / C::BT;
   const int s = split_count(p.groups, tiles, (i64)sm_count() * C::CTAS);
