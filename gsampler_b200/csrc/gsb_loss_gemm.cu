@@ -56,6 +56,7 @@ struct GmParams {
   int v0;                   // GM_PIECE: id of the piece's first column
   void* piece;              // GM_PIECE: [PL][M][ld_piece]
   i64 ld_piece, plane;
+  float* lost;              // GM_PIECE: [M] what rounding the target's element to 16 bits lost, for dx
   float* slab;              // GM_DX / GM_DW: [units along z][M][N]
   int add;
   int* err;
@@ -240,6 +241,12 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             if (col + j == hot) v[j] -= 1.f;
             v[j] = gs == 0.f ? 0.f : v[j] * gs;  // rows that do not count
           }
+          if (C::PL == 1 && (u32)(hot - col) < 64u) {
+            // g (p - 1) is as large as its row's other elements together: dx gets the lost part back
+#pragma unroll
+            for (int j = 0; j < 64; ++j)
+              if (col + j == hot) p.lost[row] = v[j] - to_float(from_float<T>(v[j]));
+          }
           const u32 out = base + C::OFF_OUT + warp * 4096;
           const int first = m * 128 + quarter * 32;
 #pragma unroll
@@ -371,15 +378,31 @@ __global__ void loss_planes_kernel(const S* __restrict__ src, i64 ld, i64 rows, 
   }
 }
 
-// out[e] = factor * sum over the slabs; rows whose `live` is zero are zeros
+// dx[i] = factor * (sum over the slabs + lost_i w_{t_i}); zeros for a row that does not count
+template <typename T>
+__global__ void loss_wide_dx_kernel(const float* __restrict__ slab, i64 N, i64 D, int slabs, float factor, const u32* __restrict__ top,
+                                    const float* __restrict__ g, const float* __restrict__ lost, const i64* __restrict__ target,
+                                    const T* __restrict__ w, i64 ldw, T* __restrict__ dx) {
+  const float f = factor * __uint_as_float(*top);
+  for (i64 e = (i64)blockIdx.x * blockDim.x + threadIdx.x; e < N * D; e += (i64)gridDim.x * blockDim.x) {
+    const i64 r = e / D;
+    float v = 0.f;
+    if (g[r] != 0.f) {
+      for (int z = 0; z < slabs; ++z) v += slab[z * (N * D) + e];
+      if (lost) v = fmaf(lost[r], to_float(w[target[r] * ldw + (e - r * D)]), v);
+    }
+    dx[e] = from_float<T>(v * f);
+  }
+}
+
+// out[e] = factor * sum over the slabs
 template <typename T>
 __global__ void loss_slabs_kernel(const float* __restrict__ slab, i64 size, int slabs, float factor, const u32* __restrict__ top,
-                                  const float* __restrict__ live, i64 D, T* __restrict__ out) {
+                                  T* __restrict__ out) {
   const float f = factor * __uint_as_float(*top);
   for (i64 e = (i64)blockIdx.x * blockDim.x + threadIdx.x; e < size; e += (i64)gridDim.x * blockDim.x) {
     float v = 0.f;
-    if (!live || live[e / D] != 0.f)
-      for (int z = 0; z < slabs; ++z) v += slab[z * size + e];
+    for (int z = 0; z < slabs; ++z) v += slab[z * size + e];
     out[e] = from_float<T>(v * f);
   }
 }
@@ -403,7 +426,7 @@ static int bn_of(int planes, i64 cols) { return planes == 3 ? (cols <= 64 ? 64 :
 static int bn_wide(int planes) { return planes == 3 ? 128 : 256; }                               // logits
 
 struct GmLayout {
-  size_t ms, x, w, piece, dx_slab, dw_slab, bytes;
+  size_t ms, x, w, piece, lost, dx_slab, dw_slab, bytes;
   i64 cols, ldp;
   int dx_slabs, dw_slabs, splits, per;
 };
@@ -424,6 +447,7 @@ static GmLayout gemm_layout(int planes, i64 N, i64 V, i64 D, bool forward, bool 
     L.dx_slabs = slab_count(N, D, L.cols, bn_of(planes, D));
     L.dw_slabs = slab_count(L.cols, D, N, bn_of(planes, D));
     L.piece = take(2 * (size_t)planes * N * packed_ld(L.cols));
+    L.lost = take(4 * (size_t)N);
     L.dx_slab = take(dx ? 4 * (size_t)L.dx_slabs * N * D : 0);
     L.dw_slab = take(dw ? 4 * (size_t)L.dw_slabs * L.cols * D : 0);
   }
@@ -543,6 +567,7 @@ int gemm_loss_backward(const LossArgs& a) {
       p.piece = piece;
       p.ld_piece = ldq;
       p.plane = a.N * ldq;
+      p.lost = (float*)(ws + L.lost);
       p.err = a.err;
       const dim3 grid = units_grid(p, 1);
       const int rc = launch_mode<T, GM_PIECE, PL>(c, ma, mb, p, grid, KID_LOSS_GRAD, a.st);
@@ -579,13 +604,15 @@ int gemm_loss_backward(const LossArgs& a) {
       const int rc = launch_mode<T, GM_DW, PL>(a.D, ma, mb, p, grid, KID_LOSS_GRAD, a.st);
       if (rc != GSB_OK) return rc;
       LaunchScope ls(KID_LOSS_JOIN, a.st);
-      loss_slabs_kernel<S><<<blocks_for(c * a.D), 256, 0, a.st>>>(dws, c * a.D, L.dw_slabs, fabsf(a.scale) * unit, a.top, nullptr, a.D,
+      loss_slabs_kernel<S><<<blocks_for(c * a.D), 256, 0, a.st>>>(dws, c * a.D, L.dw_slabs, fabsf(a.scale) * unit, a.top,
                                                                  (S*)a.dw + v0 * a.D);
     }
   }
   if (a.dx) {
     LaunchScope ls(KID_LOSS_JOIN, a.st);
-    loss_slabs_kernel<S><<<blocks_for(a.N * a.D), 256, 0, a.st>>>(dxs, a.N * a.D, L.dx_slabs, a.scale * unit, a.top, a.g, a.D, (S*)a.dx);
+    loss_wide_dx_kernel<S><<<blocks_for(a.N * a.D), 256, 0, a.st>>>(dxs, a.N, a.D, L.dx_slabs, a.scale * unit, a.top, a.g,
+                                                                    PL == 1 ? (const float*)(ws + L.lost) : nullptr, a.target, (const S*)a.w,
+                                                                    a.ldw, (S*)a.dx);
   }
   return GSB_OK;
 }

@@ -873,7 +873,8 @@ typedef TcShape<TC_GRAD_X, 64, 1, 2, 64, 4, 2, 2, true> GradX64;
 typedef TcShape<TC_GRAD_X, 128, 1, 1, 64, 4, 2, 2, true> GradX128;
 typedef TcShape<TC_GRAD_X, 256, 1, 2, 64, 3, 1, 2, true> GradX256;
 // fp32: the products are six times as many, so one tile A and small tiles B are enough to hide the rest
-typedef TcShape<TC_STATS, 64, 1, 3, 64, 5, 1, 2, true, 3> StatsF64;
+// (4000 x 50021 x 64, us: statistics with 64-row tiles 131, 128 rows 114; gradients 237 with 64, 330 with 128)
+typedef TcShape<TC_STATS, 64, 1, 2, 128, 3, 1, 2, false, 3> StatsF64;
 typedef TcShape<TC_STATS, 128, 1, 2, 64, 2, 1, 2, false, 3> StatsF128;
 typedef TcShape<TC_GRAD_X, 64, 1, 2, 64, 5, 1, 2, true, 3> GradXF64;
 typedef TcShape<TC_GRAD_X, 128, 1, 1, 64, 2, 1, 2, false, 3> GradXF128;
