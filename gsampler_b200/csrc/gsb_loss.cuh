@@ -1,5 +1,7 @@
 // Shared by the two forms of the vocabulary cross entropy (gsb_loss.cu, gsb_loss_tc.cu).
 #pragma once
+#include <atomic>
+
 #include "gsb_common.cuh"
 #include "gsb_types.cuh"
 
@@ -13,6 +15,18 @@ constexpr float MOVE_REFERENCE = 8.f;  // a row's reference moves when its maxim
 // Factor from x . w to a base-2 logit, |scale| log2 e (the sign goes into x).  Not zero, so that a
 // masked logit of -inf stays one; times any finite product 1e-38 is as good as zero.
 inline float logit_factor(float scale) { return fmaxf(fabsf(scale) * LOG2E, 1e-38f); }
+
+// Lets a kernel use `bytes` of shared memory; asked once a device, `done` is the kernel's own word.
+template <typename K>
+inline bool allow_shared(K kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
 
 inline size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 inline int blocks_for(i64 threads) {

@@ -474,7 +474,8 @@ void make_planes(const void* src, i64 ld, i64 rows, i64 D, bool negate, const fl
 
 template <typename T, typename C>
 static int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GmParams& p, dim3 grid, int kid, cudaStream_t st) {
-  GSB_CUDA_OK(cudaFuncSetAttribute(loss_gemm_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
+  static std::atomic<unsigned long long> done{0};
+  if (!allow_shared(loss_gemm_kernel<T, C>, C::BYTES, done)) return GSB_ERR_CUDA;
   LaunchScope ls(kid, st);
   loss_gemm_kernel<T, C><<<grid, C::THREADS, C::BYTES, st>>>(a, b, p);
   return GSB_OK;

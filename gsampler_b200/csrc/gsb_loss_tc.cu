@@ -981,8 +981,8 @@ static int row_bytes(const void* p, i64 ld, int size) {
 template <typename V, typename C>
 static int launch_tc(const CUtensorMap& b, const TcPlan& plan, const TcParams& p, int kid, cudaStream_t st) {
   typedef typename Planes<V>::type T;
-  // the attribute belongs to the device's copy of the kernel; setting it is cheap and not a stream operation
-  GSB_CUDA_OK(cudaFuncSetAttribute(loss_tc_kernel<T, V, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
+  static std::atomic<unsigned long long> done{0};
+  if (!allow_shared(loss_tc_kernel<T, V, C>, C::BYTES, done)) return GSB_ERR_CUDA;
   LaunchScope ls(kid, st);
   loss_tc_kernel<T, V, C><<<dim3((unsigned)plan.groups, (unsigned)plan.splits), C::THREADS, C::BYTES, st>>>(b, p);
   return GSB_OK;

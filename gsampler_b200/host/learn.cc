@@ -296,9 +296,14 @@ struct DropoutFn : public torch::autograd::Function<DropoutFn> {
   }
 };
 
-torch::Tensor DropoutApply(torch::Tensor data, double p, int64_t seed, int64_t stream, c10::optional<torch::Tensor> step) {
-  if (!Tracked(data)) return Dropout(data, p, seed, stream, step);
-  return DropoutFn::apply(data, p, seed, stream, step);
+torch::Tensor DropoutApply(torch::Tensor data, double p, c10::optional<int64_t> seed, c10::optional<int64_t> stream,
+                           c10::optional<torch::Tensor> step) {
+  TORCH_CHECK(seed.has_value() == stream.has_value(), "Dropout: give both seed and stream, or neither");
+  int64_t s, t;
+  if (seed.has_value()) std::tie(s, t) = std::make_tuple(*seed, *stream);
+  else std::tie(s, t) = NextDropoutStream();
+  if (!Tracked(data)) return Dropout(data, p, s, t, step);
+  return DropoutFn::apply(data, p, s, t, step);
 }
 
 struct LinearCrossEntropyFn : public torch::autograd::Function<LinearCrossEntropyFn> {

@@ -36,7 +36,9 @@ std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyGrad(torch::Tensor x,
 
 // The same with their gradients, for autograd.
 torch::Tensor EmbeddingLookup(torch::Tensor weight, torch::Tensor index, double scale, int64_t padding, bool sparse);
-torch::Tensor DropoutApply(torch::Tensor data, double p, int64_t seed, int64_t stream, c10::optional<torch::Tensor> step);
+// dropout without seed and stream takes them from the default state when it runs
+torch::Tensor DropoutApply(torch::Tensor data, double p, c10::optional<int64_t> seed, c10::optional<int64_t> stream,
+                           c10::optional<torch::Tensor> step);
 // reduction: 0 none, 1 sum, 2 mean
 torch::Tensor LinearCrossEntropyLoss(torch::Tensor x, torch::Tensor weight, torch::Tensor target, double scale,
                                      int64_t ignore, int64_t reduction);

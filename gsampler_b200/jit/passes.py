@@ -25,7 +25,7 @@ RANDOM = {"_CAPI_Sampling", "_CAPI_SamplingProbs", "_CAPI_SlicingSampling", "_CA
           "_CAPI_BatchRowSamplingProbs", "_CAPI_BatchFusedSlicingSampling", "_CAPI_RandomWalk",
           "_CAPI_Node2Vec", "_CAPI_BatchGraphSAGE", "_CAPI_LadiesLayer"}
 RANDOM_FUNCTIONS = ("_CAPI_ListSampling", "_CAPI_ListSamplingWithProbs", "_CAPI_BatchListSampling",
-                    "_CAPI_BatchListSamplingWithProbs")
+                    "_CAPI_BatchListSamplingWithProbs", "_CAPI_DropoutApply")
 # leaf helpers that allocate an output which an in-place operator then fills
 ALLOCATING = ("spmm_prepare", "sddmm_prepare")
 

@@ -23,6 +23,4 @@ def dropout(data: torch.Tensor, p: float = 0.5, training: bool = True, seed: int
         raise ValueError("dropout: p must lie in [0, 1], got %s" % (p,))
     if not training or p == 0.0:
         return data
-    if seed is None:
-        seed, stream = torch.ops.gs_ops._CAPI_NextDropoutStream()
-    return torch.ops.gs_ops._CAPI_DropoutApply(data, float(p), int(seed), int(stream), step)
+    return torch.ops.gs_ops._CAPI_DropoutApply(data, float(p), seed, stream, step)
