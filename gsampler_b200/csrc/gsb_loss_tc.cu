@@ -865,7 +865,9 @@ typedef TcShape<TC_STATS, 128, 2, 3, 128, 5, 1, 2, true> Stats128;
 typedef TcShape<TC_STATS, 256, 2, 2, 128, 3, 1, 2, true> Stats256;
 typedef TcShape<TC_STATS, 64, 1, 3, 64, 8, 2, 2, true> StatsFew64;
 typedef TcShape<TC_STATS, 128, 1, 2, 128, 2, 2, 2, false> StatsFew128;
-typedef TcShape<TC_STATS, 256, 1, 2, 64, 3, 2, 2, true> StatsFew256;
+typedef TcShape<TC_STATS, 256, 1, 1, 64, 2, 2, 2, true> StatsFew256;
+typedef TcShape<TC_STATS, 128, 1, 1, 64, 2, 2, 2, true> StatsTile128;
+typedef TcShape<TC_STATS, 256, 1, 2, 64, 3, 2, 2, true> StatsMid256;
 typedef TcShape<TC_PULL, 64, 1, 2, 64, 8, 2, 1, false> Pull64;
 typedef TcShape<TC_PULL, 128, 1, 2, 64, 4, 2, 1, false> Pull128;
 typedef TcShape<TC_PULL, 256, 1, 2, 64, 5, 1, 1, true> Pull256;
@@ -894,7 +896,9 @@ constexpr i64 SMALL_V = 2048;
 // less often.  Measured (bf16, ms): forward with pulls, 128 columns, two small / one large: 1024 x 232965
 // 0.107 / 0.116, 4096 x 100000 0.173 / 0.186, 8192 x 300000 0.956 / 0.975; 64 columns 8192 x 300000
 // 0.886 / 1.040.  dW: 1024 x 232965 x 128 0.149 / 0.182, 8192 x 300000 x 128 0.993 / 0.982, x 64 0.854 / 1.035.
-// Statistics alone: 8192 x 300000 x 128 0.692 / 0.620, but one row against 2.45 M 0.104 / 0.125.
+// Statistics alone: 8192 x 300000 x 128 0.692 / 0.620, but one row against 2.45 M 0.104 / 0.125; with a tile
+// or a few to run over, one S buffer and a short pipeline start sooner (300007 x 47 x 128 0.038 against 0.062,
+// x 256 0.065 / 0.085), with dozens they do not (300007 x 1000 x 256 0.204 / 0.179).
 template <int PL, typename F>
 static auto with_shape(int mode, i64 N, i64 V, i64 D, F f) {
   if constexpr (PL == 3) {
@@ -902,8 +906,12 @@ static auto with_shape(int mode, i64 N, i64 V, i64 D, F f) {
     if (mode == TC_GRAD_X) return D > 64 ? f(GradXF128()) : f(GradXF64());
     return D > 64 ? f(GradF128()) : f(GradF64());
   } else {
-    if (mode == TC_STATS && (N <= 128 || V <= SMALL_V)) return D > 128 ? f(StatsFew256()) : D > 64 ? f(StatsFew128()) : f(StatsFew64());
-    if (mode == TC_STATS) return D > 128 ? f(Stats256()) : D > 64 ? f(Stats128()) : f(Stats64());
+    if (mode == TC_STATS) {
+      const bool few = N <= 128 || V <= SMALL_V, tiny = V <= 256;
+      if (D > 128) return N <= 128 || tiny ? f(StatsFew256()) : few ? f(StatsMid256()) : f(Stats256());
+      if (D > 64) return N > 128 && tiny ? f(StatsTile128()) : few ? f(StatsFew128()) : f(Stats128());
+      return few ? f(StatsFew64()) : f(Stats64());
+    }
     if (mode == TC_PULL) return D > 128 ? f(Pull256()) : D > 64 ? f(Pull128()) : f(Pull64());
     if (mode == TC_GRAD_X) return D > 128 ? f(GradX256()) : D > 64 ? f(GradX128()) : f(GradX64());
     if (D > 64 && D <= 128 && N <= 2048) return f(GradFew128());

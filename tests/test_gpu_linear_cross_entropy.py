@@ -125,7 +125,7 @@ def test_long_sums_and_several_pieces(gsb, dt, D):
 
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("N,V,D", [(1, 5000, 128), (3, 129, 40), (200, 2500, 48), (300, 3001, 128), (257, 2100, 256), (140, 9000, 100),
-                                   (70, 3000, 260)])
+                                   (70, 3000, 260), (300, 1000, 256), (400, 250, 90), (500, 47, 200), (500, 300, 60)])
 def test_scores_without_gradients(gsb, dt, N, V, D):
     """No gradient is asked for: the pass that only keeps statistics, and with it dW alone."""
     x, w, t = make(N, V, D, dt, seed=V, ignored=0.1 if N > 4 else 0.0)
