@@ -90,9 +90,10 @@ template <typename T>
 int gemm_loss_forward(const LossArgs& a);
 template <typename T>
 int gemm_loss_backward(const LossArgs& a);
-// losses (and pulls) of all rows from the parts of their statistics (gsb_loss_tc.cu)
+// losses (and pulls) of all rows from the parts of their statistics (gsb_loss_tc.cu); with hot, the targets'
+// products, the parts leave the targets out
 template <typename T>
-void launch_loss_join(const LossArgs& a, const float2* part_ms, int parts, const float* part_o, float* pull);
+void launch_loss_join(const LossArgs& a, const float2* part_ms, int parts, const float* part_o, const float* hot, float* pull);
 
 template <typename T>
 int tc_loss_forward(const LossArgs& a, float* pull);

@@ -518,7 +518,7 @@ int gemm_loss_forward(const LossArgs& a) {
   p.err = a.err;
   const int rc = launch_mode<T, GM_STATS, PL>(a.V, ma, mb, p, dim3(p.m_tiles, L.splits), KID_LOSS, a.st);
   if (rc != GSB_OK) return rc;
-  launch_loss_join<S>(a, p.part_ms, 2 * L.splits, nullptr, nullptr);
+  launch_loss_join<S>(a, p.part_ms, 2 * L.splits, nullptr, nullptr, nullptr);
   return GSB_OK;
 }
 

@@ -9,10 +9,14 @@
 // room, which halves what the first product reads from shared memory.
 //   forward   A = rows of x, B = the vocabulary.  P = exp2(l - m) against a running reference m;
 //             O / sum P is the expected row of W, which is all that dx needs; log2 sum P + m is
-//             the log-sum-exp.  Without a gradient for x there is no second product.
+//             the log-sum-exp.  Without a gradient for x there is no second product.  With one, the
+//             target's element stays out of P and of the sum and is added to them afterwards:
+//             dx ~ sum_{j != t} p_j w_j - (1 - p_t) w_t, and the rounding of p_t, half a step however
+//             likely the target is, would be many times 1 - p_t.
 //   dW        A = rows of W, B = rows of x.  P = g (p - target) with the known log-sum-exp.
-//   dx        (small vocabularies, fp32) A = rows of x, B = the vocabulary, P = g p; the target's row is
-//             taken off in 32 bits.  Makes the logits once more instead of keeping the expected rows.
+//   dx        (small vocabularies, fp32) A = rows of x, B = the vocabulary, P = g p without the target's,
+//             whose g (p_t - 1) w_t is added in 32 bits.  Makes the logits once more instead of keeping the
+//             expected rows.
 // So training costs four products of N V D multiply-adds (five with dx by itself), and no array of
 // N x V values exists anywhere.
 //
@@ -70,13 +74,15 @@ struct TcShape {
   // truncates, which over hundreds of tiles is more than 32-bit values may lose
   static constexpr int FLUSH = PL == 3 ? 16 : 0;
   static constexpr int OFF_B = NA * A_BYTES, OFF_META = OFF_B + ST * B_BYTES;
-  static constexpr int OFF_BAR = OFF_META + ST * META;
+  static constexpr int OFF_COEF = OFF_META + ST * META;  // TC_GRAD_X: g (p_t - 1) by half and row
+  static constexpr int OFF_BAR = OFF_COEF + (MODE == TC_GRAD_X ? WG * 128 * 4 : 0);
   static constexpr int BARS = 3 * ST + 2 * NB + 3;
   static constexpr int BYTES = OFF_BAR + 8 * BARS + 16 + 1024;  // and room to align the base
   static_assert(USED <= 512 && COLS * CTAS <= 512, "TMEM");
   static_assert(BYTES * CTAS <= 226 * 1024, "shared memory");
   static_assert(MODE != TC_PULL || HV == 1, "a row's running state has one owner");
   static_assert(PL == 1 || (MODE != TC_PULL && NA == 1), "");
+  static_assert(MODE != TC_GRAD_X || NA == 1, "the halves of a row pass on its target's element");
   static_assert(HC % 32 == 0 && META % 16 == 0 && OFF_BAR % 8 == 0, "");
 };
 
@@ -94,8 +100,8 @@ struct TcParams {
   int w_bytes;
   const float* lse2;        // TC_GRAD_X, by row
   const float* g;           // TC_GRAD_X
-  const i64* target;        // TC_STATS, TC_GRAD_X
-  float* hot;               // TC_STATS: [rows_a] the target's product, where the target lies in the vocabulary
+  const i64* target;        // TC_STATS, TC_PULL, TC_GRAD_X
+  float* hot;               // TC_STATS, TC_PULL: [rows_a] the target's product, where the target lies in the vocabulary
   float2* part_ms;          // TC_STATS / TC_PULL: [parts][rows_a] reference and sum
   float* part_o;            // TC_PULL, gradients with splits: [splits][rows_a][D]
   void* out;                // gradients without splits: [rows_a][D]
@@ -376,10 +382,10 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
     };
     float m = -INFINITY, sum = 0.f;
     const u64 c2 = join2(p.c, p.c);
-    // the target, and for dx the row's scaled gradient (an infinite bias: P = 0)
+    // the target, and for dx the row's scaled gradient (an infinite bias: P = 0) and what becomes of it at the target
     int hot = -1;
-    float gs = 0.f, row_bias = -INFINITY;
-    if (C::MODE == TC_STATS && row < p.rows_a) {
+    float gs = 0.f, row_bias = -INFINITY, coef = 0.f;
+    if ((C::MODE == TC_STATS || C::MODE == TC_PULL) && row < p.rows_a) {
       const i64 t = p.target[row];
       if (t >= 0 && t < p.rows_b) hot = (int)t;
     }
@@ -473,17 +479,29 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
             exponentials(v[k], v[k + 1], k);
             part2(mul2(join2(v[k], v[k + 1]), gs2), v[k], v[k + 1]);
           }
+          const int at = hot - col0;
+          if (__any_sync(0xffffffffu, (u32)at < (u32)C::HC)) {
+            float mine = 0.f;
+#pragma unroll
+            for (int k = 0; k < C::HC; ++k)
+              if (k == at) {
+                mine = v[k];
+                v[k] = 0.f;
+              }
+            if ((u32)at < (u32)C::HC) coef = mine - gs;
+          }
         } else {
           const int col0 = (t0 + j) * C::BT + half * C::HC;
-          if (C::MODE == TC_STATS) {
-            const int at = hot - col0;
-            if (__any_sync(0xffffffffu, (u32)at < (u32)C::HC)) {  // the target's product, on its way past
-              float mine = 0.f;
+          const int at = hot - col0;
+          if (__any_sync(0xffffffffu, (u32)at < (u32)C::HC)) {  // the target's product, on its way past
+            float mine = 0.f;
 #pragma unroll
-              for (int k = 0; k < C::HC; ++k)
-                if (k == at) mine = v[k];
-              if ((u32)at < (u32)C::HC && row < p.rows_a) p.hot[row] = mine;
-            }
+            for (int k = 0; k < C::HC; ++k)
+              if (k == at) {
+                mine = v[k];
+                if (C::MODE == TC_PULL) v[k] = -INFINITY;
+              }
+            if ((u32)at < (u32)C::HC && row < p.rows_a) p.hot[row] = mine;
           }
           if (col0 + C::HC > p.rows_b) {
 #pragma unroll
@@ -561,11 +579,21 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
     if (C::MODE == TC_STATS && row < p.rows_a && ok)
       p.part_ms[(i64)(blockIdx.y * C::HV + half) * p.rows_a + row] = make_float2(m, sum);
     if (C::MODE == TC_PULL && row < p.rows_a && ok) p.part_ms[(i64)blockIdx.y * p.rows_a + row] = make_float2(m, sum);
-    // dx: the target's own row is taken off in 32 bits
+    // dx: the target's own row is added in 32 bits, by the split that has met it
     constexpr int AHEAD = C::MODE == TC_GRAD_X && C::PL == 1 ? PIECES : 1;  // pieces of it requested before the wait
     Pack<V, 32> target_row[AHEAD];
-    if (C::MODE == TC_GRAD_X && C::PL == 1 && gridDim.y == 1)
-      row_pieces(target_row, (const V*)p.w + (i64)(hot < 0 ? 0 : hot) * p.ldw + half * 32, 32 * C::HV, row_live ? p.D - half * 32 : 0, p.w_bytes);
+    const bool here = C::MODE == TC_GRAD_X && hot >= t0 * C::BT && hot < (t0 + my_tiles) * C::BT;
+    const V* target_at = (const V*)p.w + (i64)(here ? hot : 0) * p.ldw;
+    if (C::MODE == TC_GRAD_X) {
+      if (C::PL == 1) row_pieces(target_row, target_at + half * 32, 32 * C::HV, here ? p.D - half * 32 : 0, p.w_bytes);
+      // one of the halves has met it: they pass it on
+      float* passed = reinterpret_cast<float*>(smem + C::OFF_COEF) + quarter * 32 + lane;
+      passed[wg * 128] = coef;
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + quarter), "n"(32 * C::HV) : "memory");
+      coef = 0.f;
+#pragma unroll
+      for (int h = 0; h < C::HV; ++h) coef += passed[h * 128];
+    }
     if (C::SECOND && my_tiles > 0) {
       ok = ok && bar_wait(o_full, 0, gave_up, p.err);
       ok = __all_sync(0xffffffffu, ok);
@@ -587,11 +615,11 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
           }
           if (row < p.rows_a) {
             const bool slab = C::MODE == TC_PULL || gridDim.y > 1;
-            if (C::MODE == TC_GRAD_X && !slab) {
-              if (C::PL == 3) row_pieces(target_row, (const V*)p.w + (i64)(hot < 0 ? 0 : hot) * p.ldw + k, 0, row_live ? p.D - k : 0, p.w_bytes);
+            if (C::MODE == TC_GRAD_X) {
+              if (C::PL == 3) row_pieces(target_row, target_at + k, 0, here ? p.D - k : 0, p.w_bytes);
               // a row that does not count is zero
 #pragma unroll
-              for (int q = 0; q < 32; ++q) o[q] = row_live ? fmaf(-gs, to_float(target_row[AHEAD == 1 ? 0 : i].v[q]), o[q]) : 0.f;
+              for (int q = 0; q < 32; ++q) o[q] = row_live ? fmaf(coef, to_float(target_row[AHEAD == 1 ? 0 : i].v[q]), o[q]) : 0.f;
             }
             if (slab) {
               float* to = p.part_o + ((i64)blockIdx.y * p.rows_a + row) * p.D + k;
@@ -696,23 +724,27 @@ __global__ void loss_meta_kernel(const float* __restrict__ lse2, const i64* __re
 }
 
 // The statistics of a row's parts joined: the log-sum-exp in base 2 (of values held at 2^FWD_SHIFT).
-__device__ __forceinline__ float join_parts(const float2* __restrict__ part, int parts, i64 N, i64 r, int first, int step, float& m, float& s) {
-  m = -INFINITY;
+// Parts that leave the target out get it here, as its logit l2 in base 2 (-inf: they have it already);
+// `others` is the sum without it.
+__device__ __forceinline__ float join_parts(const float2* __restrict__ part, int parts, i64 N, i64 r, int first, int step, float l2, float& m,
+                                            float& others, float& s) {
+  m = l2;
   for (int k = first; k < parts; k += step) m = max_nan(m, part[(i64)k * N + r].x);
   if (step == 32) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
   }
-  s = 0.f;
+  others = 0.f;
   for (int k = first; k < parts; k += step) {
     const float2 q = part[(i64)k * N + r];
     // a part without a reference has either no finite logit (sum 0) or a NaN
-    s += q.x == -INFINITY ? q.y : q.y * exp2f(q.x - m);
+    others += q.x == -INFINITY ? q.y : q.y * exp2f(q.x - m);
   }
   if (step == 32) {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    for (int d = 16; d > 0; d >>= 1) others += __shfl_xor_sync(0xffffffffu, others, d);
   }
+  s = l2 == -INFINITY ? others : others + exp2f(l2 - m + (float)FWD_SHIFT);
   return m - (float)FWD_SHIFT + log2f(s);
 }
 constexpr float LN2 = 0.6931471805599453f;
@@ -725,8 +757,8 @@ loss_finish_kernel(const float2* __restrict__ part, int parts, int lanes, const 
   const i64 e = (i64)blockIdx.x * blockDim.x + threadIdx.x;
   const i64 r = lanes == 32 ? e >> 5 : e;
   if (r >= N) return;
-  float m, s;
-  const float total = join_parts(part, parts, N, r, lanes == 32 ? (int)(e & 31) : 0, lanes, m, s);
+  float m, others, s;
+  const float total = join_parts(part, parts, N, r, lanes == 32 ? (int)(e & 31) : 0, lanes, -INFINITY, m, others, s);
   if (lanes == 32 && (e & 31) != 0) return;
   const i64 t = target[r];
   const bool counts = t != ignore && t >= 0 && t < V;
@@ -735,32 +767,37 @@ loss_finish_kernel(const float2* __restrict__ part, int parts, int lanes, const 
   loss[r] = counts ? total * LN2 - hot[r] * scale : 0.f;
 }
 
-// A warp per row: joins the parts' statistics (and pulls), makes the target's logit.
-//   pull_i = sum_j p_ij w_j - w_{t_i}      (zeros for a row that does not count)
+// A warp per row: joins the parts' statistics (and pulls).  The target's product comes from hot, where the
+// parts leave the target out, or is made here.
+//   pull_i = sum_{j != t} p_ij w_j - (1 - p_it) w_t      (zeros for a row that does not count)
 template <typename T>
 __global__ void __launch_bounds__(256)
 loss_join_kernel(const float2* __restrict__ part, int parts, const float* __restrict__ part_o, const T* __restrict__ x, i64 ldx,
-                 i64 N, const T* __restrict__ w, i64 ldw, i64 V, int D, float scale, const i64* __restrict__ target, i64 ignore,
-                 float* __restrict__ loss, float* __restrict__ lse2, float* __restrict__ pull, int* err) {
+                 i64 N, const T* __restrict__ w, i64 ldw, i64 V, int D, float scale, float c, const i64* __restrict__ target, i64 ignore,
+                 const float* __restrict__ hot, float* __restrict__ loss, float* __restrict__ lse2, float* __restrict__ pull, int* err) {
   const i64 r = ((i64)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (r >= N) return;
-  float m, s;
-  const float total = join_parts(part, parts, N, r, lane, 32, m, s);
   const i64 t = target[r];
-  const bool counts = t != ignore && t >= 0 && t < V;
+  const bool there = t >= 0 && t < V, counts = there && t != ignore;
   if (t != ignore && !counts && lane == 0) raise(err, ERRBIT_BAD_INPUT);
-  float dot = 0.f;
-  if (counts)
-    for (int d = lane; d < D; d += 32) dot = fmaf(to_float(x[r * ldx + d]), to_float(w[t * ldw + d]), dot);
+  float m, others, s;
+  const float total = join_parts(part, parts, N, r, lane, 32, hot && there ? hot[r] * c : -INFINITY, m, others, s);
+  float logit = 0.f;
+  if (counts && hot) logit = hot[r] * fabsf(scale);  // hot holds products of +-x
+  if (!hot) {
+    if (counts)
+      for (int d = lane; d < D; d += 32) logit = fmaf(to_float(x[r * ldx + d]), to_float(w[t * ldw + d]), logit);
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+    for (int d = 16; d > 0; d >>= 1) logit += __shfl_xor_sync(0xffffffffu, logit, d);
+    logit *= scale;
+  }
   if (lane == 0) {
     lse2[r] = total;
-    loss[r] = counts ? total * LN2 - dot * scale : 0.f;
+    loss[r] = counts ? total * LN2 - logit : 0.f;
   }
   if (pull) {  // D <= 256: a lane has every 32nd column; the parts' weights go round the warp
-    const float inv = 1.f / s;
+    const float inv = 1.f / s, miss = others * inv;
     float v[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] = 0.f;
@@ -790,7 +827,7 @@ loss_join_kernel(const float2* __restrict__ part, int parts, const float* __rest
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       const int d = q * 32 + lane;
-      if (d < D) pull[r * D + d] = counts ? v[q] * inv - to_float(w[t * ldw + d]) : 0.f;
+      if (d < D) pull[r * D + d] = counts ? fmaf(-miss, to_float(w[t * ldw + d]), v[q] * inv) : 0.f;
     }
   }
 }
@@ -804,17 +841,12 @@ __global__ void loss_dx_kernel(const float* __restrict__ pull, const float* __re
   }
 }
 
-// dx[i] = sum over the slabs, less the target's row; zeros for a row that does not count
+// dx[i] = sum over the slabs
 template <typename T>
-__global__ void loss_join_dx_kernel(const float* __restrict__ slab, i64 N, int D, int slabs, const float* __restrict__ g, float scale,
-                                    const i64* __restrict__ target, const T* __restrict__ w, i64 ldw, T* __restrict__ dx) {
-  for (i64 e = (i64)blockIdx.x * blockDim.x + threadIdx.x; e < N * D; e += (i64)gridDim.x * blockDim.x) {
-    const i64 r = e / D;
+__global__ void loss_join_dx_kernel(const float* __restrict__ slab, i64 size, int slabs, T* __restrict__ dx) {
+  for (i64 e = (i64)blockIdx.x * blockDim.x + threadIdx.x; e < size; e += (i64)gridDim.x * blockDim.x) {
     float v = 0.f;
-    if (g[r] != 0.f) {
-      for (int z = 0; z < slabs; ++z) v += slab[z * (N * D) + e];
-      v = fmaf(-g[r] * scale, to_float(w[target[r] * ldw + (e - r * D)]), v);
-    }
+    for (int z = 0; z < slabs; ++z) v += slab[z * size + e];
     dx[e] = from_float<T>(v);
   }
 }
@@ -944,7 +976,7 @@ static TcFwdLayout fwd_layout(int planes, i64 N, i64 V, i64 D, bool pull) {
   auto take = [&](size_t b) { const size_t at = o; o += up256(b); return at; };
   const TcPlan p = tc_plan(planes, pull ? TC_PULL : TC_STATS, N, V, D);
   L.ms = take(8 * (size_t)p.parts * N);
-  L.hot = take(pull ? 0 : 4 * (size_t)N);
+  L.hot = take(4 * (size_t)N);
   L.o = take(pull ? 4 * (size_t)p.splits * N * D : 0);
   L.w = take(copy_bytes(planes, V, D));
   L.bytes = o;
@@ -997,10 +1029,11 @@ static int launch_tc(const CUtensorMap& b, const TcPlan& plan, const TcParams& p
 }
 
 template <typename T>
-void launch_loss_join(const LossArgs& a, const float2* part_ms, int parts, const float* part_o, float* pull) {
+void launch_loss_join(const LossArgs& a, const float2* part_ms, int parts, const float* part_o, const float* hot, float* pull) {
   LaunchScope ls(KID_LOSS_JOIN, a.st);
   loss_join_kernel<T><<<ceil_div_i(a.N, 8), 256, 0, a.st>>>(part_ms, parts, part_o, (const T*)a.x, a.ldx, a.N, (const T*)a.w, a.ldw, a.V,
-                                                            (int)a.D, a.scale, a.target, a.ignore, a.loss, a.lse2, pull, a.err);
+                                                            (int)a.D, a.scale, logit_factor(a.scale), a.target, a.ignore, hot, a.loss,
+                                                            a.lse2, pull, a.err);
 }
 
 // what the forward pass and both gradients have in common
@@ -1056,7 +1089,7 @@ int tc_loss_forward(const LossArgs& a, float* pull) {
   const int rc = with_shape<Planes<T>::count>(mode, a.N, a.V, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS, a.st); });
   if (rc != GSB_OK) return rc;
   if (pull) {
-    launch_loss_join<T>(a, p.part_ms, plan.parts, p.part_o, pull);
+    launch_loss_join<T>(a, p.part_ms, plan.parts, p.part_o, p.hot, pull);
     return GSB_OK;
   }
   const int lanes = plan.parts > 8 ? 32 : 1;
@@ -1110,7 +1143,7 @@ int tc_loss_grad_x(const LossArgs& a) {
   if (rc != GSB_OK) return rc;
   if (plan.splits > 1) {
     LaunchScope ls(KID_LOSS_JOIN, a.st);
-    loss_join_dx_kernel<T><<<blocks_for(a.N * a.D), 256, 0, a.st>>>(p.part_o, a.N, (int)a.D, plan.splits, a.g, a.scale, a.target, (const T*)a.w, a.ldw, (T*)a.dx);
+    loss_join_dx_kernel<T><<<blocks_for(a.N * a.D), 256, 0, a.st>>>(p.part_o, a.N * a.D, plan.splits, (T*)a.dx);
   }
   return GSB_OK;
 }
@@ -1121,9 +1154,9 @@ void tc_loss_dx(const LossArgs& a, const float* pull) {
   loss_dx_kernel<T><<<blocks_for(a.N * a.D), 256, 0, a.st>>>(pull, a.g, a.scale, a.N, (int)a.D, (T*)a.dx);
 }
 
-template void launch_loss_join<float>(const LossArgs&, const float2*, int, const float*, float*);
-template void launch_loss_join<__half>(const LossArgs&, const float2*, int, const float*, float*);
-template void launch_loss_join<__nv_bfloat16>(const LossArgs&, const float2*, int, const float*, float*);
+template void launch_loss_join<float>(const LossArgs&, const float2*, int, const float*, const float*, float*);
+template void launch_loss_join<__half>(const LossArgs&, const float2*, int, const float*, const float*, float*);
+template void launch_loss_join<__nv_bfloat16>(const LossArgs&, const float2*, int, const float*, const float*, float*);
 template int tc_loss_forward<float>(const LossArgs&, float*);
 template int tc_loss_forward<__half>(const LossArgs&, float*);
 template int tc_loss_forward<__nv_bfloat16>(const LossArgs&, float*);
