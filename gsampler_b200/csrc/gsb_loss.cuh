@@ -73,9 +73,26 @@ struct LossArgs {
 // How a type reaches the tensor cores: as it is, or as three bf16 planes (h + m + l, 8 bits each).
 template <typename S> struct Planes { typedef S type; static constexpr int count = 1; };
 template <> struct Planes<float> { typedef __nv_bfloat16 type; static constexpr int count = 3; };
-// dst[plane][r, :] = the planes of +-src[r, :], rows of packed_ld(D) elements; rows whose g is zero as zeros (gsb_loss_gemm.cu)
+// dst[plane][r, :] = the planes of +-src[r, :], rows of packed_ld(D) elements; with g and lse2, rows whose g is zero
+// and whose lse2 is not finite as zeros (gsb_loss_gemm.cu)
 template <typename S>
-void make_planes(const void* src, i64 ld, i64 rows, i64 D, bool negate, const float* g, void* dst, cudaStream_t st);
+void make_planes(const void* src, i64 ld, i64 rows, i64 D, bool negate, const float* g, const float* lse2, void* dst, cudaStream_t st);
+
+// Rounding to nearest would make the first plane of a finite value above this infinite (and the next ones
+// infinite the other way): it stays at the largest bf16, and the next planes hold the rest.
+__device__ __forceinline__ float first_plane(float v) {
+  constexpr float MOST = 3.3895313892515355e38f;  // (2 - 2^-7) 2^127
+  return fabsf(v) < INFINITY ? fminf(fmaxf(v, -MOST), MOST) : v;
+}
+// The two accumulators of plane products.  An infinite value is in its first plane and the others are
+// NaN, so the accumulator of the two first planes alone decides: what is not finite there stays what
+// it is, and the other counts as finite.
+__device__ __forceinline__ float finite_part(float low) {
+  float r;  // the smaller magnitude with low's sign: one instruction, where clamping takes two
+  asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(low), "f"(3.402823466e38f));
+  return r;
+}
+__device__ __forceinline__ float add_planes(float low, float high) { return high + finite_part(low); }
 
 // The streamed form (gsb_loss_tc.cu): 16-bit types of up to 256 columns, fp32 of up to 128.
 bool tc_loss_takes(int dtype, i64 D);

@@ -220,7 +220,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           tc_ld32(u, from + C::BN);
           tc_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] += u[j];
+          for (int j = 0; j < 32; ++j) v[j] = add_planes(v[j], u[j]);
         } else {
           tc_wait_ld();
         }
@@ -349,16 +349,17 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 }
 
 // dst[plane][r, :] = the planes of +-src[r, :] (one plane: the values themselves), rows of ldp elements
-// with zeros behind D.  Rows whose g is zero become zeros, so that nothing they hold reaches a product.
+// with zeros behind D.  Rows that do not count (g = 0) and hold what is not finite (lse2 is not, either)
+// become zeros, so that it reaches no product.
 template <typename S, typename T, int PL>
 __global__ void loss_planes_kernel(const S* __restrict__ src, i64 ld, i64 rows, int D, int ldp, bool negate,
-                                   const float* __restrict__ g, T* __restrict__ dst) {
+                                   const float* __restrict__ g, const float* __restrict__ lse2, T* __restrict__ dst) {
   const int chunks = ldp / 8;
   const i64 total = rows * chunks;
   for (i64 e = (i64)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (i64)gridDim.x * blockDim.x) {
     const i64 r = e / chunks;
     const int c = (int)(e - r * chunks) * 8;
-    const bool live = !g || g[r] != 0.f;
+    const bool live = !g || g[r] != 0.f || fabsf(lse2[r]) < INFINITY;
     float v[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
@@ -370,7 +371,7 @@ __global__ void loss_planes_kernel(const S* __restrict__ src, i64 ld, i64 rows, 
       Pack<T, 8> h;
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        h.v[q] = from_float<T>(v[q]);
+        h.v[q] = from_float<T>(PL > 1 && pl == 0 ? first_plane(v[q]) : v[q]);
         v[q] -= to_float(h.v[q]);
       }
       h.store(dst + (i64)pl * rows * ldp + r * ldp + c);
@@ -465,11 +466,11 @@ size_t gemm_loss_grad_workspace(int dtype, i64 N, i64 V, i64 D, bool dx, bool dw
 }
 
 template <typename S>
-void make_planes(const void* src, i64 ld, i64 rows, i64 D, bool negate, const float* g, void* dst, cudaStream_t st) {
+void make_planes(const void* src, i64 ld, i64 rows, i64 D, bool negate, const float* g, const float* lse2, void* dst, cudaStream_t st) {
   typedef typename Planes<S>::type T;
   LaunchScope ls(KID_LOSS_JOIN, st);
   loss_planes_kernel<S, T, Planes<S>::count><<<blocks_for(rows * packed_ld(D) / 8), 256, 0, st>>>(
-      (const S*)src, ld, rows, (int)D, (int)packed_ld(D), negate, g, (T*)dst);
+      (const S*)src, ld, rows, (int)D, (int)packed_ld(D), negate, g, lse2, (T*)dst);
 }
 
 template <typename T, typename C>
@@ -500,8 +501,8 @@ int gemm_loss_forward(const LossArgs& a) {
   char* ws = (char*)a.ws;
   const void *x = a.x, *w = a.w;
   i64 ldx = a.ldx, ldw = a.ldw;
-  if (PL == 3 || a.scale < 0.f || !tma_ready(x, ldx)) { make_planes<S>(x, ldx, a.N, a.D, a.scale < 0.f, nullptr, ws + L.x, a.st); x = ws + L.x; ldx = L.ldp; }
-  if (PL == 3 || !tma_ready(w, ldw)) { make_planes<S>(w, ldw, a.V, a.D, false, nullptr, ws + L.w, a.st); w = ws + L.w; ldw = L.ldp; }
+  if (PL == 3 || a.scale < 0.f || !tma_ready(x, ldx)) { make_planes<S>(x, ldx, a.N, a.D, a.scale < 0.f, nullptr, nullptr, ws + L.x, a.st); x = ws + L.x; ldx = L.ldp; }
+  if (PL == 3 || !tma_ready(w, ldw)) { make_planes<S>(w, ldw, a.V, a.D, false, nullptr, nullptr, ws + L.w, a.st); w = ws + L.w; ldw = L.ldp; }
   const int bn = bn_wide(PL);
   CUtensorMap ma, mb;
   if (!tc_map(&ma, x, IsBf16<T>::value, a.N, a.D, ldx, PL, 64, 128) || !tc_map(&mb, w, IsBf16<T>::value, a.V, a.D, ldw, PL, 64, bn)) return GSB_ERR_CUDA;
@@ -529,11 +530,11 @@ int gemm_loss_backward(const LossArgs& a) {
   constexpr bool bf = IsBf16<T>::value;
   const GmLayout L = gemm_layout(PL, a.N, a.V, a.D, false, a.dx != nullptr, a.dw != nullptr);
   char* ws = (char*)a.ws;
-  make_planes<S>(a.x, a.ldx, a.N, a.D, a.scale < 0.f, a.g, ws + L.x, a.st);
+  make_planes<S>(a.x, a.ldx, a.N, a.D, a.scale < 0.f, a.g, a.lse2, ws + L.x, a.st);
   const T* x = (const T*)(ws + L.x);
   const T* w = (const T*)a.w;
   i64 ldw = a.ldw;
-  if (PL == 3 || !tma_ready(w, ldw)) { make_planes<S>(a.w, a.ldw, a.V, a.D, false, nullptr, ws + L.w, a.st); w = (const T*)(ws + L.w); ldw = L.ldp; }
+  if (PL == 3 || !tma_ready(w, ldw)) { make_planes<S>(a.w, a.ldw, a.V, a.D, false, nullptr, nullptr, ws + L.w, a.st); w = (const T*)(ws + L.w); ldw = L.ldp; }
   void* piece = ws + L.piece;
   float* dxs = (float*)(ws + L.dx_slab);
   float* dws = (float*)(ws + L.dw_slab);
@@ -618,7 +619,7 @@ int gemm_loss_backward(const LossArgs& a) {
   return GSB_OK;
 }
 
-template void make_planes<float>(const void*, i64, i64, i64, bool, const float*, void*, cudaStream_t);
+template void make_planes<float>(const void*, i64, i64, i64, bool, const float*, const float*, void*, cudaStream_t);
 template int gemm_loss_forward<float>(const LossArgs&);
 template int gemm_loss_forward<__half>(const LossArgs&);
 template int gemm_loss_forward<__nv_bfloat16>(const LossArgs&);

@@ -34,7 +34,7 @@
 
 namespace gsb {
 
-constexpr int WIPE = -2;  // in the place of a target: the row must be zeroed
+constexpr int WIPE = -2;  // in the place of a target: the row must be zeroed, and its P with it
 
 enum { TC_STATS = 0, TC_PULL = 1, TC_GRAD_W = 2, TC_GRAD_X = 3 };
 
@@ -152,12 +152,12 @@ __device__ __forceinline__ void row_pieces(Pack<V, 32> (&to)[PIECES], const V* f
 }
 
 // Pairs of values as packed 16-bit elements; with more planes to come, the values become what this
-// plane does not hold.
+// plane does not hold.  `any`: values of any size, and this is their first plane.
 template <typename T, int N>
-__device__ __forceinline__ void take_plane(u32 (&h)[N], float* v, bool more) {
+__device__ __forceinline__ void take_plane(u32 (&h)[N], float* v, bool more, bool any) {
 #pragma unroll
   for (int q = 0; q < N; ++q) {
-    h[q] = pack2<T>(v[2 * q], v[2 * q + 1]);
+    h[q] = any ? pack2<T>(first_plane(v[2 * q]), first_plane(v[2 * q + 1])) : pack2<T>(v[2 * q], v[2 * q + 1]);
     if (more) {
       const T* t = reinterpret_cast<const T*>(h + q);
       v[2 * q] -= to_float(t[0]);
@@ -349,7 +349,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
 #pragma unroll
               for (int q = 0; q < 16; ++q) h[q] = reinterpret_cast<const u32*>(piece[i].v)[q];
             } else {
-              take_plane<T>(h, reinterpret_cast<float*>(piece[i].v), pl + 1 < C::PL);
+              take_plane<T>(h, reinterpret_cast<float*>(piece[i].v), pl + 1 < C::PL, pl == 0);
             }
 #pragma unroll
             for (int q = 0; q < 16; ++q) h[q] ^= p.a_sign;
@@ -410,7 +410,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
           tc_ld32(u, tmem + C::O_COL + C::DP + k + lanes);
           tc_wait_ld();
 #pragma unroll
-          for (int q = 0; q < 32; ++q) kept[i * 32 + q] += o[q] + u[q];
+          for (int q = 0; q < 32; ++q) kept[i * 32 + q] += add_planes(o[q], u[q]);
         }
       }
     };
@@ -440,7 +440,8 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
             tc_ld32(u, S + C::BT + k);
             tc_wait_ld();
 #pragma unroll
-            for (int q = 0; q < 32; ++q) v[k + q] += u[q];
+            for (int q = 0; q < 32; q += 2)
+              part2(add2(join2(finite_part(v[k + q]), finite_part(v[k + q + 1])), join2(u[q], u[q + 1])), v[k + q], v[k + q + 1]);
           }
         }
         tc_wait_ld();
@@ -459,11 +460,19 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
           const float* gs = reinterpret_cast<const float*>(meta + 8 * C::BT);
           bool near = false;
 #pragma unroll
-          for (int k = 0; k < C::HC / 32; ++k) near |= (u32)(tgt[k * 32 + lane] - (row - lane)) < 32u;
-          if (__any_sync(0xffffffffu, near)) {  // some row's target is one of this warp's vocabulary rows
+          for (int k = 0; k < C::HC / 32; ++k) {
+            const int t = tgt[k * 32 + lane];
+            near |= (u32)(t - (row - lane)) < 32u || t == WIPE;
+          }
+          // some row's target is one of this warp's vocabulary rows, or some row is zeros: times a masked class's
+          // infinity that is a NaN
+          if (__any_sync(0xffffffffu, near)) {
 #pragma unroll
-            for (int k = 0; k < C::HC; ++k)
-              if (tgt[k] == row) v[k] -= gs[k];
+            for (int k = 0; k < C::HC; ++k) {
+              const int t = tgt[k];
+              if (t == row) v[k] -= gs[k];
+              if (t == WIPE) v[k] = 0.f;
+            }
           }
         } else if constexpr (C::MODE == TC_GRAD_X) {
           const int col0 = (t0 + j) * C::BT + half * C::HC;
@@ -556,7 +565,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
 #pragma unroll
           for (int pl = 0; pl < C::PL; ++pl) {
             u32 h[C::HC / 2];
-            take_plane<T>(h, v, pl + 1 < C::PL);
+            take_plane<T>(h, v, pl + 1 < C::PL, false);
             if constexpr (C::MODE == TC_GRAD_W) {
               // rows with a negative upstream gradient: the sign of their whole column
               const u32* sign = reinterpret_cast<const u32*>(smem + C::OFF_META + st * C::META + 12 * C::BT) + half * (C::HC / 2);
@@ -699,7 +708,8 @@ __global__ void loss_pack_kernel(const T* __restrict__ src, i64 ld, i64 rows, in
 
 // What the dW pass needs of every row of x, by tiles of BT rows: -bias (p g = exp2(l - bias)), target,
 // |g| as P holds it, and the sign as a mask of the packed element.  Rows that do not count, and the
-// rows behind the last, have an infinite bias: P = 0.
+// rows behind the last, have an infinite bias: P = 0.  That is not enough where the row is taken as zeros,
+// behind the last and where it holds an infinity or a NaN: WIPE.
 __global__ void loss_meta_kernel(const float* __restrict__ lse2, const i64* __restrict__ target, const float* __restrict__ g,
                                  const u32* __restrict__ top, i64 N, i64 Npad, int BT, unsigned char* __restrict__ meta) {
   const i64 r = (i64)blockIdx.x * blockDim.x + threadIdx.x;
@@ -709,7 +719,7 @@ __global__ void loss_meta_kernel(const float* __restrict__ lse2, const i64* __re
   float bias = INFINITY, gs = 0.f;
   int t = -1;
   u32 sign = 0;
-  if (r < N && g[r] == 0.f && !(fabsf(lse2[r]) < INFINITY)) t = WIPE;
+  if (r >= N || (g[r] == 0.f && !(fabsf(lse2[r]) < INFINITY))) t = WIPE;
   if (r < N && g[r] != 0.f) {
     const float rel = fabsf(g[r]) / __uint_as_float(*top);
     gs = rel * (float)(1 << GRAD_SHIFT);
@@ -1059,12 +1069,13 @@ static TcParams base_params(const LossArgs& a, const TcPlan& plan, bool vocabula
   return p;
 }
 // The map of the streamed matrix; rows that TMA does not take as they lie are copied to `copy` first.
-// fp32 rows go there as planes, those whose g is zero as zeros.
+// fp32 rows go there as planes, those that must not reach a product as zeros.
 template <typename T>
-static bool stream_map(CUtensorMap* map, const void* src, i64 ld, i64 rows, i64 D, int box_rows, const float* g, void* copy, cudaStream_t st) {
+static bool stream_map(CUtensorMap* map, const void* src, i64 ld, i64 rows, i64 D, int box_rows, const float* g, const float* lse2, void* copy,
+                       cudaStream_t st) {
   constexpr int planes = Planes<T>::count;
   if constexpr (planes == 3) {
-    make_planes<T>(src, ld, rows, D, false, g, copy, st);
+    make_planes<T>(src, ld, rows, D, false, g, lse2, copy, st);
     src = copy;
     ld = packed_ld(D);
   } else if (!tma_ready(src, ld)) {
@@ -1081,7 +1092,7 @@ int tc_loss_forward(const LossArgs& a, float* pull) {
   const TcFwdLayout L = fwd_layout(Planes<T>::count, a.N, a.V, a.D, pull != nullptr);
   char* ws = (char*)a.ws;
   CUtensorMap mb;
-  if (!stream_map<T>(&mb, a.w, a.ldw, a.V, a.D, plan.BT, nullptr, ws + L.w, a.st)) return GSB_ERR_CUDA;
+  if (!stream_map<T>(&mb, a.w, a.ldw, a.V, a.D, plan.BT, nullptr, nullptr, ws + L.w, a.st)) return GSB_ERR_CUDA;
   TcParams p = base_params<T>(a, plan, false);
   p.part_ms = (float2*)(ws + L.ms);
   p.part_o = (float*)(ws + L.o);
@@ -1111,7 +1122,7 @@ int tc_loss_grad_w(const LossArgs& a) {
     loss_meta_kernel<<<ceil_div_i(npad, 256), 256, 0, a.st>>>(a.lse2, a.target, a.g, a.top, a.N, npad, plan.BT, (unsigned char*)(ws + L.meta));
   }
   CUtensorMap mb;
-  if (!stream_map<T>(&mb, a.x, a.ldx, a.N, a.D, plan.BT, a.g, ws + L.x, a.st)) return GSB_ERR_CUDA;
+  if (!stream_map<T>(&mb, a.x, a.ldx, a.N, a.D, plan.BT, a.g, a.lse2, ws + L.x, a.st)) return GSB_ERR_CUDA;
   TcParams p = base_params<T>(a, plan, true);
   p.meta = (const unsigned char*)(ws + L.meta);
   p.part_o = (float*)(ws + L.dw_slab);
@@ -1132,7 +1143,7 @@ int tc_loss_grad_x(const LossArgs& a) {
   const TcGradLayout L = grad_layout(Planes<T>::count, a.N, a.V, a.D, true, a.dw != nullptr);
   char* ws = (char*)a.ws;
   CUtensorMap mb;
-  if (!stream_map<T>(&mb, a.w, a.ldw, a.V, a.D, plan.BT, nullptr, ws + L.w, a.st)) return GSB_ERR_CUDA;
+  if (!stream_map<T>(&mb, a.w, a.ldw, a.V, a.D, plan.BT, nullptr, nullptr, ws + L.w, a.st)) return GSB_ERR_CUDA;
   TcParams p = base_params<T>(a, plan, false);
   p.w = a.w;
   p.ldw = a.ldw;
