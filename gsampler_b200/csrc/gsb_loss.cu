@@ -63,10 +63,11 @@ static int total_blocks(i64 N) {
 }
 
 // g[i] = upstream gradient of row i's loss (divided by the count for the mean), 0 where the row
-// does not count; top = bits of the largest magnitude (an integer maximum: no order matters).
+// does not count; top = bits of the largest finite magnitude (an integer maximum: no order matters).
 __global__ void loss_row_grad_kernel(const float* __restrict__ up, int per_row, const float* __restrict__ count,
                                      const i64* __restrict__ target, i64 ignore, i64 V, i64 N, float* __restrict__ g,
                                      u32* top) {
+  constexpr u32 INFINITE = 0x7F800000u;
   u32 mine = 0;
   for (i64 i = (i64)blockIdx.x * blockDim.x + threadIdx.x; i < N; i += (i64)gridDim.x * blockDim.x) {
     const i64 t = target[i];
@@ -74,10 +75,13 @@ __global__ void loss_row_grad_kernel(const float* __restrict__ up, int per_row, 
     if (t != ignore && t >= 0 && t < V) v = per_row ? up[i] : (count ? *up / *count : *up);
     g[i] = v;
     const u32 b = __float_as_uint(fabsf(v));
-    mine = b > mine ? b : mine;
+    mine = b > mine && b < INFINITE ? b : mine;
   }
   if (!per_row) {  // the same for every row that counts
-    if (blockIdx.x == 0 && threadIdx.x == 0) *top = __float_as_uint(fabsf(count ? *up / *count : *up));
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      const u32 b = __float_as_uint(fabsf(count ? *up / *count : *up));
+      *top = b < INFINITE ? b : 0;
+    }
     return;
   }
   mine = __reduce_max_sync(0xffffffffu, mine);
@@ -188,7 +192,7 @@ extern "C" int gsb_linear_ce_grad(const void* x, int dtype, int64_t ldx, int64_t
   LossArgs a = {};
   a.x = x; a.ldx = ldx; a.N = N; a.w = weight; a.ldw = ldw; a.V = V; a.D = D;
   a.target = (const i64*)target; a.ignore = ignore; a.scale = scale; a.lse2 = const_cast<float*>(lse2);
-  a.g = g; a.top = top; a.dx = dx; a.dw = dw; a.ws = ws + up256(4 * (size_t)N) + 256; a.err = d_err; a.st = st;
+  a.per_row = per_row; a.g = g; a.top = top; a.dx = dx; a.dw = dw; a.ws = ws + up256(4 * (size_t)N) + 256; a.err = d_err; a.st = st;
   int rc = GSB_OK;
   if (!tc_loss_takes(dtype, D)) {
     rc = dtype == GSB_F32 ? gemm_loss_backward<float>(a)

@@ -9,7 +9,9 @@ namespace gsb {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int FWD_SHIFT = 7;    // the forward pass holds p at 2^7 times its value relative to the row's reference
-constexpr int GRAD_SHIFT = 14;  // the backward pass holds g (p - target) at 2^14 / max |g| times its value
+// The backward pass holds g (p - target) at 2^14 / max |g| times its value for dW, whose sums run over the rows; for
+// dx g is a factor of the row, and fp16 holds p at 2^14 times its value.
+constexpr int GRAD_SHIFT = 14;
 constexpr float MOVE_REFERENCE = 8.f;  // a row's reference moves when its maximum passes it by 2^8
 
 // Factor from x . w to a base-2 logit, |scale| log2 e (the sign goes into x).  Not zero, so that a
@@ -62,8 +64,9 @@ struct LossArgs {
   float scale;
   float* loss;   // [N]
   float* lse2;   // [N], base 2
+  int per_row;     // whether rows have gradients of their own
   const float* g;  // [N] upstream gradient of every row's loss, 0 where it does not count
-  const u32* top;  // bits of the largest |g|
+  const u32* top;  // bits of the largest finite |g|: one row's infinity or NaN is not a factor of the others
   void *dx, *dw;
   void* ws;
   int* err;
@@ -74,9 +77,21 @@ struct LossArgs {
 template <typename S> struct Planes { typedef S type; static constexpr int count = 1; };
 template <> struct Planes<float> { typedef __nv_bfloat16 type; static constexpr int count = 3; };
 // dst[plane][r, :] = the planes of +-src[r, :], rows of packed_ld(D) elements; with g and lse2, rows whose g is zero
-// and whose lse2 is not finite as zeros (gsb_loss_gemm.cu)
+// and whose lse2 is not finite as zeros; with top, rows times 2^small_rows (gsb_loss_gemm.cu)
 template <typename S>
-void make_planes(const void* src, i64 ld, i64 rows, i64 D, bool negate, const float* g, const float* lse2, void* dst, cudaStream_t st);
+void make_planes(const void* src, i64 ld, i64 rows, i64 D, bool negate, const float* g, const float* lse2, const u32* top, void* dst,
+                 cudaStream_t st);
+
+// Where one array of g (p - target) serves both dx and dW, a row whose |g| is below 2^-16 of the largest would
+// lose its digits in fp16.  Such a row is held times a power of two, 2^-small_rows, that brings it there (to at
+// most top / 2^15), and its row of x takes the power back for dW.
+template <typename T>
+__device__ __forceinline__ int small_rows(float g, float top) {
+  if (sizeof(T) != 2 || IsBf16<T>::value || !(fabsf(g) < INFINITY) || g == 0.f || top == 0.f) return 0;
+  const int e = ilogbf(g) - ilogbf(top) + 16;
+  return e < 0 ? e : 0;
+}
+__device__ __forceinline__ float times_power(float v, int e) { return e == 0 ? v : scalbnf(v, e); }
 
 // Rounding to nearest would make the first plane of a finite value above this infinite (and the next ones
 // infinite the other way): it stays at the largest bf16, and the next planes hold the rest.

@@ -209,7 +209,8 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       int hot = -1;
       if (C::MODE == GM_PIECE && row < p.M && p.g[row] != 0.f) {
         lse = p.lse2[row];
-        gs = p.g[row] / __uint_as_float(*p.top) * (float)(1 << GRAD_SHIFT);
+        const float top = __uint_as_float(*p.top);
+        gs = times_power(p.g[row], -small_rows<T>(p.g[row], top)) / top * (float)(1 << GRAD_SHIFT);
         hot = (int)(p.target[row] - p.v0);
       }
       auto columns = [&](float* v, int q) {  // 32 of the tile's columns, the accumulators added
@@ -350,21 +351,24 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 
 // dst[plane][r, :] = the planes of +-src[r, :] (one plane: the values themselves), rows of ldp elements
 // with zeros behind D.  Rows that do not count (g = 0) and hold what is not finite (lse2 is not, either)
-// become zeros, so that it reaches no product.
+// become zeros, so that it reaches no product; with top, a row takes back the power of two that its g was given.
 template <typename S, typename T, int PL>
 __global__ void loss_planes_kernel(const S* __restrict__ src, i64 ld, i64 rows, int D, int ldp, bool negate,
-                                   const float* __restrict__ g, const float* __restrict__ lse2, T* __restrict__ dst) {
+                                   const float* __restrict__ g, const float* __restrict__ lse2, const u32* __restrict__ top,
+                                   T* __restrict__ dst) {
   const int chunks = ldp / 8;
   const i64 total = rows * chunks;
   for (i64 e = (i64)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (i64)gridDim.x * blockDim.x) {
     const i64 r = e / chunks;
     const int c = (int)(e - r * chunks) * 8;
     const bool live = !g || g[r] != 0.f || fabsf(lse2[r]) < INFINITY;
+    const int small = top && live ? small_rows<T>(g[r], __uint_as_float(*top)) : 0;
     float v[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       v[q] = live && c + q < D ? to_float(src[r * ld + c + q]) : 0.f;
       if (negate) v[q] = -v[q];
+      v[q] = times_power(v[q], small);
     }
 #pragma unroll
     for (int pl = 0; pl < PL; ++pl) {
@@ -384,15 +388,16 @@ template <typename T>
 __global__ void loss_wide_dx_kernel(const float* __restrict__ slab, i64 N, i64 D, int slabs, float factor, const u32* __restrict__ top,
                                     const float* __restrict__ g, const float* __restrict__ lost, const i64* __restrict__ target,
                                     const T* __restrict__ w, i64 ldw, T* __restrict__ dx) {
-  const float f = factor * __uint_as_float(*top);
+  const float largest = __uint_as_float(*top);
   for (i64 e = (i64)blockIdx.x * blockDim.x + threadIdx.x; e < N * D; e += (i64)gridDim.x * blockDim.x) {
     const i64 r = e / D;
     float v = 0.f;
     if (g[r] != 0.f) {
       for (int z = 0; z < slabs; ++z) v += slab[z * (N * D) + e];
       if (lost) v = fmaf(lost[r], to_float(w[target[r] * ldw + (e - r * D)]), v);
+      v *= factor * times_power(largest, small_rows<T>(g[r], largest));
     }
-    dx[e] = from_float<T>(v * f);
+    dx[e] = from_float<T>(v);
   }
 }
 
@@ -423,15 +428,19 @@ static i64 piece_columns(i64 N, i64 V) {
   if (c < 128) c = 128;
   return c < V ? c : V;
 }
+template <typename S>
+static constexpr int dtype_of() { return sizeof(S) == 4 ? GSB_F32 : IsBf16<S>::value ? GSB_BF16 : GSB_F16; }
 static int bn_of(int planes, i64 cols) { return planes == 3 ? (cols <= 64 ? 64 : 128) : 256; }  // dx, dW
 static int bn_wide(int planes) { return planes == 3 ? 128 : 256; }                               // logits
 
 struct GmLayout {
-  size_t ms, x, w, piece, lost, dx_slab, dw_slab, bytes;
+  size_t ms, x, x_dw, w, piece, lost, dx_slab, dw_slab, bytes;
+  bool x_dw_taken;
   i64 cols, ldp;
   int dx_slabs, dw_slabs, splits, per;
 };
-static GmLayout gemm_layout(int planes, i64 N, i64 V, i64 D, bool forward, bool dx, bool dw) {
+static GmLayout gemm_layout(int dtype, i64 N, i64 V, i64 D, bool forward, bool dx, bool dw) {
+  const int planes = dtype == GSB_F32 ? 3 : 1;
   GmLayout L = {};
   size_t o = 0;
   auto take = [&](size_t b) { const size_t at = o; o += up256(b); return at; };
@@ -449,6 +458,8 @@ static GmLayout gemm_layout(int planes, i64 N, i64 V, i64 D, bool forward, bool 
     L.dw_slabs = slab_count(L.cols, D, N, bn_of(planes, D));
     L.piece = take(2 * (size_t)planes * N * packed_ld(L.cols));
     L.lost = take(4 * (size_t)N);
+    L.x_dw_taken = dw && dtype == GSB_F16;
+    L.x_dw = take(L.x_dw_taken ? 2 * (size_t)N * L.ldp : 0);
     L.dx_slab = take(dx ? 4 * (size_t)L.dx_slabs * N * D : 0);
     L.dw_slab = take(dw ? 4 * (size_t)L.dw_slabs * L.cols * D : 0);
   }
@@ -457,20 +468,21 @@ static GmLayout gemm_layout(int planes, i64 N, i64 V, i64 D, bool forward, bool 
   return L;
 }
 size_t gemm_loss_workspace(int dtype, i64 N, i64 V, i64 D, bool pack_w) {
-  const GmLayout L = gemm_layout(dtype == GSB_F32 ? 3 : 1, N, V, D, true, false, false);
+  const GmLayout L = gemm_layout(dtype, N, V, D, true, false, false);
   return dtype == GSB_F32 || pack_w ? L.bytes : L.w;
 }
 size_t gemm_loss_grad_workspace(int dtype, i64 N, i64 V, i64 D, bool dx, bool dw, bool pack_w) {
-  const GmLayout L = gemm_layout(dtype == GSB_F32 ? 3 : 1, N, V, D, false, dx, dw);
+  const GmLayout L = gemm_layout(dtype, N, V, D, false, dx, dw);
   return dtype == GSB_F32 || pack_w ? L.bytes : L.w;
 }
 
 template <typename S>
-void make_planes(const void* src, i64 ld, i64 rows, i64 D, bool negate, const float* g, const float* lse2, void* dst, cudaStream_t st) {
+void make_planes(const void* src, i64 ld, i64 rows, i64 D, bool negate, const float* g, const float* lse2, const u32* top, void* dst,
+                 cudaStream_t st) {
   typedef typename Planes<S>::type T;
   LaunchScope ls(KID_LOSS_JOIN, st);
   loss_planes_kernel<S, T, Planes<S>::count><<<blocks_for(rows * packed_ld(D) / 8), 256, 0, st>>>(
-      (const S*)src, ld, rows, (int)D, (int)packed_ld(D), negate, g, lse2, (T*)dst);
+      (const S*)src, ld, rows, (int)D, (int)packed_ld(D), negate, g, lse2, top, (T*)dst);
 }
 
 template <typename T, typename C>
@@ -497,12 +509,12 @@ template <typename S>
 int gemm_loss_forward(const LossArgs& a) {
   typedef typename Planes<S>::type T;
   constexpr int PL = Planes<S>::count;
-  const GmLayout L = gemm_layout(PL, a.N, a.V, a.D, true, false, false);
+  const GmLayout L = gemm_layout(dtype_of<S>(), a.N, a.V, a.D, true, false, false);
   char* ws = (char*)a.ws;
   const void *x = a.x, *w = a.w;
   i64 ldx = a.ldx, ldw = a.ldw;
-  if (PL == 3 || a.scale < 0.f || !tma_ready(x, ldx)) { make_planes<S>(x, ldx, a.N, a.D, a.scale < 0.f, nullptr, nullptr, ws + L.x, a.st); x = ws + L.x; ldx = L.ldp; }
-  if (PL == 3 || !tma_ready(w, ldw)) { make_planes<S>(w, ldw, a.V, a.D, false, nullptr, nullptr, ws + L.w, a.st); w = ws + L.w; ldw = L.ldp; }
+  if (PL == 3 || a.scale < 0.f || !tma_ready(x, ldx)) { make_planes<S>(x, ldx, a.N, a.D, a.scale < 0.f, nullptr, nullptr, nullptr, ws + L.x, a.st); x = ws + L.x; ldx = L.ldp; }
+  if (PL == 3 || !tma_ready(w, ldw)) { make_planes<S>(w, ldw, a.V, a.D, false, nullptr, nullptr, nullptr, ws + L.w, a.st); w = ws + L.w; ldw = L.ldp; }
   const int bn = bn_wide(PL);
   CUtensorMap ma, mb;
   if (!tc_map(&ma, x, IsBf16<T>::value, a.N, a.D, ldx, PL, 64, 128) || !tc_map(&mb, w, IsBf16<T>::value, a.V, a.D, ldw, PL, 64, bn)) return GSB_ERR_CUDA;
@@ -528,13 +540,19 @@ int gemm_loss_backward(const LossArgs& a) {
   typedef typename Planes<S>::type T;
   constexpr int PL = Planes<S>::count;
   constexpr bool bf = IsBf16<T>::value;
-  const GmLayout L = gemm_layout(PL, a.N, a.V, a.D, false, a.dx != nullptr, a.dw != nullptr);
+  const GmLayout L = gemm_layout(dtype_of<S>(), a.N, a.V, a.D, false, a.dx != nullptr, a.dw != nullptr);
   char* ws = (char*)a.ws;
-  make_planes<S>(a.x, a.ldx, a.N, a.D, a.scale < 0.f, a.g, a.lse2, ws + L.x, a.st);
+  // x for the logits, and where rows of fp16 may have small_rows' powers, with these for dW
+  make_planes<S>(a.x, a.ldx, a.N, a.D, a.scale < 0.f, a.g, a.lse2, nullptr, ws + L.x, a.st);
   const T* x = (const T*)(ws + L.x);
+  const T* x_dw = x;
+  if (a.dw && L.x_dw_taken && a.per_row) {
+    make_planes<S>(a.x, a.ldx, a.N, a.D, a.scale < 0.f, a.g, a.lse2, a.top, ws + L.x_dw, a.st);
+    x_dw = (const T*)(ws + L.x_dw);
+  }
   const T* w = (const T*)a.w;
   i64 ldw = a.ldw;
-  if (PL == 3 || !tma_ready(w, ldw)) { make_planes<S>(a.w, a.ldw, a.V, a.D, false, nullptr, nullptr, ws + L.w, a.st); w = (const T*)(ws + L.w); ldw = L.ldp; }
+  if (PL == 3 || !tma_ready(w, ldw)) { make_planes<S>(a.w, a.ldw, a.V, a.D, false, nullptr, nullptr, nullptr, ws + L.w, a.st); w = (const T*)(ws + L.w); ldw = L.ldp; }
   void* piece = ws + L.piece;
   float* dxs = (float*)(ws + L.dx_slab);
   float* dws = (float*)(ws + L.dw_slab);
@@ -592,7 +610,7 @@ int gemm_loss_backward(const LossArgs& a) {
       if (rc != GSB_OK) return rc;
     }
     if (a.dw) {
-      if (!tc_map(&ma, piece, bf, a.N, c, ldq, PL, 64, 64) || !tc_map(&mb, x, bf, a.N, a.D, L.ldp, PL, 64, 64)) return GSB_ERR_CUDA;
+      if (!tc_map(&ma, piece, bf, a.N, c, ldq, PL, 64, 64) || !tc_map(&mb, x_dw, bf, a.N, a.D, L.ldp, PL, 64, 64)) return GSB_ERR_CUDA;
       GmParams p = {};
       p.M = (int)c;
       p.N = (int)a.D;
@@ -619,7 +637,7 @@ int gemm_loss_backward(const LossArgs& a) {
   return GSB_OK;
 }
 
-template void make_planes<float>(const void*, i64, i64, i64, bool, const float*, const float*, void*, cudaStream_t);
+template void make_planes<float>(const void*, i64, i64, i64, bool, const float*, const float*, const u32*, void*, cudaStream_t);
 template int gemm_loss_forward<float>(const LossArgs&);
 template int gemm_loss_forward<__half>(const LossArgs&);
 template int gemm_loss_forward<__nv_bfloat16>(const LossArgs&);

@@ -14,9 +14,9 @@
 //             dx ~ sum_{j != t} p_j w_j - (1 - p_t) w_t, and the rounding of p_t, half a step however
 //             likely the target is, would be many times 1 - p_t.
 //   dW        A = rows of W, B = rows of x.  P = g (p - target) with the known log-sum-exp.
-//   dx        (small vocabularies, fp32) A = rows of x, B = the vocabulary, P = g p without the target's,
-//             whose g (p_t - 1) w_t is added in 32 bits.  Makes the logits once more instead of keeping the
-//             expected rows.
+//   dx        (small vocabularies, fp32) A = rows of x, B = the vocabulary, P = p without the target's,
+//             whose (p_t - 1) w_t is added in 32 bits; the row's g is a factor at the end, so that no row's
+//             scale is another's.  Makes the logits once more instead of keeping the expected rows.
 // So training costs four products of N V D multiply-adds (five with dx by itself), and no array of
 // N x V values exists anywhere.
 //
@@ -74,7 +74,7 @@ struct TcShape {
   // truncates, which over hundreds of tiles is more than 32-bit values may lose
   static constexpr int FLUSH = PL == 3 ? 16 : 0;
   static constexpr int OFF_B = NA * A_BYTES, OFF_META = OFF_B + ST * B_BYTES;
-  static constexpr int OFF_COEF = OFF_META + ST * META;  // TC_GRAD_X: g (p_t - 1) by half and row
+  static constexpr int OFF_COEF = OFF_META + ST * META;  // TC_GRAD_X: p_t - 1 by half and row
   static constexpr int OFF_BAR = OFF_COEF + (MODE == TC_GRAD_X ? WG * 128 * 4 : 0);
   static constexpr int BARS = 3 * ST + 2 * NB + 3;
   static constexpr int BYTES = OFF_BAR + 8 * BARS + 16 + 1024;  // and room to align the base
@@ -105,8 +105,8 @@ struct TcParams {
   float2* part_ms;          // TC_STATS / TC_PULL: [parts][rows_a] reference and sum
   float* part_o;            // TC_PULL, gradients with splits: [splits][rows_a][D]
   void* out;                // gradients without splits: [rows_a][D]
-  const u32* top;           // gradients: bits of max |g|
-  float out_scale;          // scale 2^-GRAD_SHIFT
+  const u32* top;           // TC_GRAD_W: bits of the largest finite |g|
+  float out_scale;          // scale over what P is held at
   int* err;
 };
 
@@ -165,6 +165,10 @@ __device__ __forceinline__ void take_plane(u32 (&h)[N], float* v, bool more, boo
     }
   }
 }
+
+// what dx holds p times
+template <typename T>
+__host__ __device__ constexpr float dx_unit() { return IsBf16<T>::value ? 1.f : (float)(1 << GRAD_SHIFT); }
 
 // T: type of the planes, V: of the values in memory
 template <typename T, typename V, typename C>
@@ -382,16 +386,18 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
     };
     float m = -INFINITY, sum = 0.f;
     const u64 c2 = join2(p.c, p.c);
-    // the target, and for dx the row's scaled gradient (an infinite bias: P = 0) and what becomes of it at the target
+    // the target, and for dx the row's gradient (an infinite bias: P = 0) and p - 1 at the target, held as P is:
+    // p itself, and only for fp16 at 2^14 times that (by a product, an addition to the exponent would round p near 1)
+    constexpr float UNIT = dx_unit<T>();
     int hot = -1;
-    float gs = 0.f, row_bias = -INFINITY, coef = 0.f;
+    float row_grad = 0.f, row_bias = -INFINITY, coef = 0.f;
     if ((C::MODE == TC_STATS || C::MODE == TC_PULL) && row < p.rows_a) {
       const i64 t = p.target[row];
       if (t >= 0 && t < p.rows_b) hot = (int)t;
     }
     if (C::MODE == TC_GRAD_X && row_live) {
       hot = (int)p.target[row];  // in range: the row counts
-      gs = p.g[row] / __uint_as_float(*p.top) * (float)(1 << GRAD_SHIFT);
+      row_grad = p.g[row];
       row_bias = -p.lse2[row];
     }
     bool ok = true;
@@ -481,12 +487,12 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
             for (int k = 0; k < C::HC; ++k)
               if (col0 + k >= p.rows_b) v[k] = -INFINITY;
           }
-          const u64 bias2 = both(row_bias), gs2 = both(gs);
+          const u64 bias2 = both(row_bias);
 #pragma unroll
           for (int k = 0; k < C::HC; k += 2) {
             part2(fma2(join2(v[k], v[k + 1]), c2, bias2), v[k], v[k + 1]);
             exponentials(v[k], v[k + 1], k);
-            part2(mul2(join2(v[k], v[k + 1]), gs2), v[k], v[k + 1]);
+            if (UNIT != 1.f) part2(mul2(join2(v[k], v[k + 1]), both(UNIT)), v[k], v[k + 1]);
           }
           const int at = hot - col0;
           if (__any_sync(0xffffffffu, (u32)at < (u32)C::HC)) {
@@ -497,7 +503,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
                 mine = v[k];
                 v[k] = 0.f;
               }
-            if ((u32)at < (u32)C::HC) coef = mine - gs;
+            if ((u32)at < (u32)C::HC) coef = mine - UNIT;
           }
         } else {
           const int col0 = (t0 + j) * C::BT + half * C::HC;
@@ -609,7 +615,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
       if (ok && warp_live) {
         tc_after();
         if constexpr (C::FLUSH != 0) keep();
-        const float f = C::MODE == TC_PULL ? 1.f : p.out_scale * __uint_as_float(*p.top);
+        const float f = C::MODE == TC_PULL ? 1.f : p.out_scale * (C::MODE == TC_GRAD_X ? row_grad : __uint_as_float(*p.top));
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
           const int k = half * 32 + i * (32 * C::HV);
@@ -1075,7 +1081,7 @@ static bool stream_map(CUtensorMap* map, const void* src, i64 ld, i64 rows, i64 
                        cudaStream_t st) {
   constexpr int planes = Planes<T>::count;
   if constexpr (planes == 3) {
-    make_planes<T>(src, ld, rows, D, false, g, lse2, copy, st);
+    make_planes<T>(src, ld, rows, D, false, g, lse2, nullptr, copy, st);
     src = copy;
     ld = packed_ld(D);
   } else if (!tma_ready(src, ld)) {
@@ -1148,6 +1154,7 @@ int tc_loss_grad_x(const LossArgs& a) {
   p.w = a.w;
   p.ldw = a.ldw;
   p.w_bytes = row_bytes(a.w, a.ldw, sizeof(T));
+  p.out_scale = a.scale / dx_unit<typename Planes<T>::type>();
   p.out = a.dx;
   p.part_o = (float*)(ws + L.dx_slab);
   const int rc = with_shape<Planes<T>::count>(TC_GRAD_X, a.N, a.V, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS_GRAD, a.st); });
