@@ -12,6 +12,14 @@ constexpr int FWD_SHIFT = 7;    // the forward pass holds p at 2^7 times its val
 // The backward pass holds g (p - target) at 2^14 / max |g| times its value for dW, whose sums run over the rows; for
 // dx g is a factor of the row, and fp16 holds p at 2^14 times its value.
 constexpr int GRAD_SHIFT = 14;
+// Every addition into a 32-bit accumulator of the matrix units truncates, 16 products at a time: a sum of one sign
+// loses 0.3 units in the last place each time (262144 terms in a row were off by 6e-4 of their sum, 65536
+// columns by 4e-4 of the logit).  So a run of additions ends after this many terms, and its sum goes on in
+// 32-bit additions that round: at most 2^-13 of the sum is lost, 2^-17 for fp32.  The streamed form lets
+// bf16, whose half step is eight times fp16's, run eight times as long.
+constexpr int RUN_TERMS = 16384, RUN_TERMS_F32 = 1024;
+template <typename T>
+constexpr int streamed_run() { return sizeof(T) == 4 ? RUN_TERMS_F32 : IsBf16<T>::value ? 8 * RUN_TERMS : RUN_TERMS; }
 constexpr float MOVE_REFERENCE = 8.f;  // a row's reference moves when its maximum passes it by 2^8
 
 // Factor from x . w to a base-2 logit, |scale| log2 e (the sign goes into x).  Not zero, so that a
@@ -72,6 +80,9 @@ struct LossArgs {
   int* err;
   cudaStream_t st;
 };
+
+template <typename T>
+constexpr int dtype_of() { return sizeof(T) == 4 ? GSB_F32 : IsBf16<T>::value ? GSB_BF16 : GSB_F16; }
 
 // How a type reaches the tensor cores: as it is, or as three bf16 planes (h + m + l, 8 bits each).
 template <typename S> struct Planes { typedef S type; static constexpr int count = 1; };

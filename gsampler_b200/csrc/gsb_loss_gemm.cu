@@ -23,9 +23,11 @@ enum { GM_STATS = 0, GM_PIECE = 1, GM_DX = 2, GM_DW = 3 };
 
 constexpr i64 PIECE_ELEMS = 1ll << 25;
 
-template <int MODE_, int PL_, int BN_, int ST_>
+// RUN: blocks of depth (64 each) after which the accumulators' sums move on to registers, 0 where the depth is
+// never more than RUN_TERMS
+template <int MODE_, int PL_, int BN_, int ST_, int RUN_>
 struct GmShape {
-  static constexpr int MODE = MODE_, PL = PL_, BN = BN_, ST = ST_;
+  static constexpr int MODE = MODE_, PL = PL_, BN = BN_, ST = ST_, RUN = RUN_;
   static constexpr bool A_ACROSS = MODE == GM_DW, B_ACROSS = MODE == GM_DX || MODE == GM_DW;
   static constexpr int A_PLANE = 128 * 128, B_PLANE = BN * 128;
   static constexpr int STAGE = PL * (A_PLANE + B_PLANE);
@@ -40,6 +42,7 @@ struct GmShape {
   static constexpr int BYTES = OFF_BAR + 8 * BARS + 16 + 1024;
   static_assert(BYTES <= 227 * 1024 && COLS >= 128 && COLS <= 512, "");
   static_assert(MODE != GM_PIECE || BN % 128 == 0, "");
+  static_assert(!RUN || BN <= 128, "half a tile's columns in registers");
 };
 
 struct GmParams {
@@ -97,6 +100,8 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     const int k1 = min(p.K, k0 + p.k_per);
     blocks = k1 > k0 ? (k1 - k0 + 63) / 64 : 0;
   };
+  // a tile's products are made in runs, each in accumulators of its own
+  auto runs_of = [](int blocks) { return C::RUN && blocks > C::RUN ? (blocks + C::RUN - 1) / (C::RUN ? C::RUN : 1) : 1; };
 
   if (warp == 8 && lane == 0) {
     for (int s = 0; s < C::ST; ++s) { bar_init(full(s), 1); bar_init(empty(s), 1); }
@@ -152,42 +157,44 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     // ------------------------------------------------ products (the warp together, one lane issues)
     const u32 id = tc_idesc(C::PL == 3 || IsBf16<T>::value, C::BN, C::A_ACROSS, C::B_ACROSS);
     const bool leader = elect_one();
-    int it = 0, i = 0;
+    int it = 0, acc = 0;
     bool ok = true;
     int m, n, z;
-    for (; ok && tile_at(i, m, n, z); ++i) {
+    for (int i = 0; ok && tile_at(i, m, n, z); ++i) {
       int k0, blocks;
       depth(z, k0, blocks);
-      const int b = i & 1;
-      if (i >= 2) ok = bar_wait(acc_empty(b), ((i >> 1) - 1) & 1, gave_up, p.err);
-      tc_after();
-      const u32 d = tmem + b * (C::ACCS * C::BN);
-      for (int kb = 0; ok && kb < blocks; ++kb, ++it) {
-        const int st = it % C::ST;
-        ok = bar_wait(full(st), (it / C::ST) & 1, gave_up, p.err);
-        if (!ok) break;
+      for (int r = 0, runs = runs_of(blocks); ok && r < runs; ++r, ++acc) {
+        const int b = acc & 1, first = r * C::RUN, last = r + 1 < runs ? first + C::RUN : blocks;
+        if (acc >= 2) ok = bar_wait(acc_empty(b), ((acc >> 1) - 1) & 1, gave_up, p.err);
         tc_after();
-        const u64 A = tc_desc(base + st * C::STAGE, C::A_ACROSS ? 8192 : 16);
-        const u64 B = tc_desc(base + st * C::STAGE + C::PL * C::A_PLANE, C::B_ACROSS ? 8192 : 16);
-        constexpr int PAIRS = C::PL == 3 ? 6 : 1;
-        constexpr int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
-        if (leader) {
+        const u32 d = tmem + b * (C::ACCS * C::BN);
+        for (int kb = first; ok && kb < last; ++kb, ++it) {
+          const int st = it % C::ST;
+          ok = bar_wait(full(st), (it / C::ST) & 1, gave_up, p.err);
+          if (!ok) break;
+          tc_after();
+          const u64 A = tc_desc(base + st * C::STAGE, C::A_ACROSS ? 8192 : 16);
+          const u64 B = tc_desc(base + st * C::STAGE + C::PL * C::A_PLANE, C::B_ACROSS ? 8192 : 16);
+          constexpr int PAIRS = C::PL == 3 ? 6 : 1;
+          constexpr int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
+          if (leader) {
 #pragma unroll
-          for (int q = 0; q < PAIRS; ++q) {
-            const bool high = q == PAIRS - 1;
+            for (int q = 0; q < PAIRS; ++q) {
+              const bool high = q == PAIRS - 1;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              tc_mma(d + (high ? (C::ACCS - 1) * C::BN : 0), A + ((C::PL == 3 ? pa[q] : 0) * C::A_PLANE + k * (C::A_ACROSS ? 2048 : 32)) / 16,
-                     B + ((C::PL == 3 ? pb[q] : 0) * C::B_PLANE + k * (C::B_ACROSS ? 2048 : 32)) / 16, id,
-                     kb > 0 || k > 0 || (q > 0 && !high));
+              for (int k = 0; k < 4; ++k)
+                tc_mma(d + (high ? (C::ACCS - 1) * C::BN : 0), A + ((C::PL == 3 ? pa[q] : 0) * C::A_PLANE + k * (C::A_ACROSS ? 2048 : 32)) / 16,
+                       B + ((C::PL == 3 ? pb[q] : 0) * C::B_PLANE + k * (C::B_ACROSS ? 2048 : 32)) / 16, id,
+                       kb > first || k > 0 || (q > 0 && !high));
+            }
+            tc_commit(empty(st));
           }
-          tc_commit(empty(st));
         }
+        if (ok && leader) tc_commit(acc_full(b));
       }
-      if (ok && leader) tc_commit(acc_full(b));
     }
     // what was issued ends by itself; a bounded look keeps the order when a wait gave up
-    for (int j = i > 2 ? i - 2 : 0; j < i; ++j)
+    for (int j = acc > 2 ? acc - 2 : 0; j < acc; ++j)
       for (int k = 0; k < (1 << 16) && !bar_try(acc_full(j & 1), (j >> 1) & 1); ++k) __nanosleep(32);
   } else {
     // ------------------------------------------------ epilogue: a thread has a row and half the columns
@@ -196,25 +203,13 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     float run_m = -INFINITY, run_s = 0.f;
     bool ok = true;
     int m, n, z;
-    for (int i = 0; tile_at(i, m, n, z); ++i) {
-      const int b = i & 1;
-      ok = bar_wait(acc_full(b), (i >> 1) & 1, gave_up, p.err);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_after();
+    int acc = 0;
+    float kept[C::RUN ? C::BN / 2 : 1];  // the runs before a tile's last
+    for (int i = 0; ok && tile_at(i, m, n, z); ++i) {
       int k0, blocks;
       depth(z, k0, blocks);
-      const int row = m * 128 + quarter * 32 + lane;
-      float lse = INFINITY, gs = 0.f;
-      int hot = -1;
-      if (C::MODE == GM_PIECE && row < p.M && p.g[row] != 0.f) {
-        lse = p.lse2[row];
-        const float top = __uint_as_float(*p.top);
-        gs = times_power(p.g[row], -small_rows<T>(p.g[row], top)) / top * (float)(1 << GRAD_SHIFT);
-        hot = (int)(p.target[row] - p.v0);
-      }
       auto columns = [&](float* v, int q) {  // 32 of the tile's columns, the accumulators added
-        const u32 from = tmem + b * (C::ACCS * C::BN) + q + lanes;
+        const u32 from = tmem + (acc & 1) * (C::ACCS * C::BN) + q + lanes;
         tc_ld32(v, from);
         if constexpr (C::ACCS == 2) {
           float u[32];
@@ -226,16 +221,55 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           tc_wait_ld();
         }
       };
+      const int runs = runs_of(blocks);
+      if constexpr (C::RUN != 0) {
+#pragma unroll
+        for (int j = 0; j < C::BN / 2; ++j) kept[j] = 0.f;
+        for (int r = 0; r + 1 < runs; ++r, ++acc) {
+          ok = __all_sync(0xffffffffu, bar_wait(acc_full(acc & 1), (acc >> 1) & 1, gave_up, p.err));
+          if (!ok) break;
+          tc_after();
+#pragma unroll
+          for (int q = 0; q < C::BN / 2; q += 32) {
+            float v[32];
+            columns(v, half * (C::BN / 2) + q);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) kept[q + j] += v[j];
+          }
+          tc_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(acc_empty(acc & 1));
+        }
+        if (!ok) break;
+      }
+      const int b = acc & 1;
+      ok = bar_wait(acc_full(b), (acc >> 1) & 1, gave_up, p.err);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_after();
+      const int row = m * 128 + quarter * 32 + lane;
+      float lse = INFINITY, gs = 0.f;
+      int hot = -1;
+      if (C::MODE == GM_PIECE && row < p.M && p.g[row] != 0.f) {
+        lse = p.lse2[row];
+        const float top = __uint_as_float(*p.top);
+        gs = times_power(p.g[row], -small_rows<T>(p.g[row], top)) / top * (float)(1 << GRAD_SHIFT);
+        hot = (int)(p.target[row] - p.v0);
+      }
       if constexpr (C::MODE == GM_PIECE) {
         // 64 columns at a time through shared memory, so that they leave as whole lines: row by row a
         // warp's stores touch 32 lines an instruction (52 us for 4000 x 4096 columns of three planes)
-#pragma unroll 1
-        for (int q = half * (C::BN / 2); q < (half + 1) * (C::BN / 2); q += 64) {
-          const int col = n * C::BN + q;
+#pragma unroll (C::RUN ? 4 : 1)
+        for (int own = 0; own < C::BN / 2; own += 64) {
+          const int q = half * (C::BN / 2) + own, col = n * C::BN + q;
           if (col >= p.N || m * 128 + quarter * 32 >= p.M) break;
           float v[64];
           columns(v, q);
           columns(v + 32, q + 32);
+          if constexpr (C::RUN != 0) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) v[j] += kept[own + j];
+          }
 #pragma unroll
           for (int j = 0; j < 64; ++j) {
             v[j] = ex2(fmaf(v[j], p.c, -lse));
@@ -285,12 +319,16 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           }
         }
       }
-#pragma unroll 1
-      for (int q = half * (C::BN / 2); C::MODE != GM_PIECE && q < (half + 1) * (C::BN / 2); q += 32) {
-        const int col = n * C::BN + q;
+#pragma unroll (C::RUN ? 4 : 1)
+      for (int own = 0; C::MODE != GM_PIECE && own < C::BN / 2; own += 32) {
+        const int q = half * (C::BN / 2) + own, col = n * C::BN + q;
         if (col >= p.N) break;
         float v[32];
         columns(v, q);
+        if constexpr (C::RUN != 0) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += kept[own + j];
+        }
         if (blocks == 0) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = 0.f;
@@ -335,6 +373,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       tc_before();
       __syncwarp();
       if (lane == 0) bar_arrive(acc_empty(b));
+      ++acc;
     }
     if (C::MODE == GM_STATS && ok) {
       const int row = blockIdx.x * 128 + quarter * 32 + lane;
@@ -414,13 +453,15 @@ __global__ void loss_slabs_kernel(const float* __restrict__ slab, i64 size, int 
 }
 
 // ---------------------------------------------------------------- host side
-// A slab for every SM that would otherwise be idle, of at least 512 products.
-static int slab_count(i64 m, i64 n, i64 K, int bn) {
+// A slab for every SM that would otherwise be idle, of at least 512 products; and for 16-bit types, whose
+// accumulators are not emptied on the way, enough of them for RUN_TERMS products at most.
+static int slab_count(int planes, i64 m, i64 n, i64 K, int bn) {
   const i64 tiles = ((m > 0 ? m + 127 : 128) / 128) * ((n + bn - 1) / bn);
   i64 z = (i64)sm_count() / tiles;
   const i64 most = K / 512;
   if (z > most) z = most;
   if (z > 64) z = 64;
+  if (planes == 1 && z < (K + RUN_TERMS - 1) / RUN_TERMS) z = (K + RUN_TERMS - 1) / RUN_TERMS;
   return (int)(z < 1 ? 1 : z);
 }
 static i64 piece_columns(i64 N, i64 V) {
@@ -428,10 +469,9 @@ static i64 piece_columns(i64 N, i64 V) {
   if (c < 128) c = 128;
   return c < V ? c : V;
 }
-template <typename S>
-static constexpr int dtype_of() { return sizeof(S) == 4 ? GSB_F32 : IsBf16<S>::value ? GSB_BF16 : GSB_F16; }
 static int bn_of(int planes, i64 cols) { return planes == 3 ? (cols <= 64 ? 64 : 128) : 256; }  // dx, dW
-static int bn_wide(int planes) { return planes == 3 ? 128 : 256; }                               // logits
+// logits; a tile of 256 leaves no registers for the sums of several runs
+static int bn_wide(int planes, i64 D) { return planes == 3 || D > RUN_TERMS ? 128 : 256; }
 
 struct GmLayout {
   size_t ms, x, x_dw, w, piece, lost, dx_slab, dw_slab, bytes;
@@ -447,15 +487,15 @@ static GmLayout gemm_layout(int dtype, i64 N, i64 V, i64 D, bool forward, bool d
   L.ldp = packed_ld(D);
   L.x = take(2 * (size_t)planes * N * L.ldp);
   if (forward) {
-    const i64 tiles = (V + bn_wide(planes) - 1) / bn_wide(planes);
+    const i64 tiles = (V + bn_wide(planes, D) - 1) / bn_wide(planes, D);
     const int s = split_count(N > 0 ? (N + 127) / 128 : 1, tiles, sm_count());
     L.per = (int)((tiles + s - 1) / s);
     L.splits = (int)((tiles + L.per - 1) / L.per);
     L.ms = take(8 * (size_t)2 * L.splits * N);
   } else {
     L.cols = piece_columns(N, V);
-    L.dx_slabs = slab_count(N, D, L.cols, bn_of(planes, D));
-    L.dw_slabs = slab_count(L.cols, D, N, bn_of(planes, D));
+    L.dx_slabs = slab_count(planes, N, D, L.cols, bn_of(planes, D));
+    L.dw_slabs = slab_count(planes, L.cols, D, N, bn_of(planes, D));
     L.piece = take(2 * (size_t)planes * N * packed_ld(L.cols));
     L.lost = take(4 * (size_t)N);
     L.x_dw_taken = dw && dtype == GSB_F16;
@@ -493,15 +533,17 @@ static int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GmParam
   loss_gemm_kernel<T, C><<<grid, C::THREADS, C::BYTES, st>>>(a, b, p);
   return GSB_OK;
 }
-// the shape for `cols` columns of the result (dx and dW of few columns: 64 of them, with a stage more)
+// the shape for `cols` columns of the result (dx and dW of few columns: 64 of them, with a stage more) and a depth
 template <typename T, int MODE, int PL>
-static int launch_mode(i64 cols, const CUtensorMap& a, const CUtensorMap& b, const GmParams& p, dim3 grid, int kid, cudaStream_t st) {
+static int launch_mode(i64 cols, i64 depth, const CUtensorMap& a, const CUtensorMap& b, const GmParams& p, dim3 grid, int kid, cudaStream_t st) {
   if constexpr (PL == 3) {
     if constexpr (MODE == GM_DX || MODE == GM_DW)
-      if (bn_of(3, cols) == 64) return launch_gemm<T, GmShape<MODE, 3, 64, 3>>(a, b, p, grid, kid, st);
-    return launch_gemm<T, GmShape<MODE, 3, 128, 2>>(a, b, p, grid, kid, st);
+      if (bn_of(3, cols) == 64) return launch_gemm<T, GmShape<MODE, 3, 64, 3, RUN_TERMS_F32 / 64>>(a, b, p, grid, kid, st);
+    return launch_gemm<T, GmShape<MODE, 3, 128, 2, RUN_TERMS_F32 / 64>>(a, b, p, grid, kid, st);
   } else {
-    return launch_gemm<T, GmShape<MODE, 1, 256, 4>>(a, b, p, grid, kid, st);
+    if constexpr (MODE == GM_STATS || MODE == GM_PIECE)
+      if (bn_wide(1, depth) == 128) return launch_gemm<T, GmShape<MODE, 1, 128, 4, RUN_TERMS / 64>>(a, b, p, grid, kid, st);
+    return launch_gemm<T, GmShape<MODE, 1, 256, 4, 0>>(a, b, p, grid, kid, st);
   }
 }
 
@@ -515,7 +557,7 @@ int gemm_loss_forward(const LossArgs& a) {
   i64 ldx = a.ldx, ldw = a.ldw;
   if (PL == 3 || a.scale < 0.f || !tma_ready(x, ldx)) { make_planes<S>(x, ldx, a.N, a.D, a.scale < 0.f, nullptr, nullptr, nullptr, ws + L.x, a.st); x = ws + L.x; ldx = L.ldp; }
   if (PL == 3 || !tma_ready(w, ldw)) { make_planes<S>(w, ldw, a.V, a.D, false, nullptr, nullptr, nullptr, ws + L.w, a.st); w = ws + L.w; ldw = L.ldp; }
-  const int bn = bn_wide(PL);
+  const int bn = bn_wide(PL, a.D);
   CUtensorMap ma, mb;
   if (!tc_map(&ma, x, IsBf16<T>::value, a.N, a.D, ldx, PL, 64, 128) || !tc_map(&mb, w, IsBf16<T>::value, a.V, a.D, ldw, PL, 64, bn)) return GSB_ERR_CUDA;
   GmParams p = {};
@@ -529,7 +571,7 @@ int gemm_loss_forward(const LossArgs& a) {
   p.c = logit_factor(a.scale);
   p.part_ms = (float2*)(ws + L.ms);
   p.err = a.err;
-  const int rc = launch_mode<T, GM_STATS, PL>(a.V, ma, mb, p, dim3(p.m_tiles, L.splits), KID_LOSS, a.st);
+  const int rc = launch_mode<T, GM_STATS, PL>(a.V, a.D, ma, mb, p, dim3(p.m_tiles, L.splits), KID_LOSS, a.st);
   if (rc != GSB_OK) return rc;
   launch_loss_join<S>(a, p.part_ms, 2 * L.splits, nullptr, nullptr, nullptr);
   return GSB_OK;
@@ -569,7 +611,7 @@ int gemm_loss_backward(const LossArgs& a) {
     const T* wv = w + v0 * ldw;
     CUtensorMap ma, mb;
     {
-      const int bn = bn_wide(PL);
+      const int bn = bn_wide(PL, a.D);
       if (!tc_map(&ma, x, bf, a.N, a.D, L.ldp, PL, 64, 128) || !tc_map(&mb, wv, bf, c, a.D, ldw, PL, 64, bn, a.V)) return GSB_ERR_CUDA;
       GmParams p = {};
       p.M = (int)a.N;
@@ -590,7 +632,7 @@ int gemm_loss_backward(const LossArgs& a) {
       p.lost = (float*)(ws + L.lost);
       p.err = a.err;
       const dim3 grid = units_grid(p, 1);
-      const int rc = launch_mode<T, GM_PIECE, PL>(c, ma, mb, p, grid, KID_LOSS_GRAD, a.st);
+      const int rc = launch_mode<T, GM_PIECE, PL>(c, a.D, ma, mb, p, grid, KID_LOSS_GRAD, a.st);
       if (rc != GSB_OK) return rc;
     }
     if (a.dx) {
@@ -606,7 +648,7 @@ int gemm_loss_backward(const LossArgs& a) {
       p.add = v0 > 0;
       p.err = a.err;
       const dim3 grid = units_grid(p, L.dx_slabs);
-      const int rc = launch_mode<T, GM_DX, PL>(a.D, ma, mb, p, grid, KID_LOSS_GRAD, a.st);
+      const int rc = launch_mode<T, GM_DX, PL>(a.D, p.k_per, ma, mb, p, grid, KID_LOSS_GRAD, a.st);
       if (rc != GSB_OK) return rc;
     }
     if (a.dw) {
@@ -621,7 +663,7 @@ int gemm_loss_backward(const LossArgs& a) {
       p.slab = dws;
       p.err = a.err;
       const dim3 grid = units_grid(p, L.dw_slabs);
-      const int rc = launch_mode<T, GM_DW, PL>(a.D, ma, mb, p, grid, KID_LOSS_GRAD, a.st);
+      const int rc = launch_mode<T, GM_DW, PL>(a.D, p.k_per, ma, mb, p, grid, KID_LOSS_GRAD, a.st);
       if (rc != GSB_OK) return rc;
       LaunchScope ls(KID_LOSS_JOIN, a.st);
       loss_slabs_kernel<S><<<blocks_for(c * a.D), 256, 0, a.st>>>(dws, c * a.D, L.dw_slabs, fabsf(a.scale) * unit, a.top,

@@ -26,7 +26,8 @@
 //
 // The reference m moves only when a row's maximum passes it by 2^8, because moving it rescales O;
 // P stays below 2^15, which fp16 holds.  Sums and O are 32 bits; P is rounded to the type, half a
-// step each, which is the rounding that the tensor cores' operands ask for.
+// step each, which is the rounding that the tensor cores' operands ask for.  O leaves its accumulator every
+// streamed_run rows of B: fp32 keeps the sums in registers, 16-bit types in memory, 32 bits an element.
 #include "gsb_common.cuh"
 #include "gsb_loss.cuh"
 #include "gsb_tc.cuh"
@@ -45,8 +46,9 @@ enum { TC_STATS = 0, TC_PULL = 1, TC_GRAD_W = 2, TC_GRAD_X = 3 };
 // HV    warpgroups that turn an item's S into P, each an equal share of its columns
 // PL    planes: 1 for 16-bit values, 3 for fp32 as three bf16 planes and six plane products (see gsb_loss_gemm.cu)
 // ATM   tiles A in TMEM, where there is room beside O and two S buffers; else in shared memory
+// SHORT for at most RUN_TERMS rows of B
 // An item is (tile B j, tile A a), numbered w = j NA + a; it uses buffer w % NB.
-template <int MODE_, int DP_, int NA_, int NB_, int BT_, int ST_, int CTAS_, int HV_, bool ATM_, int PL_ = 1>
+template <int MODE_, int DP_, int NA_, int NB_, int BT_, int ST_, int CTAS_, int HV_, bool ATM_, int PL_ = 1, bool SHORT_ = false>
 struct TcShape {
   static constexpr int PL = PL_, ACCS = PL == 3 ? 2 : 1, SB = BT_ * ACCS;  // planes, accumulators, columns of an S buffer
   static constexpr int MODE = MODE_, DP = DP_, NA = NA_, NB = NB_, BT = BT_, ST = ST_, CTAS = CTAS_;
@@ -70,9 +72,9 @@ struct TcShape {
   static constexpr bool WIPES = MODE == TC_GRAD_W && PL == 1;
   static constexpr int THREADS = WG * 128 + 64 + (WIPES ? 32 : 0);
   static constexpr int A_BYTES = ATM ? 0 : PL * SUBS * 128 * 128;
-  // tiles B after which O is added to sums in registers: every addition to an accumulator in TMEM
-  // truncates, which over hundreds of tiles is more than 32-bit values may lose
-  static constexpr int FLUSH = PL == 3 ? 16 : 0;
+  // whether O is emptied into sums in memory; dx of 16-bit types has at most SMALL_V rows to run over
+  static constexpr bool SPILLS = PL == 1 && !SHORT_ && (MODE == TC_PULL || MODE == TC_GRAD_W);
+  static constexpr bool KEEPS = PL == 3 && SECOND;  // or in registers
   static constexpr int OFF_B = NA * A_BYTES, OFF_META = OFF_B + ST * B_BYTES;
   static constexpr int OFF_COEF = OFF_META + ST * META;  // TC_GRAD_X: p_t - 1 by half and row
   static constexpr int OFF_BAR = OFF_COEF + (MODE == TC_GRAD_X ? WG * 128 * 4 : 0);
@@ -81,8 +83,9 @@ struct TcShape {
   static_assert(USED <= 512 && COLS * CTAS <= 512, "TMEM");
   static_assert(BYTES * CTAS <= 226 * 1024, "shared memory");
   static_assert(MODE != TC_PULL || HV == 1, "a row's running state has one owner");
+  static_assert(MODE != TC_PULL || NB > 1, "a moved reference waits for the product before");
   static_assert(PL == 1 || (MODE != TC_PULL && NA == 1), "");
-  static_assert(MODE != TC_GRAD_X || NA == 1, "the halves of a row pass on its target's element");
+  static_assert(!SECOND || NA == 1, "the halves of a row pass on its target's element; runs count tiles");
   static_assert(HC % 32 == 0 && META % 16 == 0 && OFF_BAR % 8 == 0, "");
 };
 
@@ -105,6 +108,7 @@ struct TcParams {
   float2* part_ms;          // TC_STATS / TC_PULL: [parts][rows_a] reference and sum
   float* part_o;            // TC_PULL, gradients with splits: [splits][rows_a][D]
   void* out;                // gradients without splits: [rows_a][D]
+  float4* run_sums;         // O of the runs before the last, where a CTA has several: [CTA][D / 4 up to whole 32s][128 rows]
   const u32* top;           // TC_GRAD_W: bits of the largest finite |g|
   float out_scale;          // scale over what P is held at
   int* err;
@@ -195,6 +199,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
   const int my_tiles = min(p.tiles_per_split, tiles - t0);
   const int items = my_tiles * C::NA;
   const int subs = (p.D + 63) / 64, ksteps = (p.D + 15) / 16;
+  constexpr int RUN = C::SPILLS || C::KEEPS ? streamed_run<V>() / C::BT : 1 << 30;  // tiles B of a run
 
   if (warp == C::WG * 4 && lane == 0) {
     for (int s = 0; s < C::ST; ++s) {
@@ -285,7 +290,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
           tc_after();
           const u32 P = tmem + b * C::SB, d = tmem + C::O_COL + a * C::DP;
           const u64 B = tc_desc(base + C::OFF_B + st * C::B_BYTES, C::BT * 128);
-          const bool fresh = C::FLUSH ? j % (C::FLUSH ? C::FLUSH : 1) == 0 : j == 0;
+          const bool fresh = j % RUN == 0;
           if (leader) {
 #pragma unroll
             for (int q = 0; q < PAIRS; ++q) {
@@ -297,7 +302,8 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
                           B + (pb * C::SUBS * (C::BT * 128) + k * 2048) / 16, id_o, !fresh || k > 0 || (q > 0 && !high));
             }
             if (a == C::NA - 1) tc_commit(empty(st));
-            if (C::FLUSH || (C::MODE == TC_PULL && C::NA == 1 && C::NB > 1)) tc_commit(pv_done);
+            // waited for where a run ends, and in the forward pass wherever a reference moves
+            if (C::MODE == TC_PULL || (C::SECOND && (j + 1) % RUN == 0)) tc_commit(pv_done);
           }
         }
         if (w + C::NB < items) product_s(w + C::NB);
@@ -401,8 +407,9 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
       row_bias = -p.lse2[row];
     }
     bool ok = true;
-    float kept[C::FLUSH ? PIECES * 32 : 1];  // O of the tiles before the last flush, this warp's columns of it
-    if constexpr (C::FLUSH != 0) {
+    float kept[C::KEEPS ? PIECES * 32 : 1];  // O of the runs before this one, this warp's columns of it
+    float kept_m = -INFINITY;                // TC_PULL: the reference that run_sums were made against
+    if constexpr (C::KEEPS) {
 #pragma unroll
       for (int q = 0; q < PIECES * 32; ++q) kept[q] = 0.f;
     }
@@ -420,176 +427,213 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
         }
       }
     };
-    for (int w = a; w < items; w += C::NA) {
-      const int j = w / C::NA, st = j % C::ST, b = w % C::NB;
-      ok = bar_wait(s_full(b), (w / C::NB) & 1, gave_up, p.err);
-      if (C::META) ok = ok && bar_wait(ready(st), (j / C::ST) & 1, gave_up, p.err);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_after();
-      if constexpr (C::SECOND && C::FLUSH != 0) {
-        if (j > 0 && j % C::FLUSH == 0) {
-          ok = __all_sync(0xffffffffu, bar_wait(pv_done, (w - 1) & 1, gave_up, p.err));
-          if (!ok) break;
-          tc_after();
-          if (warp_live) keep();
-        }
+    // run_sums: a thread its row, pieces of four columns, so that a warp's accesses are whole lines
+    const int pieces4 = (p.D + 31) / 32 * 8;
+    float4* own_sums = p.run_sums + ((i64)(blockIdx.y * gridDim.x + blockIdx.x) * pieces4) * 128 + quarter * 32 + lane;
+    // how much what was summed against an older reference counts now
+    auto since = [&]() { return C::MODE != TC_PULL || kept_m == m ? 1.f : kept_m == -INFINITY ? 0.f : ex2(kept_m - m); };
+    auto add_sums = [&](float (&o)[32], int k, float old) {
+      float4 h[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) h[q] = own_sums[(k / 4 + q) * 128];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        o[4 * q] = fmaf(h[q].x, old, o[4 * q]);
+        o[4 * q + 1] = fmaf(h[q].y, old, o[4 * q + 1]);
+        o[4 * q + 2] = fmaf(h[q].z, old, o[4 * q + 2]);
+        o[4 * q + 3] = fmaf(h[q].w, old, o[4 * q + 3]);
       }
-      if (warp_live) {
-        const u32 S = tmem + b * C::SB + half * C::HC + lanes;
-        float v[C::HC];
-#pragma unroll
-        for (int k = 0; k < C::HC; k += 32) {
-          tc_ld32(v + k, S + k);
-          if constexpr (C::ACCS == 2) {
-            float u[32];
-            tc_ld32(u, S + C::BT + k);
-            tc_wait_ld();
-#pragma unroll
-            for (int q = 0; q < 32; q += 2)
-              part2(add2(join2(finite_part(v[k + q]), finite_part(v[k + q + 1])), join2(u[q], u[q + 1])), v[k + q], v[k + q + 1]);
-          }
-        }
+    };
+    auto spill = [&](bool first) {
+      const float old = since();
+#pragma unroll 1
+      for (int k = half * 32; k < p.D; k += 32 * C::HV) {
+        float o[32];
+        tc_ld32(o, tmem + C::O_COL + k + lanes);
         tc_wait_ld();
-        if constexpr (C::MODE == TC_GRAD_W) {
-          const unsigned char* meta = smem + C::OFF_META + st * C::META + half * C::HC * 4;
-          const ulonglong2* bias = reinterpret_cast<const ulonglong2*>(meta);  // negative
+        if (!first) add_sums(o, k, old);
 #pragma unroll
-          for (int k = 0; k < C::HC / 4; ++k) {
-            const ulonglong2 q = bias[k];
-            part2(fma2(join2(v[4 * k], v[4 * k + 1]), c2, q.x), v[4 * k], v[4 * k + 1]);
-            part2(fma2(join2(v[4 * k + 2], v[4 * k + 3]), c2, q.y), v[4 * k + 2], v[4 * k + 3]);
-          }
+        for (int q = 0; q < 8; ++q) own_sums[(k / 4 + q) * 128] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+      }
+      kept_m = m;
+    };
+    for (int w = a, run = 0;; ++run) {
+      const int run_end = C::SPILLS || C::KEEPS ? min(items, (run + 1) * RUN) : items;
+      for (; w < run_end; w += C::NA) {
+        const int j = w / C::NA, st = j % C::ST, b = w % C::NB;
+        ok = bar_wait(s_full(b), (w / C::NB) & 1, gave_up, p.err);
+        if (C::META) ok = ok && bar_wait(ready(st), (j / C::ST) & 1, gave_up, p.err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_after();
+        if (warp_live) {
+          const u32 S = tmem + b * C::SB + half * C::HC + lanes;
+          float v[C::HC];
 #pragma unroll
-          for (int k = 0; k < C::HC; k += 2) exponentials(v[k], v[k + 1], k);
-          const int* tgt = reinterpret_cast<const int*>(meta + 4 * C::BT);
-          const float* gs = reinterpret_cast<const float*>(meta + 8 * C::BT);
-          bool near = false;
+          for (int k = 0; k < C::HC; k += 32) {
+            tc_ld32(v + k, S + k);
+            if constexpr (C::ACCS == 2) {
+              float u[32];
+              tc_ld32(u, S + C::BT + k);
+              tc_wait_ld();
 #pragma unroll
-          for (int k = 0; k < C::HC / 32; ++k) {
-            const int t = tgt[k * 32 + lane];
-            near |= (u32)(t - (row - lane)) < 32u || t == WIPE;
-          }
-          // some row's target is one of this warp's vocabulary rows, or some row is zeros: times a masked class's
-          // infinity that is a NaN
-          if (__any_sync(0xffffffffu, near)) {
-#pragma unroll
-            for (int k = 0; k < C::HC; ++k) {
-              const int t = tgt[k];
-              if (t == row) v[k] -= gs[k];
-              if (t == WIPE) v[k] = 0.f;
+              for (int q = 0; q < 32; q += 2)
+                part2(add2(join2(finite_part(v[k + q]), finite_part(v[k + q + 1])), join2(u[q], u[q + 1])), v[k + q], v[k + q + 1]);
             }
           }
-        } else if constexpr (C::MODE == TC_GRAD_X) {
-          const int col0 = (t0 + j) * C::BT + half * C::HC;
-          if (col0 + C::HC > p.rows_b) {  // behind the vocabulary: a logit of 0 may lie far above the row's own
+          tc_wait_ld();
+          if constexpr (C::MODE == TC_GRAD_W) {
+            const unsigned char* meta = smem + C::OFF_META + st * C::META + half * C::HC * 4;
+            const ulonglong2* bias = reinterpret_cast<const ulonglong2*>(meta);  // negative
 #pragma unroll
-            for (int k = 0; k < C::HC; ++k)
-              if (col0 + k >= p.rows_b) v[k] = -INFINITY;
-          }
-          const u64 bias2 = both(row_bias);
+            for (int k = 0; k < C::HC / 4; ++k) {
+              const ulonglong2 q = bias[k];
+              part2(fma2(join2(v[4 * k], v[4 * k + 1]), c2, q.x), v[4 * k], v[4 * k + 1]);
+              part2(fma2(join2(v[4 * k + 2], v[4 * k + 3]), c2, q.y), v[4 * k + 2], v[4 * k + 3]);
+            }
 #pragma unroll
-          for (int k = 0; k < C::HC; k += 2) {
-            part2(fma2(join2(v[k], v[k + 1]), c2, bias2), v[k], v[k + 1]);
-            exponentials(v[k], v[k + 1], k);
-            if (UNIT != 1.f) part2(mul2(join2(v[k], v[k + 1]), both(UNIT)), v[k], v[k + 1]);
-          }
-          const int at = hot - col0;
-          if (__any_sync(0xffffffffu, (u32)at < (u32)C::HC)) {
-            float mine = 0.f;
+            for (int k = 0; k < C::HC; k += 2) exponentials(v[k], v[k + 1], k);
+            const int* tgt = reinterpret_cast<const int*>(meta + 4 * C::BT);
+            const float* gs = reinterpret_cast<const float*>(meta + 8 * C::BT);
+            bool near = false;
 #pragma unroll
-            for (int k = 0; k < C::HC; ++k)
-              if (k == at) {
-                mine = v[k];
-                v[k] = 0.f;
+            for (int k = 0; k < C::HC / 32; ++k) {
+              const int t = tgt[k * 32 + lane];
+              near |= (u32)(t - (row - lane)) < 32u || t == WIPE;
+            }
+            // some row's target is one of this warp's vocabulary rows, or some row is zeros: times a masked class's
+            // infinity that is a NaN
+            if (__any_sync(0xffffffffu, near)) {
+#pragma unroll
+              for (int k = 0; k < C::HC; ++k) {
+                const int t = tgt[k];
+                if (t == row) v[k] -= gs[k];
+                if (t == WIPE) v[k] = 0.f;
               }
-            if ((u32)at < (u32)C::HC) coef = mine - UNIT;
-          }
-        } else {
-          const int col0 = (t0 + j) * C::BT + half * C::HC;
-          const int at = hot - col0;
-          if (__any_sync(0xffffffffu, (u32)at < (u32)C::HC)) {  // the target's product, on its way past
-            float mine = 0.f;
+            }
+          } else if constexpr (C::MODE == TC_GRAD_X) {
+            const int col0 = (t0 + j) * C::BT + half * C::HC;
+            if (col0 + C::HC > p.rows_b) {  // behind the vocabulary: a logit of 0 may lie far above the row's own
 #pragma unroll
-            for (int k = 0; k < C::HC; ++k)
-              if (k == at) {
-                mine = v[k];
-                if (C::MODE == TC_PULL) v[k] = -INFINITY;
-              }
-            if ((u32)at < (u32)C::HC && row < p.rows_a) p.hot[row] = mine;
-          }
-          if (col0 + C::HC > p.rows_b) {
+              for (int k = 0; k < C::HC; ++k)
+                if (col0 + k >= p.rows_b) v[k] = -INFINITY;
+            }
+            const u64 bias2 = both(row_bias);
 #pragma unroll
-            for (int k = 0; k < C::HC; ++k)
-              if (col0 + k >= p.rows_b) v[k] = -INFINITY;
-          }
-          float top[4] = {v[0], v[1], v[2], v[3]};
+            for (int k = 0; k < C::HC; k += 2) {
+              part2(fma2(join2(v[k], v[k + 1]), c2, bias2), v[k], v[k + 1]);
+              exponentials(v[k], v[k + 1], k);
+              if (UNIT != 1.f) part2(mul2(join2(v[k], v[k + 1]), both(UNIT)), v[k], v[k + 1]);
+            }
+            const int at = hot - col0;
+            if (__any_sync(0xffffffffu, (u32)at < (u32)C::HC)) {
+              float mine = 0.f;
 #pragma unroll
-          for (int k = 4; k < C::HC; k += 4) {
-            const int q = (k >> 2) & 1 ? 2 : 0;
-            top[q] = max3(top[q], v[k], v[k + 1]);
-            top[q + 1] = max3(top[q + 1], v[k + 2], v[k + 3]);
-          }
-          const float t = fmaxf(max3(top[0], top[1], top[2]), top[3]) * p.c;
-          const bool move = t > m + MOVE_REFERENCE;
-          if (__any_sync(0xffffffffu, move)) {
-            const float f = move ? (m == -INFINITY ? 0.f : ex2(m - t)) : 1.f;
-            sum = m == -INFINITY ? sum : sum * f;
-            if (move) m = t;
-            if (C::MODE == TC_PULL && j > 0) {
-              // O was made against the old reference
-              if (C::NA == 1 && C::NB > 1) {
+              for (int k = 0; k < C::HC; ++k)
+                if (k == at) {
+                  mine = v[k];
+                  v[k] = 0.f;
+                }
+              if ((u32)at < (u32)C::HC) coef = mine - UNIT;
+            }
+          } else {
+            const int col0 = (t0 + j) * C::BT + half * C::HC;
+            const int at = hot - col0;
+            if (__any_sync(0xffffffffu, (u32)at < (u32)C::HC)) {  // the target's product, on its way past
+              float mine = 0.f;
+#pragma unroll
+              for (int k = 0; k < C::HC; ++k)
+                if (k == at) {
+                  mine = v[k];
+                  if (C::MODE == TC_PULL) v[k] = -INFINITY;
+                }
+              if ((u32)at < (u32)C::HC && row < p.rows_a) p.hot[row] = mine;
+            }
+            if (col0 + C::HC > p.rows_b) {
+#pragma unroll
+              for (int k = 0; k < C::HC; ++k)
+                if (col0 + k >= p.rows_b) v[k] = -INFINITY;
+            }
+            float top[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+            for (int k = 4; k < C::HC; k += 4) {
+              const int q = (k >> 2) & 1 ? 2 : 0;
+              top[q] = max3(top[q], v[k], v[k + 1]);
+              top[q + 1] = max3(top[q + 1], v[k + 2], v[k + 3]);
+            }
+            const float t = fmaxf(max3(top[0], top[1], top[2]), top[3]) * p.c;
+            const bool move = t > m + MOVE_REFERENCE;
+            if (__any_sync(0xffffffffu, move)) {
+              const float f = move ? (m == -INFINITY ? 0.f : ex2(m - t)) : 1.f;
+              sum = m == -INFINITY ? sum : sum * f;
+              if (move) m = t;
+              if (C::MODE == TC_PULL && j > 0) {
+                // O was made against the old reference; S of this item is issued behind the product before the last
                 ok = bar_wait(pv_done, (w - 1) & 1, gave_up, p.err);
                 tc_after();
-              }
-              for (int k = 0; k < ksteps * 16; k += 16) {
-                float o[16];
-                const u32 at = tmem + C::O_COL + a * C::DP + k + lanes;
-                tc_ld16(o, at);
-                tc_wait_ld();
+                for (int k = 0; k < ksteps * 16; k += 16) {
+                  float o[16];
+                  const u32 at = tmem + C::O_COL + a * C::DP + k + lanes;
+                  tc_ld16(o, at);
+                  tc_wait_ld();
 #pragma unroll
-                for (int q = 0; q < 16; ++q) o[q] *= f;
-                tc_st16(at, reinterpret_cast<const u32*>(o));
-              }
-            }
-          }
-          const float off = (float)FWD_SHIFT - (m == -INFINITY ? 0.f : m);
-          const u64 off2 = join2(off, off);
-          u64 add[2] = {0, 0};
-#pragma unroll
-          for (int k = 0; k < C::HC; k += 2) {
-            part2(fma2(join2(v[k], v[k + 1]), c2, off2), v[k], v[k + 1]);
-            exponentials(v[k], v[k + 1], k);
-            add[(k >> 1) & 1] = add2(add[(k >> 1) & 1], join2(v[k], v[k + 1]));
-          }
-          float lo, hi;
-          part2(add2(add[0], add[1]), lo, hi);
-          sum += lo + hi;
-        }
-        if constexpr (C::SECOND) {
-          // each half's P takes the first columns of the half's own S: a warp overwrites what it has read itself
-#pragma unroll
-          for (int pl = 0; pl < C::PL; ++pl) {
-            u32 h[C::HC / 2];
-            take_plane<T>(h, v, pl + 1 < C::PL, false);
-            if constexpr (C::MODE == TC_GRAD_W) {
-              // rows with a negative upstream gradient: the sign of their whole column
-              const u32* sign = reinterpret_cast<const u32*>(smem + C::OFF_META + st * C::META + 12 * C::BT) + half * (C::HC / 2);
-              const u32 own = sign[lane % (C::HC / 2)];
-              if (__any_sync(0xffffffffu, own != 0)) {
-#pragma unroll
-                for (int q = 0; q < C::HC / 2; ++q) h[q] ^= sign[q];
+                  for (int q = 0; q < 16; ++q) o[q] *= f;
+                  tc_st16(at, reinterpret_cast<const u32*>(o));
+                }
               }
             }
+            const float off = (float)FWD_SHIFT - (m == -INFINITY ? 0.f : m);
+            const u64 off2 = join2(off, off);
+            u64 add[2] = {0, 0};
 #pragma unroll
-            for (int q = 0; q < C::HC / 2; q += 16) tc_st16(tmem + b * C::SB + C::p_at(pl, half) + lanes + q, h + q);
+            for (int k = 0; k < C::HC; k += 2) {
+              part2(fma2(join2(v[k], v[k + 1]), c2, off2), v[k], v[k + 1]);
+              exponentials(v[k], v[k + 1], k);
+              add[(k >> 1) & 1] = add2(add[(k >> 1) & 1], join2(v[k], v[k + 1]));
+            }
+            float lo, hi;
+            part2(add2(add[0], add[1]), lo, hi);
+            sum += lo + hi;
           }
-          tc_wait_st();
+          if constexpr (C::SECOND) {
+            // each half's P takes the first columns of the half's own S: a warp overwrites what it has read itself
+#pragma unroll
+            for (int pl = 0; pl < C::PL; ++pl) {
+              u32 h[C::HC / 2];
+              take_plane<T>(h, v, pl + 1 < C::PL, false);
+              if constexpr (C::MODE == TC_GRAD_W) {
+                // rows with a negative upstream gradient: the sign of their whole column
+                const u32* sign = reinterpret_cast<const u32*>(smem + C::OFF_META + st * C::META + 12 * C::BT) + half * (C::HC / 2);
+                const u32 own = sign[lane % (C::HC / 2)];
+                if (__any_sync(0xffffffffu, own != 0)) {
+#pragma unroll
+                  for (int q = 0; q < C::HC / 2; ++q) h[q] ^= sign[q];
+                }
+              }
+#pragma unroll
+              for (int q = 0; q < C::HC / 2; q += 16) tc_st16(tmem + b * C::SB + C::p_at(pl, half) + lanes + q, h + q);
+            }
+            tc_wait_st();
+          }
         }
+        tc_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(p_full(b));
       }
-      tc_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(p_full(b));
+      if (!ok || run_end >= items) break;
+      if constexpr (C::SPILLS || C::KEEPS) {  // the run's last product, then its sum; the next run's first waits for this warp
+        // the forward pass counts every product: S of the next item says that all but the last are done, and the
+        // parity is then the last one's
+        if (C::MODE == TC_PULL) ok = bar_wait(s_full(w % C::NB), (w / C::NB) & 1, gave_up, p.err);
+        ok = __all_sync(0xffffffffu, ok && bar_wait(pv_done, (C::MODE == TC_PULL ? w - 1 : run) & 1, gave_up, p.err));
+        if (!ok) break;
+        tc_after();
+        if (warp_live) {
+          if constexpr (C::KEEPS) keep();
+          else spill(run == 0);
+        }
+        tc_before();
+      }
     }
     if (C::MODE == TC_STATS && row < p.rows_a && ok)
       p.part_ms[(i64)(blockIdx.y * C::HV + half) * p.rows_a + row] = make_float2(m, sum);
@@ -614,19 +658,21 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
       ok = __all_sync(0xffffffffu, ok);
       if (ok && warp_live) {
         tc_after();
-        if constexpr (C::FLUSH != 0) keep();
+        if constexpr (C::KEEPS) keep();
+        const float old = since();
         const float f = C::MODE == TC_PULL ? 1.f : p.out_scale * (C::MODE == TC_GRAD_X ? row_grad : __uint_as_float(*p.top));
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
           const int k = half * 32 + i * (32 * C::HV);
           if (k >= p.D) break;
           float o[32];
-          if constexpr (C::FLUSH != 0) {
+          if constexpr (C::KEEPS) {
 #pragma unroll
             for (int q = 0; q < 32; ++q) o[q] = kept[i * 32 + q];
           } else {
             tc_ld32(o, tmem + C::O_COL + a * C::DP + k + lanes);
             tc_wait_ld();
+            if (C::SPILLS && my_tiles > RUN) add_sums(o, k, old);
           }
           if (row < p.rows_a) {
             const bool slab = C::MODE == TC_PULL || gridDim.y > 1;
@@ -890,6 +936,7 @@ __global__ void __launch_bounds__(256) loss_join_dw_kernel(const float* __restri
 // ---------------------------------------------------------------- host side
 struct TcPlan {
   int BT, splits, per, parts;
+  bool spills;
   i64 groups;
 };
 template <typename C>
@@ -904,6 +951,7 @@ static TcPlan plan_of(i64 rows_a, i64 rows_b) {
   p.per = (int)((tiles + s - 1) / s);
   p.splits = (int)((tiles + p.per - 1) / p.per);
   p.parts = p.splits * (C::MODE == TC_STATS ? C::HV : 1);
+  p.spills = C::SPILLS;
   return p;
 }
 
@@ -933,7 +981,7 @@ typedef TcShape<TC_GRAD_W, 128, 1, 1, 64, 2, 1, 2, false, 3> GradF128;
 typedef TcShape<TC_GRAD_W, 64, 1, 2, 64, 8, 2, 2, true> Grad64;
 typedef TcShape<TC_GRAD_W, 128, 1, 2, 128, 4, 1, 2, true> Grad128;
 typedef TcShape<TC_GRAD_W, 256, 1, 2, 64, 5, 1, 2, true> Grad256;
-typedef TcShape<TC_GRAD_W, 128, 1, 2, 64, 4, 2, 2, false> GradFew128;
+typedef TcShape<TC_GRAD_W, 128, 1, 2, 64, 4, 2, 2, false, 1, true> GradFew128;
 
 // A vocabulary of up to this many rows: dx by making the logits again (2 V multiply-adds an element of
 // x more at 1.3 PFLOP/s, against writing and reading 16 bytes of pull at 5 TB/s: equal near 2080).
@@ -985,8 +1033,17 @@ bool tc_loss_pulls(int dtype, i64 V) { return dtype != GSB_F32 && V > SMALL_V; }
 // rows of a streamed matrix as TMA takes them: a copy where its address or row step does not do, planes for fp32
 static size_t copy_bytes(int planes, i64 rows, i64 D) { return 2 * (size_t)planes * rows * packed_ld(D); }
 
-struct TcFwdLayout { size_t ms, hot, o, w, bytes; };
-static TcFwdLayout fwd_layout(int planes, i64 N, i64 V, i64 D, bool pull) {
+static int planes_of(int dtype) { return dtype == GSB_F32 ? 3 : 1; }
+// sums of the runs before a CTA's last
+static size_t run_bytes(int dtype, const TcPlan& p, i64 D) {
+  const int run = dtype == GSB_BF16 ? streamed_run<__nv_bfloat16>() : streamed_run<__half>();
+  if (!p.spills || (i64)p.per * p.BT <= run) return 0;
+  return (size_t)p.groups * p.splits * ((D + 31) / 32 * 32) * 128 * 4;
+}
+
+struct TcFwdLayout { size_t ms, hot, o, runs, w, bytes; };
+static TcFwdLayout fwd_layout(int dtype, i64 N, i64 V, i64 D, bool pull) {
+  const int planes = planes_of(dtype);
   TcFwdLayout L;
   size_t o = 0;
   auto take = [&](size_t b) { const size_t at = o; o += up256(b); return at; };
@@ -994,24 +1051,26 @@ static TcFwdLayout fwd_layout(int planes, i64 N, i64 V, i64 D, bool pull) {
   L.ms = take(8 * (size_t)p.parts * N);
   L.hot = take(4 * (size_t)N);
   L.o = take(pull ? 4 * (size_t)p.splits * N * D : 0);
+  L.runs = take(run_bytes(dtype, p, D));
   L.w = take(copy_bytes(planes, V, D));
   L.bytes = o;
   return L;
 }
 size_t tc_loss_workspace(int dtype, i64 N, i64 V, i64 D, bool pull, bool pack_w) {
-  const int planes = dtype == GSB_F32 ? 3 : 1;
-  const TcFwdLayout L = fwd_layout(planes, N, V, D, pull);
-  return pack_w || planes == 3 ? L.bytes : L.w;
+  const TcFwdLayout L = fwd_layout(dtype, N, V, D, pull);
+  return pack_w || dtype == GSB_F32 ? L.bytes : L.w;
 }
 
-struct TcGradLayout { size_t meta, dw_slab, dx_slab, x, w, bytes; };
-static TcGradLayout grad_layout(int planes, i64 N, i64 V, i64 D, bool dx, bool dw) {
+struct TcGradLayout { size_t meta, dw_slab, dw_runs, dx_slab, x, w, bytes; };
+static TcGradLayout grad_layout(int dtype, i64 N, i64 V, i64 D, bool dx, bool dw) {
+  const int planes = planes_of(dtype);
   TcGradLayout L;
   size_t o = 0;
   auto take = [&](size_t b) { const size_t at = o; o += up256(b); return at; };
   const TcPlan w = tc_plan(planes, TC_GRAD_W, N, V, D), x = tc_plan(planes, TC_GRAD_X, N, V, D);
   L.meta = take(dw ? (size_t)((N + w.BT - 1) / w.BT) * w.BT * 14 : 0);
   L.dw_slab = take(dw && w.splits > 1 ? 4 * (size_t)w.splits * V * D : 0);
+  L.dw_runs = take(dw ? run_bytes(dtype, w, D) : 0);
   L.dx_slab = take(dx && x.splits > 1 ? 4 * (size_t)x.splits * N * D : 0);
   L.x = take(dw ? copy_bytes(planes, N, D) : 0);
   L.w = take(dx ? copy_bytes(planes, V, D) : 0);
@@ -1019,7 +1078,7 @@ static TcGradLayout grad_layout(int planes, i64 N, i64 V, i64 D, bool dx, bool d
   return L;
 }
 size_t tc_loss_grad_workspace(int dtype, i64 N, i64 V, i64 D, bool dx, bool dw) {
-  return grad_layout(dtype == GSB_F32 ? 3 : 1, N, V, D, dx, dw).bytes;
+  return grad_layout(dtype, N, V, D, dx, dw).bytes;
 }
 bool tc_loss_packs(const void* w, i64 ldw) { return !tma_ready(w, ldw); }
 
@@ -1095,7 +1154,7 @@ template <typename T>
 int tc_loss_forward(const LossArgs& a, float* pull) {
   const int mode = pull ? TC_PULL : TC_STATS;
   const TcPlan plan = tc_plan(Planes<T>::count, mode, a.N, a.V, a.D);
-  const TcFwdLayout L = fwd_layout(Planes<T>::count, a.N, a.V, a.D, pull != nullptr);
+  const TcFwdLayout L = fwd_layout(dtype_of<T>(), a.N, a.V, a.D, pull != nullptr);
   char* ws = (char*)a.ws;
   CUtensorMap mb;
   if (!stream_map<T>(&mb, a.w, a.ldw, a.V, a.D, plan.BT, nullptr, nullptr, ws + L.w, a.st)) return GSB_ERR_CUDA;
@@ -1103,6 +1162,7 @@ int tc_loss_forward(const LossArgs& a, float* pull) {
   p.part_ms = (float2*)(ws + L.ms);
   p.part_o = (float*)(ws + L.o);
   p.hot = (float*)(ws + L.hot);
+  p.run_sums = (float4*)(ws + L.runs);
   const int rc = with_shape<Planes<T>::count>(mode, a.N, a.V, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS, a.st); });
   if (rc != GSB_OK) return rc;
   if (pull) {
@@ -1120,7 +1180,7 @@ int tc_loss_forward(const LossArgs& a, float* pull) {
 template <typename T>
 int tc_loss_grad_w(const LossArgs& a) {
   const TcPlan plan = tc_plan(Planes<T>::count, TC_GRAD_W, a.N, a.V, a.D);
-  const TcGradLayout L = grad_layout(Planes<T>::count, a.N, a.V, a.D, a.dx != nullptr, true);
+  const TcGradLayout L = grad_layout(dtype_of<T>(), a.N, a.V, a.D, a.dx != nullptr, true);
   char* ws = (char*)a.ws;
   {
     const i64 npad = (a.N + plan.BT - 1) / plan.BT * plan.BT;
@@ -1132,6 +1192,7 @@ int tc_loss_grad_w(const LossArgs& a) {
   TcParams p = base_params<T>(a, plan, true);
   p.meta = (const unsigned char*)(ws + L.meta);
   p.part_o = (float*)(ws + L.dw_slab);
+  p.run_sums = (float4*)(ws + L.dw_runs);
   p.out = a.dw;
   const int rc = with_shape<Planes<T>::count>(TC_GRAD_W, a.N, a.V, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS_GRAD, a.st); });
   if (rc != GSB_OK) return rc;
@@ -1146,7 +1207,7 @@ int tc_loss_grad_w(const LossArgs& a) {
 template <typename T>
 int tc_loss_grad_x(const LossArgs& a) {
   const TcPlan plan = tc_plan(Planes<T>::count, TC_GRAD_X, a.N, a.V, a.D);
-  const TcGradLayout L = grad_layout(Planes<T>::count, a.N, a.V, a.D, true, a.dw != nullptr);
+  const TcGradLayout L = grad_layout(dtype_of<T>(), a.N, a.V, a.D, true, a.dw != nullptr);
   char* ws = (char*)a.ws;
   CUtensorMap mb;
   if (!stream_map<T>(&mb, a.w, a.ldw, a.V, a.D, plan.BT, nullptr, nullptr, ws + L.w, a.st)) return GSB_ERR_CUDA;
