@@ -244,6 +244,46 @@ using torch::autograd::variable_list;
 
 static bool Tracked(const torch::Tensor& t) { return at::GradMode::is_enabled() && t.defined() && t.requires_grad(); }
 
+// The kernels know no tangents and would drop them without a word.
+static void RefuseTangent(const torch::Tensor& t, const char* op) {
+  TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), op, ": forward-mode differentiation is not provided");
+}
+
+// The gradient of the lookup is linear in the upstream gradient, and its own gradient is the lookup.
+struct EmbeddingGradFn : public torch::autograd::Function<EmbeddingGradFn> {
+  static torch::Tensor forward(AutogradContext* ctx, torch::Tensor grad, torch::Tensor index, int64_t rows, double scale,
+                               int64_t padding) {
+    ctx->save_for_backward({index});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    return EmbeddingGrad(grad, index, rows, scale, padding);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    auto up = EmbeddingLookup(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["scale"].toDouble(),
+                              ctx->saved_data["padding"].toInt(), /*sparse=*/false);
+    return {up, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()};
+  }
+};
+
+static torch::Tensor SparseRows(torch::Tensor grad, torch::Tensor index, int64_t rows, double scale, int64_t padding) {
+  torch::Tensor ids, values;
+  std::tie(ids, values) = EmbeddingSparseGrad(grad, index, rows, scale, padding);
+  return at::_sparse_coo_tensor_unsafe(ids.unsqueeze(0), values, {rows, values.size(1)},
+                                       values.options().layout(at::kSparse), /*is_coalesced=*/true);
+}
+
+// Under create_graph: a gradient that cannot be differentiated again says so when that is tried, instead of
+// counting as a constant.
+struct EmbeddingSparseGradFn : public torch::autograd::Function<EmbeddingSparseGradFn> {
+  static torch::Tensor forward(AutogradContext*, torch::Tensor grad, torch::Tensor index, int64_t rows, double scale,
+                               int64_t padding) {
+    return SparseRows(grad, index, rows, scale, padding);
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "Embedding: gradients of gradients are not provided for the sparse form");
+  }
+};
+
 struct EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
   static torch::Tensor forward(AutogradContext* ctx, torch::Tensor weight, torch::Tensor index, double scale,
                                int64_t padding, bool sparse) {
@@ -261,10 +301,10 @@ struct EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
     const double scale = ctx->saved_data["scale"].toDouble();
     torch::Tensor dw;
     if (ctx->saved_data["sparse"].toBool()) {
-      torch::Tensor ids, values;
-      std::tie(ids, values) = EmbeddingSparseGrad(grads[0], index, rows, scale, padding);
-      dw = at::_sparse_coo_tensor_unsafe(ids.unsqueeze(0), values, {rows, values.size(1)},
-                                         values.options().layout(at::kSparse), /*is_coalesced=*/true);
+      dw = Tracked(grads[0]) ? EmbeddingSparseGradFn::apply(grads[0], index, rows, scale, padding)
+                             : SparseRows(grads[0], index, rows, scale, padding);
+    } else if (Tracked(grads[0])) {
+      dw = EmbeddingGradFn::apply(grads[0], index, rows, scale, padding);
     } else {
       dw = EmbeddingGrad(grads[0], index, rows, scale, padding);
     }
@@ -273,6 +313,7 @@ struct EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
 };
 
 torch::Tensor EmbeddingLookup(torch::Tensor weight, torch::Tensor index, double scale, int64_t padding, bool sparse) {
+  RefuseTangent(weight, "Embedding");
   if (!Tracked(weight)) return Embedding(weight, index, scale, padding);
   return EmbeddingFn::apply(weight, index, scale, padding, sparse);
 }
@@ -290,8 +331,9 @@ struct DropoutFn : public torch::autograd::Function<DropoutFn> {
     const auto saved = ctx->get_saved_variables();
     c10::optional<torch::Tensor> step;
     if (!saved.empty()) step = saved[0];
-    auto dx = Dropout(grads[0], ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(),
-                      ctx->saved_data["stream"].toInt(), step);
+    // the same map again, and so is its own gradient
+    auto dx = DropoutApply(grads[0], ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(),
+                           ctx->saved_data["stream"].toInt(), step);
     return {dx, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()};
   }
 };
@@ -299,12 +341,27 @@ struct DropoutFn : public torch::autograd::Function<DropoutFn> {
 torch::Tensor DropoutApply(torch::Tensor data, double p, c10::optional<int64_t> seed, c10::optional<int64_t> stream,
                            c10::optional<torch::Tensor> step) {
   TORCH_CHECK(seed.has_value() == stream.has_value(), "Dropout: give both seed and stream, or neither");
+  RefuseTangent(data, "Dropout");
   int64_t s, t;
   if (seed.has_value()) std::tie(s, t) = std::make_tuple(*seed, *stream);
   else std::tie(s, t) = NextDropoutStream();
   if (!Tracked(data)) return Dropout(data, p, s, t, step);
   return DropoutFn::apply(data, p, s, t, step);
 }
+
+// Under create_graph, as above.
+struct LinearCrossEntropyGradFn : public torch::autograd::Function<LinearCrossEntropyGradFn> {
+  static variable_list forward(AutogradContext*, torch::Tensor x, torch::Tensor weight, torch::Tensor target, torch::Tensor lse2,
+                               torch::Tensor pull, torch::Tensor upstream, c10::optional<torch::Tensor> count, double scale,
+                               int64_t ignore, bool want_dx, bool want_dw) {
+    torch::Tensor dx, dw;
+    std::tie(dx, dw) = LinearCrossEntropyGrad(x, weight, target, lse2, pull, upstream, count, scale, ignore, want_dx, want_dw);
+    return {dx, dw};
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "LinearCrossEntropy: gradients of gradients are not provided");
+  }
+};
 
 struct LinearCrossEntropyFn : public torch::autograd::Function<LinearCrossEntropyFn> {
   static torch::Tensor forward(AutogradContext* ctx, torch::Tensor x, torch::Tensor weight, torch::Tensor target,
@@ -324,9 +381,15 @@ struct LinearCrossEntropyFn : public torch::autograd::Function<LinearCrossEntrop
     const bool want_dx = ctx->needs_input_grad(0), want_dw = ctx->needs_input_grad(1);
     c10::optional<torch::Tensor> count;
     if (s[5].defined()) count = s[5];
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const int64_t ignore = ctx->saved_data["ignore"].toInt();
     torch::Tensor dx, dw;
-    std::tie(dx, dw) = LinearCrossEntropyGrad(s[0], s[1], s[2], s[3], s[4], grads[0], count, ctx->saved_data["scale"].toDouble(),
-                                              ctx->saved_data["ignore"].toInt(), want_dx, want_dw);
+    if (at::GradMode::is_enabled()) {
+      const auto both = LinearCrossEntropyGradFn::apply(s[0], s[1], s[2], s[3], s[4], grads[0], count, scale, ignore, want_dx, want_dw);
+      std::tie(dx, dw) = std::make_tuple(both[0], both[1]);
+    } else {
+      std::tie(dx, dw) = LinearCrossEntropyGrad(s[0], s[1], s[2], s[3], s[4], grads[0], count, scale, ignore, want_dx, want_dw);
+    }
     return {want_dx ? dx : torch::Tensor(), want_dw ? dw : torch::Tensor(), torch::Tensor(), torch::Tensor(),
             torch::Tensor(), torch::Tensor(), torch::Tensor()};
   }
@@ -335,6 +398,8 @@ struct LinearCrossEntropyFn : public torch::autograd::Function<LinearCrossEntrop
 torch::Tensor LinearCrossEntropyLoss(torch::Tensor x, torch::Tensor weight, torch::Tensor target, double scale,
                                      int64_t ignore, int64_t reduction) {
   TORCH_CHECK(reduction >= 0 && reduction <= 2, "LinearCrossEntropy: reduction must be 0, 1 or 2");
+  RefuseTangent(x, "LinearCrossEntropy");
+  RefuseTangent(weight, "LinearCrossEntropy");
   if (Tracked(x) || Tracked(weight))
     return LinearCrossEntropyFn::apply(x, weight, target, scale, ignore, reduction, Tracked(x));
   auto loss = std::get<0>(LinearCrossEntropy(x, weight, target, scale, ignore, false));

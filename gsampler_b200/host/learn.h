@@ -34,7 +34,8 @@ std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyGrad(torch::Tensor x,
                                                                 c10::optional<torch::Tensor> count, double scale,
                                                                 int64_t ignore, bool want_dx, bool want_dw);
 
-// The same with their gradients, for autograd.
+// The same with their gradients, for autograd (reverse mode; gradients of gradients for the lookup with a dense
+// gradient and for dropout, an error for the others).
 torch::Tensor EmbeddingLookup(torch::Tensor weight, torch::Tensor index, double scale, int64_t padding, bool sparse);
 // dropout without seed and stream takes them from the default state when it runs
 torch::Tensor DropoutApply(torch::Tensor data, double p, c10::optional<int64_t> seed, c10::optional<int64_t> stream,

@@ -16,7 +16,8 @@ def dropout(data: torch.Tensor, p: float = 0.5, training: bool = True, seed: int
     ``torch.ops.gs_ops._CAPI_SetDropoutSeed`` (default 7777) and a counter that advances with every
     call.  Give both to repeat a mask.  A recorded CUDA graph replays the recorded streams; ``step``, a
     one-element int64 tensor on the GPU that is added to ``stream`` when the kernel runs, gives
-    every replay a mask of its own (advance it after the backward pass, which reads it again)."""
+    every replay a mask of its own (advance it after the backward pass, which reads it again).
+    Gradients can be differentiated again; forward-mode differentiation raises."""
     if (seed is None) != (stream is None):
         raise ValueError("dropout: give both seed and stream, or neither")
     if not 0.0 <= p <= 1.0:

@@ -19,5 +19,6 @@ def embedding(weight: torch.Tensor, index: torch.Tensor, scale: float = 1.0, pad
     The gradient sums the rows of equal ids in 32 bits, in the order of their positions (the same
     inputs give the same bits), and rounds once.  ``sparse=True`` returns it as a coalesced sparse
     tensor over the touched rows, which costs one read-back of their number (so it cannot be
-    recorded into a CUDA graph); the dense form writes the whole table."""
+    recorded into a CUDA graph); the dense form writes the whole table.  The dense gradient can be
+    differentiated again; the sparse one, and forward-mode differentiation, raise."""
     return torch.ops.gs_ops._CAPI_EmbeddingLookup(weight, index, float(scale), int(padding_idx), bool(sparse))

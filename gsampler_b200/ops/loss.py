@@ -18,7 +18,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     single row is scored when serving).  A row whose target is ``ignore_index`` does not count: its
     loss and gradients are zero, whatever ``x`` holds there; "mean" over no rows is zero.  A target
     outside the vocabulary does not count either and is reported by ``check_async_errors()``.
-    Nothing here synchronises."""
+    Nothing here synchronises.  Gradients of gradients and forward-mode differentiation raise."""
     how = _REDUCTIONS.get(reduction)
     if how is None:
         raise ValueError("linear_cross_entropy: reduction must be mean, sum or none, got %r" % (reduction,))
