@@ -15,7 +15,7 @@ std::tuple<torch::Tensor, torch::Tensor> EmbeddingSparseGrad(torch::Tensor grad,
                                                              double scale, int64_t padding);
 // `step` (optional one-element int64 tensor on the GPU) is added to `stream` when the kernel runs
 torch::Tensor Dropout(torch::Tensor data, double p, int64_t seed, int64_t stream, c10::optional<torch::Tensor> step);
-// default random state of dropout: a seed and a per-process call counter, as for list sampling
+// default random state of dropout: a seed (its own, not the samplers') and a per-process call counter
 void SetDropoutSeed(int64_t seed);
 std::tuple<int64_t, int64_t> NextDropoutStream();
 
