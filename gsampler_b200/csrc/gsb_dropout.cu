@@ -49,15 +49,15 @@ __device__ __forceinline__ void drop_block(Pack<T, 8>& v, i64 g, u32 threshold, 
 // U blocks of eight a thread, all requested first; no grid-stride loop, whose last round leaves most of
 // a launch of a few rounds idle.  The copy needs about 35 KB in flight an SM: 4 M x 100 bf16 in 319 us
 // with U = 1, 267 with 2, 253 with 4 (6.3 TB/s); a small tensor has more CTAs with U = 1.
+// y may be x: a thread loads all its elements before it stores the first, and nobody else touches them.
 template <typename T, bool VECTOR, int U>
 __global__ void __launch_bounds__(256)
-dropout_kernel(const T* __restrict__ x, i64 n, u32 threshold, float scale, u64 seed, u32 stream,
-               const i64* __restrict__ stream_dev, T* __restrict__ y) {
+dropout_kernel(const T* x, i64 n, u32 threshold, float scale, u64 seed, u32 stream, const i64* __restrict__ stream_dev, T* y) {
   const i64 g0 = (i64)blockIdx.x * (256 * U) + threadIdx.x;
   if (VECTOR && ((i64)blockIdx.x + 1) * (256 * U) * 8 <= n) {  // whole blocks only
     Pack<T, 8> v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u].load(x + (g0 + u * 256) * 8);
+    for (int u = 0; u < U; ++u) v[u].load_written(x + (g0 + u * 256) * 8);
     if (stream_dev) stream += (u32)__ldg(stream_dev);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -73,7 +73,7 @@ dropout_kernel(const T* __restrict__ x, i64 n, u32 threshold, float scale, u64 s
     Pack<T, 8> v;
     const bool whole = VECTOR && e + 8 <= n;
     if (whole) {
-      v.load(x + e);
+      v.load_written(x + e);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v.v[j] = e + j < n ? x[e + j] : from_float<T>(0.f);
@@ -113,6 +113,7 @@ extern "C" int gsb_dropout(const void* x, int dtype, int64_t n, double p, uint64
   if (n < 0 || n > (1ll << 40) || !(p >= 0.0 && p <= 1.0)) return GSB_ERR_INVALID;  // the grid's limit
   if (n == 0) return GSB_OK;
   if (!x || !y) return GSB_ERR_INVALID;
+  if (!at_multiple(x, value_bytes(dtype)) || !at_multiple(y, value_bytes(dtype)) || !at_multiple(stream_dev, 8)) return GSB_ERR_INVALID;
   const u32 threshold = (u32)(p * 65536.0 + 0.5);
   const float scale = threshold >= 65536u ? 0.f : (float)(65536.0 / (65536.0 - threshold));
   cudaStream_t st = (cudaStream_t)cuda_stream;

@@ -653,6 +653,8 @@ extern "C" int gsb_embedding(const void* weight, int dtype, int64_t ld, int64_t 
   if (n < 0 || rows < 0 || D < 0 || D > GSB_EMBED_MAX_D || (rows > 1 && ld < D)) return GSB_ERR_INVALID;
   if (n == 0 || D == 0) return GSB_OK;
   if (!idx || !out || (rows > 0 && !weight)) return GSB_ERR_INVALID;
+  if (!at_multiple(weight, value_bytes(dtype)) || !at_multiple(out, value_bytes(dtype)) || !at_multiple(idx, 8) || !at_multiple(d_err, 4))
+    return GSB_ERR_INVALID;
   cudaStream_t st = (cudaStream_t)cuda_stream;
   const i64* ix = (const i64*)idx;
 #define GSB_ROWS(T, V) run_rows<T, V>(weight, ld, rows, D, ix, n, scale, padding, out, d_err, st)
@@ -698,6 +700,9 @@ extern "C" int gsb_embedding_grad(const void* grad, int dtype, int64_t D, const 
   if (!embed_sizes_ok(n, rows, D) || (dtype != GSB_F32 && dtype != GSB_F16 && dtype != GSB_BF16)) return GSB_ERR_INVALID;
   if (rows == 0 || D == 0) return GSB_OK;
   if (!out || (n > 0 && (!grad || !idx))) return GSB_ERR_INVALID;
+  if (!at_multiple(grad, value_bytes(dtype)) || !at_multiple(out, value_bytes(dtype)) || !at_multiple(idx, 8) ||
+      !at_multiple(workspace, 16) || !at_multiple(d_err, 4))
+    return GSB_ERR_INVALID;
   cudaStream_t st = (cudaStream_t)cuda_stream;
   GSB_CUDA_OK(cudaMemsetAsync(out, 0, (size_t)rows * D * (dtype == GSB_F32 ? 4 : 2), st));
   if (n == 0) return GSB_OK;
@@ -715,6 +720,8 @@ extern "C" int gsb_embedding_sort(const int64_t* idx, int64_t n, int64_t rows, i
                                   int64_t* d_num, void* workspace, size_t workspace_bytes, int* d_err,
                                   void* cuda_stream) {
   if (!embed_sizes_ok(n, rows, D) || n == 0 || !idx || !ids || !d_num) return GSB_ERR_INVALID;
+  if (!at_multiple(idx, 8) || !at_multiple(ids, 8) || !at_multiple(d_num, 8) || !at_multiple(workspace, 16) || !at_multiple(d_err, 4))
+    return GSB_ERR_INVALID;
   const EmbedLayout L = embed_layout(n, D, rows);
   if (!workspace || workspace_bytes < L.bytes) return GSB_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)cuda_stream;
@@ -741,6 +748,8 @@ extern "C" int gsb_embedding_grad_rows(const void* grad, int dtype, int64_t D, i
     return GSB_ERR_INVALID;
   if (num == 0 || D == 0) return GSB_OK;
   if (!grad || !out) return GSB_ERR_INVALID;
+  if (!at_multiple(grad, value_bytes(dtype)) || !at_multiple(out, value_bytes(dtype)) || !at_multiple(workspace, 16))
+    return GSB_ERR_INVALID;
   const EmbedLayout L = embed_layout(n, D, rows);
   if (!workspace || workspace_bytes < L.bytes) return GSB_ERR_WORKSPACE;
   char* ws = (char*)workspace;

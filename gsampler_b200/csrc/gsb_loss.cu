@@ -114,6 +114,9 @@ extern "C" int gsb_linear_ce(const void* x, int dtype, int64_t ldx, int64_t N, c
   if (pull && !gsb_linear_ce_has_pull(dtype, V, D)) return GSB_ERR_UNSUPPORTED;
   if (N == 0) return GSB_OK;
   if (!x || !weight || !target || !loss || !lse2) return GSB_ERR_INVALID;
+  if (!at_multiple(x, value_bytes(dtype)) || !at_multiple(weight, value_bytes(dtype)) || !at_multiple(target, 8) ||
+      !at_multiple(loss, 4) || !at_multiple(lse2, 4) || !at_multiple(pull, 4) || !at_multiple(workspace, 16) || !at_multiple(d_err, 4))
+    return GSB_ERR_INVALID;
   if (!workspace || workspace_bytes < gsb_linear_ce_workspace_bytes(dtype, weight, ldw, N, V, D, pull != nullptr))
     return GSB_ERR_WORKSPACE;
   LossArgs a = {};
@@ -138,6 +141,8 @@ extern "C" int gsb_linear_ce_total(const float* loss, const int64_t* target, int
                                    int mean, float* total, float* count, void* workspace, size_t workspace_bytes,
                                    void* cuda_stream) {
   if (N < 0 || !total || !count || (N > 0 && (!loss || !target))) return GSB_ERR_INVALID;
+  if (!at_multiple(loss, 4) || !at_multiple(target, 8) || !at_multiple(total, 4) || !at_multiple(count, 4) || !at_multiple(workspace, 16))
+    return GSB_ERR_INVALID;
   const int blocks = total_blocks(N);
   if (blocks > 1 && (!workspace || workspace_bytes < gsb_linear_ce_total_workspace_bytes(N))) return GSB_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)cuda_stream;
@@ -169,6 +174,10 @@ extern "C" int gsb_linear_ce_grad(const void* x, int dtype, int64_t ldx, int64_t
                                   int* d_err, void* cuda_stream) {
   if (!loss_sizes_ok(N, V, D, ldx, ldw) || !(scale - scale == 0.f)) return GSB_ERR_INVALID;
   if (dtype != GSB_F32 && dtype != GSB_F16 && dtype != GSB_BF16) return GSB_ERR_INVALID;
+  if (!at_multiple(x, value_bytes(dtype)) || !at_multiple(weight, value_bytes(dtype)) || !at_multiple(target, 8) ||
+      !at_multiple(lse2, 4) || !at_multiple(pull, 4) || !at_multiple(upstream, 4) || !at_multiple(count, 4) ||
+      !at_multiple(dx, value_bytes(dtype)) || !at_multiple(dw, value_bytes(dtype)) || !at_multiple(workspace, 16) || !at_multiple(d_err, 4))
+    return GSB_ERR_INVALID;
   cudaStream_t st = (cudaStream_t)cuda_stream;
   if (N == 0) {
     if (dw) GSB_CUDA_OK(cudaMemsetAsync(dw, 0, (size_t)V * D * (dtype == GSB_F32 ? 4 : 2), st));

@@ -108,6 +108,7 @@ struct TcParams {
   float2* part_ms;          // TC_STATS / TC_PULL: [parts][rows_a] reference and sum
   float* part_o;            // TC_PULL, gradients with splits: [splits][rows_a][D]
   void* out;                // gradients without splits: [rows_a][D]
+  int out_bytes;            // 16, 8, 4 or 2: what the address and step of its rows are multiples of
   float4* run_sums;         // O of the runs before the last, where a CTA has several: [CTA][D / 4 up to whole 32s][128 rows]
   const u32* top;           // TC_GRAD_W: bits of the largest finite |g|
   float out_scale;          // scale over what P is held at
@@ -696,7 +697,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
             } else {
               V* to = (V*)p.out + (i64)row * p.D + k;
               if constexpr (C::PL == 3) {
-                if ((p.D & 3) == 0) {
+                if (p.out_bytes == 16) {
 #pragma unroll
                   for (int q = 0; q < 8; ++q)
                     if (k + 4 * q < p.D) reinterpret_cast<float4*>(to)[q] = make_float4(o[4 * q] * f, o[4 * q + 1] * f, o[4 * q + 2] * f, o[4 * q + 3] * f);
@@ -709,15 +710,15 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
               u32 h[16];
 #pragma unroll
               for (int q = 0; q < 16; ++q) h[q] = pack2<T>(o[2 * q] * f, o[2 * q + 1] * f);
-              if ((p.D & 7) == 0) {
+              if (p.out_bytes == 16) {
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
                   if (k + 8 * q < p.D) reinterpret_cast<uint4*>(to)[q] = make_uint4(h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]);
-              } else if ((p.D & 3) == 0) {
+              } else if (p.out_bytes == 8) {
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
                   if (k + 4 * q < p.D) reinterpret_cast<uint2*>(to)[q] = make_uint2(h[2 * q], h[2 * q + 1]);
-              } else if ((p.D & 1) == 0) {
+              } else if (p.out_bytes == 4) {
 #pragma unroll
                 for (int q = 0; q < 16; ++q)
                   if (k + 2 * q < p.D) reinterpret_cast<u32*>(to)[q] = h[q];
@@ -1194,6 +1195,7 @@ int tc_loss_grad_w(const LossArgs& a) {
   p.part_o = (float*)(ws + L.dw_slab);
   p.run_sums = (float4*)(ws + L.dw_runs);
   p.out = a.dw;
+  p.out_bytes = row_bytes(a.dw, a.D, sizeof(T));
   const int rc = with_shape<Planes<T>::count>(TC_GRAD_W, a.N, a.V, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS_GRAD, a.st); });
   if (rc != GSB_OK) return rc;
   if (plan.splits > 1) {
@@ -1217,6 +1219,7 @@ int tc_loss_grad_x(const LossArgs& a) {
   p.w_bytes = row_bytes(a.w, a.ldw, sizeof(T));
   p.out_scale = a.scale / dx_unit<typename Planes<T>::type>();
   p.out = a.dx;
+  p.out_bytes = row_bytes(a.dx, a.D, sizeof(T));
   p.part_o = (float*)(ws + L.dx_slab);
   const int rc = with_shape<Planes<T>::count>(TC_GRAD_X, a.N, a.V, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS_GRAD, a.st); });
   if (rc != GSB_OK) return rc;

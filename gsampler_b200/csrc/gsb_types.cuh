@@ -3,6 +3,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "../../include/gsb200.h"
+
 namespace gsb {
 
 __device__ __forceinline__ float to_float(float x) { return x; }
@@ -17,6 +19,10 @@ template <>
 __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// Whether p (null included) is a multiple of `bytes`: what the entry points ask of every pointer.
+inline bool at_multiple(const void* p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+inline size_t value_bytes(int dtype) { return dtype == GSB_F32 ? 4 : 2; }
 
 template <typename T> struct IsBf16 { static constexpr bool value = false; };
 template <> struct IsBf16<__nv_bfloat16> { static constexpr bool value = true; };
@@ -37,6 +43,11 @@ struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
   __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
     for (int i = 0; i < BYTES / PIECE; ++i) reinterpret_cast<raw*>(v)[i] = __ldg(reinterpret_cast<const raw*>(p) + i);
+  }
+  // from memory that this kernel also writes
+  __device__ __forceinline__ void load_written(const T* p) {
+#pragma unroll
+    for (int i = 0; i < BYTES / PIECE; ++i) reinterpret_cast<raw*>(v)[i] = reinterpret_cast<const raw*>(p)[i];
   }
   __device__ __forceinline__ void store(T* p) const {
 #pragma unroll

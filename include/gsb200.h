@@ -222,7 +222,9 @@ GSB_API int gsb_gather_rows(const void* src, int64_t row_bytes, int64_t src_rows
  * What a model does with the ids that sampling and walks produce when the node
  * values are learned (no counterpart in the reference, whose examples hand that
  * to torch).  Values are fp32, fp16 or bf16 (`dtype`, GSB_F32 ...); sums are
- * held in 32 bits and rounded once.  No call allocates or synchronises.
+ * held in 32 bits and rounded once.  No call allocates or synchronises.  Pointers
+ * are multiples of their element's size and workspaces of 16 bytes; others are
+ * refused (GSB_ERR_INVALID).
  *
  * gsb_embedding: out[i,:] = scale * weight[idx[i],:], rows of D elements; a row
  * of `weight` starts ld elements after the one before.  idx[i] == padding gives
