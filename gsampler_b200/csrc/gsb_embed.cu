@@ -3,8 +3,9 @@
 //   forward   out[i] = scale * W[idx[i]]          (zeros where idx[i] is the padding id)
 //   gradient  dW[v]  = scale * sum over {i : idx[i] = v} of g[i], in ascending order of i
 //
-// The sum runs over positions sorted by (id, position), so it does not depend on the order in
-// which anything executes: same inputs, same bits.  Sums are held in 32 bits and rounded once.
+// The sum runs over positions sorted by (id, position), in consecutive runs whose sums are added in order, and where
+// the runs are cut depends on the sizes, the type and the number of SMs alone -- not on the order in which
+// anything executes, nor on addresses: same inputs, same bits.  Sums are held in 32 bits and rounded once.
 // All of it is bound by memory traffic; nothing here has arithmetic to speak of.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -423,16 +424,17 @@ embed_segsum_kernel(const u32* __restrict__ key, const u32* __restrict__ pos, i6
 
 // A group per chunk in which a segment begins and goes on: adds the partials of the chunks behind it.
 // Nearly all runs end within a chunk or two; a hub that fills thousands of chunks is left to the
-// whole CTA, whose groups take equal shares of it that are then added in order.
-template <typename T, int VEC>
+// whole CTA, whose groups take equal shares of it that are then added in order; `shares` is the number of groups
+// that rows at 16-byte boundaries have, so that NARROW accesses, with fewer groups, change no sum.
+template <typename T, int VEC, bool NARROW>
 __global__ void __launch_bounds__(256)
 embed_join_kernel(const u32* __restrict__ part_key, const float* __restrict__ part, i64 part_ld, i64 chunks, int D, int log_group,
-                  float scale, T* __restrict__ out) {
+                  int shares, float scale, T* __restrict__ out) {
   constexpr int U = 8, SHORT = 32;
   __shared__ i64 long_run[256];
   __shared__ int longs;
   __shared__ i64 lo_s, hi_s;
-  __shared__ float sums[256 * VEC];
+  __shared__ float sums[256 * (NARROW ? 16 / sizeof(T) : VEC)];  // by share and column
   const int lane = threadIdx.x & ((1 << log_group) - 1), group = threadIdx.x >> log_group, groups = 256 >> log_group;
   const i64 c = (i64)blockIdx.x * groups + group;
   const int col = (((int)blockIdx.y << log_group) + lane) * VEC;
@@ -499,19 +501,23 @@ embed_join_kernel(const u32* __restrict__ part_key, const float* __restrict__ pa
       hi = hi_s;
       __syncthreads();
     }
-    const i64 len = hi - (at + 1), per = (len + groups - 1) / groups;
+    if (!NARROW) shares = groups;
+    const i64 len = hi - (at + 1), per = (len + shares - 1) / shares;
     float acc[VEC];
+#pragma unroll 1
+    for (int g = group; g < (NARROW ? shares : group + 1); g += groups) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-    const i64 from = at + 1 + group * per;
-    add_run(acc, from, from + per < hi ? from + per : hi, k0, false);
+      for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+      const i64 from = at + 1 + g * per;
+      add_run(acc, from, from + per < hi ? from + per : hi, k0, false);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) sums[threadIdx.x * VEC + j] = acc[j];
+      for (int j = 0; j < VEC; ++j) sums[((g << log_group) + lane) * VEC + j] = acc[j];
+    }
     __syncthreads();
     if (group == 0 && live) {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) acc[j] = part[(2 * at + 1) * part_ld + col + j];
-      for (int g = 0; g < groups; ++g) {
+      for (int g = 0; g < shares; ++g) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) acc[j] += sums[((g << log_group) + lane) * VEC + j];
       }
@@ -604,6 +610,20 @@ static int launch_embed_sort(const i64* idx, i64 n, i64 rows, i64 padding, char*
   return GSB_OK;
 }
 
+// elements a thread moves at once: 16 bytes where row width and addresses allow
+static int vec_of(const void* a, const void* b, i64 D, i64 ld, int size) {
+  const uintptr_t m = (uintptr_t)a | (uintptr_t)b | (uintptr_t)(D * size) | (uintptr_t)(ld * size);
+  int bytes = 16;
+  while (bytes > size && (m & (uintptr_t)(bytes - 1))) bytes >>= 1;
+  return bytes / size;
+}
+// log2 of the lanes that take a row of D elements, vec each
+static int log_lanes(i64 D, int vec) {
+  int lg = 0;
+  while (lg < 5 && (1 << lg) < D / vec) ++lg;
+  return lg;
+}
+
 template <typename T, int VEC>
 static void launch_segsum(const u32* key, const u32* pos, i64 n, const void* grad, i64 D, u32 limit, float scale,
                           void* out, char* ws, const EmbedLayout& L, cudaStream_t st) {
@@ -611,8 +631,7 @@ static void launch_segsum(const u32* key, const u32* pos, i64 n, const void* gra
   u32* part_key = (u32*)(ws + L.part_key);
   const int chunk = first_chunk(n);
   const i64 chunks = (n + chunk - 1) / chunk, per_row = D / VEC;
-  int lg = 0;
-  while (lg < 5 && (1 << lg) < per_row) ++lg;
+  const int widest = vec_of(nullptr, nullptr, D, D, sizeof(T)), lg = log_lanes(D, VEC), shares = 256 >> log_lanes(D, widest);
   const dim3 grid((unsigned)(((chunks << lg) + 255) / 256), (unsigned)((per_row + (1 << lg) - 1) >> lg));
   {
     LaunchScope ls(KID_EMBED_GRAD, st);
@@ -621,16 +640,11 @@ static void launch_segsum(const u32* key, const u32* pos, i64 n, const void* gra
   }
   if (chunks > 1) {
     LaunchScope ls(KID_EMBED_GRAD, st);
-    embed_join_kernel<T, VEC><<<grid, 256, 0, st>>>(part_key, part, L.part_ld, chunks, (int)D, lg, scale, (T*)out);
+    if (VEC * sizeof(T) < 16 && VEC < widest)
+      embed_join_kernel<T, VEC, (VEC * sizeof(T) < 16)><<<grid, 256, 0, st>>>(part_key, part, L.part_ld, chunks, (int)D, lg, shares, scale, (T*)out);
+    else
+      embed_join_kernel<T, VEC, false><<<grid, 256, 0, st>>>(part_key, part, L.part_ld, chunks, (int)D, lg, shares, scale, (T*)out);
   }
-}
-
-// elements a thread moves at once: 16 bytes where row width and addresses allow
-static int vec_of(const void* a, const void* b, i64 D, i64 ld, int size) {
-  const uintptr_t m = (uintptr_t)a | (uintptr_t)b | (uintptr_t)(D * size) | (uintptr_t)(ld * size);
-  int bytes = 16;
-  while (bytes > size && (m & (uintptr_t)(bytes - 1))) bytes >>= 1;
-  return bytes / size;
 }
 
 }  // namespace gsb

@@ -16,8 +16,8 @@ def embedding(weight: torch.Tensor, index: torch.Tensor, scale: float = 1.0, pad
     An id equal to ``padding_idx`` gives a row of zeros and has no gradient.  Any other id outside
     the table does the same and is reported by ``check_async_errors()``; nothing here synchronises.
 
-    The gradient sums the rows of equal ids in 32 bits, in the order of their positions (the same
-    inputs give the same bits), and rounds once.  ``sparse=True`` returns it as a coalesced sparse
+    The gradient sums the rows of equal ids in 32 bits, in an order that their positions fix (the same
+    inputs give the same bits on the same kind of GPU), and rounds once.  ``sparse=True`` returns it as a coalesced sparse
     tensor over the touched rows, which costs one read-back of their number (so it cannot be
     recorded into a CUDA graph); the dense form writes the whole table.  The dense gradient can be
     differentiated again; the sparse one, and forward-mode differentiation, raise."""

@@ -236,9 +236,10 @@ GSB_API int gsb_embedding(const void* weight, int dtype, int64_t ld, int64_t row
                           int* d_err, void* cuda_stream);
 
 /* The gradient of gsb_embedding with respect to weight, dense: out[rows, D],
- * out[v,:] = scale * sum of grad[i,:] over idx[i] == v in ascending order of i
- * (grad contiguous [n, D]), zeros for rows that no id names.  The order of the
- * sums depends on the ids alone: the same inputs give the same bits.
+ * out[v,:] = scale * sum of grad[i,:] over idx[i] == v (grad contiguous [n, D]),
+ * zeros for rows that no id names.  Consecutive runs of ascending i are summed and
+ * their sums added in order; where they are cut depends on the ids, the sizes, the
+ * type and the device's number of SMs: there, the same inputs give the same bits.
  * n < 2^31, rows < 2^32 - 1. */
 GSB_API size_t gsb_embedding_grad_workspace_bytes(int64_t n, int64_t rows, int64_t D);
 GSB_API int gsb_embedding_grad(const void* grad, int dtype, int64_t D, const int64_t* idx, int64_t n,
