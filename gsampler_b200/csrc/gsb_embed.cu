@@ -664,7 +664,7 @@ static void run_rows(const void* w, i64 ld, i64 rows, i64 D, const i64* idx, i64
 
 extern "C" int gsb_embedding(const void* weight, int dtype, int64_t ld, int64_t rows, int64_t D, const int64_t* idx,
                              int64_t n, float scale, int64_t padding, void* out, int* d_err, void* cuda_stream) {
-  if (n < 0 || rows < 0 || D < 0 || D > GSB_EMBED_MAX_D || (rows > 1 && ld < D)) return GSB_ERR_INVALID;
+  if (n < 0 || rows < 0 || D < 0 || D > GSB_EMBED_MAX_D || (rows > 1 && ld < D) || !(scale - scale == 0.f)) return GSB_ERR_INVALID;
   if (n == 0 || D == 0) return GSB_OK;
   if (!idx || !out || (rows > 0 && !weight)) return GSB_ERR_INVALID;
   if (!at_multiple(weight, value_bytes(dtype)) || !at_multiple(out, value_bytes(dtype)) || !at_multiple(idx, 8) || !at_multiple(d_err, 4))
@@ -711,7 +711,7 @@ static void segsum_any(int dtype, const u32* key, const u32* pos, i64 n, const v
 extern "C" int gsb_embedding_grad(const void* grad, int dtype, int64_t D, const int64_t* idx, int64_t n, int64_t rows,
                                   float scale, int64_t padding, void* out, void* workspace, size_t workspace_bytes,
                                   int* d_err, void* cuda_stream) {
-  if (!embed_sizes_ok(n, rows, D) || (dtype != GSB_F32 && dtype != GSB_F16 && dtype != GSB_BF16)) return GSB_ERR_INVALID;
+  if (!embed_sizes_ok(n, rows, D) || !(scale - scale == 0.f) || (dtype != GSB_F32 && dtype != GSB_F16 && dtype != GSB_BF16)) return GSB_ERR_INVALID;
   if (rows == 0 || D == 0) return GSB_OK;
   if (!out || (n > 0 && (!grad || !idx))) return GSB_ERR_INVALID;
   if (!at_multiple(grad, value_bytes(dtype)) || !at_multiple(out, value_bytes(dtype)) || !at_multiple(idx, 8) ||
@@ -758,7 +758,7 @@ extern "C" int gsb_embedding_sort(const int64_t* idx, int64_t n, int64_t rows, i
 extern "C" int gsb_embedding_grad_rows(const void* grad, int dtype, int64_t D, int64_t n, int64_t rows, int64_t num,
                                        float scale, void* out, void* workspace, size_t workspace_bytes,
                                        void* cuda_stream) {
-  if (!embed_sizes_ok(n, rows, D) || num < 0 || num > n || (dtype != GSB_F32 && dtype != GSB_F16 && dtype != GSB_BF16))
+  if (!embed_sizes_ok(n, rows, D) || num < 0 || num > n || !(scale - scale == 0.f) || (dtype != GSB_F32 && dtype != GSB_F16 && dtype != GSB_BF16))
     return GSB_ERR_INVALID;
   if (num == 0 || D == 0) return GSB_OK;
   if (!grad || !out) return GSB_ERR_INVALID;

@@ -28,6 +28,10 @@ static void CheckIndex(const torch::Tensor& t, const char* op, const char* name)
   TORCH_CHECK(t.scalar_type() == torch::kInt64, op, ": ", name, " must be int64");
 }
 
+static void CheckScale(double scale, const char* op) {
+  TORCH_CHECK(std::isfinite((float)scale), op, ": scale must be finite as a float32, got ", scale);
+}
+
 static int* ErrorWord(const torch::Device& dev) { return AsyncErrorWord(dev).data_ptr<int>(); }
 
 // ------------------------------------------------------------------ embedding
@@ -36,7 +40,7 @@ torch::Tensor Embedding(torch::Tensor weight, torch::Tensor index, double scale,
   CheckIndex(index, "Embedding", "index");
   TORCH_CHECK(weight.device() == index.device(), "Embedding: weight and index live on different devices");
   TORCH_CHECK(weight.dim() == 2, "Embedding: weight must be two-dimensional");
-  TORCH_CHECK(std::isfinite(scale), "Embedding: scale must be finite");
+  CheckScale(scale, "Embedding");
   c10::cuda::CUDAGuard guard(index.device());
   // rows may be strided (a column slice of a wider table is read in place)
   if (weight.size(1) > 1 && weight.stride(1) != 1) weight = weight.contiguous();
@@ -53,7 +57,8 @@ torch::Tensor Embedding(torch::Tensor weight, torch::Tensor index, double scale,
   return out;
 }
 
-static void CheckEmbeddingGrad(const torch::Tensor& grad, const torch::Tensor& index, int64_t num_rows) {
+static void CheckEmbeddingGrad(const torch::Tensor& grad, const torch::Tensor& index, int64_t num_rows, double scale) {
+  CheckScale(scale, "EmbeddingGrad");
   CheckIndex(index, "EmbeddingGrad", "index");
   TORCH_CHECK(grad.device() == index.device(), "EmbeddingGrad: grad and index live on different devices");
   TORCH_CHECK(grad.dim() == index.dim() + 1 && grad.sizes().slice(0, index.dim()) == index.sizes(),
@@ -64,7 +69,7 @@ static void CheckEmbeddingGrad(const torch::Tensor& grad, const torch::Tensor& i
 
 torch::Tensor EmbeddingGrad(torch::Tensor grad, torch::Tensor index, int64_t num_rows, double scale, int64_t padding) {
   const int dt = ValueType(grad, "EmbeddingGrad", "grad");
-  CheckEmbeddingGrad(grad, index, num_rows);
+  CheckEmbeddingGrad(grad, index, num_rows, scale);
   c10::cuda::CUDAGuard guard(index.device());
   grad = grad.contiguous();
   index = index.contiguous();
@@ -81,7 +86,7 @@ torch::Tensor EmbeddingGrad(torch::Tensor grad, torch::Tensor index, int64_t num
 std::tuple<torch::Tensor, torch::Tensor> EmbeddingSparseGrad(torch::Tensor grad, torch::Tensor index, int64_t num_rows,
                                                              double scale, int64_t padding) {
   const int dt = ValueType(grad, "EmbeddingSparseGrad", "grad");
-  CheckEmbeddingGrad(grad, index, num_rows);
+  CheckEmbeddingGrad(grad, index, num_rows, scale);
   c10::cuda::CUDAGuard guard(index.device());
   grad = grad.contiguous();
   index = index.contiguous();
@@ -162,7 +167,7 @@ static int CheckLoss(const torch::Tensor& x, const torch::Tensor& weight, const 
   TORCH_CHECK(weight.size(0) >= 1 && weight.size(1) >= 1, op, ": weight must have a row and a column");
   TORCH_CHECK(weight.size(1) <= GSB_LOSS_MAX_D, op, ": at most ", GSB_LOSS_MAX_D, " columns");
   TORCH_CHECK(x.size(0) <= (1ll << 30) && weight.size(0) <= (1ll << 30), op, ": at most 2^30 rows");
-  TORCH_CHECK(std::isfinite(scale), op, ": scale must be finite");
+  CheckScale(scale, op);
   return dt;
 }
 
