@@ -3,7 +3,8 @@
 //
 //   statistics  tiles of x W^T whose epilogue keeps the running maximum and sum of every row
 //   piece       tiles of x W^T again, whose epilogue writes g (p - target) of at most PIECE_ELEMS
-//               elements to a workspace (its 2 or 6 bytes an element stay in L2)
+//               elements to a workspace: 64 MB of 16-bit values, which L2 holds, 192 MB of fp32's planes, which
+//               it does not; at least 128 columns, of which 16-bit tiles of 256 waste half, from 262144 rows on
 //   dx, dW      the piece times W, its transpose times x; long sums are split into 32-bit slabs that
 //               are added in a fixed order
 //

@@ -21,8 +21,8 @@
 // N x V values exists anywhere.
 //
 // Bound by the hand-over from the tensor cores to the exponentials and back: at 128 columns both take
-// 1024 cycles a tile of 128 x 128 and each is busy 56 - 58 % of the time (8192 x 60000, bf16); at 256
-// columns the products are twice as long and run at 1500 TFLOP/s (8192 x 300000).
+// 1024 cycles a tile of 128 x 128 and each is busy 58 - 59 % of the time (8192 x 60000, bf16); at 256
+// columns the products are twice as long and run at 1400 (forward) and 1490 TFLOP/s (dW; 8192 x 300000).
 //
 // The reference m moves only when a row's maximum passes it by 2^8, because moving it rescales O;
 // P stays below 2^15, which fp16 holds.  Sums and O are 32 bits; P is rounded to the type, half a
@@ -988,7 +988,8 @@ typedef TcShape<TC_GRAD_W, 128, 1, 2, 64, 4, 2, 2, false, 1, true> GradFew128;
 // x more at 1.3 PFLOP/s, against writing and reading 16 bytes of pull at 5 TB/s: equal near 2080).
 constexpr i64 SMALL_V = 2048;
 
-// f(shape) for the shape that the sizes ask for.  Two small CTAs an SM overlap one's loads and stores
+// f(shape) for the shape that the sizes ask for; the figures are those of the choice, each shape's own time has
+// moved by up to 5 % since.  Two small CTAs an SM overlap one's loads and stores
 // with the other's products, and their hand-overs fall out of step by themselves; one large CTA reads B
 // less often.  Measured (bf16, ms): forward with pulls, 128 columns, two small / one large: 1024 x 232965
 // 0.107 / 0.116, 4096 x 100000 0.173 / 0.186, 8192 x 300000 0.956 / 0.975; 64 columns 8192 x 300000

@@ -163,7 +163,8 @@ __device__ __forceinline__ u64 both(float v) { return join2(v, v); }
 // the special-function unit (16 results a cycle and SM).  x = n + f with n the nearest integer, which
 // the addition of 1.5 2^23 leaves in the low bits (127 more makes them an exponent field); 2^f by
 // the polynomial of degree 5 that is nearest to it in relative error on [-1/2, 1/2] (weighted least
-// squares on Chebyshev points, 7.5e-8; 2.1e-7 with the roundings of its evaluation).  x below -126
+// squares on Chebyshev points; 1.5e-7 with its coefficients in 32 bits, 2.1e-7 with the roundings of its
+// evaluation).  x below -126
 // gives 2^-126; a NaN and an infinity give NaN.  x < 128.
 __device__ __forceinline__ void ex2_poly(float& lo, float& hi) {
   const u64 x = join2(max_nan(lo, -126.f), max_nan(hi, -126.f));
