@@ -14,7 +14,8 @@ def dropout(data: torch.Tensor, p: float = 0.5, training: bool = True, seed: int
     The mask depends on ``seed``, ``stream`` and the element's position in row-major order only.
     Left out, they come from the process's dropout state: the seed of
     ``torch.ops.gs_ops._CAPI_SetDropoutSeed`` (by default one that no sampler starts from) and a counter
-    that advances with every call.  Give both to repeat a mask.  A seed that a graph or list sampling uses
+    that advances with every call.  Give both to repeat a mask, also where a forward pass is
+    computed twice (activation checkpointing).  A seed that a graph or list sampling uses
     too makes masks of the words that chose there, wherever the stream numbers meet: keep them apart.
     ``stream`` counts modulo 2^32.  A recorded CUDA graph replays the recorded streams; ``step``, a
     one-element int64 tensor on the GPU that is added to ``stream`` when the kernel runs, gives
