@@ -62,11 +62,35 @@ static int total_blocks(i64 N) {
   return (int)(b < 512 ? b : 512);
 }
 
+// 1 - p_t of every row that counts, from its loss.
+__device__ __forceinline__ float miss_of_loss(float loss) { return -expm1f(-loss); }
+
+// The same from the log-sum-exp and the target's logit made once more, a warp a row: to about 1e-6, the units in
+// the last place of both.
+template <typename T>
+__global__ void __launch_bounds__(256)
+loss_miss_kernel(const T* __restrict__ x, i64 ldx, i64 N, const T* __restrict__ w, i64 ldw, i64 V, int D, float scale, const i64* __restrict__ target,
+                 i64 ignore, const float* __restrict__ lse2, float* __restrict__ miss) {
+  const i64 r = ((i64)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (r >= N) return;
+  const i64 t = target[r];
+  float l = 0.f;
+  if (t != ignore && t >= 0 && t < V)
+    for (int d = lane; d < D; d += 32) l = fmaf(to_float(x[r * ldx + d]), to_float(w[t * ldw + d]), l);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  if (lane == 0) {
+    const float d = lse2[r] * 0.6931471805599453f - l * scale;
+    miss[r] = miss_of_loss(d < 0.f ? 0.f : d);
+  }
+}
+
 // g[i] = upstream gradient of row i's loss (divided by the count for the mean), 0 where the row
-// does not count; top = bits of the largest finite magnitude (an integer maximum: no order matters).
+// does not count; with loss, miss[i] = 1 - p_t; top = bits of the largest finite magnitude (an integer maximum: no order matters).
 __global__ void loss_row_grad_kernel(const float* __restrict__ up, int per_row, const float* __restrict__ count,
-                                     const i64* __restrict__ target, i64 ignore, i64 V, i64 N, float* __restrict__ g,
-                                     u32* top) {
+                                     const i64* __restrict__ target, i64 ignore, i64 V, i64 N, const float* __restrict__ loss,
+                                     float* __restrict__ g, float* __restrict__ miss, u32* top) {
   constexpr u32 INFINITE = 0x7F800000u;
   u32 mine = 0;
   for (i64 i = (i64)blockIdx.x * blockDim.x + threadIdx.x; i < N; i += (i64)gridDim.x * blockDim.x) {
@@ -74,6 +98,7 @@ __global__ void loss_row_grad_kernel(const float* __restrict__ up, int per_row, 
     float v = 0.f;
     if (t != ignore && t >= 0 && t < V) v = per_row ? up[i] : (count ? *up / *count : *up);
     g[i] = v;
+    if (loss) miss[i] = miss_of_loss(loss[i]);
     const u32 b = __float_as_uint(fabsf(v));
     mine = b > mine && b < INFINITE ? b : mine;
   }
@@ -161,7 +186,7 @@ extern "C" int gsb_linear_ce_total(const float* loss, const int64_t* target, int
 extern "C" size_t gsb_linear_ce_grad_workspace_bytes(int dtype, const void* weight, int64_t ldw, int64_t N, int64_t V, int64_t D,
                                                      int have_pull, int want_dx, int want_dw) {
   if (!loss_sizes_ok(N, V, D, D, D)) return 0;
-  const size_t head = up256(4 * (size_t)N) + 256;
+  const size_t head = 2 * up256(4 * (size_t)N) + 256;
   if (!tc_loss_takes(dtype, D))
     return head + gemm_loss_grad_workspace(dtype, N, V, D, want_dx != 0, want_dw != 0, tc_loss_packs(weight, ldw));
   return head + tc_loss_grad_workspace(dtype, N, V, D, want_dx && !have_pull, want_dw != 0);
@@ -172,10 +197,19 @@ extern "C" int gsb_linear_ce_grad(const void* x, int dtype, int64_t ldx, int64_t
                                   const float* lse2, const float* pull, const float* upstream, int per_row,
                                   const float* count, void* dx, void* dw, void* workspace, size_t workspace_bytes,
                                   int* d_err, void* cuda_stream) {
+  return gsb_linear_ce_grad_rows(x, dtype, ldx, N, weight, ldw, V, D, target, ignore, scale, nullptr, lse2, pull, upstream, per_row, count, dx,
+                                 dw, workspace, workspace_bytes, d_err, cuda_stream);
+}
+
+extern "C" int gsb_linear_ce_grad_rows(const void* x, int dtype, int64_t ldx, int64_t N, const void* weight, int64_t ldw,
+                                       int64_t V, int64_t D, const int64_t* target, int64_t ignore, float scale,
+                                       const float* loss, const float* lse2, const float* pull, const float* upstream,
+                                       int per_row, const float* count, void* dx, void* dw, void* workspace,
+                                       size_t workspace_bytes, int* d_err, void* cuda_stream) {
   if (!loss_sizes_ok(N, V, D, ldx, ldw) || !(scale - scale == 0.f)) return GSB_ERR_INVALID;
   if (dtype != GSB_F32 && dtype != GSB_F16 && dtype != GSB_BF16) return GSB_ERR_INVALID;
   if (!at_multiple(x, value_bytes(dtype)) || !at_multiple(weight, value_bytes(dtype)) || !at_multiple(target, 8) ||
-      !at_multiple(lse2, 4) || !at_multiple(pull, 4) || !at_multiple(upstream, 4) || !at_multiple(count, 4) ||
+      !at_multiple(loss, 4) || !at_multiple(lse2, 4) || !at_multiple(pull, 4) || !at_multiple(upstream, 4) || !at_multiple(count, 4) ||
       !at_multiple(dx, value_bytes(dtype)) || !at_multiple(dw, value_bytes(dtype)) || !at_multiple(workspace, 16) || !at_multiple(d_err, 4))
     return GSB_ERR_INVALID;
   cudaStream_t st = (cudaStream_t)cuda_stream;
@@ -190,18 +224,29 @@ extern "C" int gsb_linear_ce_grad(const void* x, int dtype, int64_t ldx, int64_t
     return GSB_ERR_WORKSPACE;
   char* ws = (char*)workspace;
   float* g = (float*)ws;
-  u32* top = (u32*)(ws + up256(4 * (size_t)N));
+  float* miss = (float*)(ws + up256(4 * (size_t)N));
+  u32* top = (u32*)(ws + 2 * up256(4 * (size_t)N));
   if (per_row) GSB_CUDA_OK(cudaMemsetAsync(top, 0, 4, st));
   {
     LaunchScope ls(KID_LOSS_JOIN, st);
     i64 blocks = (N + 255) / 256;
     if (blocks > sm_count() * 4) blocks = sm_count() * 4;
-    loss_row_grad_kernel<<<(int)blocks, 256, 0, st>>>(upstream, per_row, count, (const i64*)target, ignore, V, N, g, top);
+    loss_row_grad_kernel<<<(int)blocks, 256, 0, st>>>(upstream, per_row, count, (const i64*)target, ignore, V, N, loss, g, miss, top);
+  }
+  if (!loss && (dw || !pull)) {
+    LaunchScope ls(KID_LOSS_JOIN, st);
+    const int blocks = ceil_div_i(N, 8);
+    auto launch = [&](auto* xs, auto* rows_w) {
+      loss_miss_kernel<<<blocks, 256, 0, st>>>(xs, ldx, N, rows_w, ldw, V, (int)D, scale, (const i64*)target, ignore, lse2, miss);
+    };
+    if (dtype == GSB_F32) launch((const float*)x, (const float*)weight);
+    else if (dtype == GSB_F16) launch((const __half*)x, (const __half*)weight);
+    else launch((const __nv_bfloat16*)x, (const __nv_bfloat16*)weight);
   }
   LossArgs a = {};
   a.x = x; a.ldx = ldx; a.N = N; a.w = weight; a.ldw = ldw; a.V = V; a.D = D;
   a.target = (const i64*)target; a.ignore = ignore; a.scale = scale; a.lse2 = const_cast<float*>(lse2);
-  a.per_row = per_row; a.g = g; a.top = top; a.dx = dx; a.dw = dw; a.ws = ws + up256(4 * (size_t)N) + 256; a.err = d_err; a.st = st;
+  a.per_row = per_row; a.g = g; a.miss = miss; a.top = top; a.dx = dx; a.dw = dw; a.ws = ws + 2 * up256(4 * (size_t)N) + 256; a.err = d_err; a.st = st;
   int rc = GSB_OK;
   if (!tc_loss_takes(dtype, D)) {
     rc = dtype == GSB_F32 ? gemm_loss_backward<float>(a)

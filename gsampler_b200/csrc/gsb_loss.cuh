@@ -74,6 +74,7 @@ struct LossArgs {
   float* lse2;   // [N], base 2
   int per_row;     // whether rows have gradients of their own
   const float* g;  // [N] upstream gradient of every row's loss, 0 where it does not count
+  const float* miss;  // [N] 1 - p of the row's target
   const u32* top;  // bits of the largest finite |g|: one row's infinity or NaN is not a factor of the others
   void *dx, *dw;
   void* ws;
@@ -133,8 +134,8 @@ template <typename T>
 int gemm_loss_forward(const LossArgs& a);
 template <typename T>
 int gemm_loss_backward(const LossArgs& a);
-// losses (and pulls) of all rows from the parts of their statistics (gsb_loss_tc.cu); with hot, the targets'
-// products, the parts leave the targets out
+// losses (and pulls) of all rows from the parts of their statistics, which leave the targets out, and hot, the
+// targets' products (gsb_loss_tc.cu)
 template <typename T>
 void launch_loss_join(const LossArgs& a, const float2* part_ms, int parts, const float* part_o, const float* hot, float* pull);
 

@@ -1,8 +1,9 @@
 // The vocabulary cross entropy for more columns than gsb_loss_tc.cu takes: tiled products on the tensor
 // cores, with the vocabulary taken in pieces in the backward pass.
 //
-//   statistics  tiles of x W^T whose epilogue keeps the running maximum and sum of every row
-//   piece       tiles of x W^T again, whose epilogue writes g (p - target) of at most PIECE_ELEMS
+//   statistics  tiles of x W^T whose epilogue keeps the running maximum and sum of every row, its target left out
+//   piece       tiles of x W^T again, whose epilogue writes g (p - target), the target's element from the row's
+//               1 - p_t, of at most PIECE_ELEMS
 //               elements to a workspace: 64 MB of 16-bit values, which L2 holds, 192 MB of fp32's planes, which
 //               it does not; at least 128 columns, of which 16-bit tiles of 256 waste half, from 262144 rows on
 //   dx, dW      the piece times W, its transpose times x; long sums are split into 32-bit slabs that
@@ -53,9 +54,11 @@ struct GmParams {
   int k_per;                // depth of one slab, a multiple of 64
   float c;
   float2* part_ms;          // GM_STATS: [2 * splits][M]
+  float* hot;               // GM_STATS: [M] the target's product, where the target lies in the vocabulary
   const float* lse2;        // GM_PIECE, by row
   const float* g;
-  const i64* target;
+  const float* miss;
+  const i64* target;        // GM_STATS, GM_PIECE
   const u32* top;
   int v0;                   // GM_PIECE: id of the piece's first column
   void* piece;              // GM_PIECE: [PL][M][ld_piece]
@@ -251,11 +254,17 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       const int row = m * 128 + quarter * 32 + lane;
       float lse = INFINITY, gs = 0.f;
       int hot = -1;
+      float at_target = 0.f;
+      if (C::MODE == GM_STATS && row < p.M) {
+        const i64 t = p.target[row];
+        if (t >= 0 && t < p.N) hot = (int)t;
+      }
       if (C::MODE == GM_PIECE && row < p.M && p.g[row] != 0.f) {
         lse = p.lse2[row];
         const float top = __uint_as_float(*p.top);
         gs = times_power(p.g[row], -small_rows<T>(p.g[row], top)) / top * (float)(1 << GRAD_SHIFT);
         hot = (int)(p.target[row] - p.v0);
+        at_target = -p.miss[row] * gs;
       }
       if constexpr (C::MODE == GM_PIECE) {
         // 64 columns at a time through shared memory, so that they leave as whole lines: row by row a
@@ -274,8 +283,7 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 #pragma unroll
           for (int j = 0; j < 64; ++j) {
             v[j] = ex2(fmaf(v[j], p.c, -lse));
-            if (col + j == hot) v[j] -= 1.f;
-            v[j] = gs == 0.f ? 0.f : v[j] * gs;  // rows that do not count
+            v[j] = gs == 0.f ? 0.f : col + j == hot ? at_target : v[j] * gs;  // zeros for rows that do not count
           }
           if (C::PL == 1 && (u32)(hot - col) < 64u) {
             // g (p - 1) is as large as its row's other elements together: dx gets the lost part back
@@ -335,13 +343,24 @@ loss_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           for (int j = 0; j < 32; ++j) v[j] = 0.f;
         }
         if (C::MODE == GM_STATS) {
+          const int at = hot - col;
+          if (__any_sync(0xffffffffu, (u32)at < 32u)) {
+            float mine = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j == at) {
+                mine = v[j];
+                v[j] = -INFINITY;
+              }
+            if ((u32)at < 32u) p.hot[row] = mine;
+          }
           float top = -INFINITY;
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             if (col + j >= p.N) v[j] = -INFINITY;
             top = fmaxf(top, v[j]);
           }
-          const float t = top * p.c;
+          const float t = __fmul_rn(top, p.c);
           if (t > run_m + MOVE_REFERENCE) {
             run_s = run_m == -INFINITY ? run_s : run_s * ex2(run_m - t);
             run_m = t;
@@ -475,7 +494,7 @@ static int bn_of(int planes, i64 cols) { return planes == 3 ? (cols <= 64 ? 64 :
 static int bn_wide(int planes, i64 D) { return planes == 3 || D > RUN_TERMS ? 128 : 256; }
 
 struct GmLayout {
-  size_t ms, x, x_dw, w, piece, lost, dx_slab, dw_slab, bytes;
+  size_t ms, hot, x, x_dw, w, piece, lost, dx_slab, dw_slab, bytes;
   bool x_dw_taken;
   i64 cols, ldp;
   int dx_slabs, dw_slabs, splits, per;
@@ -493,6 +512,7 @@ static GmLayout gemm_layout(int dtype, i64 N, i64 V, i64 D, bool forward, bool d
     L.per = (int)((tiles + s - 1) / s);
     L.splits = (int)((tiles + L.per - 1) / L.per);
     L.ms = take(8 * (size_t)2 * L.splits * N);
+    L.hot = take(4 * (size_t)N);
   } else {
     L.cols = piece_columns(N, V);
     L.dx_slabs = slab_count(planes, N, D, L.cols, bn_of(planes, D));
@@ -571,10 +591,12 @@ int gemm_loss_forward(const LossArgs& a) {
   p.k_per = (int)((a.D + 63) / 64 * 64);
   p.c = logit_factor(a.scale);
   p.part_ms = (float2*)(ws + L.ms);
+  p.hot = (float*)(ws + L.hot);
+  p.target = a.target;
   p.err = a.err;
   const int rc = launch_mode<T, GM_STATS, PL>(a.V, a.D, ma, mb, p, dim3(p.m_tiles, L.splits), KID_LOSS, a.st);
   if (rc != GSB_OK) return rc;
-  launch_loss_join<S>(a, p.part_ms, 2 * L.splits, nullptr, nullptr, nullptr);
+  launch_loss_join<S>(a, p.part_ms, 2 * L.splits, nullptr, p.hot, nullptr);
   return GSB_OK;
 }
 
@@ -624,6 +646,7 @@ int gemm_loss_backward(const LossArgs& a) {
       p.c = logit_factor(a.scale);
       p.lse2 = a.lse2;
       p.g = a.g;
+      p.miss = a.miss;
       p.target = a.target;
       p.top = a.top;
       p.v0 = (int)v0;

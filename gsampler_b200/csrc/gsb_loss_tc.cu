@@ -9,14 +9,15 @@
 // room, which halves what the first product reads from shared memory.
 //   forward   A = rows of x, B = the vocabulary.  P = exp2(l - m) against a running reference m;
 //             O / sum P is the expected row of W, which is all that dx needs; log2 sum P + m is
-//             the log-sum-exp.  Without a gradient for x there is no second product.  With one, the
-//             target's element stays out of P and of the sum and is added to them afterwards:
-//             dx ~ sum_{j != t} p_j w_j - (1 - p_t) w_t, and the rounding of p_t, half a step however
-//             likely the target is, would be many times 1 - p_t.
+//             the log-sum-exp.  Without a gradient for x there is no second product.
 //   dW        A = rows of W, B = rows of x.  P = g (p - target) with the known log-sum-exp.
 //   dx        (small vocabularies, fp32) A = rows of x, B = the vocabulary, P = p without the target's,
 //             whose (p_t - 1) w_t is added in 32 bits; the row's g is a factor at the end, so that no row's
 //             scale is another's.  Makes the logits once more instead of keeping the expected rows.
+// The gradients are sum_{j != t} p_j w_j - (1 - p_t) w_t and the like: where the target is likely, all of it is of
+// the size of 1 - p_t, and half a step of p_t, or a unit of its logit, would be many times that.  So p_t is never
+// made: the forward pass leaves the target out of P and of the sum, the join adds it and has the row's loss as
+// log(1 + others / target), and the backward passes take 1 - p_t from the loss.
 // So training costs four products of N V D multiply-adds (five with dx by itself), and no array of
 // N x V values exists anywhere.
 //
@@ -76,8 +77,7 @@ struct TcShape {
   static constexpr bool SPILLS = PL == 1 && !SHORT_ && (MODE == TC_PULL || MODE == TC_GRAD_W);
   static constexpr bool KEEPS = PL == 3 && SECOND;  // or in registers
   static constexpr int OFF_B = NA * A_BYTES, OFF_META = OFF_B + ST * B_BYTES;
-  static constexpr int OFF_COEF = OFF_META + ST * META;  // TC_GRAD_X: p_t - 1 by half and row
-  static constexpr int OFF_BAR = OFF_COEF + (MODE == TC_GRAD_X ? WG * 128 * 4 : 0);
+  static constexpr int OFF_BAR = OFF_META + ST * META;
   static constexpr int BARS = 3 * ST + 2 * NB + 3;
   static constexpr int BYTES = OFF_BAR + 8 * BARS + 16 + 1024;  // and room to align the base
   static_assert(USED <= 512 && COLS * CTAS <= 512, "TMEM");
@@ -85,7 +85,7 @@ struct TcShape {
   static_assert(MODE != TC_PULL || HV == 1, "a row's running state has one owner");
   static_assert(MODE != TC_PULL || NB > 1, "a moved reference waits for the product before");
   static_assert(PL == 1 || (MODE != TC_PULL && NA == 1), "");
-  static_assert(!SECOND || NA == 1, "the halves of a row pass on its target's element; runs count tiles");
+  static_assert(!SECOND || NA == 1, "runs count tiles");
   static_assert(HC % 32 == 0 && META % 16 == 0 && OFF_BAR % 8 == 0, "");
 };
 
@@ -103,6 +103,7 @@ struct TcParams {
   int w_bytes;
   const float* lse2;        // TC_GRAD_X, by row
   const float* g;           // TC_GRAD_X
+  const float* miss;        // TC_GRAD_X: 1 - p of the row's target
   const i64* target;        // TC_STATS, TC_PULL, TC_GRAD_X
   float* hot;               // TC_STATS, TC_PULL: [rows_a] the target's product, where the target lies in the vocabulary
   float2* part_ms;          // TC_STATS / TC_PULL: [parts][rows_a] reference and sum
@@ -394,7 +395,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
     float m = -INFINITY, sum = 0.f;
     const u64 c2 = join2(p.c, p.c);
     // the target, and for dx the row's gradient (an infinite bias: P = 0) and p - 1 at the target, held as P is:
-    // p itself, and only for fp16 at 2^14 times that (by a product, an addition to the exponent would round p near 1)
+    // p itself, and only for fp16 at 2^14 times that
     constexpr float UNIT = dx_unit<T>();
     int hot = -1;
     float row_grad = 0.f, row_bias = -INFINITY, coef = 0.f;
@@ -406,6 +407,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
       hot = (int)p.target[row];  // in range: the row counts
       row_grad = p.g[row];
       row_bias = -p.lse2[row];
+      coef = -UNIT * p.miss[row];
     }
     bool ok = true;
     float kept[C::KEEPS ? PIECES * 32 : 1];  // O of the runs before this one, this warp's columns of it
@@ -495,7 +497,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
 #pragma unroll
             for (int k = 0; k < C::HC; k += 2) exponentials(v[k], v[k + 1], k);
             const int* tgt = reinterpret_cast<const int*>(meta + 4 * C::BT);
-            const float* gs = reinterpret_cast<const float*>(meta + 8 * C::BT);
+            const float* at_target = reinterpret_cast<const float*>(meta + 8 * C::BT);
             bool near = false;
 #pragma unroll
             for (int k = 0; k < C::HC / 32; ++k) {
@@ -508,7 +510,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
 #pragma unroll
               for (int k = 0; k < C::HC; ++k) {
                 const int t = tgt[k];
-                if (t == row) v[k] -= gs[k];
+                if (t == row) v[k] = at_target[k];
                 if (t == WIPE) v[k] = 0.f;
               }
             }
@@ -526,28 +528,18 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
               exponentials(v[k], v[k + 1], k);
               if (UNIT != 1.f) part2(mul2(join2(v[k], v[k + 1]), both(UNIT)), v[k], v[k + 1]);
             }
-            const int at = hot - col0;
-            if (__any_sync(0xffffffffu, (u32)at < (u32)C::HC)) {
-              float mine = 0.f;
+            const int at = hot - col0;  // the target is not a part of P (a branch around this costs more than it: 81 us for 77)
 #pragma unroll
-              for (int k = 0; k < C::HC; ++k)
-                if (k == at) {
-                  mine = v[k];
-                  v[k] = 0.f;
-                }
-              if ((u32)at < (u32)C::HC) coef = mine - UNIT;
-            }
+            for (int k = 0; k < C::HC; ++k) v[k] = k == at ? 0.f : v[k];
           } else {
             const int col0 = (t0 + j) * C::BT + half * C::HC;
             const int at = hot - col0;
-            if (__any_sync(0xffffffffu, (u32)at < (u32)C::HC)) {  // the target's product, on its way past
+            if (__any_sync(0xffffffffu, (u32)at < (u32)C::HC)) {  // the target's product: not a part of the sums
               float mine = 0.f;
 #pragma unroll
-              for (int k = 0; k < C::HC; ++k)
-                if (k == at) {
-                  mine = v[k];
-                  if (C::MODE == TC_PULL) v[k] = -INFINITY;
-                }
+              for (int k = 0; k < C::HC; ++k) mine = k == at ? v[k] : mine;
+#pragma unroll
+              for (int k = 0; k < C::HC; ++k) v[k] = k == at ? -INFINITY : v[k];
               if ((u32)at < (u32)C::HC && row < p.rows_a) p.hot[row] = mine;
             }
             if (col0 + C::HC > p.rows_b) {
@@ -562,7 +554,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
               top[q] = max3(top[q], v[k], v[k + 1]);
               top[q + 1] = max3(top[q + 1], v[k + 2], v[k + 3]);
             }
-            const float t = fmaxf(max3(top[0], top[1], top[2]), top[3]) * p.c;
+            const float t = __fmul_rn(fmaxf(max3(top[0], top[1], top[2]), top[3]), p.c);
             const bool move = t > m + MOVE_REFERENCE;
             if (__any_sync(0xffffffffu, move)) {
               const float f = move ? (m == -INFINITY ? 0.f : ex2(m - t)) : 1.f;
@@ -644,16 +636,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
     Pack<V, 32> target_row[AHEAD];
     const bool here = C::MODE == TC_GRAD_X && hot >= t0 * C::BT && hot < (t0 + my_tiles) * C::BT;
     const V* target_at = (const V*)p.w + (i64)(here ? hot : 0) * p.ldw;
-    if (C::MODE == TC_GRAD_X) {
-      if (C::PL == 1) row_pieces(target_row, target_at + half * 32, 32 * C::HV, here ? p.D - half * 32 : 0, p.w_bytes);
-      // one of the halves has met it: they pass it on
-      float* passed = reinterpret_cast<float*>(smem + C::OFF_COEF) + quarter * 32 + lane;
-      passed[wg * 128] = coef;
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + quarter), "n"(32 * C::HV) : "memory");
-      coef = 0.f;
-#pragma unroll
-      for (int h = 0; h < C::HV; ++h) coef += passed[h * 128];
-    }
+    if (C::MODE == TC_GRAD_X && C::PL == 1) row_pieces(target_row, target_at + half * 32, 32 * C::HV, here ? p.D - half * 32 : 0, p.w_bytes);
     if (C::SECOND && my_tiles > 0) {
       ok = ok && bar_wait(o_full, 0, gave_up, p.err);
       ok = __all_sync(0xffffffffu, ok);
@@ -760,114 +743,113 @@ __global__ void loss_pack_kernel(const T* __restrict__ src, i64 ld, i64 rows, in
 }
 
 // What the dW pass needs of every row of x, by tiles of BT rows: -bias (p g = exp2(l - bias)), target,
-// |g| as P holds it, and the sign as a mask of the packed element.  Rows that do not count, and the
+// |g| (p - 1) of the target as P holds it, and the sign of g as a mask of the packed element.  Rows that do not count, and the
 // rows behind the last, have an infinite bias: P = 0.  That is not enough where the row is taken as zeros,
 // behind the last and where it holds an infinity or a NaN: WIPE.
-__global__ void loss_meta_kernel(const float* __restrict__ lse2, const i64* __restrict__ target, const float* __restrict__ g,
+__global__ void loss_meta_kernel(const float* __restrict__ lse2, const float* __restrict__ miss, const i64* __restrict__ target, const float* __restrict__ g,
                                  const u32* __restrict__ top, i64 N, i64 Npad, int BT, unsigned char* __restrict__ meta) {
   const i64 r = (i64)blockIdx.x * blockDim.x + threadIdx.x;
   if (r >= Npad) return;
   unsigned char* tile = meta + r / BT * (BT * 14);
   const int k = (int)(r % BT);
-  float bias = INFINITY, gs = 0.f;
+  float bias = INFINITY, at_target = 0.f;
   int t = -1;
   u32 sign = 0;
   if (r >= N || (g[r] == 0.f && !(fabsf(lse2[r]) < INFINITY))) t = WIPE;
   if (r < N && g[r] != 0.f) {
     const float rel = fabsf(g[r]) / __uint_as_float(*top);
-    gs = rel * (float)(1 << GRAD_SHIFT);
+    at_target = -miss[r] * (rel * (float)(1 << GRAD_SHIFT));
     bias = lse2[r] - log2f(rel) - (float)GRAD_SHIFT;
     t = (int)target[r];
     sign = g[r] < 0.f ? 0x8000u : 0u;
   }
   reinterpret_cast<float*>(tile)[k] = -bias;
   reinterpret_cast<int*>(tile + 4 * BT)[k] = t;
-  reinterpret_cast<float*>(tile + 8 * BT)[k] = gs;
+  reinterpret_cast<float*>(tile + 8 * BT)[k] = at_target;
   reinterpret_cast<unsigned short*>(tile + 12 * BT)[k] = (unsigned short)sign;
 }
 
-// The statistics of a row's parts joined: the log-sum-exp in base 2 (of values held at 2^FWD_SHIFT).
-// Parts that leave the target out get it here, as its logit l2 in base 2 (-inf: they have it already);
-// `others` is the sum without it.
-__device__ __forceinline__ float join_parts(const float2* __restrict__ part, int parts, i64 N, i64 r, int first, int step, float l2, float& m,
-                                            float& others, float& s) {
-  m = l2;
+// The statistics of a row's parts, which leave its target out, joined with the target's logit l2 in base 2 (-inf:
+// there is none): the log-sum-exp in base 2 (of values held at 2^FWD_SHIFT).
+struct RowSums { float m, others, s; };  // reference, sum without the target, sum
+__device__ __forceinline__ float join_parts(const float2* __restrict__ part, int parts, i64 N, i64 r, int first, int step, float l2, RowSums& q) {
+  float m = l2;
   for (int k = first; k < parts; k += step) m = max_nan(m, part[(i64)k * N + r].x);
   if (step == 32) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
   }
-  others = 0.f;
+  float others = 0.f;
   for (int k = first; k < parts; k += step) {
-    const float2 q = part[(i64)k * N + r];
-    // a part without a reference has either no finite logit (sum 0) or a NaN
-    others += q.x == -INFINITY ? q.y : q.y * exp2f(q.x - m);
+    const float2 mine = part[(i64)k * N + r];
+    // a part without a reference has either no finite logit or a NaN
+    others += mine.x == -INFINITY ? mine.y * 0.f : mine.y * exp2f(mine.x - m);
   }
   if (step == 32) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) others += __shfl_xor_sync(0xffffffffu, others, d);
   }
-  s = l2 == -INFINITY ? others : others + exp2f(l2 - m + (float)FWD_SHIFT);
-  return m - (float)FWD_SHIFT + log2f(s);
+  q.m = m;
+  q.others = others;
+  q.s = l2 == -INFINITY ? others : others + exp2f(l2 - m + (float)FWD_SHIFT);
+  return m + (log2f(q.s) - (float)FWD_SHIFT);
 }
 constexpr float LN2 = 0.6931471805599453f;
+// -log p of the target: log(1 + others / its own), which has the digits of a small loss; from the difference of
+// logarithms where its own is as good as nothing
+__device__ __forceinline__ float row_loss(float total, float l2, const RowSums& q) {
+  const float d = l2 - q.m;
+  return d > -20.f ? log1pf(q.others * exp2f(-(float)FWD_SHIFT - d)) : (total - l2) * LN2;
+}
 
-// Losses from the parts and the targets' products that went past (hot): a thread a row, or a warp
-// where there are many parts.
+// Losses from the parts and the targets' products that went past (hot, of +-x: times c >= 0 a logit in base 2): a
+// thread a row, or a warp where there are many parts.
 __global__ void __launch_bounds__(256)
-loss_finish_kernel(const float2* __restrict__ part, int parts, int lanes, const float* __restrict__ hot, i64 N, i64 V, float scale,
+loss_finish_kernel(const float2* __restrict__ part, int parts, int lanes, const float* __restrict__ hot, i64 N, i64 V, float c,
                    const i64* __restrict__ target, i64 ignore, float* __restrict__ loss, float* __restrict__ lse2, int* err) {
   const i64 e = (i64)blockIdx.x * blockDim.x + threadIdx.x;
   const i64 r = lanes == 32 ? e >> 5 : e;
   if (r >= N) return;
-  float m, others, s;
-  const float total = join_parts(part, parts, N, r, lanes == 32 ? (int)(e & 31) : 0, lanes, -INFINITY, m, others, s);
-  if (lanes == 32 && (e & 31) != 0) return;
   const i64 t = target[r];
-  const bool counts = t != ignore && t >= 0 && t < V;
+  const bool there = t >= 0 && t < V, counts = there && t != ignore;
+  const float l2 = there ? __fmul_rn(hot[r], c) : -INFINITY;
+  RowSums q;
+  const float total = join_parts(part, parts, N, r, lanes == 32 ? (int)(e & 31) : 0, lanes, l2, q);
+  if (lanes == 32 && (e & 31) != 0) return;
   if (t != ignore && !counts) raise(err, ERRBIT_BAD_INPUT);
   lse2[r] = total;
-  loss[r] = counts ? total * LN2 - hot[r] * scale : 0.f;
+  loss[r] = counts ? row_loss(total, l2, q) : 0.f;
 }
 
-// A warp per row: joins the parts' statistics (and pulls).  The target's product comes from hot, where the
-// parts leave the target out, or is made here.
+// The same with pulls, a warp a row:
 //   pull_i = sum_{j != t} p_ij w_j - (1 - p_it) w_t      (zeros for a row that does not count)
 template <typename T>
 __global__ void __launch_bounds__(256)
-loss_join_kernel(const float2* __restrict__ part, int parts, const float* __restrict__ part_o, const T* __restrict__ x, i64 ldx,
-                 i64 N, const T* __restrict__ w, i64 ldw, i64 V, int D, float scale, float c, const i64* __restrict__ target, i64 ignore,
-                 const float* __restrict__ hot, float* __restrict__ loss, float* __restrict__ lse2, float* __restrict__ pull, int* err) {
+loss_join_kernel(const float2* __restrict__ part, int parts, const float* __restrict__ part_o, i64 N, const T* __restrict__ w, i64 ldw, i64 V,
+                 int D, float c, const i64* __restrict__ target, i64 ignore, const float* __restrict__ hot, float* __restrict__ loss,
+                 float* __restrict__ lse2, float* __restrict__ pull, int* err) {
   const i64 r = ((i64)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   if (r >= N) return;
   const i64 t = target[r];
   const bool there = t >= 0 && t < V, counts = there && t != ignore;
   if (t != ignore && !counts && lane == 0) raise(err, ERRBIT_BAD_INPUT);
-  float m, others, s;
-  const float total = join_parts(part, parts, N, r, lane, 32, hot && there ? hot[r] * c : -INFINITY, m, others, s);
-  float logit = 0.f;
-  if (counts && hot) logit = hot[r] * fabsf(scale);  // hot holds products of +-x
-  if (!hot) {
-    if (counts)
-      for (int d = lane; d < D; d += 32) logit = fmaf(to_float(x[r * ldx + d]), to_float(w[t * ldw + d]), logit);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) logit += __shfl_xor_sync(0xffffffffu, logit, d);
-    logit *= scale;
-  }
+  const float l2 = there ? __fmul_rn(hot[r], c) : -INFINITY;
+  RowSums q;
+  const float total = join_parts(part, parts, N, r, lane, 32, l2, q);
   if (lane == 0) {
     lse2[r] = total;
-    loss[r] = counts ? total * LN2 - logit : 0.f;
+    loss[r] = counts ? row_loss(total, l2, q) : 0.f;
   }
-  if (pull) {  // D <= 256: a lane has every 32nd column; the parts' weights go round the warp
-    const float inv = 1.f / s, miss = others * inv;
+  {  // D <= 256: a lane has every 32nd column; the parts' weights go round the warp
+    const float inv = 1.f / q.s, miss = q.others * inv;
     float v[8];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = 0.f;
     if (counts) {
       for (int k0 = 0; k0 < parts; k0 += 32) {
         const float mk = k0 + lane < parts ? part[(i64)(k0 + lane) * N + r].x : -INFINITY;
-        const float weight = mk == -INFINITY ? 1.f : exp2f(mk - m);
+        const float weight = mk == -INFINITY ? 1.f : exp2f(mk - q.m);
         const int here = parts - k0 < 32 ? parts - k0 : 32;
         for (int k = 0; k < here; k += 4) {  // four parts requested before the first is added
           float o[4][8];
@@ -875,22 +857,22 @@ loss_join_kernel(const float2* __restrict__ part, int parts, const float* __rest
           for (int u = 0; u < 4; ++u) {
             const float* from = part_o + ((i64)(k0 + (k + u < here ? k + u : 0)) * N + r) * D;
 #pragma unroll
-            for (int q = 0; q < 8; ++q) o[u][q] = q * 32 + lane < D ? __ldg(from + q * 32 + lane) : 0.f;
+            for (int i = 0; i < 8; ++i) o[u][i] = i * 32 + lane < D ? __ldg(from + i * 32 + lane) : 0.f;
           }
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             float f = __shfl_sync(0xffffffffu, weight, (k + u) & 31);
             if (k + u >= here) break;
 #pragma unroll
-            for (int q = 0; q < 8; ++q) v[q] = fmaf(o[u][q], f, v[q]);
+            for (int i = 0; i < 8; ++i) v[i] = fmaf(o[u][i], f, v[i]);
           }
         }
       }
     }
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const int d = q * 32 + lane;
-      if (d < D) pull[r * D + d] = counts ? fmaf(-miss, to_float(w[t * ldw + d]), v[q] * inv) : 0.f;
+    for (int i = 0; i < 8; ++i) {
+      const int d = i * 32 + lane;
+      if (d < D) pull[r * D + d] = counts ? fmaf(-miss, to_float(w[t * ldw + d]), v[i] * inv) : 0.f;
     }
   }
 }
@@ -1108,9 +1090,15 @@ static int launch_tc(const CUtensorMap& b, const TcPlan& plan, const TcParams& p
 template <typename T>
 void launch_loss_join(const LossArgs& a, const float2* part_ms, int parts, const float* part_o, const float* hot, float* pull) {
   LaunchScope ls(KID_LOSS_JOIN, a.st);
-  loss_join_kernel<T><<<ceil_div_i(a.N, 8), 256, 0, a.st>>>(part_ms, parts, part_o, (const T*)a.x, a.ldx, a.N, (const T*)a.w, a.ldw, a.V,
-                                                            (int)a.D, a.scale, logit_factor(a.scale), a.target, a.ignore, hot, a.loss,
-                                                            a.lse2, pull, a.err);
+  const float c = logit_factor(a.scale);
+  if (pull) {
+    loss_join_kernel<T><<<ceil_div_i(a.N, 8), 256, 0, a.st>>>(part_ms, parts, part_o, a.N, (const T*)a.w, a.ldw, a.V, (int)a.D, c, a.target,
+                                                              a.ignore, hot, a.loss, a.lse2, pull, a.err);
+    return;
+  }
+  const int lanes = parts > 8 ? 32 : 1;
+  loss_finish_kernel<<<ceil_div_i(a.N * lanes, 256), 256, 0, a.st>>>(part_ms, parts, lanes, hot, a.N, a.V, c, a.target, a.ignore, a.loss, a.lse2,
+                                                                    a.err);
 }
 
 // what the forward pass and both gradients have in common
@@ -1167,15 +1155,7 @@ int tc_loss_forward(const LossArgs& a, float* pull) {
   p.run_sums = (float4*)(ws + L.runs);
   const int rc = with_shape<Planes<T>::count>(mode, a.N, a.V, a.D, [&](auto shape) { return launch_tc<T, decltype(shape)>(mb, plan, p, KID_LOSS, a.st); });
   if (rc != GSB_OK) return rc;
-  if (pull) {
-    launch_loss_join<T>(a, p.part_ms, plan.parts, p.part_o, p.hot, pull);
-    return GSB_OK;
-  }
-  const int lanes = plan.parts > 8 ? 32 : 1;
-  LaunchScope ls(KID_LOSS_JOIN, a.st);
-  // hot holds products of +-x; loss takes them times |scale|
-  loss_finish_kernel<<<ceil_div_i(a.N * lanes, 256), 256, 0, a.st>>>(p.part_ms, plan.parts, lanes, p.hot, a.N, a.V, fabsf(a.scale), a.target,
-                                                                    a.ignore, a.loss, a.lse2, a.err);
+  launch_loss_join<T>(a, p.part_ms, plan.parts, p.part_o, p.hot, pull);
   return GSB_OK;
 }
 
@@ -1187,7 +1167,7 @@ int tc_loss_grad_w(const LossArgs& a) {
   {
     const i64 npad = (a.N + plan.BT - 1) / plan.BT * plan.BT;
     LaunchScope ls(KID_LOSS_JOIN, a.st);
-    loss_meta_kernel<<<ceil_div_i(npad, 256), 256, 0, a.st>>>(a.lse2, a.target, a.g, a.top, a.N, npad, plan.BT, (unsigned char*)(ws + L.meta));
+    loss_meta_kernel<<<ceil_div_i(npad, 256), 256, 0, a.st>>>(a.lse2, a.miss, a.target, a.g, a.top, a.N, npad, plan.BT, (unsigned char*)(ws + L.meta));
   }
   CUtensorMap mb;
   if (!stream_map<T>(&mb, a.x, a.ldx, a.N, a.D, plan.BT, a.g, a.lse2, ws + L.x, a.st)) return GSB_ERR_CUDA;
@@ -1218,6 +1198,7 @@ int tc_loss_grad_x(const LossArgs& a) {
   p.w = a.w;
   p.ldw = a.ldw;
   p.w_bytes = row_bytes(a.w, a.ldw, sizeof(T));
+  p.miss = a.miss;
   p.out_scale = a.scale / dx_unit<typename Planes<T>::type>();
   p.out = a.dx;
   p.out_bytes = row_bytes(a.dx, a.D, sizeof(T));

@@ -210,11 +210,11 @@ std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyTotal(torch::Tensor l
   return {total, count};
 }
 
-std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyGrad(torch::Tensor x, torch::Tensor weight,
-                                                                torch::Tensor target, torch::Tensor lse2,
-                                                                torch::Tensor pull, torch::Tensor upstream,
-                                                                c10::optional<torch::Tensor> count, double scale,
-                                                                int64_t ignore, bool want_dx, bool want_dw) {
+// with the rows' losses, or (undefined) without them
+static std::tuple<torch::Tensor, torch::Tensor> GradRows(torch::Tensor x, torch::Tensor weight, torch::Tensor target,
+                                                         torch::Tensor rows, torch::Tensor lse2, torch::Tensor pull,
+                                                         torch::Tensor upstream, c10::optional<torch::Tensor> count,
+                                                         double scale, int64_t ignore, bool want_dx, bool want_dw) {
   const int dt = CheckLoss(x, weight, target, scale);
   const int64_t N = x.size(0), V = weight.size(0), D = x.size(1);
   auto good = [&](const torch::Tensor& t, int64_t n) {
@@ -222,6 +222,7 @@ std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyGrad(torch::Tensor x,
   };
   const bool per_row = upstream.dim() == 1;
   TORCH_CHECK(good(lse2, N) && lse2.is_contiguous(), "LinearCrossEntropyGrad: lse2 must be float32 [N]");
+  TORCH_CHECK(!rows.defined() || (good(rows, N) && rows.is_contiguous()), "LinearCrossEntropyGrad: losses must be float32 [N]");
   const bool have_pull = pull.numel() > 0;
   TORCH_CHECK(!have_pull || (good(pull, N * D) && pull.is_contiguous()), "LinearCrossEntropyGrad: pull must be float32 [N, D]");
   TORCH_CHECK(good(upstream, per_row ? N : 1), "LinearCrossEntropyGrad: upstream must be float32, one value or [N]");
@@ -236,13 +237,23 @@ std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyGrad(torch::Tensor x,
   auto ws = NewWorkspace(gsb_linear_ce_grad_workspace_bytes(dt, weight.data_ptr(), RowStep(weight), N, V, D, have_pull, want_dx,
                                                             want_dw),
                          x.device());
-  CheckStatus(gsb_linear_ce_grad(x.data_ptr(), dt, RowStep(x), N, weight.data_ptr(), RowStep(weight), V, D,
-                                 target.data_ptr<int64_t>(), ignore, (float)scale, lse2.data_ptr<float>(),
-                                 have_pull ? pull.data_ptr<float>() : nullptr, upstream.data_ptr<float>(), per_row, count.has_value() ? count->data_ptr<float>() : nullptr,
-                                 want_dx ? dx.data_ptr() : nullptr, want_dw ? dw.data_ptr() : nullptr, ws.data_ptr(),
-                                 (size_t)ws.numel(), ErrorWord(x.device()), CurrentStream()),
+  CheckStatus(gsb_linear_ce_grad_rows(x.data_ptr(), dt, RowStep(x), N, weight.data_ptr(), RowStep(weight), V, D,
+                                      target.data_ptr<int64_t>(), ignore, (float)scale,
+                                      rows.defined() ? rows.data_ptr<float>() : nullptr, lse2.data_ptr<float>(),
+                                      have_pull ? pull.data_ptr<float>() : nullptr, upstream.data_ptr<float>(), per_row,
+                                      count.has_value() ? count->data_ptr<float>() : nullptr, want_dx ? dx.data_ptr() : nullptr,
+                                      want_dw ? dw.data_ptr() : nullptr, ws.data_ptr(), (size_t)ws.numel(), ErrorWord(x.device()),
+                                      CurrentStream()),
               "linear_ce_grad");
   return {dx, dw};
+}
+
+std::tuple<torch::Tensor, torch::Tensor> LinearCrossEntropyGrad(torch::Tensor x, torch::Tensor weight,
+                                                                torch::Tensor target, torch::Tensor lse2,
+                                                                torch::Tensor pull, torch::Tensor upstream,
+                                                                c10::optional<torch::Tensor> count, double scale,
+                                                                int64_t ignore, bool want_dx, bool want_dw) {
+  return GradRows(x, weight, target, torch::Tensor(), lse2, pull, upstream, count, scale, ignore, want_dx, want_dw);
 }
 
 // ------------------------------------------------------------------ autograd
@@ -358,11 +369,11 @@ torch::Tensor DropoutApply(torch::Tensor data, double p, c10::optional<int64_t> 
 
 // Under create_graph, as above.
 struct LinearCrossEntropyGradFn : public torch::autograd::Function<LinearCrossEntropyGradFn> {
-  static variable_list forward(AutogradContext*, torch::Tensor x, torch::Tensor weight, torch::Tensor target, torch::Tensor lse2,
-                               torch::Tensor pull, torch::Tensor upstream, c10::optional<torch::Tensor> count, double scale,
+  static variable_list forward(AutogradContext*, torch::Tensor x, torch::Tensor weight, torch::Tensor target, torch::Tensor rows,
+                               torch::Tensor lse2, torch::Tensor pull, torch::Tensor upstream, c10::optional<torch::Tensor> count, double scale,
                                int64_t ignore, bool want_dx, bool want_dw) {
     torch::Tensor dx, dw;
-    std::tie(dx, dw) = LinearCrossEntropyGrad(x, weight, target, lse2, pull, upstream, count, scale, ignore, want_dx, want_dw);
+    std::tie(dx, dw) = GradRows(x, weight, target, rows, lse2, pull, upstream, count, scale, ignore, want_dx, want_dw);
     return {dx, dw};
   }
   static variable_list backward(AutogradContext*, variable_list) {
@@ -375,10 +386,12 @@ struct LinearCrossEntropyFn : public torch::autograd::Function<LinearCrossEntrop
                                double scale, int64_t ignore, int64_t reduction, bool want_dx) {
     torch::Tensor loss, lse2, pull, count;
     std::tie(loss, lse2, pull) = LinearCrossEntropy(x, weight, target, scale, ignore, want_dx);
+    // the backward pass has 1 - p_t from the rows' losses; the ones that go out are the caller's to change
+    const auto rows = reduction == 0 ? loss.clone() : loss;
     if (reduction != 0)
       std::tie(loss, count) = LinearCrossEntropyTotal(loss, target, weight.size(0), ignore, reduction == 2);
     if (reduction != 2) count = torch::Tensor();
-    ctx->save_for_backward({x, weight, target, lse2, pull, count});
+    ctx->save_for_backward({x, weight, target, lse2, pull, count, rows});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["ignore"] = ignore;
     return loss;
@@ -392,10 +405,10 @@ struct LinearCrossEntropyFn : public torch::autograd::Function<LinearCrossEntrop
     const int64_t ignore = ctx->saved_data["ignore"].toInt();
     torch::Tensor dx, dw;
     if (at::GradMode::is_enabled()) {
-      const auto both = LinearCrossEntropyGradFn::apply(s[0], s[1], s[2], s[3], s[4], grads[0], count, scale, ignore, want_dx, want_dw);
+      const auto both = LinearCrossEntropyGradFn::apply(s[0], s[1], s[2], s[6], s[3], s[4], grads[0], count, scale, ignore, want_dx, want_dw);
       std::tie(dx, dw) = std::make_tuple(both[0], both[1]);
     } else {
-      std::tie(dx, dw) = LinearCrossEntropyGrad(s[0], s[1], s[2], s[3], s[4], grads[0], count, scale, ignore, want_dx, want_dw);
+      std::tie(dx, dw) = GradRows(s[0], s[1], s[2], s[6], s[3], s[4], grads[0], count, scale, ignore, want_dx, want_dw);
     }
     return {want_dx ? dx : torch::Tensor(), want_dw ? dw : torch::Tensor(), torch::Tensor(), torch::Tensor(),
             torch::Tensor(), torch::Tensor(), torch::Tensor()};

@@ -281,7 +281,10 @@ GSB_API int gsb_dropout(const void* x, int dtype, int64_t n, double p, uint64_t 
  * count, 0 when there are none) of the rows' losses, *count = max(that number, 1).
  * gsb_linear_ce_grad: dx[N, D] and / or dw[V, D] (either may be NULL) from the
  * upstream gradient: upstream[N] when per_row, else one value, divided by *count
- * when count is given.  Sums are made in an order that depends on the sizes and
+ * when count is given.  gsb_linear_ce_grad_rows also takes the rows' losses as
+ * gsb_linear_ce wrote them, which hold 1 - p_target with all its digits however
+ * likely the target is; without them (loss NULL, or gsb_linear_ce_grad) it is made
+ * from the target's logit once more, to about 1e-6.  Sums are made in an order that depends on the sizes and
  * on which results are asked for, nothing else.  N, V <= 2^30.  A workspace is sized for the device that is current. */
 #define GSB_LOSS_MAX_D 65536
 GSB_API int gsb_linear_ce_has_pull(int dtype, int64_t V, int64_t D);
@@ -302,6 +305,11 @@ GSB_API int gsb_linear_ce_grad(const void* x, int dtype, int64_t ldx, int64_t N,
                                const float* lse2, const float* pull, const float* upstream, int per_row,
                                const float* count, void* dx, void* dw, void* workspace, size_t workspace_bytes,
                                int* d_err, void* cuda_stream);
+GSB_API int gsb_linear_ce_grad_rows(const void* x, int dtype, int64_t ldx, int64_t N, const void* weight, int64_t ldw,
+                                    int64_t V, int64_t D, const int64_t* target, int64_t ignore, float scale,
+                                    const float* loss, const float* lse2, const float* pull, const float* upstream,
+                                    int per_row, const float* count, void* dx, void* dw, void* workspace,
+                                    size_t workspace_bytes, int* d_err, void* cuda_stream);
 
 /* ------------------------------------------------------------------ format conversion
  * CSC -> COO column expansion: out[e] = column owning edge e.  Replaces
