@@ -22,8 +22,8 @@
 // N x V values exists anywhere.
 //
 // Bound by the hand-over from the tensor cores to the exponentials and back: at 128 columns both take
-// 1024 cycles a tile of 128 x 128 and each is busy 58 - 59 % of the time (8192 x 60000, bf16); at 256
-// columns the products are twice as long and run at 1400 (forward) and 1490 TFLOP/s (dW; 8192 x 300000).
+// 1024 cycles a tile of 128 x 128 and each is busy 58 - 60 % of the time (8192 x 60000, bf16); at 256
+// columns the products are twice as long and run at 1430 (forward) and 1520 TFLOP/s (dW; 8192 x 300000).
 //
 // The reference m moves only when a row's maximum passes it by 2^8, because moving it rescales O;
 // P stays below 2^15, which fp16 holds.  Sums and O are 32 bits; P is rounded to the type, half a
@@ -528,7 +528,7 @@ loss_tc_kernel(const __grid_constant__ CUtensorMap map_b, const TcParams p) {
               exponentials(v[k], v[k + 1], k);
               if (UNIT != 1.f) part2(mul2(join2(v[k], v[k + 1]), both(UNIT)), v[k], v[k + 1]);
             }
-            const int at = hot - col0;  // the target is not a part of P (a branch around this costs more than it: 81 us for 77)
+            const int at = hot - col0;  // the target is not a part of P (100000 x 1000 x 128: 77 us, with a branch around this 81)
 #pragma unroll
             for (int k = 0; k < C::HC; ++k) v[k] = k == at ? 0.f : v[k];
           } else {
